@@ -511,6 +511,82 @@ VECOPS_HIP_EXPORT int32_t vecops_hip_matmul_i8_dequant_packed_b(const int8_t* a,
                                                                 uint64_t workspace_size, void* stream);
 
 /*
+ * 8-bit floats.  Elements are e4m3 (OCP: 4 exponent bits, 3 mantissa bits, no infinities, largest number 448) with an fp32
+ * scale for each block: an element stands for q * scale.  vecops has no 8-bit float: the dtype number is this library's own.
+ */
+#define VECOPS_HIP_DTYPE_F8E4M3 64u
+
+/*
+ * x (f32, bf16 or f16; rank 2 or 3, any strides) -> q (e4m3, the same shape, any strides) and scales (f32, any strides).
+ * block_rows = 1: a scale for each 128 elements of a row, scales [.., M, ceil(K / 128)] (activations); block_rows = 128: one
+ * for each 128 x 128 elements, scales [.., ceil(M / 128), ceil(K / 128)] (weights).  Blocks at the edges are the elements
+ * there are.  With amax the largest |x| of a block:
+ *   scale = max(amax / 448, 2^-126),   q = e4m3(x / scale)
+ * both divisions rounded to nearest in fp32, then to the nearest e4m3, ties to even.  A block of zeros gets zeros and the
+ * scale 2^-126.  A NaN makes its block's scale NaN, an infinity makes it infinite: products with such a block are NaN.
+ */
+VECOPS_HIP_EXPORT int32_t vecops_hip_quantize_fp8_block(const VecopsHipOperand* x, uint32_t block_rows, const VecopsHipOperand* q,
+                                                        const VecopsHipOperand* scales, void* stream);
+
+/*
+ * c[..,m,n] = sum_g a_scales[..,m,g] * b_scales[..,n/128,g] * sum_{k in block g} a[..,m,k] * b[..,n,k]
+ * a [..,M,K] and b [..,N,K] e4m3, a_scales [..,M,ceil(K/128)], b_scales [..,ceil(N/128),ceil(K/128)] f32 (what
+ * vecops_hip_quantize_fp8_block writes with block_rows 1 and 128), c f32, bf16 or f16; all of rank 2 or all of rank 3, any
+ * strides (a batch stride of 0 shares an operand; row strides of the scales 0 to 2^20).  A block's products are summed in
+ * fp32 by the matrix core, its sum is scaled and added in fp32, the result is rounded once.  K == 0 writes zeros.
+ * workspace: vecops_hip_matmul_fp8_block_workspace bytes, 16-byte aligned - none where the k of both operands are
+ * contiguous (rows at any alignment); an operand stored otherwise is first copied into rows there.
+ */
+VECOPS_HIP_EXPORT uint64_t vecops_hip_matmul_fp8_block_workspace(const VecopsHipOperand* a, const VecopsHipOperand* b);
+VECOPS_HIP_EXPORT int32_t vecops_hip_matmul_fp8_block(const VecopsHipOperand* a, const VecopsHipOperand* a_scales,
+                                                      const VecopsHipOperand* b, const VecopsHipOperand* b_scales,
+                                                      const VecopsHipOperand* c, void* workspace, uint64_t workspace_size,
+                                                      void* stream);
+
+/*
+ * The experts of a mixture-of-experts layer for a few tokens (decoding), no counterpart in vecops:
+ *   out[t] = sum_r weights[t,r] * down[e] . ( silu(gate[e] . x[t]) * (up[e] . x[t]) ),  e = ids[t,r]
+ * x [T,H] bf16 or f16; ids i32 and weights f32 [T,choices]; gate_up [E, 2 I, H] (an expert's gate rows, then its up rows) and
+ * down [E, H, I], both of x's type, or e4m3 with f32 scales for blocks of 128 x 128, gate_up_scales [E, ceil(2 I / 128),
+ * ceil(H / 128)] and down_scales [E, ceil(H / 128), ceil(I / 128)] (as vecops_hip_quantize_fp8_block writes them with
+ * block_rows 128; null otherwise); out [T,H] of x's type or f32.  T <= 128, choices <= 16, E <= 512.  Rows of x, gate_up and
+ * down are contiguous, at any alignment; other strides are free.  An id outside 0..E-1 names no expert and adds nothing (an
+ * expert on another device); an expert that a token names twice counts with both weights; a token that names none gets zeros.
+ * Each weight of a named expert is read once.  Sums and the inner values are held to fp32 (the inner values to 2^-17, as a
+ * pair of bf16), the result is rounded once; it does not depend on timing.  What is not finite stays not finite.
+ * workspace: vecops_hip_moe_experts_workspace bytes, 16-byte aligned.
+ */
+VECOPS_HIP_EXPORT uint64_t vecops_hip_moe_experts_workspace(const VecopsHipOperand* ids, const VecopsHipOperand* down);
+VECOPS_HIP_EXPORT int32_t vecops_hip_moe_experts(const VecopsHipOperand* x, const VecopsHipOperand* ids, const VecopsHipOperand* weights,
+                                                 const VecopsHipOperand* gate_up, const VecopsHipOperand* gate_up_scales,
+                                                 const VecopsHipOperand* down, const VecopsHipOperand* down_scales,
+                                                 const VecopsHipOperand* out, void* workspace, uint64_t workspace_size, void* stream);
+
+/*
+ * The whole layer: the router's choice, then vecops_hip_moe_experts.  router [E,H] of x's type or f32 (contiguous rows):
+ *   l = x . router^T (fp32);   score = softmax(l) or 1 / (1 + exp(-l));
+ *   ids[t] = the experts with the largest l - with a bias, the largest score + bias - in falling order, the lower index among
+ *            equals, a NaN above every number;   weights[t,r] = score (/ the sum over the choices) * scale
+ * ids and weights are outputs here ([T,choices], choices <= E).
+ */
+enum VecopsHipMoeScoring { VECOPS_HIP_MOE_SOFTMAX = 0, VECOPS_HIP_MOE_SIGMOID = 1 };
+typedef struct VecopsHipMoeRouting {
+  uint32_t struct_size;  /* sizeof(VecopsHipMoeRouting) */
+  uint32_t scoring;      /* VecopsHipMoeScoring */
+  uint32_t renormalize;  /* 1: a token's weights are divided by their sum */
+  float scale;           /* a factor of all weights, 1 for none */
+  const float* bias;     /* device, [E], added to the scores for the choice only; or null */
+} VecopsHipMoeRouting;
+VECOPS_HIP_EXPORT uint64_t vecops_hip_moe_layer_workspace(const VecopsHipOperand* x, const VecopsHipOperand* ids,
+                                                          const VecopsHipOperand* down);
+VECOPS_HIP_EXPORT int32_t vecops_hip_moe_layer(const VecopsHipOperand* x, const VecopsHipOperand* router,
+                                               const VecopsHipMoeRouting* routing, const VecopsHipOperand* gate_up,
+                                               const VecopsHipOperand* gate_up_scales, const VecopsHipOperand* down,
+                                               const VecopsHipOperand* down_scales, const VecopsHipOperand* ids,
+                                               const VecopsHipOperand* weights, const VecopsHipOperand* out, void* workspace,
+                                               uint64_t workspace_size, void* stream);
+
+/*
  * Measurement yardstick, no counterpart in vecops: `workgroups` workgroups of four wavefronts (one per SIMD) each
  * issue iters x 32 independent matrix-core instructions of the tile kernels' shape (dtype 11: v_mfma_f32_32x32x16_bf16,
  * dtype 2: v_mfma_i32_32x32x32_i8, sixteen 32x32 accumulator tiles per wavefront) on operand registers filled from

@@ -13,6 +13,7 @@ LIB_PATH = os.path.join(HERE, "lib", "libvecops_hip.so")
 
 # VecopsDType numbers
 I8, U8, I32, F16, BF16, F32, F64 = 2, 3, 6, 10, 11, 12, 13
+F8E4M3 = 64  # this library's own (VECOPS_HIP_DTYPE_F8E4M3)
 COMPUTE_BF16, COMPUTE_F32 = 0, 1
 FAMILY_NAMES = {0: "none", 1: "tile_256", 2: "tile_128", 3: "tile_64", 4: "skinny", 5: "zero_k", 6: "tile_256x128",
                 7: "tile_128x256", 8: "tile_256x352", 9: "tile_192"}
@@ -35,6 +36,8 @@ EXPORTS = [
     "vecops_hip_matmul_grouped_workspace", "vecops_hip_matmul_grouped",
     "vecops_hip_pack_a", "vecops_hip_plan_matmul_packed_a", "vecops_hip_matmul_packed_a",
     "vecops_hip_matmul_packed_ab_workspace", "vecops_hip_matmul_packed_ab",
+    "vecops_hip_quantize_fp8_block", "vecops_hip_matmul_fp8_block_workspace", "vecops_hip_matmul_fp8_block",
+    "vecops_hip_moe_experts_workspace", "vecops_hip_moe_experts", "vecops_hip_moe_layer_workspace", "vecops_hip_moe_layer",
 ]
 
 ACT_NONE, ACT_RELU, ACT_CLAMP, ACT_SIGMOID, ACT_SILU = 0, 1, 2, 3, 4
@@ -69,6 +72,12 @@ class FamilyRequest(C.Structure):
     _fields_ = [("struct_size", C.c_uint32), ("selection", C.c_uint32), ("family", C.c_uint32), ("split_k", C.c_uint32)]
 
 
+class MoeRouting(C.Structure):
+    _fields_ = [("struct_size", C.c_uint32), ("scoring", C.c_uint32), ("renormalize", C.c_uint32), ("scale", C.c_float),
+                ("bias", C.c_void_p)]
+
+
+MOE_SCORINGS = {"softmax": 0, "sigmoid": 1}
 SELECT_AUTOMATIC, SELECT_PREFER, SELECT_REQUIRE = 0, 1, 2
 FAMILY_CODES = {name: code for code, name in FAMILY_NAMES.items()}
 
@@ -167,6 +176,16 @@ def lib() -> C.CDLL:
         L.vecops_hip_matmul_grouped.argtypes = [C.c_uint32, P, P, P, P, C.c_uint32, C.c_void_p, C.c_uint64, C.c_void_p]
         L.vecops_hip_plan_matmul_fused.argtypes = [P, P, P, P, C.c_uint32, E, C.POINTER(Plan)]
         L.vecops_hip_matmul_fused.argtypes = [P, P, P, P, C.c_uint32, E, C.c_void_p, C.c_uint64, C.c_void_p]
+        L.vecops_hip_quantize_fp8_block.argtypes = [P, C.c_uint32, P, P, C.c_void_p]
+        L.vecops_hip_matmul_fp8_block_workspace.restype = C.c_uint64
+        L.vecops_hip_matmul_fp8_block_workspace.argtypes = [P, P]
+        L.vecops_hip_matmul_fp8_block.argtypes = [P, P, P, P, P, C.c_void_p, C.c_uint64, C.c_void_p]
+        L.vecops_hip_moe_experts_workspace.restype = C.c_uint64
+        L.vecops_hip_moe_experts_workspace.argtypes = [P, P]
+        L.vecops_hip_moe_experts.argtypes = [P] * 8 + [C.c_void_p, C.c_uint64, C.c_void_p]
+        L.vecops_hip_moe_layer_workspace.restype = C.c_uint64
+        L.vecops_hip_moe_layer_workspace.argtypes = [P, P, P]
+        L.vecops_hip_moe_layer.argtypes = [P, P, C.POINTER(MoeRouting)] + [P] * 7 + [C.c_void_p, C.c_uint64, C.c_void_p]
         _lib = L
     return _lib
 
@@ -214,7 +233,7 @@ def _check(rc: int) -> None:
 def _torch_dtype_code(t) -> int:
     import torch
     return {torch.int8: I8, torch.uint8: U8, torch.int32: I32, torch.float16: F16, torch.bfloat16: BF16,
-            torch.float32: F32, torch.float64: F64}[t.dtype]
+            torch.float32: F32, torch.float64: F64, torch.float8_e4m3fn: F8E4M3}[t.dtype]
 
 
 def operand(t) -> Operand:
@@ -705,3 +724,101 @@ def matmul_i8_dequant_packed_b(a, packed: PackedB, row_scales, column_scales, c,
         correction.data_ptr() if correction is not None else None, c.data_ptr(), c.stride(0), m, n, k, ws_ptr,
         ws_size, _stream_handle(stream)))
     return c
+
+
+def _on_one_device(name: str, *tensors) -> None:
+    """The kernels read through plain addresses: a tensor elsewhere is refused here."""
+    devices = {t.device for t in tensors if t is not None}
+    if len(devices) != 1 or next(iter(devices)).type != "cuda":
+        raise ValueError(f"{name}: tensors must all be on one GPU, got {sorted(map(str, devices))}")
+
+
+def quantize_fp8_block(x, q, scales, block_rows: int = 1, stream=None):
+    """x -> q (``torch.float8_e4m3fn``) and a scale for each block of ``block_rows`` (1 or 128) x 128 elements: ``q * scale``
+    stands for x.  Returns (q, scales)."""
+    if stream is None:
+        rc = (_calls or native_calls()).quantize_fp8_block(x, q, scales, block_rows)
+        if rc == 0:
+            return q, scales
+        if rc > 0:
+            _check(rc)
+    _on_one_device("quantize_fp8_block", x, q, scales)
+    ox, oq, os_ = operand(x), operand(q), operand(scales)
+    _check(lib().vecops_hip_quantize_fp8_block(C.byref(ox), block_rows, C.byref(oq), C.byref(os_), _stream_handle(stream)))
+    return q, scales
+
+
+def matmul_fp8_block(a, a_scales, b, b_scales, c, workspace=None, stream=None):
+    """c[..,M,N] = (a * its scales) . (b * its scales)^T for e4m3 operands as ``quantize_fp8_block`` writes them: a scale for
+    each 128 k of a row of a, and for each 128 x 128 block of b.  Returns c."""
+    if stream is None:
+        rc = (_calls or native_calls()).matmul_fp8_block(a, a_scales, b, b_scales, c, workspace)
+        if rc == 0:
+            return c
+        if rc > 0:
+            _check(rc)
+    import torch
+    _on_one_device("matmul_fp8_block", a, a_scales, b, b_scales, c, workspace)
+    oa, osa, ob, osb, oc = operand(a), operand(a_scales), operand(b), operand(b_scales), operand(c)
+    need = lib().vecops_hip_matmul_fp8_block_workspace(C.byref(oa), C.byref(ob))
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        workspace = torch.empty(need, dtype=torch.uint8, device=c.device)
+    ws_ptr = workspace.data_ptr() if workspace is not None else None
+    ws_size = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    _check(lib().vecops_hip_matmul_fp8_block(C.byref(oa), C.byref(osa), C.byref(ob), C.byref(osb), C.byref(oc), ws_ptr, ws_size,
+                                             _stream_handle(stream)))
+    return c
+
+
+def moe_experts(x, ids, weights, gate_up, down, out, gate_up_scales=None, down_scales=None, workspace=None, stream=None):
+    """out[t] = sum_r weights[t,r] * down[e] . (silu(gate[e] . x[t]) * (up[e] . x[t])) with e = ids[t,r], for up to 128 tokens:
+    the experts of a mixture-of-experts layer on a choice made elsewhere.  ``gate_up`` [E, 2 I, H] and ``down`` [E, H, I] are of
+    x's type, or e4m3 with ``gate_up_scales`` and ``down_scales`` for blocks of 128 x 128; ids outside 0..E-1 add nothing.
+    Returns out."""
+    if stream is None:
+        rc = (_calls or native_calls()).moe_experts(x, ids, weights, gate_up, gate_up_scales, down, down_scales, out, workspace)
+        if rc == 0:
+            return out
+        if rc > 0:
+            _check(rc)
+    import torch
+    _on_one_device("moe_experts", x, ids, weights, gate_up, gate_up_scales, down, down_scales, out, workspace)
+    o = [C.byref(operand(t)) if t is not None else None
+         for t in (x, ids, weights, gate_up, gate_up_scales, down, down_scales, out)]
+    need = lib().vecops_hip_moe_experts_workspace(o[1], o[5])
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        workspace = torch.empty(need, dtype=torch.uint8, device=out.device)
+    ws_ptr = workspace.data_ptr() if workspace is not None else None
+    ws_size = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    _check(lib().vecops_hip_moe_experts(*o, ws_ptr, ws_size, _stream_handle(stream)))
+    return out
+
+
+def moe_layer(x, router, gate_up, down, ids, weights, out, scoring: str = "softmax", renormalize: bool = True, scale: float = 1.0,
+              bias=None, gate_up_scales=None, down_scales=None, workspace=None, stream=None):
+    """A whole mixture-of-experts layer for up to 128 tokens: the router's scores, the ``ids.shape[1]`` best experts of each token
+    and their weights (written to ``ids``, int32, and ``weights``, fp32), then ``moe_experts``.  ``scoring`` is "softmax" or
+    "sigmoid"; ``bias`` (fp32, [E]) is added to the scores for the choice only; ``renormalize`` divides a token's weights by
+    their sum, ``scale`` multiplies them.  Returns out."""
+    import torch
+    if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous() or bias.shape != (router.shape[0],) or
+                             bias.device != x.device):
+        raise ValueError("moe_layer: bias must be a contiguous float32 vector on x's device with an element for each expert")
+    routing = MoeRouting(C.sizeof(MoeRouting), MOE_SCORINGS[scoring], int(renormalize), scale, bias.data_ptr() if bias is not None else None)
+    if stream is None:
+        rc = (_calls or native_calls()).moe_layer(x, router, C.addressof(routing), gate_up, gate_up_scales, down, down_scales, ids, weights,
+                                                  out, workspace)
+        if rc == 0:
+            return out
+        if rc > 0:
+            _check(rc)
+    _on_one_device("moe_layer", x, router, gate_up, gate_up_scales, down, down_scales, ids, weights, out, workspace)
+    o = [C.byref(operand(t)) if t is not None else None
+         for t in (x, router, gate_up, gate_up_scales, down, down_scales, ids, weights, out)]
+    need = lib().vecops_hip_moe_layer_workspace(o[0], o[6], o[4])
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        workspace = torch.empty(need, dtype=torch.uint8, device=out.device)
+    ws_ptr = workspace.data_ptr() if workspace is not None else None
+    ws_size = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    _check(lib().vecops_hip_moe_layer(o[0], o[1], C.byref(routing), *o[2:], ws_ptr, ws_size, _stream_handle(stream)))
+    return out

@@ -9,7 +9,9 @@
 #include <cstdio>
 #include <cstring>
 
+#include "fp8_block.h"
 #include "gemm_f64.h"
+#include "moe_few_tokens.h"
 #include "packed_row_sums.h"
 #include "skinny_dense.h"
 #include "skinny_w8a16.h"
@@ -23,7 +25,8 @@ namespace {
 using namespace vecops_hip;
 
 enum : int32_t { ST_OK = 0, ST_INVALID = 1, ST_NOT_APPLICABLE = 2, ST_EXEC = 6 };
-enum : uint32_t { DT_I8 = 2, DT_U8 = 3, DT_I32 = 6, DT_F16 = 10, DT_BF16 = 11, DT_F32 = 12, DT_F64 = 13 };
+enum : uint32_t { DT_I8 = 2, DT_U8 = 3, DT_I32 = 6, DT_F16 = 10, DT_BF16 = 11, DT_F32 = 12, DT_F64 = 13,
+                  DT_E4M3 = VECOPS_HIP_DTYPE_F8E4M3 };
 // fp64 operands run on a kernel of their own (gemm_f64.hip), outside the tile kernels' operand classes and outputs
 constexpr int kSrcF64 = 100, kOutF64 = 100;
 
@@ -2695,6 +2698,298 @@ int32_t vecops_hip_matmul_w8a16_group(const void* x, int64_t ldx, const int8_t* 
   else launch_skinny<16, 1, 1>(p, s);
   e = hipGetLastError();
   if (e != hipSuccess) return fail(ST_EXEC, "skinny kernel launch: %s", hipGetErrorString(e));
+  return ST_OK;
+}
+
+// ---- 8-bit floats with a scale for each block of 128 -----------------------------------------------------------------
+
+namespace {
+
+int real_kind(uint32_t dtype) {
+  return dtype == DT_BF16 ? FP8_REAL_BF16 : dtype == DT_F16 ? FP8_REAL_F16 : dtype == DT_F32 ? FP8_REAL_F32 : -1;
+}
+
+int64_t fp8_blocks(int64_t extent) { return (extent + kFp8Block - 1) / kFp8Block; }
+
+// What the product reads an operand through: its own rows where their k are contiguous (any alignment), else a copy of them
+// in the workspace.  (Offsets inside a tile of 256 rows are 32 bits wide.)
+bool fp8_rows_ok(const View& v) { return (v.cs == 1 || v.cols <= 1) && v.rs >= 0 && v.rs * 256 + v.cols + 128 < (int64_t{1} << 31); }
+int64_t fp8_row_bytes(const View& v) { return (v.cols + 15) / 16 * 16; }
+uint64_t fp8_copy_bytes(const View& v) {
+  if (v.batch == 0 || v.rows == 0 || v.cols == 0 || fp8_rows_ok(v)) return 0;
+  return round_up_256(static_cast<uint64_t>(v.bs == 0 ? 1 : v.batch) * static_cast<uint64_t>(v.rows) * static_cast<uint64_t>(fp8_row_bytes(v)));
+}
+
+struct Fp8Product {
+  View a, sa, b, sb, c;
+};
+
+int32_t describe_fp8(const VecopsHipOperand* a, const VecopsHipOperand* a_scales, const VecopsHipOperand* b,
+                     const VecopsHipOperand* b_scales, const VecopsHipOperand* c, Fp8Product* pr) {
+  if (!normalise(a, &pr->a) || !normalise(a_scales, &pr->sa) || !normalise(b, &pr->b) || !normalise(b_scales, &pr->sb) || !normalise(c, &pr->c))
+    return fail(ST_INVALID, "matmul_fp8_block: operands must be rank 2 or 3 with non-negative extents");
+  if (a->rank != b->rank || a->rank != c->rank || a->rank != a_scales->rank || a->rank != b_scales->rank)
+    return fail(ST_INVALID, "matmul_fp8_block: operand ranks differ");
+  if (pr->a.dtype != DT_E4M3 || pr->b.dtype != DT_E4M3 || real_kind(pr->c.dtype) < 0)
+    return fail(ST_NOT_APPLICABLE, "matmul_fp8_block: a and b must be e4m3, c f32, bf16 or f16");
+  if (pr->sa.dtype != DT_F32 || pr->sb.dtype != DT_F32) return fail(ST_INVALID, "matmul_fp8_block: scales must be f32");
+  const int64_t m = pr->a.rows, n = pr->b.rows, k = pr->a.cols, batch = pr->a.batch;
+  if (pr->b.cols != k) return fail(ST_INVALID, "matmul_fp8_block: K of a (%lld) and b (%lld) differ", (long long)k, (long long)pr->b.cols);
+  if (pr->c.rows != m || pr->c.cols != n) return fail(ST_INVALID, "matmul_fp8_block: c must be [M=%lld, N=%lld]", (long long)m, (long long)n);
+  if (pr->b.batch != batch || pr->c.batch != batch || pr->sa.batch != batch || pr->sb.batch != batch)
+    return fail(ST_INVALID, "matmul_fp8_block: batch extents differ");
+  if (pr->sa.rows != m || pr->sa.cols != fp8_blocks(k))
+    return fail(ST_INVALID, "matmul_fp8_block: a_scales must be [M=%lld, ceil(K / 128)=%lld]", (long long)m, (long long)fp8_blocks(k));
+  if (pr->sb.rows != fp8_blocks(n) || pr->sb.cols != fp8_blocks(k))
+    return fail(ST_INVALID, "matmul_fp8_block: b_scales must be [ceil(N / 128)=%lld, ceil(K / 128)=%lld]", (long long)fp8_blocks(n),
+                (long long)fp8_blocks(k));
+  if (m > INT32_MAX / 2 || n > INT32_MAX / 2 || k > INT32_MAX / 2 || batch > 65535) return fail(ST_INVALID, "matmul_fp8_block: extent too large");
+  // (a grid holds fewer than 2^32 threads: workgroups of 256 for tiles of 128 x 128, of 512 for 16 columns of a few rows)
+  if (((m + 127) / 128) * ((n + 127) / 128) >= (1 << 24) || (m <= 64 && n > (1 << 26)))
+    return fail(ST_INVALID, "matmul_fp8_block: extent too large");
+  // scales of a tile's rows are reached by 32-bit offsets
+  if (pr->sa.rs < 0 || pr->sb.rs < 0 || pr->sa.rs > (int64_t{1} << 20) || pr->sb.rs > (int64_t{1} << 20))
+    return fail(ST_NOT_APPLICABLE, "matmul_fp8_block: row strides of the scales must lie in 0 .. 2^20");
+  return ST_OK;
+}
+
+}  // namespace
+
+int32_t vecops_hip_quantize_fp8_block(const VecopsHipOperand* x, uint32_t block_rows, const VecopsHipOperand* q,
+                                      const VecopsHipOperand* scales, void* stream) {
+  View vx, vq, vs;
+  if (!normalise(x, &vx) || !normalise(q, &vq) || !normalise(scales, &vs))
+    return fail(ST_INVALID, "quantize_fp8_block: operands must be rank 2 or 3 with non-negative extents");
+  if (block_rows != 1 && block_rows != kFp8Block) return fail(ST_INVALID, "quantize_fp8_block: block_rows must be 1 or 128, got %u", block_rows);
+  if (real_kind(vx.dtype) < 0 || vq.dtype != DT_E4M3) return fail(ST_NOT_APPLICABLE, "quantize_fp8_block: x must be f32, bf16 or f16 and q e4m3");
+  if (vs.dtype != DT_F32) return fail(ST_INVALID, "quantize_fp8_block: scales must be f32");
+  if (x->rank != q->rank || x->rank != scales->rank || vx.batch != vq.batch || vx.rows != vq.rows || vx.cols != vq.cols)
+    return fail(ST_INVALID, "quantize_fp8_block: x and q differ in shape");
+  const int64_t line_blocks = (vx.rows + block_rows - 1) / block_rows, groups = fp8_blocks(vx.cols);
+  if (vs.batch != vx.batch || vs.rows != line_blocks || vs.cols != groups)
+    return fail(ST_INVALID, "quantize_fp8_block: scales must be [%lld, %lld]", (long long)line_blocks, (long long)groups);
+  if (vx.batch == 0 || vx.rows == 0 || vx.cols == 0) return ST_OK;
+  if (vx.data == nullptr || vq.data == nullptr || vs.data == nullptr) return fail(ST_INVALID, "quantize_fp8_block: null operand");
+  if (vx.batch > INT32_MAX || vx.rows > INT32_MAX / 2 || vx.cols > INT32_MAX / 2 || vx.batch * line_blocks > INT32_MAX / groups ||
+      (block_rows != 1 && vx.batch * line_blocks * groups >= (1 << 24)))   // (a workgroup of 256 each, in a grid of fewer than 2^32 threads)
+    return fail(ST_INVALID, "quantize_fp8_block: extent too large");
+  Fp8QuantizeParams p;
+  p.x = vx.data;
+  p.q = static_cast<uint8_t*>(vq.data);
+  p.scales = static_cast<float*>(vs.data);
+  p.x_bs = vx.bs, p.x_rs = vx.rs, p.x_cs = vx.cs;
+  p.q_bs = vq.bs, p.q_rs = vq.rs, p.q_cs = vq.cs;
+  p.s_bs = vs.bs, p.s_rs = vs.rs, p.s_cs = vs.cs;
+  p.batch = static_cast<int32_t>(vx.batch), p.rows = static_cast<int32_t>(vx.rows), p.k = static_cast<int32_t>(vx.cols);
+  p.groups = static_cast<int32_t>(groups);
+  p.kind = real_kind(vx.dtype);
+  const hipError_t e = launch_fp8_quantize(p, static_cast<int>(block_rows), static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(ST_EXEC, "quantize_fp8_block: kernel launch: %s", hipGetErrorString(e));
+  return ST_OK;
+}
+
+uint64_t vecops_hip_matmul_fp8_block_workspace(const VecopsHipOperand* a, const VecopsHipOperand* b) {
+  View va, vb;
+  if (!normalise(a, &va) || !normalise(b, &vb)) return 0;
+  return fp8_copy_bytes(va) + fp8_copy_bytes(vb);
+}
+
+int32_t vecops_hip_matmul_fp8_block(const VecopsHipOperand* a, const VecopsHipOperand* a_scales, const VecopsHipOperand* b,
+                                    const VecopsHipOperand* b_scales, const VecopsHipOperand* c, void* workspace,
+                                    uint64_t workspace_size, void* stream) {
+  Fp8Product pr;
+  const int32_t rc = describe_fp8(a, a_scales, b, b_scales, c, &pr);
+  if (rc != ST_OK) return rc;
+  if (pr.a.batch == 0 || pr.a.rows == 0 || pr.b.rows == 0) return ST_OK;
+  if (pr.c.data == nullptr || (pr.a.cols > 0 && (pr.a.data == nullptr || pr.b.data == nullptr || pr.sa.data == nullptr || pr.sb.data == nullptr)))
+    return fail(ST_INVALID, "matmul_fp8_block: null operand");
+  const uint64_t copy_a = fp8_copy_bytes(pr.a), copy_b = fp8_copy_bytes(pr.b);
+  if (copy_a + copy_b > 0 && (workspace == nullptr || workspace_size < copy_a + copy_b || !aligned16(workspace)))
+    return fail(ST_INVALID, "matmul_fp8_block: needs a 16-byte aligned workspace of %llu bytes", (unsigned long long)(copy_a + copy_b));
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  uint8_t* room = static_cast<uint8_t*>(workspace);
+  for (View* v : {&pr.a, &pr.b}) {
+    const uint64_t bytes = fp8_copy_bytes(*v);
+    if (bytes == 0) continue;
+    const int64_t ld = fp8_row_bytes(*v), batches = v->bs == 0 ? 1 : v->batch;
+    if (((v->rows + 63) / 64) * ((v->cols + 63) / 64) >= (1 << 24)) return fail(ST_INVALID, "matmul_fp8_block: extent too large");
+    const hipError_t e = launch_fp8_rows(static_cast<const uint8_t*>(v->data), v->bs, v->rs, v->cs, room, ld, static_cast<int32_t>(batches),
+                                         static_cast<int32_t>(v->rows), static_cast<int32_t>(v->cols), s);
+    if (e != hipSuccess) return fail(ST_EXEC, "matmul_fp8_block: kernel launch: %s", hipGetErrorString(e));
+    v->data = room;
+    v->bs = v->bs == 0 ? 0 : v->rows * ld;
+    v->rs = ld;
+    v->cs = 1;
+    room += bytes;
+  }
+  Fp8MatmulParams p;
+  p.a = static_cast<const uint8_t*>(pr.a.data), p.b = static_cast<const uint8_t*>(pr.b.data);
+  p.a_scales = static_cast<const float*>(pr.sa.data), p.b_scales = static_cast<const float*>(pr.sb.data);
+  p.c = pr.c.data;
+  p.lda = pr.a.rs, p.ldb = pr.b.rs, p.a_bs = pr.a.bs, p.b_bs = pr.b.bs;
+  p.as_rs = pr.sa.rs, p.as_gs = pr.sa.cs, p.as_bs = pr.sa.bs;
+  p.bs_rs = pr.sb.rs, p.bs_gs = pr.sb.cs, p.bs_bs = pr.sb.bs;
+  p.c_rs = pr.c.rs, p.c_cs = pr.c.cs, p.c_bs = pr.c.bs;
+  p.m = static_cast<int32_t>(pr.a.rows), p.n = static_cast<int32_t>(pr.b.rows), p.k = static_cast<int32_t>(pr.a.cols);
+  p.batch = static_cast<int32_t>(pr.a.batch);
+  p.groups = static_cast<int32_t>(fp8_blocks(pr.a.cols));
+  p.out_kind = real_kind(pr.c.dtype);
+  const hipError_t e = launch_fp8_matmul(p, s);
+  if (e != hipSuccess) return fail(ST_EXEC, "matmul_fp8_block: kernel launch: %s", hipGetErrorString(e));
+  return ST_OK;
+}
+
+// ---- mixture-of-experts layers for a few tokens ---------------------------------------------------------------------
+
+namespace {
+
+struct MoeExperts {
+  View x, ids, weights, gate_up, down, out;
+  MoeExpertsParams p;
+};
+
+int64_t moe_inner_pad(int64_t inner) { return (inner + 15) / 16 * 16; }
+uint64_t moe_middle_bytes(int64_t tokens, int64_t top, int64_t inner) {
+  return round_up_256(static_cast<uint64_t>(tokens) * static_cast<uint64_t>(top) * static_cast<uint64_t>(moe_inner_pad(inner)) * 4u);
+}
+uint64_t moe_logits_bytes(int64_t tokens, int64_t experts, int64_t hidden) {
+  return round_up_256(static_cast<uint64_t>(moe_route_parts(static_cast<int>(hidden))) * static_cast<uint64_t>(tokens) * static_cast<uint64_t>(experts) * 4u);
+}
+
+bool matrix_of(const VecopsHipOperand* o, View* v) { return normalise(o, v) && o->rank == 2; }
+
+// Checks everything but the workspace and fills the parameters; `what` names the entry point in messages.
+int32_t describe_moe(const char* what, const VecopsHipOperand* x, const VecopsHipOperand* ids, const VecopsHipOperand* weights,
+                     const VecopsHipOperand* gate_up, const VecopsHipOperand* gate_up_scales, const VecopsHipOperand* down,
+                     const VecopsHipOperand* down_scales, const VecopsHipOperand* out, MoeExperts* m) {
+  if (!matrix_of(x, &m->x) || !matrix_of(ids, &m->ids) || !matrix_of(weights, &m->weights) || !matrix_of(out, &m->out))
+    return fail(ST_INVALID, "%s: x, ids, weights and out must be rank 2", what);
+  if (!normalise(gate_up, &m->gate_up) || gate_up->rank != 3 || !normalise(down, &m->down) || down->rank != 3)
+    return fail(ST_INVALID, "%s: gate_up and down must be rank 3", what);
+  const int64_t tokens = m->x.rows, hidden = m->x.cols, top = m->ids.cols, experts = m->gate_up.batch, inner = m->down.cols;
+  if (m->ids.rows != tokens || m->weights.rows != tokens || m->weights.cols != top)
+    return fail(ST_INVALID, "%s: ids and weights must be [tokens=%lld, choices]", what, (long long)tokens);
+  if (m->gate_up.cols != hidden || m->gate_up.rows != 2 * inner || m->down.batch != experts || m->down.rows != hidden)
+    return fail(ST_INVALID, "%s: gate_up must be [experts, 2 * inner, hidden=%lld] and down [experts, hidden, inner]", what, (long long)hidden);
+  if (m->out.rows != tokens || m->out.cols != hidden) return fail(ST_INVALID, "%s: out must be [%lld, %lld]", what, (long long)tokens, (long long)hidden);
+  if (m->ids.dtype != DT_I32 || m->weights.dtype != DT_F32) return fail(ST_INVALID, "%s: ids must be i32 and weights f32", what);
+  if ((m->x.dtype != DT_BF16 && m->x.dtype != DT_F16) || (m->out.dtype != m->x.dtype && m->out.dtype != DT_F32) ||
+      m->gate_up.dtype != m->down.dtype || (m->down.dtype != m->x.dtype && m->down.dtype != DT_E4M3))
+    return fail(ST_NOT_APPLICABLE, "%s: x must be bf16 or f16, out of its type or f32, gate_up and down of its type or e4m3", what);
+  if (tokens > kMoeMostTokens || top > kMoeMostChoices || experts > kMoeMostExperts)
+    return fail(ST_NOT_APPLICABLE, "%s: serves up to %d tokens, %d choices and %d experts, got %lld, %lld and %lld", what, kMoeMostTokens,
+                kMoeMostChoices, kMoeMostExperts, (long long)tokens, (long long)top, (long long)experts);
+  if (hidden > (1 << 24) || inner > (1 << 24)) return fail(ST_INVALID, "%s: extent too large", what);
+  if ((m->x.cs != 1 && hidden > 1) || (m->gate_up.cs != 1 && hidden > 1) || (m->down.cs != 1 && inner > 1))
+    return fail(ST_NOT_APPLICABLE, "%s: rows of x, gate_up and down must be contiguous", what);
+  MoeExpertsParams& p = m->p;
+  p.gate_up_scales = p.down_scales = nullptr;
+  p.gs_es = p.gs_rs = p.gs_cs = p.ds_es = p.ds_rs = p.ds_cs = 0;
+  p.w_e4m3 = m->down.dtype == DT_E4M3;
+  if (p.w_e4m3) {
+    View gs, ds;
+    if (!normalise(gate_up_scales, &gs) || gate_up_scales->rank != 3 || gs.dtype != DT_F32 || !normalise(down_scales, &ds) ||
+        down_scales->rank != 3 || ds.dtype != DT_F32)
+      return fail(ST_INVALID, "%s: e4m3 weights need rank-3 f32 scales", what);
+    if (gs.batch != experts || gs.rows != fp8_blocks(2 * inner) || gs.cols != fp8_blocks(hidden) || ds.batch != experts ||
+        ds.rows != fp8_blocks(hidden) || ds.cols != fp8_blocks(inner))
+      return fail(ST_INVALID, "%s: scales must be [experts, ceil(rows / 128), ceil(columns / 128)] of gate_up and down", what);
+    if (experts > 0 && inner > 0 && hidden > 0 && (gs.data == nullptr || ds.data == nullptr)) return fail(ST_INVALID, "%s: null operand", what);
+    p.gate_up_scales = static_cast<const float*>(gs.data), p.down_scales = static_cast<const float*>(ds.data);
+    p.gs_es = gs.bs, p.gs_rs = gs.rs, p.gs_cs = gs.cs;
+    p.ds_es = ds.bs, p.ds_rs = ds.rs, p.ds_cs = ds.cs;
+  } else if (gate_up_scales != nullptr || down_scales != nullptr) {
+    return fail(ST_INVALID, "%s: scales belong to e4m3 weights", what);
+  }
+  if (tokens > 0 && hidden > 0) {
+    if (m->x.data == nullptr || m->out.data == nullptr || (top > 0 && (m->ids.data == nullptr || m->weights.data == nullptr)) ||
+        (experts > 0 && inner > 0 && (m->gate_up.data == nullptr || m->down.data == nullptr)))
+      return fail(ST_INVALID, "%s: null operand", what);
+  }
+  p.x = m->x.data;
+  p.ids = static_cast<const int32_t*>(m->ids.data);
+  p.weights = static_cast<const float*>(m->weights.data);
+  p.gate_up = m->gate_up.data, p.down = m->down.data, p.out = m->out.data;
+  p.ldx = m->x.rs;
+  p.ids_rs = m->ids.rs, p.ids_cs = m->ids.cs, p.weights_rs = m->weights.rs, p.weights_cs = m->weights.cs;
+  p.gate_up_es = m->gate_up.bs, p.gate_up_rs = m->gate_up.rs, p.down_es = m->down.bs, p.down_rs = m->down.rs;
+  p.out_rs = m->out.rs, p.out_cs = m->out.cs;
+  p.tokens = static_cast<int32_t>(tokens), p.experts = static_cast<int32_t>(experts), p.hidden = static_cast<int32_t>(hidden);
+  p.inner = static_cast<int32_t>(inner), p.inner_pad = static_cast<int32_t>(moe_inner_pad(inner)), p.top = static_cast<int32_t>(top);
+  p.x_f16 = m->x.dtype == DT_F16;
+  p.out_f32 = m->out.dtype == DT_F32;
+  return ST_OK;
+}
+
+}  // namespace
+
+uint64_t vecops_hip_moe_experts_workspace(const VecopsHipOperand* ids, const VecopsHipOperand* down) {
+  View vi, vd;
+  if (!matrix_of(ids, &vi) || !normalise(down, &vd)) return 0;
+  return moe_middle_bytes(vi.rows, vi.cols, vd.cols);
+}
+
+int32_t vecops_hip_moe_experts(const VecopsHipOperand* x, const VecopsHipOperand* ids, const VecopsHipOperand* weights,
+                               const VecopsHipOperand* gate_up, const VecopsHipOperand* gate_up_scales, const VecopsHipOperand* down,
+                               const VecopsHipOperand* down_scales, const VecopsHipOperand* out, void* workspace, uint64_t workspace_size,
+                               void* stream) {
+  MoeExperts m;
+  const int32_t rc = describe_moe("moe_experts", x, ids, weights, gate_up, gate_up_scales, down, down_scales, out, &m);
+  if (rc != ST_OK) return rc;
+  if (m.p.tokens == 0 || m.p.hidden == 0) return ST_OK;
+  const uint64_t need = moe_middle_bytes(m.p.tokens, m.p.top, m.p.inner);
+  if (need > 0 && (workspace == nullptr || workspace_size < need || !aligned16(workspace)))
+    return fail(ST_INVALID, "moe_experts: needs a 16-byte aligned workspace of %llu bytes", (unsigned long long)need);
+  m.p.middle = static_cast<uint16_t*>(workspace);
+  const hipError_t e = launch_moe_experts(m.p, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(ST_EXEC, "moe_experts: kernel launch: %s", hipGetErrorString(e));
+  return ST_OK;
+}
+
+uint64_t vecops_hip_moe_layer_workspace(const VecopsHipOperand* x, const VecopsHipOperand* ids, const VecopsHipOperand* down) {
+  View vx, vi, vd;
+  if (!matrix_of(x, &vx) || !matrix_of(ids, &vi) || !normalise(down, &vd) || vx.cols > (1 << 24)) return 0;
+  return moe_middle_bytes(vi.rows, vi.cols, vd.cols) + moe_logits_bytes(vx.rows, vd.batch, vx.cols);
+}
+
+int32_t vecops_hip_moe_layer(const VecopsHipOperand* x, const VecopsHipOperand* router, const VecopsHipMoeRouting* routing,
+                             const VecopsHipOperand* gate_up, const VecopsHipOperand* gate_up_scales, const VecopsHipOperand* down,
+                             const VecopsHipOperand* down_scales, const VecopsHipOperand* ids, const VecopsHipOperand* weights,
+                             const VecopsHipOperand* out, void* workspace, uint64_t workspace_size, void* stream) {
+  MoeExperts m;
+  int32_t rc = describe_moe("moe_layer", x, ids, weights, gate_up, gate_up_scales, down, down_scales, out, &m);
+  if (rc != ST_OK) return rc;
+  View vr;
+  if (!matrix_of(router, &vr) || vr.rows != m.p.experts || vr.cols != m.p.hidden)
+    return fail(ST_INVALID, "moe_layer: router must be [experts=%d, hidden=%d]", m.p.experts, m.p.hidden);
+  if (vr.dtype != m.x.dtype && vr.dtype != DT_F32) return fail(ST_NOT_APPLICABLE, "moe_layer: router must be of x's type or f32");
+  if (vr.cs != 1 && vr.cols > 1) return fail(ST_NOT_APPLICABLE, "moe_layer: rows of router must be contiguous");
+  if (routing == nullptr || routing->struct_size != sizeof(VecopsHipMoeRouting)) return fail(ST_INVALID, "moe_layer: routing record of another size");
+  if (routing->scoring > VECOPS_HIP_MOE_SIGMOID) return fail(ST_INVALID, "moe_layer: unknown scoring %u", routing->scoring);
+  if (m.p.top > m.p.experts) return fail(ST_INVALID, "moe_layer: %d choices among %d experts", m.p.top, m.p.experts);
+  if (m.p.tokens == 0 || m.p.hidden == 0) return ST_OK;
+  if (m.p.experts > 0 && vr.data == nullptr) return fail(ST_INVALID, "moe_layer: null operand");
+  const uint64_t middle = moe_middle_bytes(m.p.tokens, m.p.top, m.p.inner), need = middle + moe_logits_bytes(m.p.tokens, m.p.experts, m.p.hidden);
+  if (need > 0 && (workspace == nullptr || workspace_size < need || !aligned16(workspace)))
+    return fail(ST_INVALID, "moe_layer: needs a 16-byte aligned workspace of %llu bytes", (unsigned long long)need);
+  m.p.middle = static_cast<uint16_t*>(workspace);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (m.p.top > 0) {
+    MoeRouteParams r;
+    r.x = m.p.x, r.router = vr.data, r.bias = routing->bias;
+    r.logits = reinterpret_cast<float*>(static_cast<char*>(workspace) + middle);
+    r.ids = static_cast<int32_t*>(m.ids.data), r.weights = static_cast<float*>(m.weights.data);
+    r.ldx = m.p.ldx, r.ld_router = vr.rs;
+    r.ids_rs = m.p.ids_rs, r.ids_cs = m.p.ids_cs, r.weights_rs = m.p.weights_rs, r.weights_cs = m.p.weights_cs;
+    r.tokens = m.p.tokens, r.experts = m.p.experts, r.hidden = m.p.hidden, r.top = m.p.top;
+    r.parts = moe_route_parts(m.p.hidden);
+    r.x_f16 = m.p.x_f16, r.router_f32 = vr.dtype == DT_F32;
+    r.sigmoid = routing->scoring == VECOPS_HIP_MOE_SIGMOID, r.renormalize = routing->renormalize != 0, r.scale = routing->scale;
+    const hipError_t e = launch_moe_route(r, s);
+    if (e != hipSuccess) return fail(ST_EXEC, "moe_layer: kernel launch: %s", hipGetErrorString(e));
+  }
+  const hipError_t e = launch_moe_experts(m.p, s);
+  if (e != hipSuccess) return fail(ST_EXEC, "moe_layer: kernel launch: %s", hipGetErrorString(e));
   return ST_OK;
 }
 

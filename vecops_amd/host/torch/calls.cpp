@@ -270,6 +270,93 @@ int matmul_packed_b(PyObject* const* args) {
   });
 }
 
+// describe() for the entry points that take 8-bit floats too.
+bool describe_any(PyObject* object, VecopsHipOperand* o) {
+  const at::Tensor* t = plain_tensor(object);
+  if (t == nullptr) return false;
+  if (t->scalar_type() != at::kFloat8_e4m3fn) return describe(*t, o);
+  const int64_t rank = t->dim();
+  if (rank > 3) return false;
+  memset(o, 0, sizeof(*o));
+  o->dtype = VECOPS_HIP_DTYPE_F8E4M3;
+  o->data = t->data_ptr();
+  o->rank = static_cast<uint32_t>(rank);
+  for (int64_t i = 0; i < rank; ++i) {
+    o->sizes[i] = t->size(i);
+    o->strides[i] = t->stride(i);
+  }
+  return true;
+}
+
+// An operand that may be None.
+struct Optional {
+  VecopsHipOperand operand;
+  const VecopsHipOperand* at = nullptr;
+  bool describe(PyObject* object) {
+    if (object == Py_None) return true;
+    at = &operand;
+    return describe_any(object, &operand);
+  }
+};
+
+// quantize_fp8_block(x, q, scales, block_rows)
+int quantize_fp8_block(PyObject* const* args) {
+  VecopsHipOperand x, q, scales;
+  int64_t rows = 0;
+  if (!describe_any(args[0], &x) || !describe_any(args[1], &q) || !describe_any(args[2], &scales) || !integer(args[3], &rows) || rows < 0 ||
+      rows > UINT32_MAX)
+    return kNotPlain;
+  return without_lock([&] { return vecops_hip_quantize_fp8_block(&x, static_cast<uint32_t>(rows), &q, &scales, current_stream()); });
+}
+
+// matmul_fp8_block(a, a_scales, b, b_scales, c, workspace)
+int matmul_fp8_block(PyObject* const* args) {
+  VecopsHipOperand o[5];
+  for (int i = 0; i < 5; ++i)
+    if (!describe_any(args[i], &o[i])) return kNotPlain;
+  Given given;
+  if (!given.describe(args[5], *plain_tensor(args[4]))) return kNotPlain;
+  return without_lock([&]() -> int {
+    const Workspace workspace(given, vecops_hip_matmul_fp8_block_workspace(&o[0], &o[2]));
+    return vecops_hip_matmul_fp8_block(&o[0], &o[1], &o[2], &o[3], &o[4], workspace.data, workspace.size, current_stream());
+  });
+}
+
+// moe_experts(x, ids, weights, gate_up, gate_up_scales, down, down_scales, out, workspace)
+int moe_experts(PyObject* const* args) {
+  VecopsHipOperand x, ids, weights, gate_up, down, out;
+  Optional gate_up_scales, down_scales;
+  if (!describe_any(args[0], &x) || !describe_any(args[1], &ids) || !describe_any(args[2], &weights) || !describe_any(args[3], &gate_up) ||
+      !gate_up_scales.describe(args[4]) || !describe_any(args[5], &down) || !down_scales.describe(args[6]) || !describe_any(args[7], &out))
+    return kNotPlain;
+  Given given;
+  if (!given.describe(args[8], *plain_tensor(args[7]))) return kNotPlain;
+  return without_lock([&]() -> int {
+    const Workspace workspace(given, vecops_hip_moe_experts_workspace(&ids, &down));
+    return vecops_hip_moe_experts(&x, &ids, &weights, &gate_up, gate_up_scales.at, &down, down_scales.at, &out, workspace.data, workspace.size,
+                                  current_stream());
+  });
+}
+
+// moe_layer(x, router, the routing record's address, gate_up, gate_up_scales, down, down_scales, ids, weights, out, workspace)
+int moe_layer(PyObject* const* args) {
+  VecopsHipOperand x, router, gate_up, down, ids, weights, out;
+  Optional gate_up_scales, down_scales;
+  int64_t routing = 0;
+  if (!describe_any(args[0], &x) || !describe_any(args[1], &router) || !integer(args[2], &routing) || routing == 0 ||
+      !describe_any(args[3], &gate_up) || !gate_up_scales.describe(args[4]) || !describe_any(args[5], &down) || !down_scales.describe(args[6]) ||
+      !describe_any(args[7], &ids) || !describe_any(args[8], &weights) || !describe_any(args[9], &out))
+    return kNotPlain;
+  Given given;
+  if (!given.describe(args[10], *plain_tensor(args[9]))) return kNotPlain;
+  const auto* record = reinterpret_cast<const VecopsHipMoeRouting*>(static_cast<uintptr_t>(routing));
+  return without_lock([&]() -> int {
+    const Workspace workspace(given, vecops_hip_moe_layer_workspace(&x, &ids, &down));
+    return vecops_hip_moe_layer(&x, &router, record, &gate_up, gate_up_scales.at, &down, down_scales.at, &ids, &weights, &out, workspace.data,
+                                workspace.size, current_stream());
+  });
+}
+
 // A Python function of COUNT positional arguments around one of the above: no C++ exception leaves it.
 template <int (*CALL)(PyObject* const*), int COUNT>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t count) {
@@ -498,6 +585,10 @@ PyMethodDef methods[] = {VECOPS_ENTRY(matmul, 6),
                          VECOPS_ENTRY(matmul_i8_dequant, 8),
                          VECOPS_ENTRY(matmul_runtime_quant, 10),
                          VECOPS_ENTRY(matmul_packed_b, 7),
+                         VECOPS_ENTRY(quantize_fp8_block, 4),
+                         VECOPS_ENTRY(matmul_fp8_block, 6),
+                         VECOPS_ENTRY(moe_experts, 9),
+                         VECOPS_ENTRY(moe_layer, 11),
                          {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace
