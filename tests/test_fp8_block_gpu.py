@@ -125,13 +125,13 @@ def dequantized(q, scales, rows):
 
 def check(c, a, sa, b, sb):
     """|error| <= (terms of the inner sum + roundings of the scales and of the outer sum) 2^-24 times the sum of the terms'
-    sizes, and the rounding of the result.  16-bit results of more than 64 rows may come from the 8-bit matrix instruction: of
+    sizes, and the rounding of the result.  16-bit results of more than 16 rows may come from the 8-bit matrix instruction: of
     eight products along k the seven smaller ones may each lose 2^-13 of the largest's power of two."""
     x, w = dequantized(a, sa, 1), dequantized(b, sb, 128)
     want, size = x @ w.transpose(-1, -2), x.abs() @ w.abs().transpose(-1, -2)
     k = a.shape[-1]
     bound = (min(k, 128) + 3 + blocks(k)) * 2.0 ** -24 * size
-    if c.dtype != torch.float32 and c.shape[-2] > 64:
+    if c.dtype != torch.float32 and c.shape[-2] > 16:
         bound = bound + 7 * 2.0 ** -13 * size
     unit = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[c.dtype]
     bound = bound + unit * (want.abs() + bound) + (2.0 ** -25 if c.dtype == torch.float16 else 0.0)
@@ -146,7 +146,9 @@ def check(c, a, sa, b, sb):
 
 SIZES = [(1, 16, 128), (1, 1, 1), (1, 4096, 4096), (3, 100, 127), (16, 256, 1024), (7, 513, 16 * 1024 + 40), (17, 200, 300), (32, 128, 640),
          (33, 1000, 513), (64, 512, 17000), (65, 130, 256), (100, 257, 1000), (128, 384, 129), (130, 640, 16), (200, 300, 2049),
-         (777, 500, 130), (1100, 4400, 384), (4096, 4100, 200)]
+         (777, 500, 130), (1100, 4400, 384), (4096, 4100, 200), (9, 40, 5), (90, 300, 7), (70, 200, 15), (66, 129, 17), (5, 33, 31), (257, 513, 143),
+         (3000, 6000, 128), (2900, 6001, 4097), (64, 1000, 14336), (100, 513, 4109), (300, 700, 2304), (128, 2000, 8192),
+         (500, 5000, 1000), (900, 3000, 700), (2049, 2049, 257)]
 
 
 @pytest.mark.parametrize("m,n,k", SIZES)

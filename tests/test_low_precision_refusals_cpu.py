@@ -75,12 +75,20 @@ def test_matmul_batches_and_workspace():
     f = capi.lib().vecops_hip_matmul_fp8_block
     v = [operand(F8, 2, 5, 300), operand(F32, 2, 5, 3), operand(F8, 3, 200, 300), operand(F32, 2, 2, 3), operand(F32, 2, 5, 200)]
     refused(f(*map(C.byref, v), None, 0, None), INVALID, "batch")
-    need = capi.lib().vecops_hip_matmul_fp8_block_workspace
-    assert need(C.byref(operand(F8, 5, 300)), C.byref(operand(F8, 200, 300, strides=(333, 1)))) == 0
+    def need(*operands):
+        c = operand(F32, *operands[0].sizes[:operands[0].rank - 1], operands[2].sizes[operands[2].rank - 2])
+        return capi.lib().vecops_hip_matmul_fp8_block_workspace(*map(C.byref, operands), C.byref(c))
+    x, sx, sw = operand(F8, 5, 300), operand(F32, 5, 3), operand(F32, 2, 3)
+    assert need(x, sx, operand(F8, 200, 300, strides=(333, 1)), sw) == 0
     turned = operand(F8, 200, 300, strides=(1, 200))
-    assert need(C.byref(operand(F8, 5, 300)), C.byref(turned)) == -(-200 * 304 // 256) * 256
+    assert need(x, sx, turned, sw) == -(-200 * 304 // 256) * 256
     shared = operand(F8, 7, 200, 300, strides=(0, 1, 200))
-    assert need(C.byref(operand(F8, 7, 5, 300)), C.byref(shared)) == -(-200 * 304 // 256) * 256
+    assert need(operand(F8, 7, 5, 300), operand(F32, 7, 5, 3), shared, operand(F32, 7, 2, 3)) == -(-200 * 304 // 256) * 256
+    assert need(x, operand(F32, 5, 3, strides=(1, 5)), operand(F8, 200, 300), operand(F32, 2, 3, strides=(1, 2))) == 512
+    assert need(operand(F8, 5, 8), operand(F32, 5, 1), operand(F8, 200, 8), operand(F32, 2, 1)) == 256 + 3328
+    # few tiles and a long K: the sums of its parts
+    assert need(operand(F8, 64, 14336), operand(F32, 64, 112), operand(F8, 4096, 14336), operand(F32, 32, 112)) == 4 * 64 * 4096 * 4
+    assert need(operand(F8, 4096, 4096), operand(F32, 4096, 32), operand(F8, 4096, 4096), operand(F32, 32, 32)) == 0
     v = [operand(F8, 5, 300), operand(F32, 5, 3), turned, operand(F32, 2, 3), operand(F32, 5, 200)]
     refused(f(*map(C.byref, v), 0x10008, 1 << 20, None), INVALID, "16-byte aligned workspace")
     refused(f(*map(C.byref, v), 0x10000, 100, None), INVALID, "workspace of")

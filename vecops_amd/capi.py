@@ -178,7 +178,7 @@ def lib() -> C.CDLL:
         L.vecops_hip_matmul_fused.argtypes = [P, P, P, P, C.c_uint32, E, C.c_void_p, C.c_uint64, C.c_void_p]
         L.vecops_hip_quantize_fp8_block.argtypes = [P, C.c_uint32, P, P, C.c_void_p]
         L.vecops_hip_matmul_fp8_block_workspace.restype = C.c_uint64
-        L.vecops_hip_matmul_fp8_block_workspace.argtypes = [P, P]
+        L.vecops_hip_matmul_fp8_block_workspace.argtypes = [P] * 5
         L.vecops_hip_matmul_fp8_block.argtypes = [P, P, P, P, P, C.c_void_p, C.c_uint64, C.c_void_p]
         L.vecops_hip_moe_experts_workspace.restype = C.c_uint64
         L.vecops_hip_moe_experts_workspace.argtypes = [P, P]
@@ -760,7 +760,7 @@ def matmul_fp8_block(a, a_scales, b, b_scales, c, workspace=None, stream=None):
     import torch
     _on_one_device("matmul_fp8_block", a, a_scales, b, b_scales, c, workspace)
     oa, osa, ob, osb, oc = operand(a), operand(a_scales), operand(b), operand(b_scales), operand(c)
-    need = lib().vecops_hip_matmul_fp8_block_workspace(C.byref(oa), C.byref(ob))
+    need = lib().vecops_hip_matmul_fp8_block_workspace(C.byref(oa), C.byref(osa), C.byref(ob), C.byref(osb), C.byref(oc))
     if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
         workspace = torch.empty(need, dtype=torch.uint8, device=c.device)
     ws_ptr = workspace.data_ptr() if workspace is not None else None

@@ -2711,13 +2711,24 @@ int real_kind(uint32_t dtype) {
 
 int64_t fp8_blocks(int64_t extent) { return (extent + kFp8Block - 1) / kFp8Block; }
 
-// What the product reads an operand through: its own rows where their k are contiguous (any alignment), else a copy of them
-// in the workspace.  (Offsets inside a tile of 256 rows are 32 bits wide.)
-bool fp8_rows_ok(const View& v) { return (v.cs == 1 || v.cols <= 1) && v.rs >= 0 && v.rs * 256 + v.cols + 128 < (int64_t{1} << 31); }
+// What the product reads an operand through: its own rows where their k are contiguous (any alignment) and at least sixteen
+// (the kernels load no less), else a copy of them in the workspace, padded to sixteen with zeros.  (Offsets inside a tile of
+// 256 rows are 32 bits wide.)
+bool fp8_rows_ok(const View& v) { return v.cs == 1 && v.cols >= 16 && v.rs >= 0 && v.rs * 256 + v.cols + 128 < (int64_t{1} << 31); }
 int64_t fp8_row_bytes(const View& v) { return (v.cols + 15) / 16 * 16; }
 uint64_t fp8_copy_bytes(const View& v) {
   if (v.batch == 0 || v.rows == 0 || v.cols == 0 || fp8_rows_ok(v)) return 0;
   return round_up_256(static_cast<uint64_t>(v.bs == 0 ? 1 : v.batch) * static_cast<uint64_t>(v.rows) * static_cast<uint64_t>(fp8_row_bytes(v)));
+}
+
+// Scales likewise: a row's follow one another.
+uint64_t fp8_scale_copy_bytes(const View& v) {
+  if (v.batch == 0 || v.rows == 0 || v.cols <= 1 || v.cs == 1) return 0;
+  return round_up_256(static_cast<uint64_t>(v.bs == 0 ? 1 : v.batch) * static_cast<uint64_t>(v.rows) * static_cast<uint64_t>(v.cols) * 4u);
+}
+
+uint64_t fp8_partial_bytes(const View& a, const View& b, const Fp8Plan& plan) {
+  return plan.splits == 1 ? 0 : static_cast<uint64_t>(plan.splits) * a.batch * a.rows * b.rows * 4u;
 }
 
 struct Fp8Product {
@@ -2748,8 +2759,11 @@ int32_t describe_fp8(const VecopsHipOperand* a, const VecopsHipOperand* a_scales
   if (((m + 127) / 128) * ((n + 127) / 128) >= (1 << 24) || (m <= 64 && n > (1 << 26)))
     return fail(ST_INVALID, "matmul_fp8_block: extent too large");
   // scales of a tile's rows are reached by 32-bit offsets
-  if (pr->sa.rs < 0 || pr->sb.rs < 0 || pr->sa.rs > (int64_t{1} << 20) || pr->sb.rs > (int64_t{1} << 20))
-    return fail(ST_NOT_APPLICABLE, "matmul_fp8_block: row strides of the scales must lie in 0 .. 2^20");
+  for (const View* v : {&pr->sa, &pr->sb})
+    if (fp8_blocks(k) > (1 << 20) || (fp8_scale_copy_bytes(*v) == 0 && (v->rs < 0 || v->rs > (int64_t{1} << 20))))
+      return fail(ST_NOT_APPLICABLE, "matmul_fp8_block: row strides of the scales must lie in 0 .. 2^20");
+  if (batch * m * fp8_blocks(k) >= (int64_t{1} << 32) || batch * fp8_blocks(n) * fp8_blocks(k) >= (int64_t{1} << 32))
+    return fail(ST_INVALID, "matmul_fp8_block: extent too large");
   return ST_OK;
 }
 
@@ -2788,10 +2802,13 @@ int32_t vecops_hip_quantize_fp8_block(const VecopsHipOperand* x, uint32_t block_
   return ST_OK;
 }
 
-uint64_t vecops_hip_matmul_fp8_block_workspace(const VecopsHipOperand* a, const VecopsHipOperand* b) {
-  View va, vb;
-  if (!normalise(a, &va) || !normalise(b, &vb)) return 0;
-  return fp8_copy_bytes(va) + fp8_copy_bytes(vb);
+uint64_t vecops_hip_matmul_fp8_block_workspace(const VecopsHipOperand* a, const VecopsHipOperand* a_scales, const VecopsHipOperand* b,
+                                               const VecopsHipOperand* b_scales, const VecopsHipOperand* c) {
+  View va, vsa, vb, vsb, vc;
+  if (!normalise(a, &va) || !normalise(a_scales, &vsa) || !normalise(b, &vb) || !normalise(b_scales, &vsb) || !normalise(c, &vc)) return 0;
+  if (va.batch == 0 || va.rows == 0 || vb.rows == 0) return 0;
+  return fp8_copy_bytes(va) + fp8_copy_bytes(vb) + fp8_scale_copy_bytes(vsa) + fp8_scale_copy_bytes(vsb) +
+         fp8_partial_bytes(va, vb, fp8_plan(va.rows, vb.rows, va.cols, va.batch, real_kind(vc.dtype)));
 }
 
 int32_t vecops_hip_matmul_fp8_block(const VecopsHipOperand* a, const VecopsHipOperand* a_scales, const VecopsHipOperand* b,
@@ -2803,9 +2820,11 @@ int32_t vecops_hip_matmul_fp8_block(const VecopsHipOperand* a, const VecopsHipOp
   if (pr.a.batch == 0 || pr.a.rows == 0 || pr.b.rows == 0) return ST_OK;
   if (pr.c.data == nullptr || (pr.a.cols > 0 && (pr.a.data == nullptr || pr.b.data == nullptr || pr.sa.data == nullptr || pr.sb.data == nullptr)))
     return fail(ST_INVALID, "matmul_fp8_block: null operand");
-  const uint64_t copy_a = fp8_copy_bytes(pr.a), copy_b = fp8_copy_bytes(pr.b);
-  if (copy_a + copy_b > 0 && (workspace == nullptr || workspace_size < copy_a + copy_b || !aligned16(workspace)))
-    return fail(ST_INVALID, "matmul_fp8_block: needs a 16-byte aligned workspace of %llu bytes", (unsigned long long)(copy_a + copy_b));
+  const Fp8Plan plan = fp8_plan(pr.a.rows, pr.b.rows, pr.a.cols, pr.a.batch, real_kind(pr.c.dtype));
+  const uint64_t need = fp8_copy_bytes(pr.a) + fp8_copy_bytes(pr.b) + fp8_scale_copy_bytes(pr.sa) + fp8_scale_copy_bytes(pr.sb) +
+                        fp8_partial_bytes(pr.a, pr.b, plan);
+  if (need > 0 && (workspace == nullptr || workspace_size < need || !aligned16(workspace)))
+    return fail(ST_INVALID, "matmul_fp8_block: needs a 16-byte aligned workspace of %llu bytes", (unsigned long long)need);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   uint8_t* room = static_cast<uint8_t*>(workspace);
   for (View* v : {&pr.a, &pr.b}) {
@@ -2822,19 +2841,35 @@ int32_t vecops_hip_matmul_fp8_block(const VecopsHipOperand* a, const VecopsHipOp
     v->cs = 1;
     room += bytes;
   }
+  for (View* v : {&pr.sa, &pr.sb}) {
+    const uint64_t bytes = fp8_scale_copy_bytes(*v);
+    if (bytes == 0) continue;
+    const int64_t batches = v->bs == 0 ? 1 : v->batch;
+    const hipError_t e = launch_fp8_scales(static_cast<const float*>(v->data), v->bs, v->rs, v->cs, reinterpret_cast<float*>(room),
+                                           static_cast<int32_t>(batches), static_cast<int32_t>(v->rows), static_cast<int32_t>(v->cols), s);
+    if (e != hipSuccess) return fail(ST_EXEC, "matmul_fp8_block: kernel launch: %s", hipGetErrorString(e));
+    v->data = room;
+    v->bs = v->bs == 0 ? 0 : v->rows * v->cols;
+    v->rs = v->cols;
+    v->cs = 1;
+    room += bytes;
+  }
   Fp8MatmulParams p;
   p.a = static_cast<const uint8_t*>(pr.a.data), p.b = static_cast<const uint8_t*>(pr.b.data);
   p.a_scales = static_cast<const float*>(pr.sa.data), p.b_scales = static_cast<const float*>(pr.sb.data);
   p.c = pr.c.data;
   p.lda = pr.a.rs, p.ldb = pr.b.rs, p.a_bs = pr.a.bs, p.b_bs = pr.b.bs;
-  p.as_rs = pr.sa.rs, p.as_gs = pr.sa.cs, p.as_bs = pr.sa.bs;
-  p.bs_rs = pr.sb.rs, p.bs_gs = pr.sb.cs, p.bs_bs = pr.sb.bs;
+  p.as_rs = pr.sa.rs, p.as_bs = pr.sa.bs;
+  p.bs_rs = pr.sb.rs, p.bs_bs = pr.sb.bs;
   p.c_rs = pr.c.rs, p.c_cs = pr.c.cs, p.c_bs = pr.c.bs;
-  p.m = static_cast<int32_t>(pr.a.rows), p.n = static_cast<int32_t>(pr.b.rows), p.k = static_cast<int32_t>(pr.a.cols);
+  p.m = static_cast<int32_t>(pr.a.rows), p.n = static_cast<int32_t>(pr.b.rows);
+  p.k = static_cast<int32_t>(pr.a.cols == 0 ? 0 : std::max<int64_t>(pr.a.cols, 16));
   p.batch = static_cast<int32_t>(pr.a.batch);
   p.groups = static_cast<int32_t>(fp8_blocks(pr.a.cols));
   p.out_kind = real_kind(pr.c.dtype);
-  const hipError_t e = launch_fp8_matmul(p, s);
+  p.splits = plan.splits;
+  p.partial = reinterpret_cast<float*>(room);
+  const hipError_t e = launch_fp8_matmul(p, plan.kind, s);
   if (e != hipSuccess) return fail(ST_EXEC, "matmul_fp8_block: kernel launch: %s", hipGetErrorString(e));
   return ST_OK;
 }

@@ -158,7 +158,18 @@ __global__ __launch_bounds__(256) void fp8_quantize_tiles_kernel(const Fp8Quanti
   if (threadIdx.x == 0) p.scales[batch * p.s_bs + i * p.s_rs + g * p.s_cs] = s;
 }
 
-// Rows whose k are not contiguous, laid out so that they are: 64 x 64 elements through LDS, each side in its own order.
+// Scales whose blocks of k do not follow one another, laid out so that they do.
+__global__ __launch_bounds__(256) void fp8_scales_kernel(const float* in, int64_t bs, int64_t rs, int64_t gs, float* out, int64_t total, int32_t rows,
+                                                         int32_t groups) {
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= total) return;
+  const int64_t row = at % rows, line = at / rows;   // (consecutive lanes: consecutive rows)
+  const int64_t g = line % groups, batch = line / groups;
+  out[(batch * rows + row) * groups + g] = in[batch * bs + row * rs + g * gs];
+}
+
+// Rows whose k are not contiguous, or few, laid out so that they are, with zeros up to `ld`: 64 x 64 elements through LDS, each
+// side in its own order.
 __global__ __launch_bounds__(256) void fp8_rows_kernel(const uint8_t* in, int64_t bs, int64_t rs, int64_t cs, uint8_t* out, int64_t ld,
                                                        int32_t rows, int32_t k, uint32_t tiles_k) {
   __shared__ uint8_t tile[64][68];
@@ -168,10 +179,10 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const uint8_t* in, int64_
   in += blockIdx.y * bs;
   out += static_cast<int64_t>(blockIdx.y) * rows * ld;
   for (int i = y; i < 64; i += 4)   // consecutive lanes: consecutive rows (the contiguous side of a [K, rows] matrix)
-    if (r0 + x < rows && k0 + i < k) tile[x][i] = in[(r0 + x) * rs + (k0 + i) * cs];
+    tile[x][i] = r0 + x < rows && k0 + i < k ? in[(r0 + x) * rs + (k0 + i) * cs] : 0;
   __syncthreads();
   for (int i = y; i < 64; i += 4)
-    if (r0 + i < rows && k0 + x < k) out[(r0 + i) * ld + k0 + x] = tile[i][x];
+    if (r0 + i < rows && k0 + x < ld) out[(r0 + i) * ld + k0 + x] = tile[i][x];
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -250,19 +261,6 @@ __device__ __forceinline__ Fragments<WIDE, COUNT> fragments(const i32x8 (&bytes)
   return fragments<WIDE>(bytes, std::make_integer_sequence<int, COUNT>{});
 }
 
-// Sixteen bytes of a row from `k` on, zeros past K; reads nothing past the row's last byte.
-__device__ __forceinline__ u32x4 load_chunk_until(const VECOPS_GLOBAL uint8_t* row, int k, int k_end) {
-  u32x4 v = {0u, 0u, 0u, 0u};
-  if (k + 16 <= k_end) {
-    v = load_16(row + k);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 16; ++e)
-      if (k + e < k_end) v[e >> 2] |= static_cast<uint32_t>(row[k + e]) << (8 * (e & 3));
-  }
-  return v;
-}
-
 // COUNT consecutive results of a row from column n on (`at`: the first one's place in elements); those past n_end stay unwritten.
 template <int COUNT>
 __device__ __forceinline__ void store_results(void* c, int64_t at, int64_t cs, int out_kind, int64_t n, int64_t n_end, const float (&v)[COUNT]) {
@@ -294,52 +292,59 @@ __device__ __forceinline__ void store_results(void* c, int64_t at, int64_t cs, i
   }
 }
 
-// One 4-byte load per lane that writes LDS itself (as load_16_bytes_into_lds).
-__device__ __forceinline__ void load_4_bytes_into_lds(const u32x4& descriptor, uint32_t address, uint32_t lane_offset, uint32_t uniform_offset) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, %3 offen lds"
-               :
-               : "s"(address), "v"(lane_offset), "s"(descriptor), "s"(uniform_offset)
-               : "memory", "m0");
-#else
-  (void)descriptor; (void)address; (void)lane_offset; (void)uniform_offset;
-#endif
-}
-
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) float lds_float;
 
-__device__ __forceinline__ u32x4 read_lds(uint32_t at) { return *reinterpret_cast<const lds_u32x4*>(static_cast<uintptr_t>(at)); }
-__device__ __forceinline__ float read_lds_float(uint32_t at) { return *reinterpret_cast<const lds_float*>(static_cast<uintptr_t>(at)); }
+typedef __attribute__((address_space(3))) char lds_char;
 
-// Many rows: WN x WM wavefronts, each NT x MT blocks of 16 x 16.  A stage is one block of 128 k of both operands and the
-// activations' scales; it arrives by loads that write LDS while the stage before it is multiplied.
+// (`offset`, a constant, goes into the instruction)
+__device__ __forceinline__ u32x4 read_lds(uint32_t at, int offset) {
+  return *reinterpret_cast<const lds_u32x4*>(reinterpret_cast<const lds_char*>(static_cast<uintptr_t>(at)) + offset);
+}
+__device__ __forceinline__ float read_lds_float(uint32_t at, int offset) {
+  return *reinterpret_cast<const lds_float*>(reinterpret_cast<const lds_char*>(static_cast<uintptr_t>(at)) + offset);
+}
+
+// Many rows: WN x WM wavefronts, each NT x MT blocks of 16 x 16.  A stage is one block of 128 k of both operands and their
+// scales; STAGES of them are under way or in use, by loads that write LDS.
 // The rows of a wavefront's weights are dealt to its 16-row blocks so that a lane's results of two blocks are eight
 // consecutive n (row r of block 2 p + h is n = 32 p + 8 (r / 4) + 4 h + r % 4): sixteen bytes of a 16-bit result a store.
-template <int WN, int WM, int NT, int MT>
+template <int WN, int WM, int NT, int MT, int STAGES>
 struct Fp8Tile {
-  static constexpr int kBN = WN * NT * 16, kBM = WM * MT * 16, kThreads = 64 * WN * WM;
+  static constexpr int kBN = WN * NT * 16, kBM = WM * MT * 16, kWaves = WN * WM, kThreads = 64 * kWaves;
   static constexpr int kBytesW = kBN * 128, kBytesX = kBM * 128;
-  // behind the operands: the scales of the kBM activation rows, and those of the tile's weight blocks in 64 places
-  static constexpr int kScalesX = kBytesW + kBytesX, kScalesW = kScalesX + kBM * 4, kStage = kScalesW + 256;
-  static constexpr int kLoadsW = kBytesW / (kThreads * 16), kLoadsX = kBytesX / (kThreads * 16);
-  static_assert(kBM % 64 == 0 && kThreads >= kBM + 64, "a wavefront loads scales of 64 rows, another those of the weights");
-  static_assert(NT % 2 == 0 && 128 % (NT * 16) == 0 && kBN % 8 == 0, "a wavefront's weights share their scale");
+  static constexpr int kStage = kBytesW + kBytesX;
+  // Scales arrive four blocks of k at a time (sixteen bytes of each row: a line holds many blocks' scales of one row): the first
+  // wavefronts load those of 64 activation rows each, the others those of the weights' blocks.  In three of four stages the
+  // load fetches nothing and writes where nobody reads, so that all wavefronts have the same number of loads under way.
+  // Of four runs' places one is free again by the time that its next run is asked for, up to twelve stages ahead.
+  static constexpr int kRuns = 4, kRunX = kBM * 16, kRunW = 1024;
+  static constexpr int kScalesX = STAGES * kStage, kScalesW = kScalesX + kRuns * kRunX, kNobody = kScalesW + kRuns * kRunW, kLds = kNobody + 1024;
+  static constexpr int kLoadsW = kBytesW / (kThreads * 16), kLoadsX = kBytesX / (kThreads * 16), kLoads = kLoadsW + kLoadsX + 1;
+  static_assert(kBM % 64 == 0 && kWaves > kBM / 64 && STAGES <= 12, "wavefronts to load all scales, and room for them");
+  static_assert(NT % 2 == 0 && 128 % (NT * 16) == 0, "a wavefront's weights share their scale");
   static_assert(kBytesW % (kThreads * 16) == 0 && kBytesX % (kThreads * 16) == 0, "whole loads");
+  static_assert(kLds <= 160 * 1024 && STAGES >= 2 && (STAGES - 1) * kLoads < 64, "LDS of a compute unit; the counter of loads");
 };
 
 // slot of a chunk in its row of 128 bytes: rows that a fragment reads together lie in different slots
 __device__ __forceinline__ int slot_key_w(int row) { return (row & 3) | ((row >> 1) & 4); }
 __device__ __forceinline__ int slot_key_x(int row) { return row & 7; }
 
-template <int WN, int WM, int NT, int MT, bool WIDE>
+// What bounds the large tiles is the matrix pipe and the power it draws; a result's multiply-add every block of 128 takes half
+// the vector unit's time beside it.  So the two run side by side: a block row's multiply-adds are issued while the next one's
+// products are formed, and the stage is left, and the next one's first fragments are fetched, behind the last block row.
+template <int WN, int WM, int NT, int MT, bool WIDE, int STAGES, bool HALVES>
 __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(const Fp8MatmulParams p, uint32_t tiles_n, uint32_t tiles_m) {
-  using T = Fp8Tile<WN, WM, NT, MT>;
+  using T = Fp8Tile<WN, WM, NT, MT, STAGES>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t lds0 = lds_address_of(lds);
   const int batch = blockIdx.y;
+  // this workgroup's share of the blocks of k
+  const int g_begin = static_cast<int>(static_cast<int64_t>(p.groups) * blockIdx.z / p.splits);
+  const int g_end = static_cast<int>(static_cast<int64_t>(p.groups) * (blockIdx.z + 1) / p.splits);
 
   // neighbouring tiles on one die: each die's workgroups (every eighth) take a contiguous run of tiles, walked in groups of
   // eight tile rows
@@ -352,64 +357,83 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(const Fp8Matm
   const uint32_t height = min(tiles_m - first, 8u), in_group = pid - group * per_group;
   const uint32_t tile_m = first + in_group % height, tile_n = in_group / height;
   const int64_t m0 = static_cast<int64_t>(tile_m) * T::kBM, n0 = static_cast<int64_t>(tile_n) * T::kBN;
-  const int last_m = static_cast<int>(min(p.m - m0, static_cast<int64_t>(T::kBM))) - 1, last_n = static_cast<int>(min(p.n - n0, static_cast<int64_t>(T::kBN))) - 1;
+  const int last_m = static_cast<int>(min(p.m - m0, static_cast<int64_t>(T::kBM))) - 1;
+  const int last_n = static_cast<int>(min(p.n - n0, static_cast<int64_t>(T::kBN))) - 1;
 
   const VECOPS_GLOBAL uint8_t* w_base = (const VECOPS_GLOBAL uint8_t*)p.b + batch * p.b_bs + n0 * p.ldb;
   const VECOPS_GLOBAL uint8_t* x_base = (const VECOPS_GLOBAL uint8_t*)p.a + batch * p.a_bs + m0 * p.lda;
-  const VECOPS_GLOBAL float* sx_base = (const VECOPS_GLOBAL float*)p.a_scales + batch * p.as_bs + m0 * p.as_rs;
-  const u32x4 desc_w = tile_buffer_words((const VECOPS_GLOBAL char*)w_base);
-  const u32x4 desc_x = tile_buffer_words((const VECOPS_GLOBAL char*)x_base);
+  u32x4 desc_w = tile_buffer_words((const VECOPS_GLOBAL char*)w_base);
+  u32x4 desc_x = tile_buffer_words((const VECOPS_GLOBAL char*)x_base);
+  // the last block of k, where K ends inside it: `tail` bytes of each row.  The chunk that K ends in is fetched as the sixteen
+  // bytes in front of K (rows have at least sixteen): the same order of k on both sides, and the `again` bytes of it that the
+  // chunk before it holds too are cleared on one side when they are read.
+  const int tail = p.k % kFp8Block, again = tail % 16 ? 16 - tail % 16 : 0;
 
-  // load i of a thread: sixteen bytes of row i * threads / 8 + tid / 8, the chunk whose slot is tid % 8
-  uint32_t from_w[T::kLoadsW], from_x[T::kLoadsX];
-#pragma unroll
-  for (int i = 0; i < T::kLoadsW; ++i) {
-    const int row = i * (T::kThreads / 8) + (tid >> 3);
-    from_w[i] = static_cast<uint32_t>(min(row, last_n) * p.ldb) + (((tid & 7) ^ slot_key_w(row)) << 4);
-  }
-#pragma unroll
-  for (int i = 0; i < T::kLoadsX; ++i) {
-    const int row = i * (T::kThreads / 8) + (tid >> 3);
-    from_x[i] = static_cast<uint32_t>(min(row, last_m) * p.lda) + (((tid & 7) ^ slot_key_x(row)) << 4);
-  }
-  // scales: the first wavefronts load those of the activations, 64 rows each, the next one those of the weights
-  const bool loads_sw = wave == T::kBM / 64;
+  // load i of a thread: sixteen bytes of row i * threads / 8 + tid / 8, the chunk whose slot is tid % 8 (rows apart by threads
+  // / 8 have equal keys).  Rows past the operand's last one lie past the descriptor's end: zeros arrive.
+  constexpr int kRows = T::kThreads / 8;
+  static_assert(kRows % 16 == 0, "equal keys");
+  constexpr uint32_t kNowhere = 0x80000000u;   // past every descriptor's end
+  const int row = tid >> 3, chunk_w = ((tid & 7) ^ slot_key_w(row)) << 4, chunk_x = ((tid & 7) ^ slot_key_x(row)) << 4;
+  const uint32_t from_w = static_cast<uint32_t>(row * p.ldb) + chunk_w, from_x = static_cast<uint32_t>(row * p.lda) + chunk_x;
+  // (the tail's with their k: no part of an offset is negative.  Chosen without a branch: the loop below has to stay one block,
+  // or the compiler gathers the multiply-adds behind it.)
+  const uint32_t k_tail = static_cast<uint32_t>(p.groups - 1) * kFp8Block;
+  const uint32_t tail_w = chunk_w + 16 <= tail ? from_w + k_tail : chunk_w < tail ? from_w + k_tail - (chunk_w + 16 - tail) : kNowhere;
+  const uint32_t tail_x = chunk_x + 16 <= tail ? from_x + k_tail : chunk_x < tail ? from_x + k_tail - (chunk_x + 16 - tail) : kNowhere;
+  const uint32_t end_w = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(last_n * p.ldb + p.k));
+  const uint32_t end_x = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(last_m * p.lda + p.k));
+  const uint32_t step_w = static_cast<uint32_t>(kRows * p.ldb), step_x = static_cast<uint32_t>(kRows * p.lda);
+  const bool loads_sw = wave >= T::kBM / 64;
   const int64_t scale_row0 = n0 / kFp8Block, last_scale_row = (static_cast<int64_t>(p.n) - 1) / kFp8Block - scale_row0;
-  const VECOPS_GLOBAL float* s_base = loads_sw ? (const VECOPS_GLOBAL float*)p.b_scales + batch * p.bs_bs + scale_row0 * p.bs_rs : sx_base;
-  const int64_t s_step = loads_sw ? p.bs_gs : p.as_gs;
-  const uint32_t from_s = loads_sw ? static_cast<uint32_t>(min(static_cast<int64_t>(min(lane, T::kBN / kFp8Block)), last_scale_row) * p.bs_rs * 4)
-                                   : static_cast<uint32_t>(min(tid, last_m) * p.as_rs * 4);
+  u32x4 desc_s = tile_buffer_words((const VECOPS_GLOBAL char*)(loads_sw ? p.b_scales + batch * p.bs_bs + scale_row0 * p.bs_rs
+                                                                        : p.a_scales + batch * p.as_bs + m0 * p.as_rs));
+  const int64_t scale_rs = loads_sw ? p.bs_rs : p.as_rs, scale_rows = loads_sw ? min(static_cast<int64_t>(T::kBN / kFp8Block), last_scale_row) : last_m;
+  const uint32_t from_s = static_cast<uint32_t>(min(static_cast<int64_t>(loads_sw ? lane : tid), scale_rows) * scale_rs * 4);
+  const uint32_t end_s = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>((scale_rows * scale_rs + p.groups) * 4));
+  const uint32_t to_s = __builtin_amdgcn_readfirstlane(loads_sw ? T::kScalesW : T::kScalesX + wave * 1024);
+  const uint32_t run_shift = __builtin_amdgcn_readfirstlane(loads_sw ? 10 : T::kBM == 256 ? 12 : T::kBM == 128 ? 11 : 10);
+  static_assert(T::kBM == 256 || T::kBM == 128 || T::kBM == 64, "the shift");
 
-  auto issue = [&](int g) {
-    const uint32_t stage = lds0 + (g & 1) * T::kStage;
-    const int k0 = g * kFp8Block;
-    if (k0 + kFp8Block <= p.k) {
-#pragma unroll
-      for (int i = 0; i < T::kLoadsW; ++i)
-        load_16_bytes_into_lds(desc_w, stage, __builtin_amdgcn_readfirstlane(i * (T::kThreads * 16) + wave * 1024), from_w[i],
-                               __builtin_amdgcn_readfirstlane(k0));
-#pragma unroll
-      for (int i = 0; i < T::kLoadsX; ++i)
-        load_16_bytes_into_lds(desc_x, stage, __builtin_amdgcn_readfirstlane(T::kBytesW + i * (T::kThreads * 16) + wave * 1024),
-                               from_x[i], __builtin_amdgcn_readfirstlane(k0));
-    } else {  // the last, partial block: through registers, byte by byte where K ends
-#pragma unroll
-      for (int i = 0; i < T::kLoadsW; ++i) {
-        const int row = i * (T::kThreads / 8) + (tid >> 3), chunk = (tid & 7) ^ slot_key_w(row);
-        const u32x4 v = load_chunk_until(w_base + min(row, last_n) * p.ldb, k0 + chunk * 16, p.k);
-        *reinterpret_cast<lds_u32x4*>(static_cast<uintptr_t>(stage + i * (T::kThreads * 16) + tid * 16)) = v;
-      }
-#pragma unroll
-      for (int i = 0; i < T::kLoadsX; ++i) {
-        const int row = i * (T::kThreads / 8) + (tid >> 3), chunk = (tid & 7) ^ slot_key_x(row);
-        const u32x4 v = load_chunk_until(x_base + min(row, last_m) * p.lda, k0 + chunk * 16, p.k);
-        *reinterpret_cast<lds_u32x4*>(static_cast<uintptr_t>(stage + T::kBytesW + i * (T::kThreads * 16) + tid * 16)) = v;
-      }
+  // load PIECE of those that fill stage `slot` with block g (weights, activations, scales); past the last block nothing is
+  // fetched (but as many loads are issued)
+  auto issue_piece = [&](auto piece_tag, int g, int slot) {
+    constexpr int PIECE = decltype(piece_tag)::value;
+    const uint32_t stage = lds0 + slot * T::kStage;
+    const bool there = g < g_end, at_tail = tail != 0 && g == p.groups - 1;
+    const uint32_t k0 = at_tail ? 0u : static_cast<uint32_t>(g) * kFp8Block;
+    if constexpr (PIECE < T::kLoadsW) {
+      desc_w[2] = there ? end_w : 0u;
+      load_16_bytes_into_lds(desc_w, stage, __builtin_amdgcn_readfirstlane(PIECE * (T::kThreads * 16) + wave * 1024), at_tail ? tail_w : from_w,
+                             __builtin_amdgcn_readfirstlane(PIECE * step_w + k0));
+    } else if constexpr (PIECE < T::kLoadsW + T::kLoadsX) {
+      constexpr int AT = PIECE - T::kLoadsW;
+      desc_x[2] = there ? end_x : 0u;
+      load_16_bytes_into_lds(desc_x, stage, __builtin_amdgcn_readfirstlane(T::kBytesW + AT * (T::kThreads * 16) + wave * 1024),
+                             at_tail ? tail_x : from_x, __builtin_amdgcn_readfirstlane(AT * step_x + k0));
+    } else {
+      const bool begins = (g & 3) == 0 || g == g_begin;   // with the first stage of a run its scales
+      const uint32_t to = to_s + (static_cast<uint32_t>((g >> 2) & (T::kRuns - 1)) << run_shift);
+      desc_s[2] = there && begins ? end_s : 0u;
+      load_16_bytes_into_lds(desc_s, lds0, __builtin_amdgcn_readfirstlane(begins ? to : T::kNobody),
+                             from_s, __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(g & ~3) * 4));
     }
-    if (wave <= T::kBM / 64)
-      load_4_bytes_into_lds(tile_buffer_words((const VECOPS_GLOBAL char*)(s_base + g * s_step)),
-                            __builtin_amdgcn_readfirstlane(stage + T::kScalesX + wave * 256), from_s, 0);
   };
+  auto issue = [&](int g, int slot) { static_for<T::kLoads>([&](auto piece) { issue_piece(piece, g, slot); }); };
+  // HALVES: a stage's buffer is refilled in two parts.  The first, once every wavefront has passed the middle of the stage: the
+  // activations (in registers since the stage began), the weights of the block rows done, the scales; the second, the rest,
+  // behind the stage's end.  Each load stands among matrix instructions: all of them together would hold those up for as long
+  // as the loads take to be accepted.
+  constexpr int kSecond = HALVES ? T::kLoadsW / 2 : 0, kFirst = T::kLoads - kSecond;
+  // loads that are issued behind the wait of a stage's end, among the matrix instructions of its last block row
+  constexpr int kLate = HALVES ? (kFirst > (NT / 2 - 1) * MT ? kFirst - (NT / 2 - 1) * MT : 0) : T::kLoads - (NT - 1) * MT * T::kLoads / (NT * MT);
+  static_assert(HALVES || STAGES >= 3, "a stage that is asked for while another one is multiplied");
+  static_assert(!HALVES || (STAGES == 2 && kSecond <= MT && kFirst <= NT / 2 * MT), "loads among a stage's matrix instructions");
+  auto issue_first = [&](auto nth, int g, int slot) {   // nth of kFirst: weights 0, 2, .., then the others
+    constexpr int N = decltype(nth)::value;
+    issue_piece(std::integral_constant<int, N < T::kLoadsW / 2 ? 2 * N : N + T::kLoadsW / 2>{}, g, slot);
+  };
+  auto issue_second = [&](auto nth, int g, int slot) { issue_piece(std::integral_constant<int, 2 * decltype(nth)::value + 1>{}, g, slot); };
 
   const int wn = wave / WM, wm = wave % WM;
   const int col = lane & 15, quarter = lane >> 4;
@@ -421,44 +445,137 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(const Fp8Matm
     at_w[h] = lds0 + row_w * 128 + ((chunk ^ slot_key_w(row_w)) << 4);
     at_x[h] = lds0 + T::kBytesW + row_x * 128 + ((chunk ^ slot_key_x(row_x)) << 4);
   }
-  const uint32_t at_sx = lds0 + T::kScalesX + (wm * (MT * 16) + col) * 4;
-  const uint32_t at_sw = lds0 + T::kScalesW + static_cast<uint32_t>((n0 + wn * (NT * 16)) / kFp8Block - scale_row0) * 4;
+  const uint32_t at_sx = lds0 + T::kScalesX + (wm * (MT * 16) + col) * 16;
+  const uint32_t at_sw = lds0 + T::kScalesW + static_cast<uint32_t>((n0 + wn * (NT * 16)) / kFp8Block - scale_row0) * 16;
+  auto read_w = [&](uint32_t stage, int i) {
+    // block 2 p + h starts 32 p + 4 h rows down; 4 rows down the key stays
+    const int down = (i >> 1) * 4096 + (i & 1) * 512;
+    return fragment_of(read_lds(at_w[0] + stage, down), read_lds(at_w[1] + stage, down));
+  };
 
-  f32x4 acc[NT][MT];
+  f32x4 acc[NT][MT], part[2][MT];
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
+  for (int j = 0; j < MT; ++j) {
+    part[0][j] = part[1][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < NT; ++i) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  i32x8 xb[MT], wb[2];
+  float scale[MT], next_scale[MT];
+#pragma unroll
+  for (int j = 0; j < MT; ++j) scale[j] = 0.f;
 
-  if (p.groups > 0) issue(0);
-  for (int g = 0; g < p.groups; ++g) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");   // this stage has landed
-    __builtin_amdgcn_s_barrier();                                 // and every wavefront has left the one before it
-    asm volatile("" ::: "memory");
-    if (g + 1 < p.groups) issue(g + 1);
-    const uint32_t stage = (g & 1) * T::kStage;
-    const float sw = read_lds_float(at_sw + stage);
-    float scale[MT];
-    i32x8 xb[MT];
+  auto read_x = [&](uint32_t stage, int j) { xb[j] = fragment_of(read_lds(at_x[0] + stage, j * 2048), read_lds(at_x[1] + stage, j * 2048)); };
+  auto read_scales = [&](int g) {
+    const uint32_t run = (g >> 2) & (T::kRuns - 1), in_run = (g & 3) * 4;
+    const float sw = read_lds_float(at_sw + run * T::kRunW + in_run, 0);
 #pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      xb[j] = fragment_of(read_lds(at_x[0] + stage + j * 2048), read_lds(at_x[1] + stage + j * 2048));
-      scale[j] = read_lds_float(at_sx + stage + j * 64) * sw;
-    }
-    const auto x = fragments<WIDE>(xb);
+    for (int j = 0; j < MT; ++j) next_scale[j] = read_lds_float(at_sx + run * T::kRunX + in_run, j * 256) * sw;
+  };
+  // clears what the chunk that K ends in repeats
+  auto clear_again = [&] {
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      // block 2 p + h starts 32 p + 4 h rows down; 4 rows down the key stays
-      const uint32_t down = stage + (i >> 1) * 4096 + (i & 1) * 512;
-      const Fragment<WIDE> w(fragment_of(read_lds(at_w[0] + down), read_lds(at_w[1] + down)));
+    for (int h = 0; h < 2; ++h) {
+      const bool mine = quarter + 4 * h == (tail >> 4);
 #pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        const f32x4 part = w.dot(x.v[j]);
+      for (int d = 0; d < 4; ++d) {
+        const int z = again - 4 * d;   // bytes of this word to clear
+        const uint32_t mask = !mine || z <= 0 ? 0xffffffffu : z >= 4 ? 0u : 0xffffffffu << (8 * z);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[i][j][r] = fmaf(part[r], scale[j], acc[i][j][r]);
+        for (int j = 0; j < MT; ++j) xb[j][4 * h + d] = static_cast<int>(static_cast<uint32_t>(xb[j][4 * h + d]) & mask);
       }
     }
+  };
+
+  // one block of k: the block rows in turn, and behind the last one the next stage's first fragments
+  auto multiply = [&](auto last_tag, int g, uint32_t stage, uint32_t next, int slot, int next_slot) {
+    constexpr bool LAST = decltype(last_tag)::value;
+    const auto x = fragments<WIDE>(xb);
+    float mine[MT];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) mine[j] = next_scale[j];
+    static_for<NT>([&](auto row_tag) {
+      constexpr int i = decltype(row_tag)::value;
+      __builtin_amdgcn_sched_barrier(0);
+      const Fragment<WIDE> w(wb[i & 1]);
+      if constexpr (HALVES && !LAST && i == NT / 2) {   // every wavefront is past the first half of this stage
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      }
+      if constexpr (i + 1 < NT) {
+        wb[(i + 1) & 1] = read_w(stage, i + 1);
+      } else if constexpr (!LAST) {
+        // every fragment of this stage is in registers: the next one has landed, and this one is free for all wavefronts
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(HALVES ? kFirst - kLate : (STAGES - 2) * T::kLoads - kLate) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      }
+      static_for<MT>([&](auto column_tag) {
+        constexpr int j = decltype(column_tag)::value;
+        part[i & 1][j] = w.dot(x.v[j]);
+        if constexpr (!LAST && i + 1 == NT) {
+          __builtin_amdgcn_sched_barrier(0);   // (its registers take the next fragment)
+          read_x(next, j);
+        }
+        // the block row before this one (in front of the first one: the last of the stage before, by that stage's scale)
+        constexpr int kBefore = i == 0 ? NT - 1 : i - 1;
+        const f32x4 from = part[(i & 1) ^ 1][j];
+        const float by = i == 0 ? scale[j] : mine[j];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[kBefore][j][r] = fmaf(from[r], by, acc[kBefore][j][r]);
+        if constexpr (HALVES && !LAST) {
+          if constexpr (i == 0 && j < kSecond) issue_second(column_tag, g + 1, next_slot);
+          constexpr int kStep = (i - NT / 2) * MT + j;
+          if constexpr (kStep >= 0 && kStep < kFirst) issue_first(std::integral_constant<int, kStep < 0 ? 0 : kStep>{}, g + 2, slot);
+          __builtin_amdgcn_sched_barrier(0);
+        } else if constexpr (!LAST) {   // a stage's loads evenly among the matrix instructions
+          constexpr int kFrom = (i * MT + j) * T::kLoads / (NT * MT), kTo = (i * MT + j + 1) * T::kLoads / (NT * MT);
+          static_for<kTo - kFrom>([&](auto nth) {
+            issue_piece(std::integral_constant<int, kFrom + decltype(nth)::value>{}, g + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
+          });
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      });
+      if constexpr (!LAST && i + 1 == NT) {
+        wb[0] = read_w(next, 0);
+        read_scales(g + 1);
+      }
+    });
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < MT; ++j) scale[j] = mine[j];
+  };
+
+  if (g_begin < g_end) {
+    if constexpr (HALVES) {
+      issue(g_begin, 0);
+      static_for<kFirst>([&](auto nth) { issue_first(nth, g_begin + 1, 1); });
+    } else {
+#pragma unroll
+      for (int g = 0; g < STAGES - 1; ++g) issue(g_begin + g, g);
+    }
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(HALVES ? kFirst : (STAGES - 2) * T::kLoads) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int j = 0; j < MT; ++j) read_x(0, j);
+    wb[0] = read_w(0, 0);
+    read_scales(g_begin);
+    int slot = 0;
+    for (int g = g_begin; g + 1 < g_end; ++g) {
+      const int next_slot = slot + 1 == STAGES ? 0 : slot + 1;
+      multiply(std::integral_constant<bool, false>{}, g, slot * T::kStage, next_slot * T::kStage, slot, next_slot);
+      slot = next_slot;
+    }
+    if (again != 0 && g_end == p.groups) clear_again();
+    multiply(std::integral_constant<bool, true>{}, g_end - 1, slot * T::kStage, 0, slot, 0);
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) acc[NT - 1][j][r] = fmaf(part[(NT - 1) & 1][j][r], scale[j], acc[NT - 1][j][r]);
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (no load may write LDS once the workgroup is gone)
 
 #pragma unroll
   for (int j = 0; j < MT; ++j) {
@@ -469,17 +586,45 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void fp8_tile_kernel(const Fp8Matm
         const int64_t n = n0 + wn * (NT * 16) + i * 16 + quarter * 8;
         const float v[8] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3],
                             acc[i + 1][j][0], acc[i + 1][j][1], acc[i + 1][j][2], acc[i + 1][j][3]};
-        store_results<8>(p.c, batch * p.c_bs + m * p.c_rs + n * p.c_cs, p.c_cs, p.out_kind, n, p.n, v);
+        if (p.splits == 1) {
+          store_results<8>(p.c, batch * p.c_bs + m * p.c_rs + n * p.c_cs, p.c_cs, p.out_kind, n, p.n, v);
+        } else {
+          const int64_t line = (static_cast<int64_t>(blockIdx.z) * p.batch + batch) * p.m + m;
+          store_results<8>(p.partial, line * p.n + n, 1, FP8_REAL_F32, n, p.n, v);
+        }
       }
     }
   }
+}
+
+// The shares of a split K added, in order: a thread four columns.
+__global__ __launch_bounds__(256) void fp8_join_kernel(const Fp8MatmulParams p, uint32_t quads, int64_t total) {
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= total) return;
+  const int64_t line = at / quads, n = (at - line * quads) * 4, batch = line / p.m, m = line - batch * p.m;
+  const int64_t share = static_cast<int64_t>(p.batch) * p.m * p.n;
+  const VECOPS_GLOBAL float* from = (const VECOPS_GLOBAL float*)p.partial + line * p.n + n;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  if (n + 4 <= p.n) {
+    for (int s = 0; s < p.splits; ++s) {
+      const u32x4 w = load_16(from + s * share);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] += __uint_as_float(w[e]);
+    }
+  } else {
+    for (int s = 0; s < p.splits; ++s)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (n + e < p.n) v[e] += from[s * share + e];
+  }
+  store_results<4>(p.c, batch * p.c_bs + m * p.c_rs + n * p.c_cs, p.c_cs, p.out_kind, n, p.n, v);
 }
 
 // Few rows (m <= 16 MT): bound by HBM.  A workgroup owns 16 NT weight rows and all m; its wavefronts take the blocks of k in
 // turn, loads of DEPTH blocks under way in each, and their sums meet in LDS.  The scales sa sb of a run of blocks are
 // multiplied beforehand into a table in LDS.
 template <int NT, int MT, int WAVES, int DEPTH>
-__global__ __launch_bounds__(64 * WAVES) void fp8_skinny_kernel(const Fp8MatmulParams p) {
+__global__ __launch_bounds__(64 * WAVES, MT == 1 ? 4 : 2) void fp8_skinny_kernel(const Fp8MatmulParams p) {
   constexpr int RUN = 128, ROWS = MT * 16;
   constexpr int kTable = RUN * ROWS, kSums = WAVES * NT * MT * 256;
   __shared__ float shared[kTable > kSums ? kTable : kSums];
@@ -500,22 +645,26 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_skinny_kernel(const Fp8MatmulP
     constexpr int slot = decltype(slot_tag)::value;
     if (g >= p.groups) return;
     const int k0 = g * kFp8Block + quarter * 16;
-    if ((g + 1) * kFp8Block <= p.k) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < 2; ++h) {
+      // a chunk that K ends in, or in front of, is the sixteen bytes in front of K (rows have at least sixteen), the same on both
+      // sides; of the activations only those are kept that no other chunk has
+      const int k = k0 + 64 * h, at = min(k, p.k - 16);
 #pragma unroll
-        for (int i = 0; i < NT; ++i) wv[slot][i][h] = load_16(w[i] + k0 + 64 * h);
+      for (int i = 0; i < NT; ++i) wv[slot][i][h] = load_16(w[i] + at);
 #pragma unroll
-        for (int j = 0; j < MT; ++j) xv[slot][j][h] = load_16(x[j] + k0 + 64 * h);
-      }
-    } else {
+      for (int j = 0; j < MT; ++j) xv[slot][j][h] = load_16(x[j] + at);
+    }
+    if ((g + 1) * kFp8Block > p.k) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < NT; ++i) wv[slot][i][h] = load_chunk_until(w[i], k0 + 64 * h, p.k);
+        for (int d = 0; d < 4; ++d) {
+          const int z = k0 + 64 * h + 16 - p.k - 4 * d;   // bytes of this word to clear
+          const uint32_t mask = z <= 0 ? 0xffffffffu : z >= 4 ? 0u : 0xffffffffu << (8 * z);
 #pragma unroll
-        for (int j = 0; j < MT; ++j) xv[slot][j][h] = load_chunk_until(x[j], k0 + 64 * h, p.k);
-      }
+          for (int j = 0; j < MT; ++j) xv[slot][j][h][d] &= mask;
+        }
     }
   };
   f32x4 acc[NT][MT];
@@ -532,10 +681,10 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_skinny_kernel(const Fp8MatmulP
     float sx[ENTRIES], sw[ENTRIES];
 #pragma unroll
     for (int e = 0; e < ENTRIES; ++e) {   // (in front of the operands' loads, which the table then does not wait for)
-      const int at = e * (64 * WAVES) + tid, g = run + at / ROWS, m = min(at % ROWS, p.m - 1);
+      const int at = e * (64 * WAVES) + tid, g = run + at % RUN, m = min(at / RUN, p.m - 1);   // (consecutive lanes: consecutive blocks of a row)
       if (g < end) {
-        sx[e] = sx_base[m * p.as_rs + g * p.as_gs];
-        sw[e] = sw_base[g * p.bs_gs];
+        sx[e] = sx_base[m * p.as_rs + g];
+        sw[e] = sw_base[g];
       }
     }
     static_for<DEPTH>([&](auto u) { load(u, run + wave + decltype(u)::value * WAVES); });
@@ -543,7 +692,7 @@ __global__ __launch_bounds__(64 * WAVES) void fp8_skinny_kernel(const Fp8MatmulP
 #pragma unroll
     for (int e = 0; e < ENTRIES; ++e) {
       const int at = e * (64 * WAVES) + tid;
-      if (run + at / ROWS < end) shared[at] = sx[e] * sw[e];
+      if (run + at % RUN < end) shared[at % RUN * ROWS + at / RUN] = sx[e] * sw[e];
     }
     __syncthreads();
     for (int g0 = run + wave; g0 < end; g0 += DEPTH * WAVES) {
@@ -600,17 +749,22 @@ hipError_t launch_skinny(const Fp8MatmulParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <int WN, int WM, int NT, int MT, bool WIDE>
+template <int WN, int WM, int NT, int MT, bool WIDE, int STAGES, bool HALVES = false>
 hipError_t launch_tile(const Fp8MatmulParams& p, hipStream_t stream) {
-  using T = Fp8Tile<WN, WM, NT, MT>;
-  const void* kernel = reinterpret_cast<const void*>(&fp8_tile_kernel<WN, WM, NT, MT, WIDE>);
-  if constexpr (2 * T::kStage > 65536) {
-    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * T::kStage);
+  using T = Fp8Tile<WN, WM, NT, MT, STAGES>;
+  const void* kernel = reinterpret_cast<const void*>(&fp8_tile_kernel<WN, WM, NT, MT, WIDE, STAGES, HALVES>);
+  if constexpr (T::kLds > 65536) {
+    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds);
     if (e != hipSuccess) return e;
   }
   const uint32_t tiles_n = static_cast<uint32_t>((p.n + T::kBN - 1) / T::kBN), tiles_m = static_cast<uint32_t>((p.m + T::kBM - 1) / T::kBM);
-  hipLaunchKernelGGL((fp8_tile_kernel<WN, WM, NT, MT, WIDE>), dim3(tiles_n * tiles_m, static_cast<uint32_t>(p.batch)), dim3(T::kThreads),
-                     2 * T::kStage, stream, p, tiles_n, tiles_m);
+  hipLaunchKernelGGL((fp8_tile_kernel<WN, WM, NT, MT, WIDE, STAGES, HALVES>), dim3(tiles_n * tiles_m, static_cast<uint32_t>(p.batch), static_cast<uint32_t>(p.splits)),
+                     dim3(T::kThreads), T::kLds, stream, p, tiles_n, tiles_m);
+  if (p.splits > 1) {
+    const uint32_t quads = static_cast<uint32_t>((p.n + 3) / 4);
+    const int64_t total = static_cast<int64_t>(p.batch) * p.m * quads;
+    hipLaunchKernelGGL(fp8_join_kernel, dim3(static_cast<uint32_t>((total + 255) / 256)), dim3(256), 0, stream, p, quads, total);
+  }
   return hipGetLastError();
 }
 
@@ -641,14 +795,63 @@ hipError_t launch_fp8_rows(const uint8_t* in, int64_t bs, int64_t rs, int64_t cs
   return hipGetLastError();
 }
 
-hipError_t launch_fp8_matmul(const Fp8MatmulParams& p, hipStream_t stream) {
-  if (p.m <= 16) return launch_skinny<1, 1, 8, 4>(p, stream);
-  if (p.m <= 32) return launch_skinny<1, 2, 8, 4>(p, stream);
-  if (p.m <= 64) return launch_skinny<2, 4, 8, 2>(p, stream);
-  if (p.out_kind == FP8_REAL_F32) return launch_tile<2, 2, 4, 4, true>(p, stream);
-  const int64_t tiles_256 = ((static_cast<int64_t>(p.m) + 255) / 256) * ((static_cast<int64_t>(p.n) + 255) / 256) * p.batch;
-  if (tiles_256 >= 256) return launch_tile<2, 4, 8, 4, false>(p, stream);
-  return launch_tile<2, 2, 4, 4, false>(p, stream);
+hipError_t launch_fp8_scales(const float* in, int64_t bs, int64_t rs, int64_t gs, float* out, int32_t batch, int32_t rows, int32_t groups,
+                             hipStream_t stream) {
+  const int64_t total = static_cast<int64_t>(batch) * rows * groups;
+  hipLaunchKernelGGL(fp8_scales_kernel, dim3(static_cast<uint32_t>((total + 255) / 256)), dim3(256), 0, stream, in, bs, rs, gs, out, total, rows,
+                     groups);
+  return hipGetLastError();
+}
+
+// Which kernel a product takes, and in how many shares of K: the cheapest by an estimate whose numbers were fitted to 2400 times
+// on one MI355X - 24 to 3000 rows, 512 to 14336 columns, K 1024 to 14336, every tile, K whole, in two and in four (by it the
+// product takes 1.004 times the best of them on average, 1.2 times at the worst).
+//   time = start + rounds * (tile start + blocks of k * time a block) + join,  at least the operands' bytes at 6.7 TB/s
+// Tiles of which two share a compute unit take `alone` a block with at most one on each, `paired` else.
+Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t k, int64_t batch, int out_kind) {
+  if (m <= 16) return {FP8_FEW_ROWS, 1};
+  if (k == 0) return {FP8_TILE_64, 1};
+  struct Cost {
+    int kind, n, m, slots;
+    double start[2], alone[2], paired[2];   // us; [1]: fp32 results
+  };
+  static constexpr Cost kCosts[] = {
+      {FP8_TILE_64, 64, 64, 512, {1.83, 2.08}, {0.313, 0.489}, {0.470, 0.711}},
+      {FP8_TILE_128X64, 64, 128, 256, {2.28, 2.33}, {0.430, 0.704}, {0.430, 0.704}},
+      {FP8_TILE_128_ALONE, 128, 128, 256, {2.55, 3.23}, {0.592, 1.000}, {0.592, 1.000}},
+      {FP8_TILE_128_PAIRED, 128, 128, 512, {3.19, 3.93}, {0.718, 1.079}, {1.036, 1.683}},
+      {FP8_TILE_256, 256, 256, 256, {6.11, 1e9}, {1.458, 0.0}, {1.458, 0.0}},
+  };
+  const int wide = out_kind == FP8_REAL_F32;
+  const int64_t groups = (k + kFp8Block - 1) / kFp8Block;
+  Fp8Plan best = {FP8_TILE_64, 1};
+  double least = 1e30;
+  for (const Cost& c : kCosts) {
+    for (int splits = 1; splits <= 4; splits *= 2) {
+      if (splits > 1 && groups < 4 * splits) break;
+      const int64_t units = ((m + c.m - 1) / c.m) * ((n + c.n - 1) / c.n) * batch * splits, blocks = (groups + splits - 1) / splits;
+      const int64_t rounds = units / c.slots, rest = units - rounds * c.slots;
+      double us = rounds * (c.start[wide] + c.paired[wide] * blocks);
+      if (rest > 0) us += c.start[wide] + (rest <= 256 ? c.alone[wide] : c.paired[wide]) * blocks;
+      us = std::max(us, static_cast<double>(m + n) * k * batch / 6.7e6);
+      if (splits > 1) us += 2.5 + 8.0 * splits * m * n * batch / 4.9e6;
+      if (us < least) least = us, best = {c.kind, splits};
+    }
+  }
+  return best;
+}
+
+hipError_t launch_fp8_matmul(const Fp8MatmulParams& p, int kind, hipStream_t stream) {
+  const bool wide = p.out_kind == FP8_REAL_F32;
+  switch (kind) {
+    case FP8_FEW_ROWS: return launch_skinny<1, 1, 8, 4>(p, stream);
+    case FP8_TILE_64: return wide ? launch_tile<2, 2, 2, 2, true, 4>(p, stream) : launch_tile<2, 2, 2, 2, false, 4>(p, stream);
+    case FP8_TILE_128X64: return wide ? launch_tile<2, 4, 2, 2, true, 4>(p, stream) : launch_tile<2, 4, 2, 2, false, 4>(p, stream);
+    case FP8_TILE_128_ALONE: return wide ? launch_tile<2, 4, 4, 2, true, 3>(p, stream) : launch_tile<2, 4, 4, 2, false, 3>(p, stream);
+    case FP8_TILE_128_PAIRED: return wide ? launch_tile<2, 2, 4, 4, true, 2, true>(p, stream) : launch_tile<2, 2, 4, 4, false, 2, true>(p, stream);
+    case FP8_TILE_256: return wide ? hipErrorInvalidValue : launch_tile<2, 4, 8, 4, false, 2, true>(p, stream);
+  }
+  return hipErrorInvalidValue;
 }
 
 }  // namespace vecops_hip

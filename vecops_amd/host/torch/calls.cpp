@@ -317,7 +317,7 @@ int matmul_fp8_block(PyObject* const* args) {
   Given given;
   if (!given.describe(args[5], *plain_tensor(args[4]))) return kNotPlain;
   return without_lock([&]() -> int {
-    const Workspace workspace(given, vecops_hip_matmul_fp8_block_workspace(&o[0], &o[2]));
+    const Workspace workspace(given, vecops_hip_matmul_fp8_block_workspace(&o[0], &o[1], &o[2], &o[3], &o[4]));
     return vecops_hip_matmul_fp8_block(&o[0], &o[1], &o[2], &o[3], &o[4], workspace.data, workspace.size, current_stream());
   });
 }
