@@ -125,13 +125,13 @@ def dequantized(q, scales, rows):
 
 def check(c, a, sa, b, sb):
     """|error| <= (terms of the inner sum + roundings of the scales and of the outer sum) 2^-24 times the sum of the terms'
-    sizes, and the rounding of the result.  16-bit results of more than 16 rows may come from the 8-bit matrix instruction: of
+    sizes, and the rounding of the result.  16-bit results come from the 8-bit matrix instruction: of
     eight products along k the seven smaller ones may each lose 2^-13 of the largest's power of two."""
     x, w = dequantized(a, sa, 1), dequantized(b, sb, 128)
     want, size = x @ w.transpose(-1, -2), x.abs() @ w.abs().transpose(-1, -2)
     k = a.shape[-1]
     bound = (min(k, 128) + 3 + blocks(k)) * 2.0 ** -24 * size
-    if c.dtype != torch.float32 and c.shape[-2] > 16:
+    if c.dtype != torch.float32:
         bound = bound + 7 * 2.0 ** -13 * size
     unit = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[c.dtype]
     bound = bound + unit * (want.abs() + bound) + (2.0 ** -25 if c.dtype == torch.float16 else 0.0)
