@@ -163,6 +163,25 @@ def test_experts_not_finite(device):
     assert not bool(ok[3, 8]) and int((~ok[3]).sum()) == 1
 
 
+@pytest.mark.parametrize("weights", ["bf16", "f16"])
+@pytest.mark.parametrize("at", [1, 2, 9, 30])
+def test_experts_infinite_weights(device, weights, at):
+    """An infinite weight gives the infinity that the formula gives, and touches nothing else; rows end inside a load."""
+    t, e, top, h, i = 3, 3, 1, 99, 43
+    x, gate_up, _, down, _ = case(t, e, top, h, i, weights)
+    ids, w = torch.tensor([[0], [1], [2]], dtype=torch.int32), torch.ones(t, 1)
+    plain, bound = experts64(x, ids, w, gate_up, None, down, None)
+    gate_up[0, i + 5, h - at], down[1, 8, i - at] = float("inf"), float("inf")
+    want, _ = experts64(x, ids, w, gate_up, None, down, None)
+    assert bool(torch.isinf(want[0]).all()) and bool(torch.isinf(want[1, 8]))
+    out = torch.zeros((t, h), device=device)
+    capi.moe_experts(*to(device, x, ids, w, gate_up, down), out)
+    got = out.cpu().double()
+    assert torch.equal(got[0], want[0]) and got[1, 8] == want[1, 8]
+    got[0], got[1, 8] = plain[0], plain[1, 8]
+    assert bool(((got - plain).abs() <= bound).all())
+
+
 def test_experts_large_values_of_half_precision(device):
     """Inner values past the largest f16 number (they are held in bf16 pairs)."""
     t, e, top, h, i = 2, 2, 1, 64, 32

@@ -2887,6 +2887,20 @@ int64_t moe_inner_pad(int64_t inner) { return (inner + 15) / 16 * 16; }
 uint64_t moe_middle_bytes(int64_t tokens, int64_t top, int64_t inner) {
   return round_up_256(static_cast<uint64_t>(tokens) * static_cast<uint64_t>(top) * static_cast<uint64_t>(moe_inner_pad(inner)) * 4u);
 }
+// the inner values, the parts of the result and their counters
+uint64_t moe_experts_bytes(int64_t tokens, int64_t top, int64_t hidden, int64_t inner) {
+  const uint64_t columns = static_cast<uint64_t>((hidden + 15) / 16);
+  if (tokens == 0 || hidden == 0) return 0;
+  return moe_middle_bytes(tokens, top, inner) + round_up_256(columns * 4u) +
+         round_up_256(static_cast<uint64_t>(moe_down_shares(static_cast<int>(hidden))) * columns * static_cast<uint64_t>(tokens) * 64u);
+}
+void place_moe_workspace(MoeExpertsParams* p, void* workspace) {
+  char* at = static_cast<char*>(workspace);
+  p->middle = reinterpret_cast<uint16_t*>(at);
+  at += moe_middle_bytes(p->tokens, p->top, p->inner);
+  p->arrived = reinterpret_cast<int32_t*>(at);
+  p->shares = reinterpret_cast<float*>(at + round_up_256(static_cast<uint64_t>((p->hidden + 15) / 16) * 4u));
+}
 uint64_t moe_logits_bytes(int64_t tokens, int64_t experts, int64_t hidden) {
   return round_up_256(static_cast<uint64_t>(moe_route_parts(static_cast<int>(hidden))) * static_cast<uint64_t>(tokens) * static_cast<uint64_t>(experts) * 4u);
 }
@@ -2960,8 +2974,8 @@ int32_t describe_moe(const char* what, const VecopsHipOperand* x, const VecopsHi
 
 uint64_t vecops_hip_moe_experts_workspace(const VecopsHipOperand* ids, const VecopsHipOperand* down) {
   View vi, vd;
-  if (!matrix_of(ids, &vi) || !normalise(down, &vd)) return 0;
-  return moe_middle_bytes(vi.rows, vi.cols, vd.cols);
+  if (!matrix_of(ids, &vi) || !normalise(down, &vd) || vd.rows > (1 << 24)) return 0;
+  return moe_experts_bytes(vi.rows, vi.cols, vd.rows, vd.cols);
 }
 
 int32_t vecops_hip_moe_experts(const VecopsHipOperand* x, const VecopsHipOperand* ids, const VecopsHipOperand* weights,
@@ -2972,10 +2986,10 @@ int32_t vecops_hip_moe_experts(const VecopsHipOperand* x, const VecopsHipOperand
   const int32_t rc = describe_moe("moe_experts", x, ids, weights, gate_up, gate_up_scales, down, down_scales, out, &m);
   if (rc != ST_OK) return rc;
   if (m.p.tokens == 0 || m.p.hidden == 0) return ST_OK;
-  const uint64_t need = moe_middle_bytes(m.p.tokens, m.p.top, m.p.inner);
+  const uint64_t need = moe_experts_bytes(m.p.tokens, m.p.top, m.p.hidden, m.p.inner);
   if (need > 0 && (workspace == nullptr || workspace_size < need || !aligned16(workspace)))
     return fail(ST_INVALID, "moe_experts: needs a 16-byte aligned workspace of %llu bytes", (unsigned long long)need);
-  m.p.middle = static_cast<uint16_t*>(workspace);
+  place_moe_workspace(&m.p, workspace);
   const hipError_t e = launch_moe_experts(m.p, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return fail(ST_EXEC, "moe_experts: kernel launch: %s", hipGetErrorString(e));
   return ST_OK;
@@ -2984,7 +2998,7 @@ int32_t vecops_hip_moe_experts(const VecopsHipOperand* x, const VecopsHipOperand
 uint64_t vecops_hip_moe_layer_workspace(const VecopsHipOperand* x, const VecopsHipOperand* ids, const VecopsHipOperand* down) {
   View vx, vi, vd;
   if (!matrix_of(x, &vx) || !matrix_of(ids, &vi) || !normalise(down, &vd) || vx.cols > (1 << 24)) return 0;
-  return moe_middle_bytes(vi.rows, vi.cols, vd.cols) + moe_logits_bytes(vx.rows, vd.batch, vx.cols);
+  return moe_experts_bytes(vi.rows, vi.cols, vx.cols, vd.cols) + moe_logits_bytes(vx.rows, vd.batch, vx.cols);
 }
 
 int32_t vecops_hip_moe_layer(const VecopsHipOperand* x, const VecopsHipOperand* router, const VecopsHipMoeRouting* routing,
@@ -3004,15 +3018,15 @@ int32_t vecops_hip_moe_layer(const VecopsHipOperand* x, const VecopsHipOperand* 
   if (m.p.top > m.p.experts) return fail(ST_INVALID, "moe_layer: %d choices among %d experts", m.p.top, m.p.experts);
   if (m.p.tokens == 0 || m.p.hidden == 0) return ST_OK;
   if (m.p.experts > 0 && vr.data == nullptr) return fail(ST_INVALID, "moe_layer: null operand");
-  const uint64_t middle = moe_middle_bytes(m.p.tokens, m.p.top, m.p.inner), need = middle + moe_logits_bytes(m.p.tokens, m.p.experts, m.p.hidden);
+  const uint64_t experts = moe_experts_bytes(m.p.tokens, m.p.top, m.p.hidden, m.p.inner), need = experts + moe_logits_bytes(m.p.tokens, m.p.experts, m.p.hidden);
   if (need > 0 && (workspace == nullptr || workspace_size < need || !aligned16(workspace)))
     return fail(ST_INVALID, "moe_layer: needs a 16-byte aligned workspace of %llu bytes", (unsigned long long)need);
-  m.p.middle = static_cast<uint16_t*>(workspace);
+  place_moe_workspace(&m.p, workspace);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (m.p.top > 0) {
     MoeRouteParams r;
     r.x = m.p.x, r.router = vr.data, r.bias = routing->bias;
-    r.logits = reinterpret_cast<float*>(static_cast<char*>(workspace) + middle);
+    r.logits = reinterpret_cast<float*>(static_cast<char*>(workspace) + experts);
     r.ids = static_cast<int32_t*>(m.ids.data), r.weights = static_cast<float*>(m.weights.data);
     r.ldx = m.p.ldx, r.ld_router = vr.rs;
     r.ids_rs = m.p.ids_rs, r.ids_cs = m.p.ids_cs, r.weights_rs = m.p.weights_rs, r.weights_cs = m.p.weights_cs;

@@ -7,7 +7,7 @@
 
 namespace vecops_hip {
 
-constexpr int kMoeMostTokens = 128, kMoeMostExperts = 512, kMoeMostChoices = 16;
+constexpr int kMoeMostTokens = 128, kMoeMostExperts = 512, kMoeMostChoices = 16, kMoeMostShares = 8;
 
 struct MoeRouteParams {
   const void* x;       // [tokens][hidden], bf16 or f16
@@ -34,6 +34,8 @@ struct MoeExpertsParams {
   const float* gate_up_scales;  // e4m3: [experts][ceil(2 inner / 128)][ceil(hidden / 128)]
   const float* down_scales;     // e4m3: [experts][ceil(hidden / 128)][ceil(inner / 128)]
   uint16_t* middle;      // [2][tokens * top][inner_pad]: the experts' inner values, weighted, as a bf16 and what that leaves
+  float* shares;         // [moe_down_shares][ceil(hidden / 16)][tokens][16]: parts of the result
+  int32_t* arrived;      // [ceil(hidden / 16)]: how many of them are there
   void* out;             // [tokens][hidden], x's type or fp32
   int64_t ldx, ids_rs, ids_cs, weights_rs, weights_cs;
   int64_t gate_up_es, gate_up_rs, down_es, down_rs;  // in elements
@@ -44,6 +46,7 @@ struct MoeExpertsParams {
 };
 
 int moe_route_parts(int hidden);
+int moe_down_shares(int hidden);
 hipError_t launch_moe_route(const MoeRouteParams& p, hipStream_t stream);
 hipError_t launch_moe_experts(const MoeExpertsParams& p, hipStream_t stream);
 

@@ -38,6 +38,14 @@ __device__ __forceinline__ u32x4 load_16_until(const VECOPS_GLOBAL char* row, in
   return v;
 }
 
+// The first elements of a 16-bit chunk cleared: those that lie below `clear` (0 or less: none).
+__device__ __forceinline__ u32x4 cleared(const u32x4& v, int clear) {
+  u32x4 out;
+#pragma unroll
+  for (int d = 0; d < 4; ++d) out[d] = v[d] & (clear <= 2 * d ? 0xffffffffu : clear == 2 * d + 1 ? 0xffff0000u : 0u);
+  return out;
+}
+
 template <bool F16>
 __device__ __forceinline__ f32x4 mfma_16(const u32x4& w, const u32x4& x, const f32x4& acc) {
   if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w), __builtin_bit_cast(f16x8, x), acc, 0, 0, 0);
@@ -202,27 +210,74 @@ __global__ __launch_bounds__(64) void moe_choose_kernel(const MoeRouteParams p) 
 // Experts.  A place (token, choice) whose expert an earlier choice of the same token names too adds its weight to that one.
 // ---------------------------------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ int expert_at(const MoeExpertsParams& p, int token, int choice) { return p.ids[token * p.ids_rs + choice * p.ids_cs]; }
-
-__device__ __forceinline__ bool named_before(const MoeExpertsParams& p, int token, int choice, int expert) {
-  for (int r = 0; r < choice; ++r)
-    if (expert_at(p, token, r) == expert) return true;
-  return false;
+__device__ __forceinline__ int expert_at(const MoeExpertsParams& p, int place) {
+  const int t = place / p.top;
+  return p.ids[t * p.ids_rs + (place - t * p.top) * p.ids_cs];
 }
 
-// element index, in a block of 128 k, of chunk c (eight elements) of quarter q: a 16-byte load of weights is two chunks of
-// e4m3, one of 16-bit elements
-template <bool W8>
-__device__ __forceinline__ int chunk_k(int c, int quarter) { return W8 ? (c >> 1) * 64 + quarter * 16 + (c & 1) * 8 : c * 32 + quarter * 8; }
+// Whether an earlier choice of a place's token names the same expert (ids: all of them, by place).
+__device__ __forceinline__ bool named_before(const int* ids, int place, int choice) {
+  bool found = false;
+  for (int r = 1; r <= choice; ++r) found |= ids[place - r] == ids[place];
+  return found;
+}
+
+// A row ends where it ends: a 16-byte load of weights that the end lies in, or in front of, is the sixteen bytes in front of the
+// end, and so are the activations that go with it; what another load has is cleared when they are used, in both, since either
+// may hold an infinity (an e4m3 has none, and its NaN reaches the result from the other load as well).  (Rows of less than
+// sixteen bytes, TINY, are read element by element.)  Loads of a block of 128 k, all at this lane's places:
+template <bool W8, bool TINY>
+struct Chunks {
+  static constexpr int EB = W8 ? 1 : 2, EPL = 16 / EB, LOADS = W8 ? 2 : 4;   // bytes, elements a load, loads of weights
+  __device__ __forceinline__ static int first(int c, int quarter) { return c * (4 * EPL) + quarter * EPL; }   // of load c
+  __device__ __forceinline__ static int from(int k, int count) { return min(k, count - EPL); }
+  __device__ __forceinline__ static void weights(u32x4 (&v)[LOADS], const VECOPS_GLOBAL char* row, int k0, int quarter, int count) {
+#pragma unroll
+    for (int c = 0; c < LOADS; ++c) {
+      const int k = k0 + first(c, quarter);
+      if constexpr (TINY) v[c] = load_16_until<EB>(row, k, count);
+      else v[c] = load_16(row + static_cast<int64_t>(from(k, count)) * EB);
+    }
+  }
+  // four chunks of eight 16-bit elements, in the order of the weights
+  __device__ __forceinline__ static void activations(u32x4 (&v)[4], const VECOPS_GLOBAL char* row, int k0, int quarter, int count, bool there) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int in = W8 ? (c & 1) * 8 : 0, k = k0 + first(W8 ? c >> 1 : c, quarter);
+      v[c] = u32x4{0u, 0u, 0u, 0u};
+      if (there) {
+        if constexpr (TINY) v[c] = load_16_until<2>(row, k + in, count);
+        else v[c] = load_16(row + static_cast<int64_t>(from(k, count) + in) * 2);
+      }
+    }
+  }
+  // at the block that `count` lies in
+  __device__ __forceinline__ static void clear(u32x4 (&v)[4], int k0, int quarter, int count) {
+    if constexpr (!TINY) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int k = k0 + first(W8 ? c >> 1 : c, quarter);
+        v[c] = cleared(v[c], k - from(k, count) - (W8 ? (c & 1) * 8 : 0));
+      }
+    }
+  }
+  __device__ __forceinline__ static void clear_weights(u32x4 (&v)[LOADS], int k0, int quarter, int count) {
+    if constexpr (!TINY && !W8) clear(v, k0, quarter, count);
+  }
+};
 
 constexpr int kUpWaves = 4;
 
-// gate and up.  A workgroup: one expert, the tokens that name it (16 MT at a time), blocks of sixteen gate rows and their up
-// rows.  Its wavefronts take the blocks of 128 of the hidden axis in turn.
-template <bool F16, bool W8, int MT>
-__global__ __launch_bounds__(64 * kUpWaves) void moe_up_kernel(const MoeExpertsParams p, int by_place) {
-  constexpr int EB = W8 ? 1 : 2, LOADS = W8 ? 2 : 4;
-  __shared__ float meet[kUpWaves][2][MT][256];
+// gate and up.  A workgroup: one expert, the tokens that name it (16 MT at a time), every gridDim.x-th block of sixteen gate rows
+// and their up rows.  Its wavefronts take the blocks of 128 of the hidden axis in turn, the loads of DEPTH of them under way,
+// across the ends of row blocks; their sums meet in LDS.
+// (Loads return in order: activations asked for when they are needed would wait for the weights asked for ahead of them.)
+template <bool F16, bool W8, int MT, bool TINY>
+__global__ __launch_bounds__(64 * kUpWaves, MT == 1 && !W8 ? 3 : MT == 4 ? 1 : 2) void moe_up_kernel(const MoeExpertsParams p, int by_place) {
+  using C = Chunks<W8, TINY>;
+  constexpr int EB = C::EB, LOADS = C::LOADS, DEPTH = TINY ? 1 : W8 && MT == 1 ? 4 : W8 && MT == 2 ? 3 : 2, THREADS = 64 * kUpWaves;
+  __shared__ f32x4 meet[2][kUpWaves][2][MT][64];
+  __shared__ int ids[kMoeMostTokens * kMoeMostChoices];
   __shared__ int places[kMoeMostTokens];
   __shared__ float weight[kMoeMostTokens];
   __shared__ int found;
@@ -230,24 +285,27 @@ __global__ __launch_bounds__(64 * kUpWaves) void moe_up_kernel(const MoeExpertsP
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int total = p.tokens * p.top;
 
+  if (blockIdx.x == 0 && blockIdx.y == 0)
+    for (int at = tid; at < (p.hidden + 15) / 16; at += THREADS) p.arrived[at] = 0;   // for the kernel behind this one
+  for (int s = tid; s < total; s += THREADS) ids[s] = expert_at(p, s);
+  if (tid == 0) found = 0;
+  __syncthreads();
   // the expert: blockIdx.y itself, or the one that place blockIdx.y is the first to name
   int expert = blockIdx.y;
   if (by_place) {
     const int mine = blockIdx.y;
-    expert = expert_at(p, mine / p.top, mine % p.top);
+    expert = ids[mine];
     if (expert < 0 || expert >= p.experts) return;
     int earlier = 0;
-    for (int s = tid; s < mine; s += 64 * kUpWaves) earlier |= expert_at(p, s / p.top, s % p.top) == expert;
+    for (int s = tid; s < mine; s += THREADS) earlier |= ids[s] == expert;
     if (__syncthreads_or(earlier)) return;
   }
-  if (tid == 0) found = 0;
-  __syncthreads();
-  for (int s = tid; s < total; s += 64 * kUpWaves) {
+  for (int s = tid; s < total; s += THREADS) {
     const int t = s / p.top, r = s - t * p.top;
-    if (expert_at(p, t, r) == expert && !named_before(p, t, r, expert)) {
+    if (ids[s] == expert && !named_before(ids, s, r)) {
       float w = p.weights[t * p.weights_rs + r * p.weights_cs];
       for (int u = r + 1; u < p.top; ++u)
-        if (expert_at(p, t, u) == expert) w += p.weights[t * p.weights_rs + u * p.weights_cs];
+        if (ids[t * p.top + u] == expert) w += p.weights[t * p.weights_rs + u * p.weights_cs];
       const int at = atomicAdd(&found, 1);   // (in any order: a token's column does not touch its numbers)
       places[at] = s;
       weight[at] = w;
@@ -260,6 +318,9 @@ __global__ __launch_bounds__(64 * kUpWaves) void moe_up_kernel(const MoeExpertsP
   const VECOPS_GLOBAL char* w_base = (const VECOPS_GLOBAL char*)p.gate_up + expert * p.gate_up_es * EB;
   const VECOPS_GLOBAL float* s_base = (const VECOPS_GLOBAL float*)p.gate_up_scales + expert * p.gs_es;
   const int blocks = (p.hidden + 127) / 128, tiles = p.inner_pad / 16;
+  const int mine = wave < blocks ? (blocks - wave + kUpWaves - 1) / kUpWaves : 0;   // this wavefront's blocks of a row block
+  const int tile_count = (tiles - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
+  const int steps = mine * tile_count;
   for (int base = 0; base < rows; base += 16 * MT) {
     const VECOPS_GLOBAL char* x[MT];
     bool there[MT];
@@ -269,134 +330,173 @@ __global__ __launch_bounds__(64 * kUpWaves) void moe_up_kernel(const MoeExpertsP
       there[j] = at < rows;
       x[j] = (const VECOPS_GLOBAL char*)p.x + (places[min(at, rows - 1)] / p.top) * p.ldx * 2;
     }
-    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-      const int i0 = tile * 16, i = min(i0 + col, p.inner - 1);
+    u32x4 wv[DEPTH][2][LOADS], xv[DEPTH][MT][4];
+    float sv[DEPTH][2][2];
+    // where the next loads go: row block, block of k
+    int load_tile = blockIdx.x, load_block = wave;
+    auto load = [&](auto slot_tag) __attribute__((always_inline)) {
+      constexpr int slot = decltype(slot_tag)::value;
+      const int i0 = load_tile * 16, i = min(i0 + col, p.inner - 1), k0 = load_block * 128;
       const VECOPS_GLOBAL char* w[2] = {w_base + i * p.gate_up_rs * EB, w_base + (static_cast<int64_t>(p.inner) + i) * p.gate_up_rs * EB};
-      f32x4 acc[2][MT];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) C::weights(wv[slot][h], w[h], k0, quarter, p.hidden);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) C::activations(xv[slot][j], x[j], k0, quarter, p.hidden, there[j]);
+      if constexpr (W8) {   // the scales of a lane's first row and of its last one, which may lie in another block of rows
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            sv[slot][h][e] = s_base[(((h ? p.inner : 0) + min(i0 + quarter * 4 + 3 * e, p.inner - 1)) >> 7) * p.gs_rs + load_block * p.gs_cs];
+      }
+      load_block += kUpWaves;
+      if (load_block >= blocks) load_block = wave, load_tile += gridDim.x;
+    };
+    f32x4 acc[2][MT];
+    int tile = blockIdx.x, nth = 0, block = 0;   // the row block that is multiplied, its number here, and the block of k
+    auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int j = 0; j < MT; ++j) acc[h][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      for (int b = wave; b < blocks; b += kUpWaves) {
-        const int k0 = b * 128;
-        u32x4 wv[2][LOADS], xv[MT][4];
-        float scale[2][4];
-        const bool whole = k0 + 128 <= p.hidden;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int c = 0; c < LOADS; ++c) {
-            const int k = k0 + chunk_k<W8>(W8 ? 2 * c : c, quarter);
-            wv[h][c] = whole ? load_16(w[h] + k * EB) : load_16_until<EB>(w[h], k, p.hidden);
-          }
-#pragma unroll
-        for (int j = 0; j < MT; ++j)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int k = k0 + chunk_k<W8>(c, quarter);
-            xv[j][c] = u32x4{0u, 0u, 0u, 0u};
-            if (there[j]) xv[j][c] = whole ? load_16(x[j] + k * 2) : load_16_until<2>(x[j], k, p.hidden);
-          }
-        if constexpr (W8) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {   // (rows past the last one: a scale that exists)
-              const int row = (h ? p.inner : 0) + min(i0 + quarter * 4 + r, p.inner - 1);
-              scale[h][r] = s_base[(row >> 7) * p.gs_rs + b * p.gs_cs];
-            }
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int j = 0; j < MT; ++j) {
-            if constexpr (W8) {
-              f32x4 part = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-              for (int c = 0; c < 4; ++c) part = mfma_16<F16>(widen<F16>(wv[h][c >> 1][(c & 1) * 2], wv[h][c >> 1][(c & 1) * 2 + 1]), xv[j][c], part);
-#pragma unroll
-              for (int r = 0; r < 4; ++r) acc[h][j][r] = fmaf(part[r], scale[h][r], acc[h][j][r]);
-            } else {
-#pragma unroll
-              for (int c = 0; c < 4; ++c) acc[h][j] = mfma_16<F16>(wv[h][c], xv[j][c], acc[h][j]);
-            }
-          }
-      }
-      __syncthreads();   // (the last tile's sums have been read)
+    };
+    // the end of a row block: sums, activation, the inner values' pairs
+    auto finish = [&]() __attribute__((always_inline)) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int j = 0; j < MT; ++j) *reinterpret_cast<f32x4*>(&meet[wave][h][j][lane * 4]) = acc[h][j];
-      __syncthreads();
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        const int in_tile = (tid >> 6) * 4 + (tid & 3), row = base + j * 16 + ((tid >> 2) & 15);   // (lane tid / 4, its result tid % 4)
+        for (int j = 0; j < MT; ++j) meet[nth & 1][wave][h][j][lane] = acc[h][j];
+      __syncthreads();   // (the other half of `meet` is written next: its readers have passed this)
+      for (int at = tid; at < MT * 256; at += THREADS) {
+        const int j = at >> 8, in = at & 255, in_tile = (in >> 6) * 4 + (in & 3), row = base + j * 16 + ((in >> 2) & 15);   // (lane in / 4, its result in % 4)
         if (row < rows) {
           float g = 0.f, u = 0.f;
 #pragma unroll
-          for (int s = 0; s < kUpWaves; ++s) g += meet[s][0][j][tid], u += meet[s][1][j][tid];
-          const float v = i0 + in_tile < p.inner ? g / (1.0f + expf(-g)) * u * weight[row] : 0.0f;
+          for (int s = 0; s < kUpWaves; ++s) {
+            g += reinterpret_cast<const float*>(&meet[nth & 1][s][0][j][0])[in];
+            u += reinterpret_cast<const float*>(&meet[nth & 1][s][1][j][0])[in];
+          }
+          const int i = tile * 16 + in_tile;
+          const float v = i < p.inner ? g / (1.0f + expf(-g)) * u * weight[row] : 0.0f;
           const uint32_t hi = bf16_bits_rne(v);
           const uint32_t lo = (hi & 0x7f80u) == 0x7f80u ? 0u : bf16_bits_rne(v - __uint_as_float(hi << 16));
-          const int64_t at = static_cast<int64_t>(places[row]) * p.inner_pad + i0 + in_tile;
-          p.middle[at] = static_cast<uint16_t>(hi);
-          p.middle[static_cast<int64_t>(total) * p.inner_pad + at] = static_cast<uint16_t>(lo);
+          const int64_t to = static_cast<int64_t>(places[row]) * p.inner_pad + i;
+          p.middle[to] = static_cast<uint16_t>(hi);
+          p.middle[static_cast<int64_t>(total) * p.inner_pad + to] = static_cast<uint16_t>(lo);
         }
       }
+      tile += gridDim.x;
+      ++nth;
+      block = 0;
+      clear();
+    };
+    clear();
+    static_for<DEPTH>([&](auto u) {
+      if (decltype(u)::value < steps) load(u);
+    });
+    if (mine == 0) {   // (fewer blocks than wavefronts)
+      for (int t = 0; t < tile_count; ++t) finish();
     }
+    for (int s0 = 0; s0 < steps; s0 += DEPTH) {
+      static_for<DEPTH>([&](auto slot_tag) {
+        constexpr int slot = decltype(slot_tag)::value;
+        if (s0 + slot < steps) {
+          const int i0 = tile * 16 + quarter * 4, k0 = (wave + block * kUpWaves) * 128;
+          if (k0 + 128 > p.hidden) {
+#pragma unroll
+            for (int j = 0; j < MT; ++j) C::clear(xv[slot][j], k0, quarter, p.hidden);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) C::clear_weights(wv[slot][h], k0, quarter, p.hidden);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+              if constexpr (W8) {
+                f32x4 part = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                  part = mfma_16<F16>(widen<F16>(wv[slot][h][c >> 1][(c & 1) * 2], wv[slot][h][c >> 1][(c & 1) * 2 + 1]), xv[slot][j][c], part);
+                const int row = (h ? p.inner : 0) + i0;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[h][j][r] = fmaf(part[r], ((row + r) ^ row) >> 7 ? sv[slot][h][1] : sv[slot][h][0], acc[h][j][r]);
+              } else {
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[h][j] = mfma_16<F16>(wv[slot][h][c], xv[slot][j][c], acc[h][j]);
+              }
+            }
+          if (s0 + slot + DEPTH < steps) load(slot_tag);
+          if (++block == mine) finish();
+        }
+      });
+    }
+    if (base + 16 * MT < rows) __syncthreads();   // (`meet` begins again)
   }
 }
 
-constexpr int kDownWaves = 8;
-
-// A block of 16-bit weights as bf16: itself, or (f16) a bf16 and what that leaves, together exact.
+// f16 weights as a bf16 and what that leaves, together exact (an infinity leaves nothing).
 __device__ __forceinline__ void split_f16(const u32x4& v, u32x4& hi, u32x4& lo) {
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     const float a = f16_bits_to_f32(v[c] & 0xffffu), b = f16_bits_to_f32(v[c] >> 16);
     hi[c] = cvt_pk_bf16(a, b);
-    lo[c] = cvt_pk_bf16(a - __uint_as_float(hi[c] << 16), b - __uint_as_float(hi[c] & 0xffff0000u));
+    const float la = a - __uint_as_float(hi[c] << 16), lb = b - __uint_as_float(hi[c] & 0xffff0000u);
+    lo[c] = cvt_pk_bf16(la == la ? la : 0.0f, lb == lb ? lb : 0.0f);
   }
 }
 
-// down, and the sum over a token's experts.  A workgroup owns sixteen columns of the result for all tokens: its wavefronts
-// share the (expert, block of 128 inner) pairs out evenly, in order; a wavefront adds an expert's columns to its own sums of
-// the tokens in LDS when it leaves the expert, and the wavefronts' sums are added at the end.  No sum depends on timing.
-template <bool F16, bool W8, int MT>
-__global__ __launch_bounds__(64 * kDownWaves) void moe_down_kernel(const MoeExpertsParams p) {
-  constexpr int EB = W8 ? 1 : 2, LOADS = W8 ? 2 : 4;
+// down, and the sum over a token's experts.  A workgroup owns sixteen columns of the result for all tokens, and one of gridDim.y
+// shares of the work: the tokens of an expert, 8 MT at most, are a segment, and the wavefronts of all shares split the (segment,
+// block of 128 inner) pairs evenly among them, in order, the loads of DEPTH pairs under way across the ends of segments.  Of a
+// matrix instruction's sixteen columns eight take the upper halves of eight tokens' inner values and eight the lower ones,
+// which meet when a wavefront leaves a segment and adds its columns to its own sums of the tokens in LDS.  The wavefronts' sums
+// are added at the end, and the shares' by the workgroup that comes last, in order: no sum depends on timing.
+constexpr int kDownWaves = 8;
+
+template <bool F16, bool W8, int MT, bool TINY>
+__global__ __launch_bounds__(64 * kDownWaves, 2) void moe_down_kernel(const MoeExpertsParams p) {
+  using C = Chunks<W8, TINY>;
+  constexpr int EB = C::EB, LOADS = C::LOADS, DEPTH = TINY ? 1 : MT == 1 ? (W8 ? 6 : 4) : MT == 2 ? (W8 ? 4 : 3) : 2;
   constexpr bool SPLIT = F16 && !W8;   // f16 weights against bf16 pairs
+  constexpr int THREADS = 64 * kDownWaves, PLACES = kMoeMostTokens * kMoeMostChoices / THREADS, TOKENS = 8 * MT;
+  constexpr int SEGMENTS = kMoeMostExperts + kMoeMostTokens * kMoeMostChoices / TOKENS;
+  static_assert(THREADS >= kMoeMostExperts, "a thread an expert");
   extern __shared__ __attribute__((aligned(16))) float sums[];   // [wavefronts][tokens][16]
-  __shared__ uint32_t named[kMoeMostExperts];                    // how often; then packed: first place of its run << 16 | length, of the active ones
-  __shared__ uint16_t active[kMoeMostExperts];
-  __shared__ uint16_t order[kMoeMostTokens * kMoeMostChoices];   // places by expert
+  __shared__ int ids[kMoeMostTokens * kMoeMostChoices];
+  __shared__ uint32_t naming[kMoeMostExperts][kMoeMostTokens / 32];   // by expert: a bit for each token that names it
+  __shared__ uint16_t first_of[kMoeMostExperts];                 // where an expert's run in `order` begins
+  __shared__ uint32_t segment[SEGMENTS];                         // expert << 20 | tokens << 12 | first of them in `order`
+  __shared__ uint16_t order[kMoeMostTokens * kMoeMostChoices];   // places by expert, then by token: the same in every workgroup
   __shared__ uint32_t carry[kDownWaves];
-  __shared__ int count;
+  __shared__ int count, last;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, quarter = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int total = p.tokens * p.top;
-  constexpr int THREADS = 64 * kDownWaves, PLACES = kMoeMostTokens * kMoeMostChoices / THREADS;
-  static_assert(THREADS >= kMoeMostExperts, "a thread an expert");
 
-  named[tid] = 0;
+#pragma unroll
+  for (int w = 0; w < kMoeMostTokens / 32; ++w) naming[tid][w] = 0;
+  for (int s = tid; s < total; s += THREADS) ids[s] = expert_at(p, s);
   for (int at = tid; at < kDownWaves * p.tokens * 16; at += THREADS) sums[at] = 0.f;
   __syncthreads();
-  int expert_of[PLACES], nth[PLACES];
+  int expert_of[PLACES];   // of this thread's places: -1 for those that name none, or none for the first time
 #pragma unroll
   for (int u = 0; u < PLACES; ++u) {
     const int s = u * THREADS + tid;
     expert_of[u] = -1;
     if (s < total) {
-      const int t = s / p.top, r = s - t * p.top, e = expert_at(p, t, r);
-      if (e >= 0 && e < p.experts && !named_before(p, t, r, e)) {
+      const int e = ids[s], t = s / p.top;
+      if (e >= 0 && e < p.experts && !named_before(ids, s, s - t * p.top)) {
         expert_of[u] = e;
-        nth[u] = static_cast<int>(atomicAdd(&named[e], 1u));   // (in any order, as above)
+        atomicOr(&naming[e][t >> 5], 1u << (t & 31));
       }
     }
   }
   __syncthreads();
-  // running sums over the experts of (places, active experts), packed
-  const uint32_t mine = named[tid], pair = mine << 16 | (mine != 0 ? 1u : 0u);
+  // running sums over the experts of (places, segments), packed
+  uint32_t mine = 0;
+#pragma unroll
+  for (int w = 0; w < kMoeMostTokens / 32; ++w) mine += __popc(naming[tid][w]);
+  const uint32_t segments = (mine + TOKENS - 1) / TOKENS, pair = mine << 16 | segments;
   uint32_t run = pair;
 #pragma unroll
   for (int d = 1; d < 64; d *= 2) {
@@ -405,116 +505,176 @@ __global__ __launch_bounds__(64 * kDownWaves) void moe_down_kernel(const MoeExpe
   }
   if (lane == 63) carry[wave] = run;
   __syncthreads();
-  uint32_t before = 0;
-  for (int w = 0; w < wave; ++w) before += carry[w];
-  run += before;
+  for (int w = 0; w < wave; ++w) run += carry[w];
   const uint32_t start = run - pair;   // what lies in front of this expert
   if (tid == THREADS - 1) count = static_cast<int>(run & 0xffffu);
-  named[tid] = start >> 16;   // the first place of this expert's run
+  first_of[tid] = static_cast<uint16_t>(start >> 16);
+  for (uint32_t g = 0; g < segments; ++g)
+    segment[(start & 0xffffu) + g] = static_cast<uint32_t>(tid) << 20 | min(mine - g * TOKENS, static_cast<uint32_t>(TOKENS)) << 12 | ((start >> 16) + g * TOKENS);
   __syncthreads();
 #pragma unroll
   for (int u = 0; u < PLACES; ++u)
-    if (expert_of[u] >= 0) order[named[expert_of[u]] + nth[u]] = static_cast<uint16_t>(u * THREADS + tid);
-  __syncthreads();
-  if (mine != 0) active[start & 0xffffu] = static_cast<uint16_t>(tid);
-  __syncthreads();
-  named[tid] = (start >> 16) << 16 | mine;   // by expert: its run's first place and length
+    if (expert_of[u] >= 0) {
+      const int s = u * THREADS + tid, t = s / p.top;
+      int at = first_of[expert_of[u]];
+#pragma unroll
+      for (int w = 0; w < kMoeMostTokens / 32; ++w) {
+        const uint32_t bits = naming[expert_of[u]][w];
+        at += __popc(t >= 32 * (w + 1) ? bits : t < 32 * w ? 0u : bits & ((1u << (t & 31)) - 1u));
+      }
+      order[at] = static_cast<uint16_t>(s);
+    }
   __syncthreads();
 
   const int h0 = blockIdx.x * 16;
-  const int blocks = (p.inner + 127) / 128, units = count * blocks;
+  const int blocks = (p.inner + 127) / 128;
+  const int64_t units = static_cast<int64_t>(count) * blocks;
   const int64_t row = min(h0 + col, p.hidden - 1);
-  const int64_t lo_plane = static_cast<int64_t>(total) * p.inner_pad * 2;
-  int unit = static_cast<int>(static_cast<int64_t>(units) * wave / kDownWaves);
-  const int unit_end = static_cast<int>(static_cast<int64_t>(units) * (wave + 1) / kDownWaves);
-  while (unit < unit_end) {
-    const int nth_expert = unit / blocks, first = unit - nth_expert * blocks;
-    const int last = min(blocks, first + unit_end - unit);
-    const int expert = __builtin_amdgcn_readfirstlane(active[nth_expert]);
-    const uint32_t its = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(named[expert])));
-    const int from = static_cast<int>(its >> 16), rows = static_cast<int>(its & 0xffffu);
-    const VECOPS_GLOBAL char* w = (const VECOPS_GLOBAL char*)p.down + (expert * p.down_es + row * p.down_rs) * EB;
-    const VECOPS_GLOBAL float* s_base = (const VECOPS_GLOBAL float*)p.down_scales + expert * p.ds_es + (h0 >> 7) * p.ds_rs;
-    for (int base = 0; base < rows; base += 16 * MT) {
-      const VECOPS_GLOBAL char* x[MT];
-      bool there[MT];
-      int token[MT];
+  const int shares = gridDim.y * kDownWaves, share = blockIdx.y * kDownWaves + wave;
+  const int begin = static_cast<int>(units * share / shares), end = static_cast<int>(units * (share + 1) / shares);
+  if (begin < end) {
+    const VECOPS_GLOBAL char* w_row = (const VECOPS_GLOBAL char*)p.down + row * p.down_rs * EB;
+    const VECOPS_GLOBAL float* s_row = (const VECOPS_GLOBAL float*)p.down_scales + (h0 >> 7) * p.ds_rs;
+    // upper halves for the columns below eight, lower ones for the others
+    const VECOPS_GLOBAL char* x_plane = (const VECOPS_GLOBAL char*)p.middle + (col >> 3) * (static_cast<int64_t>(total) * p.inner_pad * 2);
+    u32x4 wv[DEPTH][LOADS], xv[DEPTH][MT][4];
+    float sv[DEPTH];
+    // where the next loads go
+    int load_segment = begin / blocks, load_block = begin - load_segment * blocks;
+    int64_t load_expert = 0;
+    const VECOPS_GLOBAL char* x[MT];
+    bool there[MT];
+    auto aim = [&]() __attribute__((always_inline)) {
+      const uint32_t its = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(segment[min(load_segment, count - 1)])));
+      const int from = static_cast<int>(its & 0xfffu), rows = static_cast<int>(its >> 12 & 0xffu);
+      load_expert = static_cast<int64_t>(its >> 20);
 #pragma unroll
       for (int j = 0; j < MT; ++j) {
-        const int at = base + j * 16 + col, place = order[from + min(at, rows - 1)];
+        const int at = j * 8 + (col & 7);
         there[j] = at < rows;
-        token[j] = place / p.top;
-        x[j] = (const VECOPS_GLOBAL char*)p.middle + static_cast<int64_t>(place) * p.inner_pad * 2;
+        x[j] = x_plane + static_cast<int64_t>(order[from + min(at, rows - 1)]) * p.inner_pad * 2;
       }
-      f32x4 acc[MT];
+    };
+    auto load = [&](auto slot_tag) __attribute__((always_inline)) {
+      constexpr int slot = decltype(slot_tag)::value;
+      const VECOPS_GLOBAL char* w = w_row + load_expert * p.down_es * EB;
+      const int k0 = load_block * 128;
+      C::weights(wv[slot], w, k0, quarter, p.inner);
 #pragma unroll
-      for (int j = 0; j < MT; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-      for (int b = first; b < last; ++b) {
-        const int k0 = b * 128;
-        const bool whole = k0 + 128 <= p.inner;
-        u32x4 wv[LOADS], xh[MT][4], xl[MT][4];
-        float scale = 1.0f;
+      for (int j = 0; j < MT; ++j) C::activations(xv[slot][j], x[j], k0, quarter, p.inner, there[j]);
+      if constexpr (W8) sv[slot] = s_row[load_expert * p.ds_es + load_block * p.ds_cs];
+      if (++load_block == blocks) {
+        load_block = 0;
+        ++load_segment;
+        aim();
+      }
+    };
+    f32x4 acc[MT], less[SPLIT ? MT : 1];   // `less`: what a weight's second half gives
+    int at_segment = load_segment, block = load_block;
+    auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int c = 0; c < LOADS; ++c) {
-          const int k = k0 + chunk_k<W8>(W8 ? 2 * c : c, quarter);
-          wv[c] = whole ? load_16(w + k * EB) : load_16_until<EB>(w, k, p.inner);
+      for (int j = 0; j < MT; ++j) {
+        acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if constexpr (SPLIT) less[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+    };
+    auto leave = [&]() __attribute__((always_inline)) {
+      const uint32_t its = segment[at_segment];
+      const int from = static_cast<int>(its & 0xfffu), rows = static_cast<int>(its >> 12 & 0xffu);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        f32x4 v;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          // what the second halves give; next to an infinity it may be a NaN, or of the other sign
+          float second = __shfl_xor(acc[j][r], 8, 64);
+          if constexpr (SPLIT) second += less[j][r] + __shfl_xor(less[j][r], 8, 64);
+          v[r] = acc[j][r] + (fabsf(acc[j][r]) < __builtin_huge_valf() ? second : 0.0f);
         }
-        if constexpr (W8) scale = s_base[b * p.ds_cs];
+        const int at = j * 8 + col;
+        if (col < 8 && at < rows) {
+          f32x4* to = reinterpret_cast<f32x4*>(&sums[(wave * p.tokens + order[from + at] / p.top) * 16 + quarter * 4]);
+          const f32x4 old = *to;
 #pragma unroll
-        for (int j = 0; j < MT; ++j)
+          for (int r = 0; r < 4; ++r) v[r] += old[r];
+          *to = v;
+        }
+      }
+    };
+    aim();
+    static_for<DEPTH>([&](auto u) {
+      if (begin + decltype(u)::value < end) load(u);
+    });
+    clear();
+    for (int u0 = begin; u0 < end; u0 += DEPTH) {
+      static_for<DEPTH>([&](auto slot_tag) {
+        constexpr int slot = decltype(slot_tag)::value;
+        if (u0 + slot < end) {
+          if ((block + 1) * 128 > p.inner) {
+#pragma unroll
+            for (int j = 0; j < MT; ++j) C::clear(xv[slot][j], block * 128, quarter, p.inner);
+            C::clear_weights(wv[slot], block * 128, quarter, p.inner);
+          }
+          f32x4 part[MT];
+#pragma unroll
+          for (int j = 0; j < MT; ++j) part[j] = W8 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[j];
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const int k = k0 + chunk_k<W8>(c, quarter);
-            xh[j][c] = xl[j][c] = u32x4{0u, 0u, 0u, 0u};
-            if (there[j] && k < p.inner) {   // (inner_pad, a multiple of sixteen, holds zeros past inner)
-              xh[j][c] = load_16(x[j] + k * 2);
-              xl[j][c] = load_16(x[j] + lo_plane + k * 2);
+            u32x4 wh, wl;
+            if constexpr (W8) wh = widen<false>(wv[slot][c >> 1][(c & 1) * 2], wv[slot][c >> 1][(c & 1) * 2 + 1]);
+            else if constexpr (SPLIT) split_f16(wv[slot][c], wh, wl);
+            else wh = wv[slot][c];
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+              part[j] = mfma_16<false>(wh, xv[slot][j][c], part[j]);
+              if constexpr (SPLIT) less[j] = mfma_16<false>(wl, xv[slot][j][c], less[j]);
             }
           }
-        f32x4 part[MT];
-#pragma unroll
-        for (int j = 0; j < MT; ++j) part[j] = W8 ? f32x4{0.f, 0.f, 0.f, 0.f} : acc[j];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          u32x4 wh, wl;
-          if constexpr (W8) wh = widen<false>(wv[c >> 1][(c & 1) * 2], wv[c >> 1][(c & 1) * 2 + 1]);
-          else if constexpr (SPLIT) split_f16(wv[c], wh, wl);
-          else wh = wv[c];
 #pragma unroll
           for (int j = 0; j < MT; ++j) {
-            part[j] = mfma_16<false>(wh, xh[j][c], part[j]);
-            part[j] = mfma_16<false>(wh, xl[j][c], part[j]);
-            if constexpr (SPLIT) part[j] = mfma_16<false>(wl, xh[j][c], part[j]);
+            if constexpr (W8) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r) acc[j][r] = fmaf(part[j][r], sv[slot], acc[j][r]);
+            } else {
+              acc[j] = part[j];
+            }
+          }
+          if (u0 + slot + DEPTH < end) load(slot_tag);
+          if (++block == blocks || u0 + slot + 1 == end) {
+            leave();
+            clear();
+            block = 0;
+            ++at_segment;
           }
         }
-#pragma unroll
-        for (int j = 0; j < MT; ++j) {
-          if constexpr (W8) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[j][r] = fmaf(part[j][r], scale, acc[j][r]);
-          } else {
-            acc[j] = part[j];
-          }
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < MT; ++j)
-        if (there[j]) {
-          f32x4* at = reinterpret_cast<f32x4*>(&sums[(wave * p.tokens + token[j]) * 16 + quarter * 4]);
-          f32x4 v = *at;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] += acc[j][r];
-          *at = v;
-        }
+      });
     }
-    unit += last - first;
   }
   __syncthreads();
+  const bool alone = gridDim.y == 1;
+  for (int at = tid; at < p.tokens * 16; at += THREADS) {
+    float v = 0.f;
+#pragma unroll
+    for (int w = 0; w < kDownWaves; ++w) v += sums[w * p.tokens * 16 + at];
+    if (alone) sums[at] = v;   // (this thread's own number of the first wavefront's)
+    else __hip_atomic_store(&p.shares[(static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * p.tokens * 16 + at], v, __ATOMIC_RELAXED,
+                            __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (!alone) {
+    __syncthreads();
+    if (tid == 0) last = __hip_atomic_fetch_add(&p.arrived[blockIdx.x], 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == static_cast<int>(gridDim.y) - 1;
+    __syncthreads();
+    if (!last) return;
+  }
   for (int at = tid; at < p.tokens * 16; at += THREADS) {
     const int t = at >> 4, h = h0 + (at & 15);
     float v = 0.f;
-#pragma unroll
-    for (int w = 0; w < kDownWaves; ++w) v += sums[(w * p.tokens + t) * 16 + (at & 15)];
+    if (alone) {
+      v = sums[at];
+    } else {
+      for (uint32_t s = 0; s < gridDim.y; ++s)
+        v += __hip_atomic_load(&p.shares[(static_cast<int64_t>(s) * gridDim.x + blockIdx.x) * p.tokens * 16 + at], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
     if (h < p.hidden) {
       const int64_t to = t * p.out_rs + h * p.out_cs;
       if (p.out_f32) static_cast<float*>(p.out)[to] = v;
@@ -523,36 +683,56 @@ __global__ __launch_bounds__(64 * kDownWaves) void moe_down_kernel(const MoeExpe
   }
 }
 
-template <bool F16, bool W8, int MT>
+template <bool F16, bool W8, int MT, bool TINY = false>
 hipError_t launch_experts(const MoeExpertsParams& p, hipStream_t stream) {
   const int places = p.tokens * p.top;
-  if (places > 0 && p.inner > 0 && p.experts > 0) {
+  const bool work = places > 0 && p.inner > 0 && p.experts > 0;
+  if (work) {
     // a workgroup an expert, or one a place where the places are fewer
     const int by_place = places < p.experts;
-    const int tiles = p.inner_pad / 16;
-    hipLaunchKernelGGL((moe_up_kernel<F16, W8, MT>), dim3(static_cast<uint32_t>(tiles), static_cast<uint32_t>(by_place ? places : p.experts)),
-                       dim3(64 * kUpWaves), 0, stream, p, by_place);
+    const int tiles = p.inner_pad / 16, lines = by_place ? places : p.experts;
+    // About six workgroups a compute unit, of equally many blocks of rows: fewer leave compute units without work where experts
+    // are named unevenly (4 tokens x 6 of 64 experts, 2048 x 1408: 89 us with 512, 76 with 1536), more have each too little
+    // behind its search for tokens (64 x 8 of 128, 2048 x 768 in e4m3: 147 us with 1536, 170 with 4096).
+    constexpr int kUpWorkgroups = 1536;
+    const int each = std::max(1, tiles * lines / kUpWorkgroups);
+    const int across = (tiles + each - 1) / each;
+    hipLaunchKernelGGL((moe_up_kernel<F16, W8, MT, TINY>), dim3(static_cast<uint32_t>(across), static_cast<uint32_t>(lines)), dim3(64 * kUpWaves), 0, stream,
+                       p, by_place);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }
-  const void* kernel = reinterpret_cast<const void*>(&moe_down_kernel<F16, W8, MT>);
+  const void* kernel = reinterpret_cast<const void*>(&moe_down_kernel<F16, W8, MT, TINY>);
   const int lds = kDownWaves * p.tokens * 16 * static_cast<int>(sizeof(float));
   if (lds > 32 * 1024) {
     const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, kDownWaves * kMoeMostTokens * 16 * 4);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL((moe_down_kernel<F16, W8, MT>), dim3(static_cast<uint32_t>((p.hidden + 15) / 16)), dim3(64 * kDownWaves), lds, stream, p);
+  const uint32_t columns = static_cast<uint32_t>((p.hidden + 15) / 16);
+  hipLaunchKernelGGL((moe_down_kernel<F16, W8, MT, TINY>), dim3(columns, static_cast<uint32_t>(work ? moe_down_shares(p.hidden) : 1)), dim3(64 * kDownWaves), lds,
+                     stream, p);
   return hipGetLastError();
 }
 
+// Columns of sixteen (in down eight) tokens that a pass over an expert's weights serves: as many as an expert has on average, since
+// more take registers from the loads ahead and fewer read the weights again.  Measured with one, two and four (us): 4 tokens an
+// expert (128 of 2048 x 768, e4m3) 147, 151, 208; 8 (8 of 4096 x 4096, bf16) 178, 169, 179; 12 (64 of 2048 x 1408, bf16) 352, 291,
+// 311; 32 (8 of 4096 x 4096, bf16) 472, 347, 304.
 template <bool F16, bool W8>
 hipError_t launch_experts_for(const MoeExpertsParams& p, hipStream_t stream) {
-  if (p.tokens <= 16) return launch_experts<F16, W8, 1>(p, stream);
-  if (p.tokens <= 32) return launch_experts<F16, W8, 2>(p, stream);
+  const int mean = p.experts > 0 ? p.tokens * p.top / p.experts : 0;
+  if (std::min(p.hidden, p.inner) < 16) return launch_experts<F16, W8, 1, true>(p, stream);
+  if (mean <= 4 || p.tokens <= 8) return launch_experts<F16, W8, 1>(p, stream);
+  if (mean <= 24 || p.tokens <= 16) return launch_experts<F16, W8, 2>(p, stream);
   return launch_experts<F16, W8, 4>(p, stream);
 }
 
 }  // namespace
+
+// A workgroup a compute unit: without shares the few columns of a small hidden axis leave units idle (1001 x 1411, f16, five tokens:
+// 62 us with 63 workgroups, 24.6 with 252), and with more than one a unit the sums that meet in memory cost more than they
+// bring (37 us with 504; 2048 x 768, 64 tokens: 98 us with 128 workgroups, 63 with 256, 75 with 512).
+int moe_down_shares(int hidden) { return std::max(1, std::min(kMoeMostShares, 256 / std::max((hidden + 15) / 16, 1))); }
 
 int moe_route_parts(int hidden) {
   const int steps = (hidden + 31) / 32;
