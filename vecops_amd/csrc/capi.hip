@@ -3023,21 +3023,17 @@ int32_t vecops_hip_moe_layer(const VecopsHipOperand* x, const VecopsHipOperand* 
     return fail(ST_INVALID, "moe_layer: needs a 16-byte aligned workspace of %llu bytes", (unsigned long long)need);
   place_moe_workspace(&m.p, workspace);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (m.p.top > 0) {
-    MoeRouteParams r;
-    r.x = m.p.x, r.router = vr.data, r.bias = routing->bias;
-    r.logits = reinterpret_cast<float*>(static_cast<char*>(workspace) + experts);
-    r.ids = static_cast<int32_t*>(m.ids.data), r.weights = static_cast<float*>(m.weights.data);
-    r.ldx = m.p.ldx, r.ld_router = vr.rs;
-    r.ids_rs = m.p.ids_rs, r.ids_cs = m.p.ids_cs, r.weights_rs = m.p.weights_rs, r.weights_cs = m.p.weights_cs;
-    r.tokens = m.p.tokens, r.experts = m.p.experts, r.hidden = m.p.hidden, r.top = m.p.top;
-    r.parts = moe_route_parts(m.p.hidden);
-    r.x_f16 = m.p.x_f16, r.router_f32 = vr.dtype == DT_F32;
-    r.sigmoid = routing->scoring == VECOPS_HIP_MOE_SIGMOID, r.renormalize = routing->renormalize != 0, r.scale = routing->scale;
-    const hipError_t e = launch_moe_route(r, s);
-    if (e != hipSuccess) return fail(ST_EXEC, "moe_layer: kernel launch: %s", hipGetErrorString(e));
-  }
-  const hipError_t e = launch_moe_experts(m.p, s);
+  MoeRouteParams r;
+  r.x = m.p.x, r.router = vr.data, r.bias = routing->bias;
+  r.logits = reinterpret_cast<float*>(static_cast<char*>(workspace) + experts);
+  r.ids = static_cast<int32_t*>(m.ids.data), r.weights = static_cast<float*>(m.weights.data);
+  r.ldx = m.p.ldx, r.ld_router = vr.rs;
+  r.ids_rs = m.p.ids_rs, r.ids_cs = m.p.ids_cs, r.weights_rs = m.p.weights_rs, r.weights_cs = m.p.weights_cs;
+  r.tokens = m.p.tokens, r.experts = m.p.experts, r.hidden = m.p.hidden, r.top = m.p.top;
+  r.parts = moe_route_parts(m.p.hidden);
+  r.x_f16 = m.p.x_f16, r.router_f32 = vr.dtype == DT_F32;
+  r.sigmoid = routing->scoring == VECOPS_HIP_MOE_SIGMOID, r.renormalize = routing->renormalize != 0, r.scale = routing->scale;
+  const hipError_t e = launch_moe_layer(r, m.p, s);
   if (e != hipSuccess) return fail(ST_EXEC, "moe_layer: kernel launch: %s", hipGetErrorString(e));
   return ST_OK;
 }

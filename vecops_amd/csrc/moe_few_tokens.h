@@ -47,8 +47,8 @@ struct MoeExpertsParams {
 
 int moe_route_parts(int hidden);
 int moe_down_shares(int hidden);
-hipError_t launch_moe_route(const MoeRouteParams& p, hipStream_t stream);
 hipError_t launch_moe_experts(const MoeExpertsParams& p, hipStream_t stream);
+hipError_t launch_moe_layer(const MoeRouteParams& route, const MoeExpertsParams& p, hipStream_t stream);
 
 }  // namespace vecops_hip
 #endif

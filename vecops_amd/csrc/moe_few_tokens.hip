@@ -1,8 +1,8 @@
 // A mixture-of-experts layer for a few tokens:
 //   l = x . router^T;  the experts of the largest scores;  out = sum_r w_r down[e_r] . (silu(gate[e_r] . x) * (up[e_r] . x))
 // What bounds it: the weights of the experts that the tokens name are read once from HBM, against a handful of rows; the rest
-// is latency.  Four launches: the logits, the choice, gate and up with the activation, down with the sum over a token's
-// experts.  The tokens of an expert are the columns of a matrix instruction whose rows are sixteen rows of weights, which go
+// is latency.  Launches: the logits, the choice (for a few tokens in front of the next, in it), gate and up with the
+// activation, down with the sum over a token's experts.  The tokens of an expert are the columns of a matrix instruction whose rows are sixteen rows of weights, which go
 // from memory straight into its operand registers.
 #include "moe_few_tokens.h"
 
@@ -75,12 +75,13 @@ __device__ __forceinline__ u32x4 widen(uint32_t lo, uint32_t hi) {
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Router: logits in fp32.  A workgroup has sixteen experts, sixteen tokens and one of `parts` shares of the hidden axis, which
-// its wavefronts split again; the shares are added where the experts are chosen.
+// its wavefronts split again; the shares are added where the experts are chosen.  A wavefront asks for all that it multiplies at
+// once (64 tokens, 128 experts, hidden 2048: 8.4 us with a step's loads behind the step before, 4.7 so).
 // ---------------------------------------------------------------------------------------------------------------------
 
 constexpr int kRouteWaves = 4, kRouteSteps = 4;  // steps of 32 that a wavefront has at most in its share
 
-template <bool F16, bool R32>
+template <bool F16, bool R32, bool TINY>
 __global__ __launch_bounds__(64 * kRouteWaves) void moe_logits_kernel(const MoeRouteParams p) {
   __shared__ float meet[kRouteWaves][256];
   const int lane = threadIdx.x & 63, col = lane & 15, quarter = lane >> 4;
@@ -90,20 +91,35 @@ __global__ __launch_bounds__(64 * kRouteWaves) void moe_logits_kernel(const MoeR
   const VECOPS_GLOBAL char* x = (const VECOPS_GLOBAL char*)p.x + static_cast<int64_t>(min(t0 + col, p.tokens - 1)) * p.ldx * 2;
   const int steps = (p.hidden + 31) / 32, first = static_cast<int>(static_cast<int64_t>(steps) * blockIdx.y / p.parts),
             end = static_cast<int>(static_cast<int64_t>(steps) * (blockIdx.y + 1) / p.parts);
+  u32x4 xv[kRouteSteps], rv[kRouteSteps][R32 ? 2 : 1];
+  int clear[kRouteSteps];   // of the eight elements, those that another step or lane has
+#pragma unroll
+  for (int u = 0; u < kRouteSteps; ++u) {
+    const int s = first + wave + u * kRouteWaves, k = s * 32 + quarter * 8, from = TINY ? k : min(k, p.hidden - 8);
+    clear[u] = s < end ? k - from : 8;
+    if constexpr (TINY) {
+      xv[u] = load_16_until<2>(x, k, p.hidden);
+      rv[u][0] = load_16_until<R32 ? 4 : 2>(r, k, p.hidden);
+      if constexpr (R32) rv[u][1] = load_16_until<4>(r, k + 4, p.hidden);
+    } else {
+      xv[u] = load_16(x + static_cast<int64_t>(from) * 2);
+      rv[u][0] = load_16(r + static_cast<int64_t>(from) * (R32 ? 4 : 2));
+      if constexpr (R32) rv[u][1] = load_16(r + static_cast<int64_t>(from) * 4 + 16);
+    }
+  }
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int s = first + wave; s < end; s += kRouteWaves) {
-    const int k = s * 32 + quarter * 8;
-    const u32x4 xv = load_16_until<2>(x, k, p.hidden);
+#pragma unroll
+  for (int u = 0; u < kRouteSteps; ++u) {
+    const u32x4 xs = cleared(xv[u], clear[u]);
     if constexpr (R32) {
-      const u32x4 lo = load_16_until<4>(r, k, p.hidden), hi = load_16_until<4>(r, k + 4, p.hidden);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {   // instruction i multiplies element i of every lane
-        const uint32_t bits = (xv[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+        const uint32_t bits = (xs[i >> 1] >> (16 * (i & 1))) & 0xffffu;
         const float xf = F16 ? f16_bits_to_f32(bits) : __uint_as_float(bits << 16);
-        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(i < 4 ? lo[i & 3] : hi[i & 3]), xf, acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(i >= clear[u] ? __uint_as_float(rv[u][i >> 2][i & 3]) : 0.0f, xf, acc, 0, 0, 0);
       }
     } else {
-      acc = mfma_16<F16>(load_16_until<2>(r, k, p.hidden), xv, acc);
+      acc = mfma_16<F16>(cleared(rv[u][0], clear[u]), xs, acc);
     }
   }
   *reinterpret_cast<f32x4*>(&meet[wave][lane * 4]) = acc;
@@ -122,23 +138,36 @@ __device__ __forceinline__ uint32_t order_of(float v) {
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) v = fmaxf(v, __shfl_xor(v, d, 64));
+// A reduction over the wavefront, by moves within rows of sixteen lanes and from row to row: the last lane has all of it.
+template <typename Join>
+__device__ __forceinline__ uint32_t over_wave(uint32_t v, uint32_t none, Join join) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  v = join(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(none, v, 0x111, 0xf, 0xf, false)));   // from one, two, four, eight
+  v = join(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(none, v, 0x112, 0xf, 0xf, false)));   // lanes below in the row
+  v = join(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(none, v, 0x114, 0xf, 0xf, false)));
+  v = join(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(none, v, 0x118, 0xf, 0xf, false)));
+  v = join(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(none, v, 0x142, 0xa, 0xf, false)));   // rows 0, 2 into 1, 3
+  v = join(v, static_cast<uint32_t>(__builtin_amdgcn_update_dpp(none, v, 0x143, 0xc, 0xf, false)));   // row 1 into 2, 3
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 63));
+#else
+  (void)none; (void)join;
   return v;
+#endif
+}
+__device__ __forceinline__ float wave_max(float v) {
+  return __uint_as_float(over_wave(__float_as_uint(v), 0xff800000u, [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
 }
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d, 64);
-  return v;
+  return __uint_as_float(over_wave(__float_as_uint(v), 0u, [](uint32_t a, uint32_t b) { return __float_as_uint(__uint_as_float(a) + __uint_as_float(b)); }));
 }
 
-// The choice: a wavefront a token, lane l has the experts l, l + 64, ...; `top` times the largest that is left, the lower
-// index among equals.
-__global__ __launch_bounds__(64) void moe_choose_kernel(const MoeRouteParams p) {
+// The choice for a token, by a wavefront: lane l has the experts l, l + 64, ...; `top` times the largest that is left, the lower
+// index among equals.  Lane r returns choice r and its weight.  What bounds it
+// is the chain from choice to choice: each is a reduction of 32 bits by moves between lanes and a search for the first lane that
+// has them, none of it through LDS (64 tokens, 8 of 128 experts: 5.5 us).
+__device__ __forceinline__ void choose(const MoeRouteParams& p, int t, int lane, int& id, float& weight) {
   constexpr int MOST = kMoeMostExperts / 64;
-  const int t = blockIdx.x, lane = threadIdx.x;
-  float score[MOST];
+  float score[MOST], bias[MOST];
   uint32_t key[MOST];
   float most = -__builtin_huge_valf();
 #pragma unroll
@@ -146,8 +175,11 @@ __global__ __launch_bounds__(64) void moe_choose_kernel(const MoeRouteParams p) 
     const int e = lane + 64 * j;
     score[j] = -__builtin_huge_valf();
     key[j] = 0;
+    bias[j] = 0.f;
     if (e < p.experts) {
+      if (p.bias != nullptr) bias[j] = p.bias[e];
       float l = 0.f;
+#pragma unroll 4
       for (int s = 0; s < p.parts; ++s) l += p.logits[(static_cast<int64_t>(s) * p.tokens + t) * p.experts + e];
       score[j] = l;
       key[j] = order_of(l);   // (0 is below every number's)
@@ -156,15 +188,17 @@ __global__ __launch_bounds__(64) void moe_choose_kernel(const MoeRouteParams p) 
   }
   if (p.sigmoid) {
 #pragma unroll
-    for (int j = 0; j < MOST; ++j) score[j] = 1.0f / (1.0f + expf(-score[j]));
+    for (int j = 0; j < MOST; ++j)
+      if (64 * j < p.experts) score[j] = 1.0f / (1.0f + expf(-score[j]));
   } else {
     most = wave_max(most);
     float sum = 0.f;
 #pragma unroll
-    for (int j = 0; j < MOST; ++j) {
-      score[j] = lane + 64 * j < p.experts ? expf(score[j] - most) : 0.f;
-      sum += score[j];
-    }
+    for (int j = 0; j < MOST; ++j)
+      if (64 * j < p.experts) {
+        score[j] = lane + 64 * j < p.experts ? expf(score[j] - most) : 0.f;
+        sum += score[j];
+      }
     sum = wave_sum(sum);
 #pragma unroll
     for (int j = 0; j < MOST; ++j) score[j] /= sum;
@@ -172,37 +206,43 @@ __global__ __launch_bounds__(64) void moe_choose_kernel(const MoeRouteParams p) 
   if (p.bias != nullptr) {
 #pragma unroll
     for (int j = 0; j < MOST; ++j)
-      if (lane + 64 * j < p.experts) key[j] = order_of(score[j] + p.bias[lane + 64 * j]);
+      if (lane + 64 * j < p.experts) key[j] = order_of(score[j] + bias[j]);
   }
   float chosen = 0.f, total = 0.f;   // lane r keeps the score of choice r
-  int id = 0;
+  id = 0;
   for (int r = 0; r < p.top; ++r) {
-    uint64_t best = 0;   // (the order, then the lower index first)
+    uint32_t mine = 0;
+#pragma unroll
+    for (int j = 0; j < MOST; ++j) mine = max(mine, key[j]);
+    const uint32_t best = over_wave(mine, 0u, [](uint32_t a, uint32_t b) { return max(a, b); });
+    int e = -1;
     float its = 0.f;
 #pragma unroll
     for (int j = 0; j < MOST; ++j) {
-      const uint64_t mine = static_cast<uint64_t>(key[j]) << 32 | static_cast<uint32_t>(~(lane + 64 * j));
-      if (key[j] != 0 && mine > best) best = mine, its = score[j];
+      if (e < 0 && 64 * j < p.experts) {   // (the same in all lanes)
+        const uint64_t have = __ballot(key[j] == best);
+        if (have != 0) {
+          const int first = __builtin_ctzll(have);
+          e = 64 * j + first;
+          its = __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(__float_as_uint(score[j])), first)));
+          if (lane == first) key[j] = 0;   // taken
+        }
+      }
     }
-    uint64_t top = best;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const uint32_t hi = static_cast<uint32_t>(__shfl_xor(static_cast<int>(top >> 32), d, 64));
-      const uint32_t lo = static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d, 64));
-      const uint64_t other = static_cast<uint64_t>(hi) << 32 | lo;
-      top = other > top ? other : top;
-    }
-    const int e = static_cast<int>(~static_cast<uint32_t>(top));
-    its = __shfl(its, e & 63, 64);
-#pragma unroll
-    for (int j = 0; j < MOST; ++j)
-      if (e == lane + 64 * j) key[j] = 0;   // taken
     if (lane == r) chosen = its, id = e;
     total += its;
   }
+  weight = (p.renormalize ? chosen / total : chosen) * p.scale;
+}
+
+__global__ __launch_bounds__(64) void moe_choose_kernel(const MoeRouteParams p) {
+  const int t = blockIdx.x, lane = threadIdx.x;
+  int id;
+  float weight;
+  choose(p, t, lane, id, weight);
   if (lane < p.top) {
     p.ids[t * p.ids_rs + lane * p.ids_cs] = id;
-    p.weights[t * p.weights_rs + lane * p.weights_cs] = (p.renormalize ? chosen / total : chosen) * p.scale;
+    p.weights[t * p.weights_rs + lane * p.weights_cs] = weight;
   }
 }
 
@@ -272,14 +312,16 @@ constexpr int kUpWaves = 4;
 // and their up rows.  Its wavefronts take the blocks of 128 of the hidden axis in turn, the loads of DEPTH of them under way,
 // across the ends of row blocks; their sums meet in LDS.
 // (Loads return in order: activations asked for when they are needed would wait for the weights asked for ahead of them.)
-template <bool F16, bool W8, int MT, bool TINY>
-__global__ __launch_bounds__(64 * kUpWaves, MT == 1 && !W8 ? 3 : MT == 4 ? 1 : 2) void moe_up_kernel(const MoeExpertsParams p, int by_place) {
+// CHOOSES: the experts are not chosen yet, and every workgroup chooses them, a wavefront a token; the first one writes the choice.
+template <bool F16, bool W8, int MT, bool TINY, bool CHOOSES>
+__global__ __launch_bounds__(64 * kUpWaves, MT == 1 && !W8 ? 3 : MT == 4 ? 1 : 2) void moe_up_kernel(const MoeExpertsParams p, const MoeRouteParams route, int by_place) {
   using C = Chunks<W8, TINY>;
   constexpr int EB = C::EB, LOADS = C::LOADS, DEPTH = TINY ? 1 : W8 && MT == 1 ? 4 : W8 && MT == 2 ? 3 : 2, THREADS = 64 * kUpWaves;
   __shared__ f32x4 meet[2][kUpWaves][2][MT][64];
   __shared__ int ids[kMoeMostTokens * kMoeMostChoices];
   __shared__ int places[kMoeMostTokens];
   __shared__ float weight[kMoeMostTokens];
+  __shared__ float chosen[CHOOSES ? kUpWaves * kMoeMostChoices : 1];   // the weights
   __shared__ int found;
   const int tid = threadIdx.x, lane = tid & 63, col = lane & 15, quarter = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -287,7 +329,23 @@ __global__ __launch_bounds__(64 * kUpWaves, MT == 1 && !W8 ? 3 : MT == 4 ? 1 : 2
 
   if (blockIdx.x == 0 && blockIdx.y == 0)
     for (int at = tid; at < (p.hidden + 15) / 16; at += THREADS) p.arrived[at] = 0;   // for the kernel behind this one
-  for (int s = tid; s < total; s += THREADS) ids[s] = expert_at(p, s);
+  if constexpr (CHOOSES) {
+    if (wave < p.tokens) {
+      int id;
+      float w;
+      choose(route, wave, lane, id, w);
+      if (lane < p.top) {
+        ids[wave * p.top + lane] = id;
+        chosen[wave * p.top + lane] = w;
+        if (blockIdx.x == 0 && blockIdx.y == 0) {
+          route.ids[wave * p.ids_rs + lane * p.ids_cs] = id;
+          route.weights[wave * p.weights_rs + lane * p.weights_cs] = w;
+        }
+      }
+    }
+  } else {
+    for (int s = tid; s < total; s += THREADS) ids[s] = expert_at(p, s);
+  }
   if (tid == 0) found = 0;
   __syncthreads();
   // the expert: blockIdx.y itself, or the one that place blockIdx.y is the first to name
@@ -303,9 +361,14 @@ __global__ __launch_bounds__(64 * kUpWaves, MT == 1 && !W8 ? 3 : MT == 4 ? 1 : 2
   for (int s = tid; s < total; s += THREADS) {
     const int t = s / p.top, r = s - t * p.top;
     if (ids[s] == expert && !named_before(ids, s, r)) {
-      float w = p.weights[t * p.weights_rs + r * p.weights_cs];
-      for (int u = r + 1; u < p.top; ++u)
-        if (ids[t * p.top + u] == expert) w += p.weights[t * p.weights_rs + u * p.weights_cs];
+      float w;
+      if constexpr (CHOOSES) {   // (no expert twice)
+        w = chosen[s];
+      } else {
+        w = p.weights[t * p.weights_rs + r * p.weights_cs];
+        for (int u = r + 1; u < p.top; ++u)
+          if (ids[t * p.top + u] == expert) w += p.weights[t * p.weights_rs + u * p.weights_cs];
+      }
       const int at = atomicAdd(&found, 1);   // (in any order: a token's column does not touch its numbers)
       places[at] = s;
       weight[at] = w;
@@ -683,23 +746,33 @@ __global__ __launch_bounds__(64 * kDownWaves, 2) void moe_down_kernel(const MoeE
   }
 }
 
+bool has_work(const MoeExpertsParams& p) { return p.tokens * p.top > 0 && p.inner > 0 && p.experts > 0; }
+// Rows of less than sixteen bytes of e4m3.
+bool is_tiny(const MoeExpertsParams& p) { return std::min(p.hidden, p.inner) < 16; }
+
+template <bool F16, bool W8, int MT, bool TINY, bool CHOOSES>
+hipError_t launch_up(const MoeExpertsParams& p, const MoeRouteParams& route, hipStream_t stream) {
+  // a workgroup an expert, or one a place where the places are fewer
+  const int places = p.tokens * p.top, by_place = places < p.experts;
+  const int tiles = p.inner_pad / 16, lines = by_place ? places : p.experts;
+  // About six workgroups a compute unit, of equally many blocks of rows: fewer leave compute units without work where experts
+  // are named unevenly (4 tokens x 6 of 64 experts, 2048 x 1408: 89 us with 512, 76 with 1536), more have each too little
+  // behind its search for tokens (64 x 8 of 128, 2048 x 768 in e4m3: 147 us with 1536, 170 with 4096).
+  constexpr int kUpWorkgroups = 1536;
+  const int each = std::max(1, tiles * lines / kUpWorkgroups);
+  const int across = (tiles + each - 1) / each;
+  hipLaunchKernelGGL((moe_up_kernel<F16, W8, MT, TINY, CHOOSES>), dim3(static_cast<uint32_t>(across), static_cast<uint32_t>(lines)), dim3(64 * kUpWaves), 0,
+                     stream, p, route, by_place);
+  return hipGetLastError();
+}
+
 template <bool F16, bool W8, int MT, bool TINY = false>
-hipError_t launch_experts(const MoeExpertsParams& p, hipStream_t stream) {
-  const int places = p.tokens * p.top;
-  const bool work = places > 0 && p.inner > 0 && p.experts > 0;
+hipError_t launch_experts(const MoeExpertsParams& p, const MoeRouteParams* route, hipStream_t stream) {
+  const bool work = has_work(p);
   if (work) {
-    // a workgroup an expert, or one a place where the places are fewer
-    const int by_place = places < p.experts;
-    const int tiles = p.inner_pad / 16, lines = by_place ? places : p.experts;
-    // About six workgroups a compute unit, of equally many blocks of rows: fewer leave compute units without work where experts
-    // are named unevenly (4 tokens x 6 of 64 experts, 2048 x 1408: 89 us with 512, 76 with 1536), more have each too little
-    // behind its search for tokens (64 x 8 of 128, 2048 x 768 in e4m3: 147 us with 1536, 170 with 4096).
-    constexpr int kUpWorkgroups = 1536;
-    const int each = std::max(1, tiles * lines / kUpWorkgroups);
-    const int across = (tiles + each - 1) / each;
-    hipLaunchKernelGGL((moe_up_kernel<F16, W8, MT, TINY>), dim3(static_cast<uint32_t>(across), static_cast<uint32_t>(lines)), dim3(64 * kUpWaves), 0, stream,
-                       p, by_place);
-    const hipError_t e = hipGetLastError();
+    hipError_t e;
+    if constexpr (MT == 1 && !TINY) e = route != nullptr ? launch_up<F16, W8, MT, TINY, true>(p, *route, stream) : launch_up<F16, W8, MT, TINY, false>(p, MoeRouteParams{}, stream);
+    else e = launch_up<F16, W8, MT, TINY, false>(p, MoeRouteParams{}, stream);
     if (e != hipSuccess) return e;
   }
   const void* kernel = reinterpret_cast<const void*>(&moe_down_kernel<F16, W8, MT, TINY>);
@@ -719,12 +792,12 @@ hipError_t launch_experts(const MoeExpertsParams& p, hipStream_t stream) {
 // expert (128 of 2048 x 768, e4m3) 147, 151, 208; 8 (8 of 4096 x 4096, bf16) 178, 169, 179; 12 (64 of 2048 x 1408, bf16) 352, 291,
 // 311; 32 (8 of 4096 x 4096, bf16) 472, 347, 304.
 template <bool F16, bool W8>
-hipError_t launch_experts_for(const MoeExpertsParams& p, hipStream_t stream) {
+hipError_t launch_experts_for(const MoeExpertsParams& p, const MoeRouteParams* route, hipStream_t stream) {
   const int mean = p.experts > 0 ? p.tokens * p.top / p.experts : 0;
-  if (std::min(p.hidden, p.inner) < 16) return launch_experts<F16, W8, 1, true>(p, stream);
-  if (mean <= 4 || p.tokens <= 8) return launch_experts<F16, W8, 1>(p, stream);
-  if (mean <= 24 || p.tokens <= 16) return launch_experts<F16, W8, 2>(p, stream);
-  return launch_experts<F16, W8, 4>(p, stream);
+  if (is_tiny(p)) return launch_experts<F16, W8, 1, true>(p, route, stream);
+  if (mean <= 4 || p.tokens <= 8) return launch_experts<F16, W8, 1>(p, route, stream);
+  if (mean <= 24 || p.tokens <= 16) return launch_experts<F16, W8, 2>(p, route, stream);
+  return launch_experts<F16, W8, 4>(p, route, stream);
 }
 
 }  // namespace
@@ -739,24 +812,39 @@ int moe_route_parts(int hidden) {
   return std::max(1, (steps + kRouteWaves * kRouteSteps - 1) / (kRouteWaves * kRouteSteps));
 }
 
-hipError_t launch_moe_route(const MoeRouteParams& p, hipStream_t stream) {
+namespace {
+
+template <bool F16, bool R32>
+hipError_t launch_logits(const MoeRouteParams& p, hipStream_t stream) {
   const dim3 grid(static_cast<uint32_t>((p.experts + 15) / 16), static_cast<uint32_t>(p.parts), static_cast<uint32_t>((p.tokens + 15) / 16));
-  if (p.router_f32) {
-    if (p.x_f16) hipLaunchKernelGGL((moe_logits_kernel<true, true>), grid, dim3(64 * kRouteWaves), 0, stream, p);
-    else hipLaunchKernelGGL((moe_logits_kernel<false, true>), grid, dim3(64 * kRouteWaves), 0, stream, p);
-  } else {
-    if (p.x_f16) hipLaunchKernelGGL((moe_logits_kernel<true, false>), grid, dim3(64 * kRouteWaves), 0, stream, p);
-    else hipLaunchKernelGGL((moe_logits_kernel<false, false>), grid, dim3(64 * kRouteWaves), 0, stream, p);
-  }
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(moe_choose_kernel, dim3(static_cast<uint32_t>(p.tokens)), dim3(64), 0, stream, p);
+  if (p.hidden < 8) hipLaunchKernelGGL((moe_logits_kernel<F16, R32, true>), grid, dim3(64 * kRouteWaves), 0, stream, p);
+  else hipLaunchKernelGGL((moe_logits_kernel<F16, R32, false>), grid, dim3(64 * kRouteWaves), 0, stream, p);
   return hipGetLastError();
 }
 
-hipError_t launch_moe_experts(const MoeExpertsParams& p, hipStream_t stream) {
-  if (p.x_f16) return p.w_e4m3 ? launch_experts_for<true, true>(p, stream) : launch_experts_for<true, false>(p, stream);
-  return p.w_e4m3 ? launch_experts_for<false, true>(p, stream) : launch_experts_for<false, false>(p, stream);
+hipError_t launch_for(const MoeExpertsParams& p, const MoeRouteParams* route, hipStream_t stream) {
+  if (p.x_f16) return p.w_e4m3 ? launch_experts_for<true, true>(p, route, stream) : launch_experts_for<true, false>(p, route, stream);
+  return p.w_e4m3 ? launch_experts_for<false, true>(p, route, stream) : launch_experts_for<false, false>(p, route, stream);
+}
+
+}  // namespace
+
+hipError_t launch_moe_experts(const MoeExpertsParams& p, hipStream_t stream) { return launch_for(p, nullptr, stream); }
+
+hipError_t launch_moe_layer(const MoeRouteParams& r, const MoeExpertsParams& p, hipStream_t stream) {
+  if (r.top > 0) {
+    hipError_t e;
+    if (r.router_f32) e = r.x_f16 ? launch_logits<true, true>(r, stream) : launch_logits<false, true>(r, stream);
+    else e = r.x_f16 ? launch_logits<true, false>(r, stream) : launch_logits<false, false>(r, stream);
+    if (e != hipSuccess) return e;
+    // For as many tokens as a workgroup of gate and up has wavefronts the choice is its first work: for one token of 6 of 64
+    // experts of 2048 x 1408 a launch of its own makes the layer 41.9 us instead of 40.1.
+    if (r.tokens <= kUpWaves && has_work(p) && !is_tiny(p)) return launch_for(p, &r, stream);
+    hipLaunchKernelGGL(moe_choose_kernel, dim3(static_cast<uint32_t>(r.tokens)), dim3(64), 0, stream, r);
+    e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return launch_for(p, nullptr, stream);
 }
 
 }  // namespace vecops_hip
