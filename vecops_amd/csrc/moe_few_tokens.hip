@@ -2,8 +2,8 @@
 //   l = x . router^T;  the experts of the largest scores;  out = sum_r w_r down[e_r] . (silu(gate[e_r] . x) * (up[e_r] . x))
 // What bounds it: the weights of the experts that the tokens name are read once from HBM, against a handful of rows; the rest
 // is latency.  Launches: the logits, the choice (for a few tokens in front of the next, in it), gate and up with the
-// activation, down with the sum over a token's experts.  The tokens of an expert are the columns of a matrix instruction whose rows are sixteen rows of weights, which go
-// from memory straight into its operand registers.
+// activation, down with the sum over a token's experts.  The tokens of an expert are the columns of a matrix instruction whose
+// rows are sixteen rows of weights, which go from memory straight into registers.
 #include "moe_few_tokens.h"
 
 #include <algorithm>
@@ -262,47 +262,80 @@ __device__ __forceinline__ bool named_before(const int* ids, int place, int choi
   return found;
 }
 
-// A row ends where it ends: a 16-byte load of weights that the end lies in, or in front of, is the sixteen bytes in front of the
-// end, and so are the activations that go with it; what another load has is cleared when they are used, in both, since either
+// Weights from memory into a matrix instruction's operand: a lane there holds sixteen bytes of row (lane % 16), the lanes of a
+// quarter of the wavefront the same bytes of their rows.  Loaded like that every lane is a look-up in the cache of its own, and
+// those bound the kernels (0.7 of them a cycle).  So neighbouring lanes load neighbouring sixteen bytes of one row, as many as
+// there are loads (four, or two of e4m3, whose scales end a block of 128 k), a load each of as many rows, and exchange them, and
+// activations likewise.  Gate and up, then down (us): 5 tokens, 4 of 60 of 1001 x 1411 in f16 35, 25.4 -> 24.4, 22.7; 64 tokens,
+// 8 of 128 of 2048 x 768 in e4m3 90, 59 -> 86, 53; 16 tokens, 2 of 8 of 4096 x 14336 in bf16 315, 196 -> 309 (6.1 TB/s), 174 (5.4).
+// Lane l holds then, of a block of 128 k, the thirty-two from 32 (l / 16) on, and so it has the activations.
+//
+// A row ends where it ends: sixteen bytes that the end lies in, or in front of, are replaced by those in front of the end, and so
+// are the activations that go with them; what another lane or load has is cleared when they are used, in both, since either
 // may hold an infinity (an e4m3 has none, and its NaN reaches the result from the other load as well).  (Rows of less than
-// sixteen bytes, TINY, are read element by element.)  Loads of a block of 128 k, all at this lane's places:
-template <bool W8, bool TINY>
+// sixteen bytes, TINY, are read element by element.)
+template <bool W8, bool TINY, bool SHARED>
 struct Chunks {
   static constexpr int EB = W8 ? 1 : 2, EPL = 16 / EB, LOADS = W8 ? 2 : 4;   // bytes, elements a load, loads of weights
-  __device__ __forceinline__ static int first(int c, int quarter) { return c * (4 * EPL) + quarter * EPL; }   // of load c
   __device__ __forceinline__ static int from(int k, int count) { return min(k, count - EPL); }
-  __device__ __forceinline__ static void weights(u32x4 (&v)[LOADS], const VECOPS_GLOBAL char* row, int k0, int quarter, int count) {
-#pragma unroll
-    for (int c = 0; c < LOADS; ++c) {
-      const int k = k0 + first(c, quarter);
-      if constexpr (TINY) v[c] = load_16_until<EB>(row, k, count);
-      else v[c] = load_16(row + static_cast<int64_t>(from(k, count)) * EB);
+  // which of sixteen rows load c of this lane is of
+  __device__ __forceinline__ static int row(int c, int lane) { return (lane & 15 & ~(LOADS - 1)) + c; }
+  __device__ __forceinline__ static u32x4 weight(const VECOPS_GLOBAL char* row, int k0, int lane, int count) {
+    const int k = k0 + (lane >> 4) * 32 + (lane & (LOADS - 1)) * EPL;
+    if constexpr (TINY) return load_16_until<EB>(row, k, count);
+    else return load_16(row + static_cast<int64_t>(from(k, count)) * EB);
+  }
+  // load c of lane l becomes load l % COUNT of lane c of its group
+  template <int COUNT>
+  __device__ __forceinline__ static void exchange(u32x4 (&v)[COUNT], int lane) {
+    swap<0xb1>(v[0], v[1], lane & 1);
+    if constexpr (COUNT == 4) {
+      swap<0xb1>(v[2], v[3], lane & 1);
+      swap<0x4e>(v[0], v[2], lane & 2);
+      swap<0x4e>(v[1], v[3], lane & 2);
     }
   }
-  // four chunks of eight 16-bit elements, in the order of the weights
-  __device__ __forceinline__ static void activations(u32x4 (&v)[4], const VECOPS_GLOBAL char* row, int k0, int quarter, int count, bool there) {
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int in = W8 ? (c & 1) * 8 : 0, k = k0 + first(W8 ? c >> 1 : c, quarter);
-      v[c] = u32x4{0u, 0u, 0u, 0u};
-      if (there) {
-        if constexpr (TINY) v[c] = load_16_until<2>(row, k + in, count);
-        else v[c] = load_16(row + static_cast<int64_t>(from(k, count) + in) * 2);
-      }
+  // four chunks of eight 16-bit elements: of a token each as a load of weights is of a row each (SHARED), or of this lane's token
+  __device__ __forceinline__ static int token(int c, int lane) { return SHARED ? (lane & 12) + c : lane & 15; }
+  __device__ __forceinline__ static u32x4 activation(const VECOPS_GLOBAL char* row, int k0, int c, int lane, int count, bool there) {
+    const int chunk = SHARED ? lane & 3 : c, in = W8 ? (chunk & 1) * 8 : 0, k = k0 + (lane >> 4) * 32 + chunk * 8 - in;
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (there) {
+      if constexpr (TINY) v = load_16_until<2>(row, k + in, count);
+      else v = load_16(row + static_cast<int64_t>(from(k, count) + in) * 2);
     }
+    return v;
+  }
+  __device__ __forceinline__ static void exchange_activations(u32x4 (&v)[4], int lane) {
+    if constexpr (SHARED) exchange(v, lane);
   }
   // at the block that `count` lies in
   __device__ __forceinline__ static void clear(u32x4 (&v)[4], int k0, int quarter, int count) {
     if constexpr (!TINY) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const int k = k0 + first(W8 ? c >> 1 : c, quarter);
-        v[c] = cleared(v[c], k - from(k, count) - (W8 ? (c & 1) * 8 : 0));
+        const int in = W8 ? (c & 1) * 8 : 0, k = k0 + quarter * 32 + c * 8 - in;
+        v[c] = cleared(v[c], k - from(k, count) - in);
       }
     }
   }
   __device__ __forceinline__ static void clear_weights(u32x4 (&v)[LOADS], int k0, int quarter, int count) {
     if constexpr (!TINY && !W8) clear(v, k0, quarter, count);
+  }
+
+ private:
+  // between lanes that CONTROL pairs: the first one's `b` and the second one's `a` change places
+  template <int CONTROL>
+  __device__ __forceinline__ static void swap(u32x4& a, u32x4& b, bool second) {
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+    for (int d = 0; d < 4; ++d) {
+      const uint32_t from_b = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0u, b[d], CONTROL, 0xf, 0xf, true));
+      const uint32_t from_a = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0u, a[d], CONTROL, 0xf, 0xf, true));
+      a[d] = second ? from_b : a[d];
+      b[d] = second ? b[d] : from_a;
+    }
+#endif
   }
 };
 
@@ -315,7 +348,9 @@ constexpr int kUpWaves = 4;
 // CHOOSES: the experts are not chosen yet, and every workgroup chooses them, a wavefront a token; the first one writes the choice.
 template <bool F16, bool W8, int MT, bool TINY, bool CHOOSES>
 __global__ __launch_bounds__(64 * kUpWaves, MT == 1 && !W8 ? 3 : MT == 4 ? 1 : 2) void moe_up_kernel(const MoeExpertsParams p, const MoeRouteParams route, int by_place) {
-  using C = Chunks<W8, TINY>;
+  // (Exchanged activations cost gate and up more than they bring between two columns and the registers of e4m3: 64 tokens, 2 of
+  // 8 of 4096 x 4096: 152 us for 143; the others gain: 100 tokens, 4 of 30 of 1501 x 2411 in f16: 247 us to 219.)
+  using C = Chunks<W8, TINY, !(W8 && MT == 2)>;
   constexpr int EB = C::EB, LOADS = C::LOADS, DEPTH = TINY ? 1 : W8 && MT == 1 ? 4 : W8 && MT == 2 ? 3 : 2, THREADS = 64 * kUpWaves;
   __shared__ f32x4 meet[2][kUpWaves][2][MT][64];
   __shared__ int ids[kMoeMostTokens * kMoeMostChoices];
@@ -385,26 +420,34 @@ __global__ __launch_bounds__(64 * kUpWaves, MT == 1 && !W8 ? 3 : MT == 4 ? 1 : 2
   const int tile_count = (tiles - static_cast<int>(blockIdx.x) + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x);
   const int steps = mine * tile_count;
   for (int base = 0; base < rows; base += 16 * MT) {
-    const VECOPS_GLOBAL char* x[MT];
-    bool there[MT];
+    const VECOPS_GLOBAL char* x[MT][4];
+    bool there[MT][4];
 #pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      const int at = base + j * 16 + col;
-      there[j] = at < rows;
-      x[j] = (const VECOPS_GLOBAL char*)p.x + (places[min(at, rows - 1)] / p.top) * p.ldx * 2;
-    }
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int at = base + j * 16 + C::token(c, lane);
+        there[j][c] = at < rows;
+        x[j][c] = (const VECOPS_GLOBAL char*)p.x + (places[min(at, rows - 1)] / p.top) * p.ldx * 2;
+      }
     u32x4 wv[DEPTH][2][LOADS], xv[DEPTH][MT][4];
     float sv[DEPTH][2][2];
     // where the next loads go: row block, block of k
     int load_tile = blockIdx.x, load_block = wave;
     auto load = [&](auto slot_tag) __attribute__((always_inline)) {
       constexpr int slot = decltype(slot_tag)::value;
-      const int i0 = load_tile * 16, i = min(i0 + col, p.inner - 1), k0 = load_block * 128;
-      const VECOPS_GLOBAL char* w[2] = {w_base + i * p.gate_up_rs * EB, w_base + (static_cast<int64_t>(p.inner) + i) * p.gate_up_rs * EB};
+      const int i0 = load_tile * 16, k0 = load_block * 128;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) C::weights(wv[slot][h], w[h], k0, quarter, p.hidden);
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int j = 0; j < MT; ++j) C::activations(xv[slot][j], x[j], k0, quarter, p.hidden, there[j]);
+        for (int c = 0; c < LOADS; ++c) {
+          const int64_t row = (h ? p.inner : 0) + min(i0 + C::row(c, lane), p.inner - 1);
+          wv[slot][h][c] = C::weight(w_base + row * p.gate_up_rs * EB, k0, lane, p.hidden);
+        }
+#pragma unroll
+      for (int j = 0; j < MT; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) xv[slot][j][c] = C::activation(x[j][c], k0, c, lane, p.hidden, there[j][c]);
       if constexpr (W8) {   // the scales of a lane's first row and of its last one, which may lie in another block of rows
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -465,6 +508,10 @@ __global__ __launch_bounds__(64 * kUpWaves, MT == 1 && !W8 ? 3 : MT == 4 ? 1 : 2
         constexpr int slot = decltype(slot_tag)::value;
         if (s0 + slot < steps) {
           const int i0 = tile * 16 + quarter * 4, k0 = (wave + block * kUpWaves) * 128;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) C::exchange(wv[slot][h], lane);
+#pragma unroll
+          for (int j = 0; j < MT; ++j) C::exchange_activations(xv[slot][j], lane);
           if (k0 + 128 > p.hidden) {
 #pragma unroll
             for (int j = 0; j < MT; ++j) C::clear(xv[slot][j], k0, quarter, p.hidden);
@@ -518,7 +565,7 @@ constexpr int kDownWaves = 8;
 
 template <bool F16, bool W8, int MT, bool TINY>
 __global__ __launch_bounds__(64 * kDownWaves, 2) void moe_down_kernel(const MoeExpertsParams p) {
-  using C = Chunks<W8, TINY>;
+  using C = Chunks<W8, TINY, true>;
   constexpr int EB = C::EB, LOADS = C::LOADS, DEPTH = TINY ? 1 : MT == 1 ? (W8 ? 6 : 4) : MT == 2 ? (W8 ? 4 : 3) : 2;
   constexpr bool SPLIT = F16 && !W8;   // f16 weights against bf16 pairs
   constexpr int THREADS = 64 * kDownWaves, PLACES = kMoeMostTokens * kMoeMostChoices / THREADS, TOKENS = 8 * MT;
@@ -592,11 +639,13 @@ __global__ __launch_bounds__(64 * kDownWaves, 2) void moe_down_kernel(const MoeE
   const int h0 = blockIdx.x * 16;
   const int blocks = (p.inner + 127) / 128;
   const int64_t units = static_cast<int64_t>(count) * blocks;
-  const int64_t row = min(h0 + col, p.hidden - 1);
   const int shares = gridDim.y * kDownWaves, share = blockIdx.y * kDownWaves + wave;
   const int begin = static_cast<int>(units * share / shares), end = static_cast<int>(units * (share + 1) / shares);
   if (begin < end) {
-    const VECOPS_GLOBAL char* w_row = (const VECOPS_GLOBAL char*)p.down + row * p.down_rs * EB;
+    const VECOPS_GLOBAL char* w_row[LOADS];
+#pragma unroll
+    for (int c = 0; c < LOADS; ++c)
+      w_row[c] = (const VECOPS_GLOBAL char*)p.down + static_cast<int64_t>(min(h0 + C::row(c, lane), p.hidden - 1)) * p.down_rs * EB;
     const VECOPS_GLOBAL float* s_row = (const VECOPS_GLOBAL float*)p.down_scales + (h0 >> 7) * p.ds_rs;
     // upper halves for the columns below eight, lower ones for the others
     const VECOPS_GLOBAL char* x_plane = (const VECOPS_GLOBAL char*)p.middle + (col >> 3) * (static_cast<int64_t>(total) * p.inner_pad * 2);
@@ -605,26 +654,30 @@ __global__ __launch_bounds__(64 * kDownWaves, 2) void moe_down_kernel(const MoeE
     // where the next loads go
     int load_segment = begin / blocks, load_block = begin - load_segment * blocks;
     int64_t load_expert = 0;
-    const VECOPS_GLOBAL char* x[MT];
-    bool there[MT];
+    const VECOPS_GLOBAL char* x[MT][4];
+    bool there[MT][4];
     auto aim = [&]() __attribute__((always_inline)) {
       const uint32_t its = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(segment[min(load_segment, count - 1)])));
       const int from = static_cast<int>(its & 0xfffu), rows = static_cast<int>(its >> 12 & 0xffu);
       load_expert = static_cast<int64_t>(its >> 20);
 #pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        const int at = j * 8 + (col & 7);
-        there[j] = at < rows;
-        x[j] = x_plane + static_cast<int64_t>(order[from + min(at, rows - 1)]) * p.inner_pad * 2;
-      }
+      for (int j = 0; j < MT; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int at = j * 8 + (C::token(c, lane) & 7);
+          there[j][c] = at < rows;
+          x[j][c] = x_plane + static_cast<int64_t>(order[from + min(at, rows - 1)]) * p.inner_pad * 2;
+        }
     };
     auto load = [&](auto slot_tag) __attribute__((always_inline)) {
       constexpr int slot = decltype(slot_tag)::value;
-      const VECOPS_GLOBAL char* w = w_row + load_expert * p.down_es * EB;
       const int k0 = load_block * 128;
-      C::weights(wv[slot], w, k0, quarter, p.inner);
 #pragma unroll
-      for (int j = 0; j < MT; ++j) C::activations(xv[slot][j], x[j], k0, quarter, p.inner, there[j]);
+      for (int c = 0; c < LOADS; ++c) wv[slot][c] = C::weight(w_row[c] + load_expert * p.down_es * EB, k0, lane, p.inner);
+#pragma unroll
+      for (int j = 0; j < MT; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) xv[slot][j][c] = C::activation(x[j][c], k0, c, lane, p.inner, there[j][c]);
       if constexpr (W8) sv[slot] = s_row[load_expert * p.ds_es + load_block * p.ds_cs];
       if (++load_block == blocks) {
         load_block = 0;
@@ -673,6 +726,9 @@ __global__ __launch_bounds__(64 * kDownWaves, 2) void moe_down_kernel(const MoeE
       static_for<DEPTH>([&](auto slot_tag) {
         constexpr int slot = decltype(slot_tag)::value;
         if (u0 + slot < end) {
+          C::exchange(wv[slot], lane);
+#pragma unroll
+          for (int j = 0; j < MT; ++j) C::exchange_activations(xv[slot][j], lane);
           if ((block + 1) * 128 > p.inner) {
 #pragma unroll
             for (int j = 0; j < MT; ++j) C::clear(xv[slot][j], block * 128, quarter, p.inner);
