@@ -5,7 +5,7 @@
 #include <algorithm>
 #include <utility>
 
-#include "tile_gemm.h"
+#include "lane_exchange.h"
 
 namespace vecops_hip {
 
@@ -644,10 +644,16 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 4 : 2) void fp8_few_rows_kern
       operand((const VECOPS_GLOBAL char*)(p.a_scales + batch * p.as_bs), ((p.m - 1) * p.as_rs + p.groups) * 4);
   const __amdgpu_buffer_rsrc_t desc_sw =
       operand((const VECOPS_GLOBAL char*)(p.b_scales + batch * p.bs_bs + n0 / kFp8Block * p.bs_rs), static_cast<int64_t>(p.groups) * 4);
-  uint32_t from_w[NT];
+  // Two neighbouring lanes load thirty-two bytes of one row, once of either's, and exchange them: sixteen bytes of a row each
+  // are a look-up in the cache for every lane.
+  uint32_t from_w[NT][2], from_x[2];
 #pragma unroll
-  for (int i = 0; i < NT; ++i) from_w[i] = static_cast<uint32_t>((i * 16 + col) * p.ldb) + quarter * 16;
-  const uint32_t from_x = static_cast<uint32_t>(col * p.lda) + quarter * 16;
+  for (int h = 0; h < 2; ++h) {
+    const int row = (col & 14) + h, k = quarter * 32 + (col & 1) * 16;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) from_w[i][h] = static_cast<uint32_t>((i * 16 + row) * p.ldb) + k;
+    from_x[h] = static_cast<uint32_t>(row * p.lda) + k;
+  }
   const uint32_t from_sx = static_cast<uint32_t>(min(col, p.m - 1) * p.as_rs * 4);
 
   const int whole = p.k / kFp8Block;   // blocks of k without the partial one
@@ -659,8 +665,8 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 4 : 2) void fp8_few_rows_kern
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int i = 0; i < NT; ++i) wv[slot][i][h] = __builtin_amdgcn_raw_buffer_load_b128(desc_w, from_w[i] + 64 * h, k0, 0);
-      xv[slot][h] = __builtin_amdgcn_raw_buffer_load_b128(desc_x, from_x + 64 * h, k0, 0);
+      for (int i = 0; i < NT; ++i) wv[slot][i][h] = __builtin_amdgcn_raw_buffer_load_b128(desc_w, from_w[i][h], k0, 0);
+      xv[slot][h] = __builtin_amdgcn_raw_buffer_load_b128(desc_x, from_x[h], k0, 0);
     }
   };
   f32x4 acc[NT], sx, sw;
@@ -685,14 +691,21 @@ __global__ __launch_bounds__(64 * WAVES, NT == 1 ? 4 : 2) void fp8_few_rows_kern
         const int g = g0 + slot;
         if (g < end) {
           f32x4 part[NT];
+          exchange_lanes<kNextLane>(xv[slot][0], xv[slot][1], lane & 1);
           const Fragment<WIDE> x(fragment_of(xv[slot][0], xv[slot][1]));
 #pragma unroll
+          for (int i = 0; i < NT; ++i) exchange_lanes<kNextLane>(wv[slot][i][0], wv[slot][i][1], lane & 1);
+#pragma unroll
           for (int i = 0; i < NT; ++i) part[i] = Fragment<WIDE>(fragment_of(wv[slot][i][0], wv[slot][i][1])).dot(x);
-          if (g + DEPTH < end) load(u, g + DEPTH);
+          // (In front of the branch below: the compiler has been seen to leave too few wait states between a matrix instruction
+          // and the use of its result where one path between them is longer than the other.)
 #pragma unroll
           for (int i = 0; i < NT; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) acc[i][r] = fmaf(part[i][r], scale[slot], acc[i][r]);
+#pragma unroll
+          for (int i = 0; i < NT; ++i) asm volatile("" : "+v"(acc[i]));   // (held here)
+          if (g + DEPTH < end) load(u, g + DEPTH);
         }
       });
     }
@@ -745,13 +758,13 @@ hipError_t launch_few_rows_as(const Fp8MatmulParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// us, weights past the caches: 16 x 14336 x 4096 in blocks of 64 weight rows, which read the activations a fourth as often,
-// 15.5, of 16 rows 19.2 (4 rows of activations 15.1 and 14.5); 1 x 4096 x 14336 with eight wavefronts a block 13.2, with four
-// 14.9 (1 x 14336 x 4096 16.6 and 14.1, 1 x 4096 x 4096 6.6 and 5.6).
+// us, weights past the caches.  Blocks of 64 weight rows, which read the activations a fourth as often: 16 x 14336 x 4096 13.9,
+// of 16 rows 16.0 (8 rows of activations 13.6 and 13.7, 4 rows 13.5 and 13.3).  Eight wavefronts a block, for a workgroup a
+// compute unit or fewer: 1 x 4096 x 14336 12.9, four 14.4 (16 x 8192 x 8192 16.7 and 15.5, 1 x 4096 x 4096 7.3 and 6.3).
 hipError_t launch_few_rows(const Fp8MatmulParams& p, hipStream_t stream) {
   const auto blocks = [&](int rows) { return (static_cast<int64_t>(p.n) + rows - 1) / rows * p.batch; };
   if (p.m > 8 && blocks(64) >= 160) return launch_few_rows_as<4, 4>(p, stream);
-  if (blocks(16) <= 512 && p.groups >= 64) return launch_few_rows_as<8, 1>(p, stream);
+  if (blocks(16) <= 256 && p.groups >= 64) return launch_few_rows_as<8, 1>(p, stream);
   return launch_few_rows_as<4, 1>(p, stream);
 }
 

@@ -8,7 +8,7 @@
 
 #include <algorithm>
 
-#include "tile_gemm.h"
+#include "lane_exchange.h"
 
 namespace vecops_hip {
 
@@ -288,11 +288,11 @@ struct Chunks {
   // load c of lane l becomes load l % COUNT of lane c of its group
   template <int COUNT>
   __device__ __forceinline__ static void exchange(u32x4 (&v)[COUNT], int lane) {
-    swap<0xb1>(v[0], v[1], lane & 1);
+    exchange_lanes<kNextLane>(v[0], v[1], lane & 1);
     if constexpr (COUNT == 4) {
-      swap<0xb1>(v[2], v[3], lane & 1);
-      swap<0x4e>(v[0], v[2], lane & 2);
-      swap<0x4e>(v[1], v[3], lane & 2);
+      exchange_lanes<kNextLane>(v[2], v[3], lane & 1);
+      exchange_lanes<kNextButOne>(v[0], v[2], lane & 2);
+      exchange_lanes<kNextButOne>(v[1], v[3], lane & 2);
     }
   }
   // four chunks of eight 16-bit elements: of a token each as a load of weights is of a row each (SHARED), or of this lane's token
@@ -321,21 +321,6 @@ struct Chunks {
   }
   __device__ __forceinline__ static void clear_weights(u32x4 (&v)[LOADS], int k0, int quarter, int count) {
     if constexpr (!TINY && !W8) clear(v, k0, quarter, count);
-  }
-
- private:
-  // between lanes that CONTROL pairs: the first one's `b` and the second one's `a` change places
-  template <int CONTROL>
-  __device__ __forceinline__ static void swap(u32x4& a, u32x4& b, bool second) {
-#if defined(__HIP_DEVICE_COMPILE__)
-#pragma unroll
-    for (int d = 0; d < 4; ++d) {
-      const uint32_t from_b = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0u, b[d], CONTROL, 0xf, 0xf, true));
-      const uint32_t from_a = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0u, a[d], CONTROL, 0xf, 0xf, true));
-      a[d] = second ? from_b : a[d];
-      b[d] = second ? b[d] : from_a;
-    }
-#endif
   }
 };
 
