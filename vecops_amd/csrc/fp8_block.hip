@@ -121,12 +121,14 @@ __global__ __launch_bounds__(256) void fp8_quantize_rows_kernel(const Fp8Quantiz
 }
 
 // A scale for each block of 128 x 128: a workgroup a block, which stays in its registers between the maximum and the
-// quotients.  Bound by HBM.
+// quotients.  Bound by HBM.  Workgroups go to the eight dies in turn, each with a cache of its own; with `runs`, of a grid of a
+// multiple of eight every die takes a run of neighbouring blocks, so that the lines that two blocks share meet in one cache.
 template <int KIND>
-__global__ __launch_bounds__(256) void fp8_quantize_tiles_kernel(const Fp8QuantizeParams p, uint32_t row_blocks) {
+__global__ __launch_bounds__(256) void fp8_quantize_tiles_kernel(const Fp8QuantizeParams p, uint32_t row_blocks, bool runs) {
   __shared__ uint32_t meet[4];
-  const uint32_t line = blockIdx.x / static_cast<uint32_t>(p.groups), g = blockIdx.x - line * p.groups;
+  const uint32_t block = runs ? (blockIdx.x & 7u) * (gridDim.x >> 3) + (blockIdx.x >> 3) : blockIdx.x, line = block / static_cast<uint32_t>(p.groups), g = block - line * p.groups;
   const uint32_t batch = line / row_blocks, i = line - batch * row_blocks;
+  if (batch >= static_cast<uint32_t>(p.batch)) return;
   const int k = static_cast<int>(g) * kFp8Block + (threadIdx.x & 15) * 8;
   const bool there = k + 8 <= p.k;
   float v[8][8];
@@ -798,10 +800,13 @@ hipError_t launch_fp8_quantize(const Fp8QuantizeParams& p, int block_rows, hipSt
     else hipLaunchKernelGGL((fp8_quantize_rows_kernel<FP8_REAL_F32>), grid, dim3(256), 0, stream, p, blocks);
   } else {
     const uint32_t row_blocks = static_cast<uint32_t>((p.rows + kFp8Block - 1) / kFp8Block);
-    const dim3 grid(static_cast<uint32_t>(p.batch) * row_blocks * static_cast<uint32_t>(p.groups));
-    if (p.kind == FP8_REAL_BF16) hipLaunchKernelGGL((fp8_quantize_tiles_kernel<FP8_REAL_BF16>), grid, dim3(256), 0, stream, p, row_blocks);
-    else if (p.kind == FP8_REAL_F16) hipLaunchKernelGGL((fp8_quantize_tiles_kernel<FP8_REAL_F16>), grid, dim3(256), 0, stream, p, row_blocks);
-    else hipLaunchKernelGGL((fp8_quantize_tiles_kernel<FP8_REAL_F32>), grid, dim3(256), 0, stream, p, row_blocks);
+    const uint32_t total = static_cast<uint32_t>(p.batch) * row_blocks * static_cast<uint32_t>(p.groups);
+    // Runs of blocks a die where rows are not whole lines: 11000 x 4001 in bf16 45.4 us without, 39.6 with; 8192 x 4096 28.1 and 29.8.
+    const bool runs = (p.x_rs * (p.kind == FP8_REAL_F32 ? 4 : 2) % 128 != 0 || p.q_rs % 128 != 0) && total <= (1u << 24) - 16;
+    const dim3 grid(runs ? (total + 7) / 8 * 8 : total);
+    if (p.kind == FP8_REAL_BF16) hipLaunchKernelGGL((fp8_quantize_tiles_kernel<FP8_REAL_BF16>), grid, dim3(256), 0, stream, p, row_blocks, runs);
+    else if (p.kind == FP8_REAL_F16) hipLaunchKernelGGL((fp8_quantize_tiles_kernel<FP8_REAL_F16>), grid, dim3(256), 0, stream, p, row_blocks, runs);
+    else hipLaunchKernelGGL((fp8_quantize_tiles_kernel<FP8_REAL_F32>), grid, dim3(256), 0, stream, p, row_blocks, runs);
   }
   return hipGetLastError();
 }
