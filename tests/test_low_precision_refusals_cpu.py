@@ -172,3 +172,21 @@ def test_nothing_to_do():
     none = {"x": operand(BF16, 0, 256, data=None), "ids": operand(I32, 0, 2, data=None), "weights": operand(F32, 0, 2, data=None),
             "out": operand(BF16, 0, 256, data=None), "ws": None, "size": 0}
     assert layer(**none) == 0 and experts(**none) == 0
+
+
+def test_tensors_that_are_not_on_a_gpu():
+    """The kernels read through plain addresses: the Python entry points refuse tensors in host memory, or on two devices."""
+    torch = pytest.importorskip("torch")
+    x, q, s = torch.zeros(4, 128), torch.zeros(4, 128).to(torch.float8_e4m3fn), torch.zeros(4, 1)
+    with pytest.raises(ValueError, match="one GPU"):
+        capi.quantize_fp8_block(x, q, s)
+    with pytest.raises(ValueError, match="one GPU"):
+        capi.matmul_fp8_block(q, s, q, torch.zeros(1, 1), torch.zeros(4, 4))
+    ids, weights, experts = torch.zeros((4, 1), dtype=torch.int32), torch.zeros(4, 1), torch.zeros(2, 16, 128)
+    with pytest.raises(ValueError, match="one GPU"):
+        capi.moe_experts(x.bfloat16(), ids, weights, experts.bfloat16(), torch.zeros(2, 128, 8).bfloat16(), x)
+    with pytest.raises(ValueError, match="one GPU"):
+        capi.moe_layer(x.bfloat16(), torch.zeros(2, 128), experts.bfloat16(), torch.zeros(2, 128, 8).bfloat16(), ids, weights, x)
+    with pytest.raises(ValueError, match="bias"):
+        capi.moe_layer(x.bfloat16(), torch.zeros(2, 128), experts.bfloat16(), torch.zeros(2, 128, 8).bfloat16(), ids, weights, x,
+                       bias=torch.zeros(3))
