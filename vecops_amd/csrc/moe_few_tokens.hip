@@ -328,15 +328,16 @@ constexpr int kUpWaves = 4;
 
 // gate and up.  A workgroup: one expert, the tokens that name it (16 MT at a time), every gridDim.x-th block of sixteen gate rows
 // and their up rows.  Its wavefronts take the blocks of 128 of the hidden axis in turn, the loads of DEPTH of them under way,
-// across the ends of row blocks; their sums meet in LDS.
+// across the ends of row blocks; their sums meet in LDS.  (Two workgroups a compute unit with one block under way each do better
+// than one with two: 128 tokens, 2 of 8 of 4096 x 4096 in bf16 225 us and 286.)
 // (Loads return in order: activations asked for when they are needed would wait for the weights asked for ahead of them.)
 // CHOOSES: the experts are not chosen yet, and every workgroup chooses them, a wavefront a token; the first one writes the choice.
 template <bool F16, bool W8, int MT, bool TINY, bool CHOOSES>
-__global__ __launch_bounds__(64 * kUpWaves, MT == 1 && !W8 ? 3 : MT == 4 ? 1 : 2) void moe_up_kernel(const MoeExpertsParams p, const MoeRouteParams route, int by_place) {
+__global__ __launch_bounds__(64 * kUpWaves, MT == 4 || (MT == 1 && W8) ? 2 : 3) void moe_up_kernel(const MoeExpertsParams p, const MoeRouteParams route, int by_place) {
   // (Exchanged activations cost gate and up more than they bring between two columns and the registers of e4m3: 64 tokens, 2 of
   // 8 of 4096 x 4096: 152 us for 143; the others gain: 100 tokens, 4 of 30 of 1501 x 2411 in f16: 247 us to 219.)
   using C = Chunks<W8, TINY, !(W8 && MT == 2)>;
-  constexpr int EB = C::EB, LOADS = C::LOADS, DEPTH = TINY ? 1 : W8 && MT == 1 ? 4 : W8 && MT == 2 ? 3 : 2, THREADS = 64 * kUpWaves;
+  constexpr int EB = C::EB, LOADS = C::LOADS, DEPTH = TINY ? 1 : W8 && MT == 1 ? 4 : MT == 1 ? 2 : 1, THREADS = 64 * kUpWaves;
   __shared__ f32x4 meet[2][kUpWaves][2][MT][64];
   __shared__ int ids[kMoeMostTokens * kMoeMostChoices];
   __shared__ int places[kMoeMostTokens];
@@ -551,7 +552,7 @@ constexpr int kDownWaves = 8;
 template <bool F16, bool W8, int MT, bool TINY>
 __global__ __launch_bounds__(64 * kDownWaves, 2) void moe_down_kernel(const MoeExpertsParams p) {
   using C = Chunks<W8, TINY, true>;
-  constexpr int EB = C::EB, LOADS = C::LOADS, DEPTH = TINY ? 1 : MT == 1 ? (W8 ? 6 : 4) : MT == 2 ? (W8 ? 4 : 3) : 2;
+  constexpr int EB = C::EB, LOADS = C::LOADS, DEPTH = TINY ? 1 : MT == 1 ? (W8 ? 6 : 4) : MT == 2 ? 2 : 1;
   constexpr bool SPLIT = F16 && !W8;   // f16 weights against bf16 pairs
   constexpr int THREADS = 64 * kDownWaves, PLACES = kMoeMostTokens * kMoeMostChoices / THREADS, TOKENS = 8 * MT;
   constexpr int SEGMENTS = kMoeMostExperts + kMoeMostTokens * kMoeMostChoices / TOKENS;
@@ -828,16 +829,17 @@ hipError_t launch_experts(const MoeExpertsParams& p, const MoeRouteParams* route
   return hipGetLastError();
 }
 
-// Columns of sixteen (in down eight) tokens that a pass over an expert's weights serves: as many as an expert has on average, since
-// more take registers from the loads ahead and fewer read the weights again.  Measured with one, two and four (us): 4 tokens an
-// expert (128 of 2048 x 768, e4m3) 147, 151, 208; 8 (8 of 4096 x 4096, bf16) 178, 169, 179; 12 (64 of 2048 x 1408, bf16) 352, 291,
-// 311; 32 (8 of 4096 x 4096, bf16) 472, 347, 304.
+// Columns of sixteen (in down eight) tokens that a pass over an expert's weights serves, by the tokens an expert has on average: more
+// take registers from the loads ahead, fewer read the weights again.  Measured with one, two and four (us): 6 (64 tokens, 6 of 64
+// of 2048 x 1408, bf16) 217, 220, 245; 8 (128 tokens, 8 of 128 of 2048 x 768) e4m3 169, 179, 248, bf16 251, 244, 270; 10 (40
+// tokens, 2 of 8 of 4096 x 4096, bf16) 170, 161, 176; 25 (128 tokens, 2 of 10 of 2048 x 4096, e4m3) 140, 123, 133; 32 (128
+// tokens, 2 of 8 of 4096 x 4096, bf16) 356, 241, 224.
 template <bool F16, bool W8>
 hipError_t launch_experts_for(const MoeExpertsParams& p, const MoeRouteParams* route, hipStream_t stream) {
   const int mean = p.experts > 0 ? p.tokens * p.top / p.experts : 0;
   if (is_tiny(p)) return launch_experts<F16, W8, 1, true>(p, route, stream);
-  if (mean <= 4 || p.tokens <= 8) return launch_experts<F16, W8, 1>(p, route, stream);
-  if (mean <= 24 || p.tokens <= 16) return launch_experts<F16, W8, 2>(p, route, stream);
+  if (mean <= 8 || p.tokens <= 8) return launch_experts<F16, W8, 1>(p, route, stream);
+  if (mean <= 28 || p.tokens <= 32) return launch_experts<F16, W8, 2>(p, route, stream);
   return launch_experts<F16, W8, 4>(p, route, stream);
 }
 
