@@ -274,7 +274,7 @@ __device__ __forceinline__ bool named_before(const int* ids, int place, int choi
 // are the activations that go with them; what another lane or load has is cleared when they are used, in both, since either
 // may hold an infinity (an e4m3 has none, and its NaN reaches the result from the other load as well).  (Rows of less than
 // sixteen bytes, TINY, are read element by element.)
-template <bool W8, bool TINY, bool SHARED>
+template <bool W8, bool TINY>
 struct Chunks {
   static constexpr int EB = W8 ? 1 : 2, EPL = 16 / EB, LOADS = W8 ? 2 : 4;   // bytes, elements a load, loads of weights
   __device__ __forceinline__ static int from(int k, int count) { return min(k, count - EPL); }
@@ -295,19 +295,16 @@ struct Chunks {
       exchange_lanes<kNextButOne>(v[1], v[3], lane & 2);
     }
   }
-  // four chunks of eight 16-bit elements: of a token each as a load of weights is of a row each (SHARED), or of this lane's token
-  __device__ __forceinline__ static int token(int c, int lane) { return SHARED ? (lane & 12) + c : lane & 15; }
-  __device__ __forceinline__ static u32x4 activation(const VECOPS_GLOBAL char* row, int k0, int c, int lane, int count, bool there) {
-    const int chunk = SHARED ? lane & 3 : c, in = W8 ? (chunk & 1) * 8 : 0, k = k0 + (lane >> 4) * 32 + chunk * 8 - in;
+  // four chunks of eight 16-bit elements, of a token each as a load of weights is of a row each
+  __device__ __forceinline__ static int token(int c, int lane) { return (lane & 12) + c; }
+  __device__ __forceinline__ static u32x4 activation(const VECOPS_GLOBAL char* row, int k0, int lane, int count, bool there) {
+    const int chunk = lane & 3, in = W8 ? (chunk & 1) * 8 : 0, k = k0 + (lane >> 4) * 32 + chunk * 8 - in;
     u32x4 v = {0u, 0u, 0u, 0u};
     if (there) {
       if constexpr (TINY) v = load_16_until<2>(row, k + in, count);
       else v = load_16(row + static_cast<int64_t>(from(k, count) + in) * 2);
     }
     return v;
-  }
-  __device__ __forceinline__ static void exchange_activations(u32x4 (&v)[4], int lane) {
-    if constexpr (SHARED) exchange(v, lane);
   }
   // at the block that `count` lies in
   __device__ __forceinline__ static void clear(u32x4 (&v)[4], int k0, int quarter, int count) {
@@ -328,16 +325,15 @@ constexpr int kUpWaves = 4;
 
 // gate and up.  A workgroup: one expert, the tokens that name it (16 MT at a time), every gridDim.x-th block of sixteen gate rows
 // and their up rows.  Its wavefronts take the blocks of 128 of the hidden axis in turn, the loads of DEPTH of them under way,
-// across the ends of row blocks; their sums meet in LDS.  (Two workgroups a compute unit with one block under way each do better
-// than one with two: 128 tokens, 2 of 8 of 4096 x 4096 in bf16 225 us and 286.)
+// across the ends of row blocks; their sums meet in LDS.  (More workgroups a compute unit do better than more blocks
+// under way in each: 128 tokens, 2 of 8 of 4096 x 4096 in bf16, two with one block 225 us, one with two 286; 64 tokens, 8 of 128
+// of 2048 x 768 in e4m3, three with two blocks 138, two with four 144.)
 // (Loads return in order: activations asked for when they are needed would wait for the weights asked for ahead of them.)
 // CHOOSES: the experts are not chosen yet, and every workgroup chooses them, a wavefront a token; the first one writes the choice.
 template <bool F16, bool W8, int MT, bool TINY, bool CHOOSES>
-__global__ __launch_bounds__(64 * kUpWaves, MT == 4 || (MT == 1 && W8) ? 2 : 3) void moe_up_kernel(const MoeExpertsParams p, const MoeRouteParams route, int by_place) {
-  // (Exchanged activations cost gate and up more than they bring between two columns and the registers of e4m3: 64 tokens, 2 of
-  // 8 of 4096 x 4096: 152 us for 143; the others gain: 100 tokens, 4 of 30 of 1501 x 2411 in f16: 247 us to 219.)
-  using C = Chunks<W8, TINY, !(W8 && MT == 2)>;
-  constexpr int EB = C::EB, LOADS = C::LOADS, DEPTH = TINY ? 1 : W8 && MT == 1 ? 4 : MT == 1 ? 2 : 1, THREADS = 64 * kUpWaves;
+__global__ __launch_bounds__(64 * kUpWaves, MT == 4 ? 2 : 3) void moe_up_kernel(const MoeExpertsParams p, const MoeRouteParams route, int by_place) {
+  using C = Chunks<W8, TINY>;
+  constexpr int EB = C::EB, LOADS = C::LOADS, DEPTH = !TINY && MT == 1 ? 2 : 1, THREADS = 64 * kUpWaves;
   __shared__ f32x4 meet[2][kUpWaves][2][MT][64];
   __shared__ int ids[kMoeMostTokens * kMoeMostChoices];
   __shared__ int places[kMoeMostTokens];
@@ -433,7 +429,7 @@ __global__ __launch_bounds__(64 * kUpWaves, MT == 4 || (MT == 1 && W8) ? 2 : 3) 
 #pragma unroll
       for (int j = 0; j < MT; ++j)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) xv[slot][j][c] = C::activation(x[j][c], k0, c, lane, p.hidden, there[j][c]);
+        for (int c = 0; c < 4; ++c) xv[slot][j][c] = C::activation(x[j][c], k0, lane, p.hidden, there[j][c]);
       if constexpr (W8) {   // the scales of a lane's first row and of its last one, which may lie in another block of rows
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -497,7 +493,7 @@ __global__ __launch_bounds__(64 * kUpWaves, MT == 4 || (MT == 1 && W8) ? 2 : 3) 
 #pragma unroll
           for (int h = 0; h < 2; ++h) C::exchange(wv[slot][h], lane);
 #pragma unroll
-          for (int j = 0; j < MT; ++j) C::exchange_activations(xv[slot][j], lane);
+          for (int j = 0; j < MT; ++j) C::exchange(xv[slot][j], lane);
           if (k0 + 128 > p.hidden) {
 #pragma unroll
             for (int j = 0; j < MT; ++j) C::clear(xv[slot][j], k0, quarter, p.hidden);
@@ -551,7 +547,7 @@ constexpr int kDownWaves = 8;
 
 template <bool F16, bool W8, int MT, bool TINY>
 __global__ __launch_bounds__(64 * kDownWaves, 2) void moe_down_kernel(const MoeExpertsParams p) {
-  using C = Chunks<W8, TINY, true>;
+  using C = Chunks<W8, TINY>;
   constexpr int EB = C::EB, LOADS = C::LOADS, DEPTH = TINY ? 1 : MT == 1 ? (W8 ? 6 : 4) : MT == 2 ? 2 : 1;
   constexpr bool SPLIT = F16 && !W8;   // f16 weights against bf16 pairs
   constexpr int THREADS = 64 * kDownWaves, PLACES = kMoeMostTokens * kMoeMostChoices / THREADS, TOKENS = 8 * MT;
@@ -663,7 +659,7 @@ __global__ __launch_bounds__(64 * kDownWaves, 2) void moe_down_kernel(const MoeE
 #pragma unroll
       for (int j = 0; j < MT; ++j)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) xv[slot][j][c] = C::activation(x[j][c], k0, c, lane, p.inner, there[j][c]);
+        for (int c = 0; c < 4; ++c) xv[slot][j][c] = C::activation(x[j][c], k0, lane, p.inner, there[j][c]);
       if constexpr (W8) sv[slot] = s_row[load_expert * p.ds_es + load_block * p.ds_cs];
       if (++load_block == blocks) {
         load_block = 0;
@@ -714,7 +710,7 @@ __global__ __launch_bounds__(64 * kDownWaves, 2) void moe_down_kernel(const MoeE
         if (u0 + slot < end) {
           C::exchange(wv[slot], lane);
 #pragma unroll
-          for (int j = 0; j < MT; ++j) C::exchange_activations(xv[slot][j], lane);
+          for (int j = 0; j < MT; ++j) C::exchange(xv[slot][j], lane);
           if ((block + 1) * 128 > p.inner) {
 #pragma unroll
             for (int j = 0; j < MT; ++j) C::clear(xv[slot][j], block * 128, quarter, p.inner);
