@@ -196,7 +196,7 @@ __global__ __launch_bounds__(256) void fp8_rows_kernel(const uint8_t* in, int64_
 //
 // Two ways to an inner sum.  v_mfma_f32_16x16x128_f8f6f4 takes the bytes as they are, at 2.8 times the rate of bf16 (random
 // bytes, nothing but the instruction: 3200 TFLOP/s, bf16 1145).  It aligns each eight products that lie together along k to
-// the largest of them and drops what is 2^-13 of its power of two or less (2^16 + 2^2 gave 2^16, 2^16 + 2^3 was exact; across
+// the largest of them and drops what is below 2^-13 of its power of two (2^16 + 2^2 gave 2^16, 2^16 + 2^3 was exact; across
 // eights nothing is lost): on normally distributed operands results are 1.4e-5 off, which a 16-bit result does not show (its
 // own rounding: bf16 1.7e-3, f16 2.1e-4).  For fp32 results the bytes are widened to bf16, exactly, and the bf16
 // instruction sums exact products in fp32.
