@@ -558,8 +558,9 @@ VECOPS_HIP_EXPORT int32_t vecops_hip_matmul_fp8_block(const VecopsHipOperand* a,
  * block_rows 128; null otherwise); out [T,H] of x's type or f32.  T <= 128, choices <= 16, E <= 512.  Rows of x, gate_up and
  * down are contiguous, at any alignment; other strides are free.  An id outside 0..E-1 names no expert and adds nothing (an
  * expert on another device); an expert that a token names twice counts with both weights; a token that names none gets zeros.
- * The weights of a named expert are read once for every 8 to 64 tokens that name it.  Sums and the inner values are held to fp32 (the inner values to 2^-17, as a
- * pair of bf16), the result is rounded once; it does not depend on timing.  What is not finite stays not finite.
+ * The weights of a named expert are read once for every 8 to 64 tokens that name it.  Sums and the inner values are held to
+ * fp32 (the inner values to 2^-17, as a pair of bf16), the result is rounded once; it does not depend on timing.  What is not
+ * finite stays not finite, and an infinite weight gives the formula's infinity.
  * workspace: vecops_hip_moe_experts_workspace bytes, 16-byte aligned.
  */
 VECOPS_HIP_EXPORT uint64_t vecops_hip_moe_experts_workspace(const VecopsHipOperand* ids, const VecopsHipOperand* down);
