@@ -542,7 +542,7 @@ __device__ __forceinline__ void split_f16(const u32x4& v, u32x4& hi, u32x4& lo) 
 // block of 128 inner) pairs evenly among them, in order, the loads of DEPTH pairs under way across the ends of segments.  Of a
 // matrix instruction's sixteen columns eight take the upper halves of eight tokens' inner values and eight the lower ones,
 // which meet when a wavefront leaves a segment and adds its columns to its own sums of the tokens in LDS.  The wavefronts' sums
-// are added at the end, and the shares' by the workgroup that comes last, in order: no sum depends on timing.
+// are added at the end, and the shares' by the workgroup that comes last, in order: no sum depends on which one that is.
 constexpr int kDownWaves = 8;
 
 template <bool F16, bool W8, int MT, bool TINY>
@@ -762,6 +762,10 @@ __global__ __launch_bounds__(64 * kDownWaves, 2) void moe_down_kernel(const MoeE
                             __HIP_MEMORY_SCOPE_AGENT);
   }
   if (!alone) {
+    // Each wavefront's numbers have to be in memory before the counter says so: neither the barrier nor the release below, which
+    // is one wavefront's, waits for another one's stores.  (A release by every wavefront would, but it writes the
+    // die's cache back each time.)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     if (tid == 0) last = __hip_atomic_fetch_add(&p.arrived[blockIdx.x], 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == static_cast<int>(gridDim.y) - 1;
     __syncthreads();
