@@ -539,7 +539,9 @@ VECOPS_HIP_EXPORT int32_t vecops_hip_quantize_fp8_block(const VecopsHipOperand* 
  * bf16 gives 1.7e-3 and to f16 2.1e-4.  K == 0 writes zeros.
  * workspace: vecops_hip_matmul_fp8_block_workspace bytes, 16-byte aligned.  It holds the sums of parts of K, where few tiles
  * would leave the chip short of work (they are added in a fixed order), and copies of operands whose k are not contiguous
- * (rows may lie at any alignment), of scales where those of a row are not, and of operands with K < 16.
+ * (rows may lie at any alignment), of scales where those of a row are not, of operands with K < 16 and of rows too far apart.
+ * The rows of a tile - up to 256 of either operand, with M <= 16 sixteen of a and sixteen or 64 of b - are reached by offsets
+ * below 2 GiB: a K so long that even a copy does not fit there (from 2^23 on with many rows and columns) is refused.
  */
 VECOPS_HIP_EXPORT uint64_t vecops_hip_matmul_fp8_block_workspace(const VecopsHipOperand* a, const VecopsHipOperand* a_scales,
                                                                  const VecopsHipOperand* b, const VecopsHipOperand* b_scales,

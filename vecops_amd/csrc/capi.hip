@@ -8,6 +8,7 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
+#include <utility>
 
 #include "fp8_block.h"
 #include "gemm_f64.h"
@@ -2711,13 +2712,14 @@ int real_kind(uint32_t dtype) {
 
 int64_t fp8_blocks(int64_t extent) { return (extent + kFp8Block - 1) / kFp8Block; }
 
-// What the product reads an operand through: its own rows where their k are contiguous (any alignment) and at least sixteen
-// (the kernels load no less), else a copy of them in the workspace, padded to sixteen with zeros.  (Offsets inside a tile of
-// 256 rows are 32 bits wide.)
-bool fp8_rows_ok(const View& v) { return v.cs == 1 && v.cols >= 16 && v.rs >= 0 && v.rs * 256 + v.cols + 128 < (int64_t{1} << 31); }
+// What the product reads an operand through: its own rows where their k are contiguous (any alignment), at least sixteen
+// (the kernels load no less) and near enough to one another for the offsets of the plan's kernel, `rows` of them, else a copy of
+// them in the workspace, padded to sixteen with zeros.
+bool fp8_rows_reached(int64_t rows, int64_t ld, int64_t k) { return ld <= INT32_MAX && (rows - 1) * ld + k + 128 < (int64_t{1} << 31); }
+bool fp8_rows_ok(const View& v, int64_t rows) { return v.cs == 1 && v.cols >= 16 && v.rs >= 0 && fp8_rows_reached(rows, v.rs, v.cols); }
 int64_t fp8_row_bytes(const View& v) { return (v.cols + 15) / 16 * 16; }
-uint64_t fp8_copy_bytes(const View& v) {
-  if (v.batch == 0 || v.rows == 0 || v.cols == 0 || fp8_rows_ok(v)) return 0;
+uint64_t fp8_copy_bytes(const View& v, int64_t rows) {
+  if (v.batch == 0 || v.rows == 0 || v.cols == 0 || fp8_rows_ok(v, rows)) return 0;
   return round_up_256(static_cast<uint64_t>(v.bs == 0 ? 1 : v.batch) * static_cast<uint64_t>(v.rows) * static_cast<uint64_t>(fp8_row_bytes(v)));
 }
 
@@ -2733,6 +2735,7 @@ uint64_t fp8_partial_bytes(const View& a, const View& b, const Fp8Plan& plan) {
 
 struct Fp8Product {
   View a, sa, b, sb, c;
+  Fp8Plan plan;
 };
 
 int32_t describe_fp8(const VecopsHipOperand* a, const VecopsHipOperand* a_scales, const VecopsHipOperand* b,
@@ -2764,6 +2767,11 @@ int32_t describe_fp8(const VecopsHipOperand* a, const VecopsHipOperand* a_scales
       return fail(ST_NOT_APPLICABLE, "matmul_fp8_block: row strides of the scales must lie in 0 .. 2^20");
   if (batch * m * fp8_blocks(k) >= (int64_t{1} << 32) || batch * fp8_blocks(n) * fp8_blocks(k) >= (int64_t{1} << 32))
     return fail(ST_INVALID, "matmul_fp8_block: extent too large");
+  pr->plan = fp8_plan(m, n, k, batch, real_kind(pr->c.dtype));
+  // a copy brings rows together, but no nearer than their length
+  for (const auto& [v, rows] : {std::make_pair(&pr->a, pr->plan.rows_a), std::make_pair(&pr->b, pr->plan.rows_b)})
+    if (m > 0 && n > 0 && k > 0 && !fp8_rows_ok(*v, rows) && !fp8_rows_reached(rows, fp8_row_bytes(*v), k))
+      return fail(ST_NOT_APPLICABLE, "matmul_fp8_block: K=%lld is too long: %d rows must lie within 2 GiB", (long long)k, rows);
   return ST_OK;
 }
 
@@ -2807,8 +2815,9 @@ uint64_t vecops_hip_matmul_fp8_block_workspace(const VecopsHipOperand* a, const 
   View va, vsa, vb, vsb, vc;
   if (!normalise(a, &va) || !normalise(a_scales, &vsa) || !normalise(b, &vb) || !normalise(b_scales, &vsb) || !normalise(c, &vc)) return 0;
   if (va.batch == 0 || va.rows == 0 || vb.rows == 0) return 0;
-  return fp8_copy_bytes(va) + fp8_copy_bytes(vb) + fp8_scale_copy_bytes(vsa) + fp8_scale_copy_bytes(vsb) +
-         fp8_partial_bytes(va, vb, fp8_plan(va.rows, vb.rows, va.cols, va.batch, real_kind(vc.dtype)));
+  const Fp8Plan plan = fp8_plan(va.rows, vb.rows, va.cols, va.batch, real_kind(vc.dtype));
+  return fp8_copy_bytes(va, plan.rows_a) + fp8_copy_bytes(vb, plan.rows_b) + fp8_scale_copy_bytes(vsa) + fp8_scale_copy_bytes(vsb) +
+         fp8_partial_bytes(va, vb, plan);
 }
 
 int32_t vecops_hip_matmul_fp8_block(const VecopsHipOperand* a, const VecopsHipOperand* a_scales, const VecopsHipOperand* b,
@@ -2820,15 +2829,15 @@ int32_t vecops_hip_matmul_fp8_block(const VecopsHipOperand* a, const VecopsHipOp
   if (pr.a.batch == 0 || pr.a.rows == 0 || pr.b.rows == 0) return ST_OK;
   if (pr.c.data == nullptr || (pr.a.cols > 0 && (pr.a.data == nullptr || pr.b.data == nullptr || pr.sa.data == nullptr || pr.sb.data == nullptr)))
     return fail(ST_INVALID, "matmul_fp8_block: null operand");
-  const Fp8Plan plan = fp8_plan(pr.a.rows, pr.b.rows, pr.a.cols, pr.a.batch, real_kind(pr.c.dtype));
-  const uint64_t need = fp8_copy_bytes(pr.a) + fp8_copy_bytes(pr.b) + fp8_scale_copy_bytes(pr.sa) + fp8_scale_copy_bytes(pr.sb) +
+  const Fp8Plan& plan = pr.plan;
+  const uint64_t need = fp8_copy_bytes(pr.a, plan.rows_a) + fp8_copy_bytes(pr.b, plan.rows_b) + fp8_scale_copy_bytes(pr.sa) + fp8_scale_copy_bytes(pr.sb) +
                         fp8_partial_bytes(pr.a, pr.b, plan);
   if (need > 0 && (workspace == nullptr || workspace_size < need || !aligned16(workspace)))
     return fail(ST_INVALID, "matmul_fp8_block: needs a 16-byte aligned workspace of %llu bytes", (unsigned long long)need);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   uint8_t* room = static_cast<uint8_t*>(workspace);
   for (View* v : {&pr.a, &pr.b}) {
-    const uint64_t bytes = fp8_copy_bytes(*v);
+    const uint64_t bytes = fp8_copy_bytes(*v, v == &pr.a ? plan.rows_a : plan.rows_b);
     if (bytes == 0) continue;
     const int64_t ld = fp8_row_bytes(*v), batches = v->bs == 0 ? 1 : v->batch;
     if (((v->rows + 63) / 64) * ((v->cols + 63) / 64) >= (1 << 24)) return fail(ST_INVALID, "matmul_fp8_block: extent too large");

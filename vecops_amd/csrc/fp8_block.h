@@ -57,6 +57,9 @@ enum Fp8Kind : int { FP8_FEW_ROWS = 0, FP8_TILE_64, FP8_TILE_128X64, FP8_TILE_12
 struct Fp8Plan {
   int kind;
   int splits;  // shares of K; more than one need `partial`
+  // Rows of a and of b that a workgroup reaches from its first one, by offsets of 32 bits whose upper half means nothing there:
+  // (rows - 1) * ld + k + 128 has to stay below 2^31.
+  int rows_a, rows_b;
 };
 Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t k, int64_t batch, int out_kind);
 hipError_t launch_fp8_matmul(const Fp8MatmulParams& p, int kind, hipStream_t stream);

@@ -763,10 +763,11 @@ hipError_t launch_few_rows_as(const Fp8MatmulParams& p, hipStream_t stream) {
 // us, weights past the caches.  Blocks of 64 weight rows, which read the activations a fourth as often: 16 x 14336 x 4096 13.9,
 // of 16 rows 16.0 (8 rows of activations 13.6 and 13.7, 4 rows 13.5 and 13.3).  Eight wavefronts a block, for a workgroup a
 // compute unit or fewer: 1 x 4096 x 14336 12.9, four 14.4 (16 x 8192 x 8192 16.7 and 15.5, 1 x 4096 x 4096 7.3 and 6.3).
+int few_rows_weights(int64_t m, int64_t n, int64_t batch) { return m > 8 && (n + 63) / 64 * batch >= 160 ? 64 : 16; }
+
 hipError_t launch_few_rows(const Fp8MatmulParams& p, hipStream_t stream) {
-  const auto blocks = [&](int rows) { return (static_cast<int64_t>(p.n) + rows - 1) / rows * p.batch; };
-  if (p.m > 8 && blocks(64) >= 160) return launch_few_rows_as<4, 4>(p, stream);
-  if (blocks(16) <= 256 && p.groups >= 64) return launch_few_rows_as<8, 1>(p, stream);
+  if (few_rows_weights(p.m, p.n, p.batch) == 64) return launch_few_rows_as<4, 4>(p, stream);
+  if ((static_cast<int64_t>(p.n) + 15) / 16 * p.batch <= 256 && p.groups >= 64) return launch_few_rows_as<8, 1>(p, stream);
   return launch_few_rows_as<4, 1>(p, stream);
 }
 
@@ -833,8 +834,8 @@ hipError_t launch_fp8_scales(const float* in, int64_t bs, int64_t rs, int64_t gs
 //   time = start + rounds * (tile start + blocks of k * time a block) + join,  at least the operands' bytes at 6.7 TB/s
 // Tiles of which two share a compute unit take `alone` a block with at most one on each, `paired` else.
 Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t k, int64_t batch, int out_kind) {
-  if (m <= 16) return {FP8_FEW_ROWS, 1};
-  if (k == 0) return {FP8_TILE_64, 1};
+  if (m <= 16) return {FP8_FEW_ROWS, 1, 16, few_rows_weights(m, n, batch)};
+  if (k == 0) return {FP8_TILE_64, 1, 64, 64};
   struct Cost {
     int kind, n, m, slots;
     double start[2], alone[2], paired[2];   // us; [1]: fp32 results
@@ -848,7 +849,7 @@ Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t k, int64_t batch, int out_kind) {
   };
   const int wide = out_kind == FP8_REAL_F32;
   const int64_t groups = (k + kFp8Block - 1) / kFp8Block;
-  Fp8Plan best = {FP8_TILE_64, 1};
+  Fp8Plan best = {FP8_TILE_64, 1, 64, 64};
   double least = 1e30;
   for (const Cost& c : kCosts) {
     for (int splits = 1; splits <= 4; splits *= 2) {
@@ -859,7 +860,7 @@ Fp8Plan fp8_plan(int64_t m, int64_t n, int64_t k, int64_t batch, int out_kind) {
       if (rest > 0) us += c.start[wide] + (rest <= 256 ? c.alone[wide] : c.paired[wide]) * blocks;
       us = std::max(us, static_cast<double>(m + n) * k * batch / 6.7e6);
       if (splits > 1) us += 2.5 + 8.0 * splits * m * n * batch / 4.9e6;
-      if (us < least) least = us, best = {c.kind, splits};
+      if (us < least) least = us, best = {c.kind, splits, c.m, c.n};
     }
   }
   return best;
