@@ -733,6 +733,20 @@ def _on_one_device(name: str, *tensors) -> None:
         raise ValueError(f"{name}: tensors must all be on one GPU, got {sorted(map(str, devices))}")
 
 
+def _scratch(need: int, workspace, device, stream):
+    """(tensor, address, bytes): the caller's workspace if it is large enough, else one of torch's allocator.  That one is taken
+    on the stream that the work goes to: it was free there before, and is again only behind the work."""
+    import torch
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        if stream is not None and not hasattr(stream, "device"):
+            stream = torch.cuda.ExternalStream(stream.cuda_stream, device)
+        with torch.cuda.stream(stream):
+            workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    if workspace is None:
+        return None, None, 0
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
 def quantize_fp8_block(x, q, scales, block_rows: int = 1, stream=None):
     """x -> q (``torch.float8_e4m3fn``) and a scale for each block of ``block_rows`` (1 or 128) x 128 elements: ``q * scale``
     stands for x.  Returns (q, scales)."""
@@ -750,21 +764,18 @@ def quantize_fp8_block(x, q, scales, block_rows: int = 1, stream=None):
 
 def matmul_fp8_block(a, a_scales, b, b_scales, c, workspace=None, stream=None):
     """c[..,M,N] = (a * its scales) . (b * its scales)^T for e4m3 operands as ``quantize_fp8_block`` writes them: a scale for
-    each 128 k of a row of a, and for each 128 x 128 block of b.  Returns c."""
+    each 128 k of a row of a, and for each 128 x 128 block of b.  With ``stream`` the work goes there, and so does scratch that
+    no ``workspace`` holds.  Returns c."""
     if stream is None:
         rc = (_calls or native_calls()).matmul_fp8_block(a, a_scales, b, b_scales, c, workspace)
         if rc == 0:
             return c
         if rc > 0:
             _check(rc)
-    import torch
     _on_one_device("matmul_fp8_block", a, a_scales, b, b_scales, c, workspace)
     oa, osa, ob, osb, oc = operand(a), operand(a_scales), operand(b), operand(b_scales), operand(c)
     need = lib().vecops_hip_matmul_fp8_block_workspace(C.byref(oa), C.byref(osa), C.byref(ob), C.byref(osb), C.byref(oc))
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        workspace = torch.empty(need, dtype=torch.uint8, device=c.device)
-    ws_ptr = workspace.data_ptr() if workspace is not None else None
-    ws_size = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    workspace, ws_ptr, ws_size = _scratch(need, workspace, c.device, stream)
     _check(lib().vecops_hip_matmul_fp8_block(C.byref(oa), C.byref(osa), C.byref(ob), C.byref(osb), C.byref(oc), ws_ptr, ws_size,
                                              _stream_handle(stream)))
     return c
@@ -774,22 +785,18 @@ def moe_experts(x, ids, weights, gate_up, down, out, gate_up_scales=None, down_s
     """out[t] = sum_r weights[t,r] * down[e] . (silu(gate[e] . x[t]) * (up[e] . x[t])) with e = ids[t,r], for up to 128 tokens:
     the experts of a mixture-of-experts layer on a choice made elsewhere.  ``gate_up`` [E, 2 I, H] and ``down`` [E, H, I] are of
     x's type, or e4m3 with ``gate_up_scales`` and ``down_scales`` for blocks of 128 x 128; ids outside 0..E-1 add nothing.
-    Returns out."""
+    ``workspace`` and ``stream`` as in ``matmul_fp8_block``.  Returns out."""
     if stream is None:
         rc = (_calls or native_calls()).moe_experts(x, ids, weights, gate_up, gate_up_scales, down, down_scales, out, workspace)
         if rc == 0:
             return out
         if rc > 0:
             _check(rc)
-    import torch
     _on_one_device("moe_experts", x, ids, weights, gate_up, gate_up_scales, down, down_scales, out, workspace)
     o = [C.byref(operand(t)) if t is not None else None
          for t in (x, ids, weights, gate_up, gate_up_scales, down, down_scales, out)]
     need = lib().vecops_hip_moe_experts_workspace(o[1], o[5])
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        workspace = torch.empty(need, dtype=torch.uint8, device=out.device)
-    ws_ptr = workspace.data_ptr() if workspace is not None else None
-    ws_size = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    workspace, ws_ptr, ws_size = _scratch(need, workspace, out.device, stream)
     _check(lib().vecops_hip_moe_experts(*o, ws_ptr, ws_size, _stream_handle(stream)))
     return out
 
@@ -799,7 +806,7 @@ def moe_layer(x, router, gate_up, down, ids, weights, out, scoring: str = "softm
     """A whole mixture-of-experts layer for up to 128 tokens: the router's scores, the ``ids.shape[1]`` best experts of each token
     and their weights (written to ``ids``, int32, and ``weights``, fp32), then ``moe_experts``.  ``scoring`` is "softmax" or
     "sigmoid"; ``bias`` (fp32, [E]) is added to the scores for the choice only; ``renormalize`` divides a token's weights by
-    their sum, ``scale`` multiplies them.  Returns out."""
+    their sum, ``scale`` multiplies them.  ``workspace`` and ``stream`` as in ``matmul_fp8_block``.  Returns out."""
     import torch
     if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous() or bias.shape != (router.shape[0],) or
                              bias.device != x.device):
@@ -816,9 +823,6 @@ def moe_layer(x, router, gate_up, down, ids, weights, out, scoring: str = "softm
     o = [C.byref(operand(t)) if t is not None else None
          for t in (x, router, gate_up, gate_up_scales, down, down_scales, ids, weights, out)]
     need = lib().vecops_hip_moe_layer_workspace(o[0], o[6], o[4])
-    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
-        workspace = torch.empty(need, dtype=torch.uint8, device=out.device)
-    ws_ptr = workspace.data_ptr() if workspace is not None else None
-    ws_size = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    workspace, ws_ptr, ws_size = _scratch(need, workspace, out.device, stream)
     _check(lib().vecops_hip_moe_layer(o[0], o[1], C.byref(routing), *o[2:], ws_ptr, ws_size, _stream_handle(stream)))
     return out
