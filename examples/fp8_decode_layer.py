@@ -71,6 +71,7 @@ def main() -> None:
     layer = Layer(asked.tokens, hidden=2048, inner=768, experts=64, top=6)
     attended = torch.randn((asked.tokens, 2048), device="cuda").bfloat16()
     side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())   # (which makes the weights)
     with torch.cuda.stream(side):   # (once before the capture: kernels are loaded on their first call)
         layer.step(attended)
     torch.cuda.current_stream().wait_stream(side)
