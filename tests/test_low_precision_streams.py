@@ -49,7 +49,8 @@ def test_scratch_is_taken_on_the_stream_that_is_named(name, monkeypatch):
         return empty(*a, **k)
 
     monkeypatch.setattr(capi, "lib", Library)
-    monkeypatch.setattr(capi, "_on_one_device", lambda *a: None)
+    monkeypatch.setattr(capi, "_on_one_device", lambda *a: stream.device)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
     monkeypatch.setattr(torch.cuda, "stream", on)
     monkeypatch.setattr(torch, "empty", counted)
     call(stream)

@@ -726,11 +726,21 @@ def matmul_i8_dequant_packed_b(a, packed: PackedB, row_scales, column_scales, c,
     return c
 
 
-def _on_one_device(name: str, *tensors) -> None:
-    """The kernels read through plain addresses: a tensor elsewhere is refused here."""
+def _on_one_device(name: str, *tensors):
+    """The device of all of them.  The kernels read through plain addresses: a tensor elsewhere is refused here."""
     devices = {t.device for t in tensors if t is not None}
     if len(devices) != 1 or next(iter(devices)).type != "cuda":
         raise ValueError(f"{name}: tensors must all be on one GPU, got {sorted(map(str, devices))}")
+    return devices.pop()
+
+
+def _on_their_device(name: str, stream, *tensors):
+    """A context in which the tensors' device is the current one; a stream that is named has to be that device's."""
+    import torch
+    device = _on_one_device(name, *tensors)
+    if getattr(stream, "device", device) != device:
+        raise ValueError(f"{name}: the tensors are on {device}, the stream is {stream.device}'s")
+    return torch.cuda.device(device)
 
 
 def _scratch(need: int, workspace, device, stream):
@@ -756,9 +766,9 @@ def quantize_fp8_block(x, q, scales, block_rows: int = 1, stream=None):
             return q, scales
         if rc > 0:
             _check(rc)
-    _on_one_device("quantize_fp8_block", x, q, scales)
-    ox, oq, os_ = operand(x), operand(q), operand(scales)
-    _check(lib().vecops_hip_quantize_fp8_block(C.byref(ox), block_rows, C.byref(oq), C.byref(os_), _stream_handle(stream)))
+    with _on_their_device("quantize_fp8_block", stream, x, q, scales):
+        ox, oq, os_ = operand(x), operand(q), operand(scales)
+        _check(lib().vecops_hip_quantize_fp8_block(C.byref(ox), block_rows, C.byref(oq), C.byref(os_), _stream_handle(stream)))
     return q, scales
 
 
@@ -772,12 +782,12 @@ def matmul_fp8_block(a, a_scales, b, b_scales, c, workspace=None, stream=None):
             return c
         if rc > 0:
             _check(rc)
-    _on_one_device("matmul_fp8_block", a, a_scales, b, b_scales, c, workspace)
-    oa, osa, ob, osb, oc = operand(a), operand(a_scales), operand(b), operand(b_scales), operand(c)
-    need = lib().vecops_hip_matmul_fp8_block_workspace(C.byref(oa), C.byref(osa), C.byref(ob), C.byref(osb), C.byref(oc))
-    workspace, ws_ptr, ws_size = _scratch(need, workspace, c.device, stream)
-    _check(lib().vecops_hip_matmul_fp8_block(C.byref(oa), C.byref(osa), C.byref(ob), C.byref(osb), C.byref(oc), ws_ptr, ws_size,
-                                             _stream_handle(stream)))
+    with _on_their_device("matmul_fp8_block", stream, a, a_scales, b, b_scales, c, workspace):
+        oa, osa, ob, osb, oc = operand(a), operand(a_scales), operand(b), operand(b_scales), operand(c)
+        need = lib().vecops_hip_matmul_fp8_block_workspace(C.byref(oa), C.byref(osa), C.byref(ob), C.byref(osb), C.byref(oc))
+        workspace, ws_ptr, ws_size = _scratch(need, workspace, c.device, stream)
+        _check(lib().vecops_hip_matmul_fp8_block(C.byref(oa), C.byref(osa), C.byref(ob), C.byref(osb), C.byref(oc), ws_ptr, ws_size,
+                                                 _stream_handle(stream)))
     return c
 
 
@@ -792,12 +802,12 @@ def moe_experts(x, ids, weights, gate_up, down, out, gate_up_scales=None, down_s
             return out
         if rc > 0:
             _check(rc)
-    _on_one_device("moe_experts", x, ids, weights, gate_up, gate_up_scales, down, down_scales, out, workspace)
-    o = [C.byref(operand(t)) if t is not None else None
-         for t in (x, ids, weights, gate_up, gate_up_scales, down, down_scales, out)]
-    need = lib().vecops_hip_moe_experts_workspace(o[1], o[5])
-    workspace, ws_ptr, ws_size = _scratch(need, workspace, out.device, stream)
-    _check(lib().vecops_hip_moe_experts(*o, ws_ptr, ws_size, _stream_handle(stream)))
+    with _on_their_device("moe_experts", stream, x, ids, weights, gate_up, gate_up_scales, down, down_scales, out, workspace):
+        o = [C.byref(operand(t)) if t is not None else None
+             for t in (x, ids, weights, gate_up, gate_up_scales, down, down_scales, out)]
+        need = lib().vecops_hip_moe_experts_workspace(o[1], o[5])
+        workspace, ws_ptr, ws_size = _scratch(need, workspace, out.device, stream)
+        _check(lib().vecops_hip_moe_experts(*o, ws_ptr, ws_size, _stream_handle(stream)))
     return out
 
 
@@ -819,10 +829,10 @@ def moe_layer(x, router, gate_up, down, ids, weights, out, scoring: str = "softm
             return out
         if rc > 0:
             _check(rc)
-    _on_one_device("moe_layer", x, router, gate_up, gate_up_scales, down, down_scales, ids, weights, out, workspace)
-    o = [C.byref(operand(t)) if t is not None else None
-         for t in (x, router, gate_up, gate_up_scales, down, down_scales, ids, weights, out)]
-    need = lib().vecops_hip_moe_layer_workspace(o[0], o[6], o[4])
-    workspace, ws_ptr, ws_size = _scratch(need, workspace, out.device, stream)
-    _check(lib().vecops_hip_moe_layer(o[0], o[1], C.byref(routing), *o[2:], ws_ptr, ws_size, _stream_handle(stream)))
+    with _on_their_device("moe_layer", stream, x, router, gate_up, gate_up_scales, down, down_scales, ids, weights, out, workspace):
+        o = [C.byref(operand(t)) if t is not None else None
+             for t in (x, router, gate_up, gate_up_scales, down, down_scales, ids, weights, out)]
+        need = lib().vecops_hip_moe_layer_workspace(o[0], o[6], o[4])
+        workspace, ws_ptr, ws_size = _scratch(need, workspace, out.device, stream)
+        _check(lib().vecops_hip_moe_layer(o[0], o[1], C.byref(routing), *o[2:], ws_ptr, ws_size, _stream_handle(stream)))
     return out

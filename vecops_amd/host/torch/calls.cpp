@@ -14,6 +14,7 @@
 #include <torch/library.h>
 
 #include <ATen/ATen.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 
 #include <deque>
@@ -299,12 +300,25 @@ struct Optional {
   }
 };
 
+// Whether tensors (described before, or None) are all on the device whose stream the work goes to: the kernels read through
+// plain addresses.
+bool on_current_device(std::initializer_list<PyObject*> objects) {
+  c10::Device device{c10::DeviceType::CPU};
+  for (PyObject* object : objects) {
+    if (object == Py_None) continue;
+    const c10::Device its = THPVariable_Unpack(object).device();
+    if (device.is_cpu()) device = its;
+    else if (its != device) return false;
+  }
+  return device.index() == c10::hip::current_device();
+}
+
 // quantize_fp8_block(x, q, scales, block_rows)
 int quantize_fp8_block(PyObject* const* args) {
   VecopsHipOperand x, q, scales;
   int64_t rows = 0;
   if (!describe_any(args[0], &x) || !describe_any(args[1], &q) || !describe_any(args[2], &scales) || !integer(args[3], &rows) || rows < 0 ||
-      rows > UINT32_MAX)
+      rows > UINT32_MAX || !on_current_device({args[0], args[1], args[2]}))
     return kNotPlain;
   return without_lock([&] { return vecops_hip_quantize_fp8_block(&x, static_cast<uint32_t>(rows), &q, &scales, current_stream()); });
 }
@@ -315,7 +329,7 @@ int matmul_fp8_block(PyObject* const* args) {
   for (int i = 0; i < 5; ++i)
     if (!describe_any(args[i], &o[i])) return kNotPlain;
   Given given;
-  if (!given.describe(args[5], *plain_tensor(args[4]))) return kNotPlain;
+  if (!given.describe(args[5], *plain_tensor(args[4])) || !on_current_device({args[0], args[1], args[2], args[3], args[4], args[5]})) return kNotPlain;
   return without_lock([&]() -> int {
     const Workspace workspace(given, vecops_hip_matmul_fp8_block_workspace(&o[0], &o[1], &o[2], &o[3], &o[4]));
     return vecops_hip_matmul_fp8_block(&o[0], &o[1], &o[2], &o[3], &o[4], workspace.data, workspace.size, current_stream());
@@ -330,7 +344,9 @@ int moe_experts(PyObject* const* args) {
       !gate_up_scales.describe(args[4]) || !describe_any(args[5], &down) || !down_scales.describe(args[6]) || !describe_any(args[7], &out))
     return kNotPlain;
   Given given;
-  if (!given.describe(args[8], *plain_tensor(args[7]))) return kNotPlain;
+  if (!given.describe(args[8], *plain_tensor(args[7])) ||
+      !on_current_device({args[0], args[1], args[2], args[3], args[4], args[5], args[6], args[7], args[8]}))
+    return kNotPlain;
   return without_lock([&]() -> int {
     const Workspace workspace(given, vecops_hip_moe_experts_workspace(&ids, &down));
     return vecops_hip_moe_experts(&x, &ids, &weights, &gate_up, gate_up_scales.at, &down, down_scales.at, &out, workspace.data, workspace.size,
@@ -348,7 +364,9 @@ int moe_layer(PyObject* const* args) {
       !describe_any(args[7], &ids) || !describe_any(args[8], &weights) || !describe_any(args[9], &out))
     return kNotPlain;
   Given given;
-  if (!given.describe(args[10], *plain_tensor(args[9]))) return kNotPlain;
+  if (!given.describe(args[10], *plain_tensor(args[9])) ||
+      !on_current_device({args[0], args[1], args[3], args[4], args[5], args[6], args[7], args[8], args[9], args[10]}))
+    return kNotPlain;
   const auto* record = reinterpret_cast<const VecopsHipMoeRouting*>(static_cast<uintptr_t>(routing));
   return without_lock([&]() -> int {
     const Workspace workspace(given, vecops_hip_moe_layer_workspace(&x, &ids, &down));
