@@ -537,7 +537,7 @@ VECOPS_HIP_EXPORT int32_t vecops_hip_quantize_fp8_block(const VecopsHipOperand* 
  * are exact.  16-bit results take the matrix core's 8-bit instruction, which aligns each eight products along k to the largest
  * of them and drops what lies 2^-14 below: results of normally distributed operands are 1.4e-5 off, where rounding them to
  * bf16 gives 1.7e-3 and to f16 2.1e-4.  K == 0 writes zeros.
- * workspace: vecops_hip_matmul_fp8_block_workspace bytes, 16-byte aligned.  It holds the sums of parts of K, where few tiles
+ * workspace: vecops_hip_matmul_fp8_block_workspace bytes (0 for operands that the call refuses), 16-byte aligned.  It holds the sums of parts of K, where few tiles
  * would leave the chip short of work (they are added in a fixed order), and copies of operands whose k are not contiguous
  * (rows may lie at any alignment), of scales where those of a row are not, of operands with K < 16 and of rows too far apart.
  * The rows of a tile - up to 256 of either operand, with M <= 16 sixteen of a and sixteen or 64 of b - are reached by offsets
@@ -563,7 +563,7 @@ VECOPS_HIP_EXPORT int32_t vecops_hip_matmul_fp8_block(const VecopsHipOperand* a,
  * The weights of a named expert are read once for every 8 to 64 tokens that name it.  Sums and the inner values are held to
  * fp32 (the inner values to 2^-17, as a pair of bf16), the result is rounded once; it does not depend on timing.  What is not
  * finite stays not finite, and an infinite weight gives the formula's infinity.
- * workspace: vecops_hip_moe_experts_workspace bytes, 16-byte aligned.
+ * workspace: vecops_hip_moe_experts_workspace bytes (0 for extents that the call refuses), 16-byte aligned.
  */
 VECOPS_HIP_EXPORT uint64_t vecops_hip_moe_experts_workspace(const VecopsHipOperand* ids, const VecopsHipOperand* down);
 VECOPS_HIP_EXPORT int32_t vecops_hip_moe_experts(const VecopsHipOperand* x, const VecopsHipOperand* ids, const VecopsHipOperand* weights,

@@ -48,3 +48,41 @@ def test_rows_that_an_offset_spans_are_taken_as_they_are():
     apart = product(1000, 1000, 4096, a=2 ** 22, b=2 ** 62)
     assert need(apart) == 1000 * 4096
     refused(multiply(apart), INVALID, "workspace of")
+
+
+I32, F16 = capi.I32, capi.F16
+
+
+def moe_need(tokens=4, top=2, experts=8, hidden=256, inner=96, dtype=BF16):
+    """(experts, layer): what the queries say."""
+    x, ids, down = operand(dtype, tokens, hidden), operand(I32, tokens, top), operand(dtype, experts, hidden, inner)
+    return (capi.lib().vecops_hip_moe_experts_workspace(C.byref(ids), C.byref(down)),
+            capi.lib().vecops_hip_moe_layer_workspace(C.byref(x), C.byref(ids), C.byref(down)))
+
+
+def test_nothing_is_asked_for_a_layer_that_is_refused():
+    """A prompt's tokens, and whatever else the calls refuse, need no workspace: a caller that allocates what the query says
+    meets the refusal and not the allocator's."""
+    assert all(n > 0 for n in moe_need()) and all(n > 0 for n in moe_need(128, 16, 512))
+    for refused_extent in ({"tokens": 129}, {"tokens": 65536, "top": 8, "inner": 14336}, {"top": 17}, {"experts": 513}, {"hidden": 2 ** 24 + 1},
+                           {"inner": 2 ** 24 + 1}):
+        assert moe_need(**refused_extent) == (0, 0), refused_extent
+    assert moe_need(top=9)[1] == 0   # more choices than experts: a layer's refusal
+    x, ids, down = operand(BF16, 5, 256), operand(I32, 4, 2), operand(BF16, 8, 256, 96)
+    assert capi.lib().vecops_hip_moe_layer_workspace(C.byref(x), C.byref(ids), C.byref(down)) == 0
+    x = operand(BF16, 4, 255)
+    assert capi.lib().vecops_hip_moe_layer_workspace(C.byref(x), C.byref(ids), C.byref(down)) == 0
+
+
+def test_nothing_is_asked_for_a_product_that_is_refused():
+    k_strided = product(1000, 1000, 4096)
+    k_strided[2] = operand(F8, 1000, 4096, strides=(1, 1000))
+    assert need(k_strided) == 1000 * 4096
+    for at, wrong in ((0, operand(capi.I8, 1000, 4096)), (4, operand(BF16, 1000, 999)), (1, operand(F32, 1000, 31)), (3, operand(F32, 1, 32)),
+                      (0, operand(F8, 1000, 4095))):
+        v = list(k_strided)
+        v[at] = wrong
+        assert need(v) == 0, at
+    k_strided = product(64, 64, 2 ** 25)
+    k_strided[2] = operand(F8, 64, 2 ** 25, strides=(1, 64))
+    assert need(k_strided) == 0

@@ -2738,6 +2738,12 @@ struct Fp8Product {
   Fp8Plan plan;
 };
 
+uint64_t fp8_workspace_bytes(const Fp8Product& pr) {
+  if (pr.a.batch == 0 || pr.a.rows == 0 || pr.b.rows == 0) return 0;
+  return fp8_copy_bytes(pr.a, pr.plan.rows_a) + fp8_copy_bytes(pr.b, pr.plan.rows_b) + fp8_scale_copy_bytes(pr.sa) + fp8_scale_copy_bytes(pr.sb) +
+         fp8_partial_bytes(pr.a, pr.b, pr.plan);
+}
+
 int32_t describe_fp8(const VecopsHipOperand* a, const VecopsHipOperand* a_scales, const VecopsHipOperand* b,
                      const VecopsHipOperand* b_scales, const VecopsHipOperand* c, Fp8Product* pr) {
   if (!normalise(a, &pr->a) || !normalise(a_scales, &pr->sa) || !normalise(b, &pr->b) || !normalise(b_scales, &pr->sb) || !normalise(c, &pr->c))
@@ -2812,12 +2818,9 @@ int32_t vecops_hip_quantize_fp8_block(const VecopsHipOperand* x, uint32_t block_
 
 uint64_t vecops_hip_matmul_fp8_block_workspace(const VecopsHipOperand* a, const VecopsHipOperand* a_scales, const VecopsHipOperand* b,
                                                const VecopsHipOperand* b_scales, const VecopsHipOperand* c) {
-  View va, vsa, vb, vsb, vc;
-  if (!normalise(a, &va) || !normalise(a_scales, &vsa) || !normalise(b, &vb) || !normalise(b_scales, &vsb) || !normalise(c, &vc)) return 0;
-  if (va.batch == 0 || va.rows == 0 || vb.rows == 0) return 0;
-  const Fp8Plan plan = fp8_plan(va.rows, vb.rows, va.cols, va.batch, real_kind(vc.dtype));
-  return fp8_copy_bytes(va, plan.rows_a) + fp8_copy_bytes(vb, plan.rows_b) + fp8_scale_copy_bytes(vsa) + fp8_scale_copy_bytes(vsb) +
-         fp8_partial_bytes(va, vb, plan);
+  Fp8Product pr;
+  if (describe_fp8(a, a_scales, b, b_scales, c, &pr) != ST_OK) return 0;   // (the call says why)
+  return fp8_workspace_bytes(pr);
 }
 
 int32_t vecops_hip_matmul_fp8_block(const VecopsHipOperand* a, const VecopsHipOperand* a_scales, const VecopsHipOperand* b,
@@ -2830,8 +2833,7 @@ int32_t vecops_hip_matmul_fp8_block(const VecopsHipOperand* a, const VecopsHipOp
   if (pr.c.data == nullptr || (pr.a.cols > 0 && (pr.a.data == nullptr || pr.b.data == nullptr || pr.sa.data == nullptr || pr.sb.data == nullptr)))
     return fail(ST_INVALID, "matmul_fp8_block: null operand");
   const Fp8Plan& plan = pr.plan;
-  const uint64_t need = fp8_copy_bytes(pr.a, plan.rows_a) + fp8_copy_bytes(pr.b, plan.rows_b) + fp8_scale_copy_bytes(pr.sa) + fp8_scale_copy_bytes(pr.sb) +
-                        fp8_partial_bytes(pr.a, pr.b, plan);
+  const uint64_t need = fp8_workspace_bytes(pr);
   if (need > 0 && (workspace == nullptr || workspace_size < need || !aligned16(workspace)))
     return fail(ST_INVALID, "matmul_fp8_block: needs a 16-byte aligned workspace of %llu bytes", (unsigned long long)need);
   const hipStream_t s = static_cast<hipStream_t>(stream);
@@ -2892,6 +2894,8 @@ struct MoeExperts {
   MoeExpertsParams p;
 };
 
+bool moe_counts_ok(int64_t tokens, int64_t top, int64_t experts) { return tokens <= kMoeMostTokens && top <= kMoeMostChoices && experts <= kMoeMostExperts; }
+bool moe_widths_ok(int64_t hidden, int64_t inner) { return hidden <= (1 << 24) && inner <= (1 << 24); }
 int64_t moe_inner_pad(int64_t inner) { return (inner + 15) / 16 * 16; }
 uint64_t moe_middle_bytes(int64_t tokens, int64_t top, int64_t inner) {
   return round_up_256(static_cast<uint64_t>(tokens) * static_cast<uint64_t>(top) * static_cast<uint64_t>(moe_inner_pad(inner)) * 4u);
@@ -2934,10 +2938,10 @@ int32_t describe_moe(const char* what, const VecopsHipOperand* x, const VecopsHi
   if ((m->x.dtype != DT_BF16 && m->x.dtype != DT_F16) || (m->out.dtype != m->x.dtype && m->out.dtype != DT_F32) ||
       m->gate_up.dtype != m->down.dtype || (m->down.dtype != m->x.dtype && m->down.dtype != DT_E4M3))
     return fail(ST_NOT_APPLICABLE, "%s: x must be bf16 or f16, out of its type or f32, gate_up and down of its type or e4m3", what);
-  if (tokens > kMoeMostTokens || top > kMoeMostChoices || experts > kMoeMostExperts)
+  if (!moe_counts_ok(tokens, top, experts))
     return fail(ST_NOT_APPLICABLE, "%s: serves up to %d tokens, %d choices and %d experts, got %lld, %lld and %lld", what, kMoeMostTokens,
                 kMoeMostChoices, kMoeMostExperts, (long long)tokens, (long long)top, (long long)experts);
-  if (hidden > (1 << 24) || inner > (1 << 24)) return fail(ST_INVALID, "%s: extent too large", what);
+  if (!moe_widths_ok(hidden, inner)) return fail(ST_INVALID, "%s: extent too large", what);
   if ((m->x.cs != 1 && hidden > 1) || (m->gate_up.cs != 1 && hidden > 1) || (m->down.cs != 1 && inner > 1))
     return fail(ST_NOT_APPLICABLE, "%s: rows of x, gate_up and down must be contiguous", what);
   MoeExpertsParams& p = m->p;
@@ -2983,7 +2987,7 @@ int32_t describe_moe(const char* what, const VecopsHipOperand* x, const VecopsHi
 
 uint64_t vecops_hip_moe_experts_workspace(const VecopsHipOperand* ids, const VecopsHipOperand* down) {
   View vi, vd;
-  if (!matrix_of(ids, &vi) || !normalise(down, &vd) || vd.rows > (1 << 24)) return 0;
+  if (!matrix_of(ids, &vi) || !normalise(down, &vd) || !moe_counts_ok(vi.rows, vi.cols, vd.batch) || !moe_widths_ok(vd.rows, vd.cols)) return 0;
   return moe_experts_bytes(vi.rows, vi.cols, vd.rows, vd.cols);
 }
 
@@ -3006,7 +3010,9 @@ int32_t vecops_hip_moe_experts(const VecopsHipOperand* x, const VecopsHipOperand
 
 uint64_t vecops_hip_moe_layer_workspace(const VecopsHipOperand* x, const VecopsHipOperand* ids, const VecopsHipOperand* down) {
   View vx, vi, vd;
-  if (!matrix_of(x, &vx) || !matrix_of(ids, &vi) || !normalise(down, &vd) || vx.cols > (1 << 24)) return 0;
+  if (!matrix_of(x, &vx) || !matrix_of(ids, &vi) || !normalise(down, &vd) || !moe_counts_ok(vi.rows, vi.cols, vd.batch) ||
+      !moe_widths_ok(vd.rows, vd.cols) || vx.rows != vi.rows || vx.cols != vd.rows || vi.cols > vd.batch)
+    return 0;
   return moe_experts_bytes(vi.rows, vi.cols, vx.cols, vd.cols) + moe_logits_bytes(vx.rows, vd.batch, vx.cols);
 }
 
