@@ -829,7 +829,8 @@ hipError_t launch_experts(const MoeExpertsParams& p, const MoeRouteParams* route
   return hipGetLastError();
 }
 
-// Columns of sixteen (in down eight) tokens that a pass over an expert's weights serves, by the tokens an expert has on average: more
+// Columns of sixteen (in down eight) tokens that a pass over an expert's weights serves, by the tokens an expert has on average
+// (known here; how many really name it, and how many ids name none, only the kernels know): more
 // take registers from the loads ahead, fewer read the weights again.  Measured with one, two and four (us): 6 (64 tokens, 6 of 64
 // of 2048 x 1408, bf16) 217, 220, 245; 8 (128 tokens, 8 of 128 of 2048 x 768) e4m3 169, 179, 248, bf16 251, 244, 270; 10 (40
 // tokens, 2 of 8 of 4096 x 4096, bf16) 170, 161, 176; 25 (128 tokens, 2 of 10 of 2048 x 4096, e4m3) 140, 123, 133; 32 (128
