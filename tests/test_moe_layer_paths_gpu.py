@@ -58,3 +58,25 @@ def test_an_expert_that_many_tokens_name(device, t, e, top, hot, weights):
         out = torch.full((t, h), float("nan"), dtype=dtype, device=device)
         capi.moe_experts(dx, dids, dw, dg, dd, out, gate_up_scales=dgs, down_scales=dds)
         check(out, want, bound)
+
+
+@pytest.mark.parametrize("weights", ["bf16", "fp8_f16"])
+@pytest.mark.parametrize("t,h", [(5, 200), (37, 512), (128, 256), (128, 1040)])
+def test_shares_of_a_result_are_added_whole(device, t, h, weights):
+    """Where few columns leave compute units idle, workgroups share a column block and the last one adds: from a workspace that
+    holds NaN before each call, so that a number that was not there yet would show."""
+    e, top, i = 12, 3, 272
+    x, gate_up, gs, down, ds = case(t, e, top, h, i, weights)
+    ids, w = choices(t, e, top)
+    want, bound = experts64(x, ids, w, gate_up, gs, down, ds)
+    dx, dids, dw, dg, dgs, dd, dds = to(device, x, ids, w, gate_up, gs, down, ds)
+    workspace = torch.empty(64 << 20, dtype=torch.uint8, device=device)
+    first = None
+    for _ in range(12):
+        workspace.fill_(0xff)
+        out = torch.full((t, h), float("nan"), device=device)
+        capi.moe_experts(dx, dids, dw, dg, dd, out, gate_up_scales=dgs, down_scales=dds, workspace=workspace)
+        if first is None:
+            first = out
+            check(out, want, bound)
+        assert torch.equal(out, first)
