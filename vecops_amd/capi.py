@@ -13,7 +13,7 @@ LIB_PATH = os.path.join(HERE, "lib", "libvecops_hip.so")
 
 # VecopsDType numbers
 I8, U8, I32, F16, BF16, F32, F64 = 2, 3, 6, 10, 11, 12, 13
-F8E4M3 = 64  # this library's own (VECOPS_HIP_DTYPE_F8E4M3)
+F8E4M3, F4E2M1X2, F8E8M0 = 64, 65, 66  # this library's own (VECOPS_HIP_DTYPE_F8E4M3, _F4E2M1X2, _F8E8M0)
 COMPUTE_BF16, COMPUTE_F32 = 0, 1
 FAMILY_NAMES = {0: "none", 1: "tile_256", 2: "tile_128", 3: "tile_64", 4: "skinny", 5: "zero_k", 6: "tile_256x128",
                 7: "tile_128x256", 8: "tile_256x352", 9: "tile_192"}
@@ -37,6 +37,8 @@ EXPORTS = [
     "vecops_hip_pack_a", "vecops_hip_plan_matmul_packed_a", "vecops_hip_matmul_packed_a",
     "vecops_hip_matmul_packed_ab_workspace", "vecops_hip_matmul_packed_ab",
     "vecops_hip_quantize_fp8_block", "vecops_hip_matmul_fp8_block_workspace", "vecops_hip_matmul_fp8_block",
+    "vecops_hip_quantize_mx", "vecops_hip_dequantize_mx", "vecops_hip_matmul_mx_workspace", "vecops_hip_matmul_mx",
+    "vecops_hip_rms_norm", "vecops_hip_silu_mul_quantize",
     "vecops_hip_moe_experts_workspace", "vecops_hip_moe_experts", "vecops_hip_moe_layer_workspace", "vecops_hip_moe_layer",
 ]
 
@@ -180,6 +182,13 @@ def lib() -> C.CDLL:
         L.vecops_hip_matmul_fp8_block_workspace.restype = C.c_uint64
         L.vecops_hip_matmul_fp8_block_workspace.argtypes = [P] * 5
         L.vecops_hip_matmul_fp8_block.argtypes = [P, P, P, P, P, C.c_void_p, C.c_uint64, C.c_void_p]
+        L.vecops_hip_quantize_mx.argtypes = [P, P, P, C.c_void_p]
+        L.vecops_hip_dequantize_mx.argtypes = [P, P, P, C.c_void_p]
+        L.vecops_hip_matmul_mx_workspace.restype = C.c_uint64
+        L.vecops_hip_matmul_mx_workspace.argtypes = [P] * 5
+        L.vecops_hip_matmul_mx.argtypes = [P] * 5 + [C.c_void_p, C.c_uint64, C.c_void_p]
+        L.vecops_hip_rms_norm.argtypes = [P, P, C.c_float] + [P] * 5 + [C.c_void_p]
+        L.vecops_hip_silu_mul_quantize.argtypes = [P, P, P, C.c_void_p]
         L.vecops_hip_moe_experts_workspace.restype = C.c_uint64
         L.vecops_hip_moe_experts_workspace.argtypes = [P, P]
         L.vecops_hip_moe_experts.argtypes = [P] * 8 + [C.c_void_p, C.c_uint64, C.c_void_p]
@@ -233,11 +242,12 @@ def _check(rc: int) -> None:
 def _torch_dtype_code(t) -> int:
     import torch
     return {torch.int8: I8, torch.uint8: U8, torch.int32: I32, torch.float16: F16, torch.bfloat16: BF16,
-            torch.float32: F32, torch.float64: F64, torch.float8_e4m3fn: F8E4M3}[t.dtype]
+            torch.float32: F32, torch.float64: F64, torch.float8_e4m3fn: F8E4M3, torch.float4_e2m1fn_x2: F4E2M1X2,
+            torch.float8_e8m0fnu: F8E8M0}[t.dtype]
 
 
 def operand(t) -> Operand:
-    """Describe a torch tensor (rank 2 or 3, any strides) living in device memory."""
+    """Describe a torch tensor (rank 2 or 3, any strides; a norm's weight is rank 1) living in device memory."""
     o = Operand()
     o.data = t.data_ptr()
     o.dtype = _torch_dtype_code(t)
@@ -789,6 +799,88 @@ def matmul_fp8_block(a, a_scales, b, b_scales, c, workspace=None, stream=None):
         _check(lib().vecops_hip_matmul_fp8_block(C.byref(oa), C.byref(osa), C.byref(ob), C.byref(osb), C.byref(oc), ws_ptr, ws_size,
                                                  _stream_handle(stream)))
     return c
+
+
+def quantize_mx(x, q, scales, stream=None):
+    """x [.., M, K] -> q and a power of two for each 32 elements of a row (``scales``, ``torch.float8_e8m0fnu``, [.., M, ceil(K / 32)]):
+    ``q * scale`` stands for x.  q is ``torch.float8_e4m3fn`` [.., M, K], or ``torch.float4_e2m1fn_x2`` [.., M, K / 2], two elements a
+    byte.  Returns (q, scales)."""
+    if stream is None:
+        rc = (_calls or native_calls()).quantize_mx(x, q, scales)
+        if rc == 0:
+            return q, scales
+        if rc > 0:
+            _check(rc)
+    with _on_their_device("quantize_mx", stream, x, q, scales):
+        ox, oq, os_ = operand(x), operand(q), operand(scales)
+        _check(lib().vecops_hip_quantize_mx(C.byref(ox), C.byref(oq), C.byref(os_), _stream_handle(stream)))
+    return q, scales
+
+
+def dequantize_mx(q, scales, out, stream=None):
+    """What ``quantize_mx`` has written, as numbers: out [.., M, K] (f32, bf16 or f16) = q * scales.  Returns out."""
+    if stream is None:
+        rc = (_calls or native_calls()).dequantize_mx(q, scales, out)
+        if rc == 0:
+            return out
+        if rc > 0:
+            _check(rc)
+    with _on_their_device("dequantize_mx", stream, q, scales, out):
+        oq, os_, oo = operand(q), operand(scales), operand(out)
+        _check(lib().vecops_hip_dequantize_mx(C.byref(oq), C.byref(os_), C.byref(oo), _stream_handle(stream)))
+    return out
+
+
+def matmul_mx(a, a_scales, b, b_scales, c, workspace=None, stream=None):
+    """c[..,M,N] = (a * its scales) . (b * its scales)^T for operands as ``quantize_mx`` writes them: 4-bit weights b, 4-bit or
+    8-bit activations a.  ``workspace`` and ``stream`` as in ``matmul_fp8_block``.  Returns c."""
+    if stream is None:
+        rc = (_calls or native_calls()).matmul_mx(a, a_scales, b, b_scales, c, workspace)
+        if rc == 0:
+            return c
+        if rc > 0:
+            _check(rc)
+    with _on_their_device("matmul_mx", stream, a, a_scales, b, b_scales, c, workspace):
+        oa, osa, ob, osb, oc = operand(a), operand(a_scales), operand(b), operand(b_scales), operand(c)
+        need = lib().vecops_hip_matmul_mx_workspace(C.byref(oa), C.byref(osa), C.byref(ob), C.byref(osb), C.byref(oc))
+        workspace, ws_ptr, ws_size = _scratch(need, workspace, c.device, stream)
+        _check(lib().vecops_hip_matmul_mx(C.byref(oa), C.byref(osa), C.byref(ob), C.byref(osb), C.byref(oc), ws_ptr, ws_size,
+                                          _stream_handle(stream)))
+    return c
+
+
+def rms_norm(x, weight, q=None, scales=None, out=None, residual=None, summed=None, eps: float = 1e-6, stream=None):
+    """y = h / sqrt(mean(h^2) + eps) * weight for the rows h = x + residual, which are written to ``summed`` (None: in the
+    residual's place).  ``out`` gets y in x's type; ``q`` and ``scales`` get it quantised, by their types: int8 with float32
+    [.., M, 1] (activations and row scales of ``matmul_i8_dequant``), ``float8_e4m3fn`` with float32 [.., M, ceil(K / 128)] (of
+    ``matmul_fp8_block``), ``float8_e4m3fn`` or ``float4_e2m1fn_x2`` with ``float8_e8m0fnu`` (of ``matmul_mx``).  Returns what
+    was asked for, (q, scales), out, or (q, scales, out)."""
+    done = (q, scales) if out is None else out if q is None else (q, scales, out)
+    if stream is None:
+        rc = (_calls or native_calls()).rms_norm(x, weight, residual, summed, q, scales, out, eps)
+        if rc == 0:
+            return done
+        if rc > 0:
+            _check(rc)
+    with _on_their_device("rms_norm", stream, x, weight, residual, summed, q, scales, out):
+        ox, ow, *others = [C.byref(operand(t)) if t is not None else None for t in (x, weight, residual, summed, q, scales, out)]
+        _check(lib().vecops_hip_rms_norm(ox, ow, eps, *others, _stream_handle(stream)))
+    return done
+
+
+def silu_mul_quantize(gate_up, q, scales, stream=None):
+    """silu(gate) * up for gate_up [.., M, 2 I], an expert's or a layer's gates and then their factors, quantised to ``q`` and
+    ``scales`` in the formats of ``rms_norm``: the operand of the down projection.  Returns (q, scales)."""
+    if stream is None:
+        rc = (_calls or native_calls()).silu_mul_quantize(gate_up, q, scales)
+        if rc == 0:
+            return q, scales
+        if rc > 0:
+            _check(rc)
+    with _on_their_device("silu_mul_quantize", stream, gate_up, q, scales):
+        ox, oq, os_ = operand(gate_up), operand(q), operand(scales)
+        _check(lib().vecops_hip_silu_mul_quantize(C.byref(ox), C.byref(oq), C.byref(os_), _stream_handle(stream)))
+    return q, scales
 
 
 def moe_experts(x, ids, weights, gate_up, down, out, gate_up_scales=None, down_scales=None, workspace=None, stream=None):

@@ -13,7 +13,9 @@
 #include "fp8_block.h"
 #include "gemm_f64.h"
 #include "moe_few_tokens.h"
+#include "mx_block.h"
 #include "packed_row_sums.h"
+#include "row_quantize.h"
 #include "skinny_dense.h"
 #include "skinny_w8a16.h"
 #include "tile_gemm_launch.h"
@@ -27,7 +29,7 @@ using namespace vecops_hip;
 
 enum : int32_t { ST_OK = 0, ST_INVALID = 1, ST_NOT_APPLICABLE = 2, ST_EXEC = 6 };
 enum : uint32_t { DT_I8 = 2, DT_U8 = 3, DT_I32 = 6, DT_F16 = 10, DT_BF16 = 11, DT_F32 = 12, DT_F64 = 13,
-                  DT_E4M3 = VECOPS_HIP_DTYPE_F8E4M3 };
+                  DT_E4M3 = VECOPS_HIP_DTYPE_F8E4M3, DT_E2M1X2 = VECOPS_HIP_DTYPE_F4E2M1X2, DT_E8M0 = VECOPS_HIP_DTYPE_F8E8M0 };
 // fp64 operands run on a kernel of their own (gemm_f64.hip), outside the tile kernels' operand classes and outputs
 constexpr int kSrcF64 = 100, kOutF64 = 100;
 
@@ -2882,6 +2884,289 @@ int32_t vecops_hip_matmul_fp8_block(const VecopsHipOperand* a, const VecopsHipOp
   p.partial = reinterpret_cast<float*>(room);
   const hipError_t e = launch_fp8_matmul(p, plan.kind, s);
   if (e != hipSuccess) return fail(ST_EXEC, "matmul_fp8_block: kernel launch: %s", hipGetErrorString(e));
+  return ST_OK;
+}
+
+// ---- microscaled operands, and the operators between products ---------------------------------------------------------
+
+namespace {
+
+int64_t mx_blocks(int64_t extent) { return (extent + kMxBlock - 1) / kMxBlock; }
+bool rows_contiguous(const View& v) { return v.cs == 1 || v.cols <= 1; }
+bool same_shape(const View& a, const View& b) { return a.batch == b.batch && a.rows == b.rows && a.cols == b.cols; }
+
+// A matrix and its microscaled copy; *nothing: there is no element.
+int32_t describe_mx_copy(const char* name, const VecopsHipOperand* x, const VecopsHipOperand* q, const VecopsHipOperand* scales, MxCopyParams* p,
+                         bool* nothing) {
+  View vx, vq, vs;
+  if (!normalise(x, &vx) || !normalise(q, &vq) || !normalise(scales, &vs))
+    return fail(ST_INVALID, "%s: operands must be rank 2 or 3 with non-negative extents", name);
+  if (real_kind(vx.dtype) < 0) return fail(ST_NOT_APPLICABLE, "%s: the matrix must be f32, bf16 or f16", name);
+  if (vq.dtype != DT_E4M3 && vq.dtype != DT_E2M1X2) return fail(ST_NOT_APPLICABLE, "%s: q must be e4m3, or e2m1 two a byte", name);
+  if (vs.dtype != DT_E8M0) return fail(ST_INVALID, "%s: scales must be e8m0", name);
+  const int64_t per_byte = vq.dtype == DT_E2M1X2 ? 2 : 1, groups = mx_blocks(vx.cols);
+  if (vx.cols % per_byte != 0) return fail(ST_INVALID, "%s: rows of e2m1 must have an even number of elements, got %lld", name, (long long)vx.cols);
+  if (x->rank != q->rank || x->rank != scales->rank || vx.batch != vq.batch || vx.rows != vq.rows || vx.cols / per_byte != vq.cols)
+    return fail(ST_INVALID, "%s: the matrix and q differ in shape (a byte of e2m1 holds two elements)", name);
+  if (vs.batch != vx.batch || vs.rows != vx.rows || vs.cols != groups)
+    return fail(ST_INVALID, "%s: scales must be [%lld, %lld]", name, (long long)vx.rows, (long long)groups);
+  *nothing = vx.batch == 0 || vx.rows == 0 || vx.cols == 0;
+  if (*nothing) return ST_OK;
+  if (vx.data == nullptr || vq.data == nullptr || vs.data == nullptr) return fail(ST_INVALID, "%s: null operand", name);
+  if (vx.batch > INT32_MAX || vx.rows > INT32_MAX || vx.cols > INT32_MAX / 2 || vx.batch * vx.rows > INT32_MAX / (4 * groups))
+    return fail(ST_INVALID, "%s: extent too large", name);
+  p->x = vx.data;
+  p->q = static_cast<uint8_t*>(vq.data);
+  p->scales = static_cast<uint8_t*>(vs.data);
+  p->x_bs = vx.bs, p->x_rs = vx.rs, p->x_cs = vx.cs;
+  p->q_bs = vq.bs, p->q_rs = vq.rs, p->q_cs = vq.cs;
+  p->s_bs = vs.bs, p->s_rs = vs.rs, p->s_cs = vs.cs;
+  p->batch = static_cast<int32_t>(vx.batch), p->rows = static_cast<int32_t>(vx.rows), p->k = static_cast<int32_t>(vx.cols);
+  p->groups = static_cast<int32_t>(groups);
+  p->kind = real_kind(vx.dtype);
+  p->format = vq.dtype == DT_E2M1X2 ? ROW_MX_E2M1 : ROW_MX_E4M3;
+  return ST_OK;
+}
+
+// What the product reads an operand through: its own rows where their bytes follow one another, their blocks are whole and they lie near enough
+// to one another for the offsets of the plan's kernel, `rows` of them, else a copy in the workspace, padded to whole blocks with zeros.
+bool mx_rows_reached(int64_t rows, int64_t ld, int64_t bytes) { return ld <= INT32_MAX && (rows - 1) * ld + bytes + 512 < (int64_t{1} << 31); }
+bool mx_rows_ok(const View& v, int64_t k, int64_t rows) { return (v.cs == 1 || v.cols == 1) && k % kMxBlock == 0 && v.rs >= 0 && mx_rows_reached(rows, v.rs, v.cols); }
+int64_t mx_row_bytes(const View& v) { return mx_blocks(v.dtype == DT_E2M1X2 ? 2 * v.cols : v.cols) * (v.dtype == DT_E2M1X2 ? kMxBlock / 2 : kMxBlock); }
+uint64_t mx_copy_bytes(const View& v, int64_t k, int64_t rows) {
+  if (v.batch == 0 || v.rows == 0 || k == 0 || mx_rows_ok(v, k, rows)) return 0;
+  return round_up_256(static_cast<uint64_t>(v.bs == 0 ? 1 : v.batch) * static_cast<uint64_t>(v.rows) * static_cast<uint64_t>(mx_row_bytes(v)));
+}
+
+// Scales likewise: a row's follow one another, at least four of them, rows up to 2^20 apart.
+bool mx_scales_ok(const View& v) { return v.cs == 1 && v.cols >= 4 && v.rs >= 0 && v.rs <= (int64_t{1} << 20); }
+int64_t mx_scale_row_bytes(const View& v) { return (v.cols + 3) / 4 * 4; }
+uint64_t mx_scale_copy_bytes(const View& v) {
+  if (v.batch == 0 || v.rows == 0 || v.cols == 0 || mx_scales_ok(v)) return 0;
+  return round_up_256(static_cast<uint64_t>(v.bs == 0 ? 1 : v.batch) * static_cast<uint64_t>(v.rows) * static_cast<uint64_t>(mx_scale_row_bytes(v)));
+}
+
+struct MxProduct {
+  View a, sa, b, sb, c;
+  int64_t k;
+  MxPlan plan;
+};
+
+uint64_t mx_workspace_bytes(const MxProduct& pr) {
+  if (pr.a.batch == 0 || pr.a.rows == 0 || pr.b.rows == 0) return 0;
+  return mx_copy_bytes(pr.a, pr.k, pr.plan.rows_a) + mx_copy_bytes(pr.b, pr.k, pr.plan.rows_b) + mx_scale_copy_bytes(pr.sa) + mx_scale_copy_bytes(pr.sb) +
+         (pr.plan.splits == 1 ? 0 : static_cast<uint64_t>(pr.plan.splits) * pr.a.batch * pr.a.rows * pr.b.rows * 4u);
+}
+
+int32_t describe_mx(const VecopsHipOperand* a, const VecopsHipOperand* a_scales, const VecopsHipOperand* b, const VecopsHipOperand* b_scales,
+                    const VecopsHipOperand* c, MxProduct* pr) {
+  if (!normalise(a, &pr->a) || !normalise(a_scales, &pr->sa) || !normalise(b, &pr->b) || !normalise(b_scales, &pr->sb) || !normalise(c, &pr->c))
+    return fail(ST_INVALID, "matmul_mx: operands must be rank 2 or 3 with non-negative extents");
+  if (a->rank != b->rank || a->rank != c->rank || a->rank != a_scales->rank || a->rank != b_scales->rank)
+    return fail(ST_INVALID, "matmul_mx: operand ranks differ");
+  if ((pr->a.dtype != DT_E2M1X2 && pr->a.dtype != DT_E4M3) || pr->b.dtype != DT_E2M1X2 || real_kind(pr->c.dtype) < 0)
+    return fail(ST_NOT_APPLICABLE, "matmul_mx: a must be e2m1 (two a byte) or e4m3, b e2m1, c f32, bf16 or f16");
+  if (pr->sa.dtype != DT_E8M0 || pr->sb.dtype != DT_E8M0) return fail(ST_INVALID, "matmul_mx: scales must be e8m0");
+  const int64_t m = pr->a.rows, n = pr->b.rows, batch = pr->a.batch;
+  if (pr->b.cols > INT32_MAX / 4 || pr->a.cols > INT32_MAX / 2) return fail(ST_INVALID, "matmul_mx: extent too large");
+  const int64_t k = pr->k = 2 * pr->b.cols;
+  if (pr->a.cols * (pr->a.dtype == DT_E2M1X2 ? 2 : 1) != k)
+    return fail(ST_INVALID, "matmul_mx: K of a (%lld) and b (%lld) differ", (long long)(pr->a.cols * (pr->a.dtype == DT_E2M1X2 ? 2 : 1)), (long long)k);
+  if (pr->c.rows != m || pr->c.cols != n) return fail(ST_INVALID, "matmul_mx: c must be [M=%lld, N=%lld]", (long long)m, (long long)n);
+  if (pr->b.batch != batch || pr->c.batch != batch || pr->sa.batch != batch || pr->sb.batch != batch) return fail(ST_INVALID, "matmul_mx: batch extents differ");
+  if (pr->sa.rows != m || pr->sa.cols != mx_blocks(k))
+    return fail(ST_INVALID, "matmul_mx: a_scales must be [M=%lld, ceil(K / 32)=%lld]", (long long)m, (long long)mx_blocks(k));
+  if (pr->sb.rows != n || pr->sb.cols != mx_blocks(k))
+    return fail(ST_INVALID, "matmul_mx: b_scales must be [N=%lld, ceil(K / 32)=%lld]", (long long)n, (long long)mx_blocks(k));
+  // (a grid holds fewer than 2^32 threads: workgroups of 256 for tiles of 128 x 128 or sixteen columns of a few rows, of 512 for larger tiles)
+  if (m > INT32_MAX / 2 || n > (1 << 27) || batch > 65535 || ((m + 63) / 64) * ((n + 63) / 64) >= (1 << 24)) return fail(ST_INVALID, "matmul_mx: extent too large");
+  pr->plan = mx_plan(m, n, k, batch, pr->a.dtype == DT_E4M3);
+  if (m == 0 || n == 0 || batch == 0) return ST_OK;
+  for (const auto& [v, rows] : {std::make_pair(&pr->a, pr->plan.rows_a), std::make_pair(&pr->b, pr->plan.rows_b)}) {
+    if (mx_copy_bytes(*v, k, rows) == 0) continue;
+    // a copy brings rows together, but no nearer than their length
+    if (!mx_rows_reached(rows, mx_row_bytes(*v), v->cols)) return fail(ST_NOT_APPLICABLE, "matmul_mx: K=%lld is too long: %d rows must lie within 2 GiB", (long long)k, rows);
+    if (((v->rows + 63) / 64) * ((v->cols + 63) / 64) >= (1 << 24)) return fail(ST_INVALID, "matmul_mx: extent too large");
+  }
+  return ST_OK;
+}
+
+// How rows of K results are held, by the types of q and scales; ROW_NONE where neither is given, -1 for another pair.
+int row_format(const View& q, const View& scales) {
+  if (q.dtype == DT_I8 && scales.dtype == DT_F32) return ROW_INT8;
+  if (q.dtype == DT_E4M3 && scales.dtype == DT_F32) return ROW_E4M3_128;
+  if (q.dtype == DT_E4M3 && scales.dtype == DT_E8M0) return ROW_MX_E4M3;
+  if (q.dtype == DT_E2M1X2 && scales.dtype == DT_E8M0) return ROW_MX_E2M1;
+  return -1;
+}
+
+// q and scales of `batch` x `rows` rows of k results.
+int32_t describe_row_results(const char* name, const VecopsHipOperand* q, const VecopsHipOperand* scales, uint32_t rank, int64_t batch, int64_t rows,
+                             int64_t k, RowQuantizeParams* p) {
+  View vq, vs;
+  if (!normalise(q, &vq) || !normalise(scales, &vs) || q->rank != rank || scales->rank != rank)
+    return fail(ST_INVALID, "%s: q and scales must have the rank of the matrix (2 or 3) and non-negative extents", name);
+  p->format = row_format(vq, vs);
+  if (p->format < 0)
+    return fail(ST_NOT_APPLICABLE, "%s: q and scales must be int8 and f32, e4m3 and f32, e4m3 and e8m0, or e2m1 (two a byte) and e8m0", name);
+  const int64_t per_byte = p->format == ROW_MX_E2M1 ? 2 : 1;
+  if (k % per_byte != 0) return fail(ST_INVALID, "%s: rows of e2m1 must have an even number of elements, got %lld", name, (long long)k);
+  if (vq.batch != batch || vq.rows != rows || vq.cols != k / per_byte)
+    return fail(ST_INVALID, "%s: q must be [%lld, %lld]", name, (long long)rows, (long long)(k / per_byte));
+  const int64_t groups = p->format == ROW_INT8 ? 1 : p->format == ROW_E4M3_128 ? fp8_blocks(k) : mx_blocks(k);
+  if (vs.batch != batch || vs.rows != rows || vs.cols != groups) return fail(ST_INVALID, "%s: scales must be [%lld, %lld]", name, (long long)rows, (long long)groups);
+  if (!rows_contiguous(vq)) return fail(ST_NOT_APPLICABLE, "%s: rows of q must be contiguous", name);
+  if (batch * rows * k > 0 && (vq.data == nullptr || vs.data == nullptr)) return fail(ST_INVALID, "%s: null operand", name);
+  p->q = static_cast<uint8_t*>(vq.data);
+  p->scales = vs.data;
+  p->q_bs = vq.bs, p->q_rs = vq.rs;
+  p->s_bs = vs.bs, p->s_rs = vs.rs, p->s_cs = vs.cs;
+  p->groups = static_cast<int32_t>(groups);
+  return ST_OK;
+}
+
+bool row_extents_ok(int64_t batch, int64_t rows, int64_t k) { return batch <= INT32_MAX && rows <= INT32_MAX && k <= (1 << 30) && (rows == 0 || batch <= INT32_MAX / rows); }
+
+}  // namespace
+
+int32_t vecops_hip_quantize_mx(const VecopsHipOperand* x, const VecopsHipOperand* q, const VecopsHipOperand* scales, void* stream) {
+  MxCopyParams p;
+  bool nothing;
+  const int32_t rc = describe_mx_copy("quantize_mx", x, q, scales, &p, &nothing);
+  if (rc != ST_OK || nothing) return rc;
+  const hipError_t e = launch_mx_quantize(p, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(ST_EXEC, "quantize_mx: kernel launch: %s", hipGetErrorString(e));
+  return ST_OK;
+}
+
+int32_t vecops_hip_dequantize_mx(const VecopsHipOperand* q, const VecopsHipOperand* scales, const VecopsHipOperand* out, void* stream) {
+  MxCopyParams p;
+  bool nothing;
+  const int32_t rc = describe_mx_copy("dequantize_mx", out, q, scales, &p, &nothing);
+  if (rc != ST_OK || nothing) return rc;
+  const hipError_t e = launch_mx_dequantize(p, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(ST_EXEC, "dequantize_mx: kernel launch: %s", hipGetErrorString(e));
+  return ST_OK;
+}
+
+uint64_t vecops_hip_matmul_mx_workspace(const VecopsHipOperand* a, const VecopsHipOperand* a_scales, const VecopsHipOperand* b,
+                                        const VecopsHipOperand* b_scales, const VecopsHipOperand* c) {
+  MxProduct pr;
+  if (describe_mx(a, a_scales, b, b_scales, c, &pr) != ST_OK) return 0;   // (the call says why)
+  return mx_workspace_bytes(pr);
+}
+
+int32_t vecops_hip_matmul_mx(const VecopsHipOperand* a, const VecopsHipOperand* a_scales, const VecopsHipOperand* b, const VecopsHipOperand* b_scales,
+                             const VecopsHipOperand* c, void* workspace, uint64_t workspace_size, void* stream) {
+  MxProduct pr;
+  const int32_t rc = describe_mx(a, a_scales, b, b_scales, c, &pr);
+  if (rc != ST_OK) return rc;
+  if (pr.a.batch == 0 || pr.a.rows == 0 || pr.b.rows == 0) return ST_OK;
+  if (pr.c.data == nullptr || (pr.k > 0 && (pr.a.data == nullptr || pr.b.data == nullptr || pr.sa.data == nullptr || pr.sb.data == nullptr)))
+    return fail(ST_INVALID, "matmul_mx: null operand");
+  const uint64_t need = mx_workspace_bytes(pr);
+  if (need > 0 && (workspace == nullptr || workspace_size < need || !aligned16(workspace)))
+    return fail(ST_INVALID, "matmul_mx: needs a 16-byte aligned workspace of %llu bytes", (unsigned long long)need);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  uint8_t* room = static_cast<uint8_t*>(workspace);
+  const auto copy = [&](View* v, uint64_t bytes, int64_t ld) {
+    if (bytes == 0) return hipSuccess;
+    const hipError_t e = launch_fp8_rows(static_cast<const uint8_t*>(v->data), v->bs, v->rs, v->cs, room, ld, static_cast<int32_t>(v->bs == 0 ? 1 : v->batch),
+                                         static_cast<int32_t>(v->rows), static_cast<int32_t>(v->cols), s);
+    v->data = room;
+    v->bs = v->bs == 0 ? 0 : v->rows * ld;
+    v->rs = ld;
+    v->cs = 1;
+    room += bytes;
+    return e;
+  };
+  for (const hipError_t e : {copy(&pr.a, mx_copy_bytes(pr.a, pr.k, pr.plan.rows_a), mx_row_bytes(pr.a)), copy(&pr.b, mx_copy_bytes(pr.b, pr.k, pr.plan.rows_b), mx_row_bytes(pr.b)),
+                             copy(&pr.sa, mx_scale_copy_bytes(pr.sa), mx_scale_row_bytes(pr.sa)), copy(&pr.sb, mx_scale_copy_bytes(pr.sb), mx_scale_row_bytes(pr.sb))})
+    if (e != hipSuccess) return fail(ST_EXEC, "matmul_mx: kernel launch: %s", hipGetErrorString(e));
+  MxMatmulParams p;
+  p.a = static_cast<const uint8_t*>(pr.a.data), p.b = static_cast<const uint8_t*>(pr.b.data);
+  p.a_scales = static_cast<const uint8_t*>(pr.sa.data), p.b_scales = static_cast<const uint8_t*>(pr.sb.data);
+  p.c = pr.c.data;
+  p.lda = pr.a.rs, p.ldb = pr.b.rs, p.a_bs = pr.a.bs, p.b_bs = pr.b.bs;
+  p.as_rs = pr.sa.rs, p.as_bs = pr.sa.bs, p.bs_rs = pr.sb.rs, p.bs_bs = pr.sb.bs;
+  p.c_rs = pr.c.rs, p.c_cs = pr.c.cs, p.c_bs = pr.c.bs;
+  p.m = static_cast<int32_t>(pr.a.rows), p.n = static_cast<int32_t>(pr.b.rows), p.batch = static_cast<int32_t>(pr.a.batch);
+  p.groups = static_cast<int32_t>(mx_blocks(pr.k));
+  p.row_scales = std::max(p.groups, 4);   // (rows of fewer have been padded with zeros, which stand for numbers; their elements are not there)
+  p.a_wide = pr.a.dtype == DT_E4M3;
+  p.out_kind = real_kind(pr.c.dtype);
+  p.splits = pr.plan.splits;
+  p.partial = reinterpret_cast<float*>(room);
+  const hipError_t e = launch_mx_matmul(p, pr.plan.kind, s);
+  if (e != hipSuccess) return fail(ST_EXEC, "matmul_mx: kernel launch: %s", hipGetErrorString(e));
+  return ST_OK;
+}
+
+int32_t vecops_hip_rms_norm(const VecopsHipOperand* x, const VecopsHipOperand* weight, float eps, const VecopsHipOperand* residual,
+                            const VecopsHipOperand* summed, const VecopsHipOperand* q, const VecopsHipOperand* scales, const VecopsHipOperand* out,
+                            void* stream) {
+  View vx, vr = {}, vh = {}, vo = {};
+  if (!normalise(x, &vx)) return fail(ST_INVALID, "rms_norm: x must be rank 2 or 3 with non-negative extents");
+  if (real_kind(vx.dtype) < 0) return fail(ST_NOT_APPLICABLE, "rms_norm: x must be f32, bf16 or f16");
+  const int64_t k = vx.cols;
+  if (weight == nullptr || weight->rank != 1 || weight->sizes[0] != k || (k > 1 && weight->strides[0] != 1))
+    return fail(ST_INVALID, "rms_norm: weight must be a contiguous vector of %lld elements", (long long)k);
+  if (weight->dtype != vx.dtype && weight->dtype != DT_F32) return fail(ST_NOT_APPLICABLE, "rms_norm: weight must be of x's type or f32");
+  if (summed != nullptr && residual == nullptr) return fail(ST_INVALID, "rms_norm: a sum is written where there is a residual");
+  if (residual != nullptr && summed == nullptr) summed = residual;
+  if ((q == nullptr) != (scales == nullptr)) return fail(ST_INVALID, "rms_norm: q and scales come together");
+  if (q == nullptr && out == nullptr) return fail(ST_INVALID, "rms_norm: no result is asked for");
+  struct Beside {
+    const VecopsHipOperand* operand;
+    View* view;
+    const char* name;
+  };
+  for (const Beside& b : {Beside{residual, &vr, "residual"}, Beside{summed, &vh, "summed"}, Beside{out, &vo, "out"}}) {
+    if (b.operand == nullptr) continue;
+    if (!normalise(b.operand, b.view) || b.operand->rank != x->rank || !same_shape(*b.view, vx)) return fail(ST_INVALID, "rms_norm: %s must have x's shape", b.name);
+    if (b.view->dtype != vx.dtype) return fail(ST_NOT_APPLICABLE, "rms_norm: %s must be of x's type", b.name);
+    if (!rows_contiguous(*b.view)) return fail(ST_NOT_APPLICABLE, "rms_norm: rows of %s must be contiguous", b.name);
+    if (vx.batch * vx.rows * k > 0 && b.view->data == nullptr) return fail(ST_INVALID, "rms_norm: null operand");
+  }
+  if (!rows_contiguous(vx)) return fail(ST_NOT_APPLICABLE, "rms_norm: rows of x must be contiguous");
+  if (!row_extents_ok(vx.batch, vx.rows, k)) return fail(ST_INVALID, "rms_norm: extent too large");
+  RowQuantizeParams p = {};
+  p.format = ROW_NONE;
+  if (q != nullptr) {
+    const int32_t rc = describe_row_results("rms_norm", q, scales, x->rank, vx.batch, vx.rows, k, &p);
+    if (rc != ST_OK) return rc;
+  }
+  if (vx.batch == 0 || vx.rows == 0 || k == 0) return ST_OK;
+  if (vx.data == nullptr || weight->data == nullptr) return fail(ST_INVALID, "rms_norm: null operand");
+  p.x = vx.data, p.residual = vr.data, p.summed = vh.data, p.weight = weight->data, p.out = vo.data;
+  p.x_bs = vx.bs, p.x_rs = vx.rs, p.residual_bs = vr.bs, p.residual_rs = vr.rs, p.summed_bs = vh.bs, p.summed_rs = vh.rs, p.out_bs = vo.bs, p.out_rs = vo.rs;
+  p.batch = static_cast<int32_t>(vx.batch), p.rows = static_cast<int32_t>(vx.rows), p.k = static_cast<int32_t>(k);
+  p.kind = real_kind(vx.dtype);
+  p.weight_kind = real_kind(weight->dtype);
+  p.eps = eps;
+  const hipError_t e = launch_rms_norm(p, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(ST_EXEC, "rms_norm: kernel launch: %s", hipGetErrorString(e));
+  return ST_OK;
+}
+
+int32_t vecops_hip_silu_mul_quantize(const VecopsHipOperand* gate_up, const VecopsHipOperand* q, const VecopsHipOperand* scales, void* stream) {
+  View vx;
+  if (!normalise(gate_up, &vx)) return fail(ST_INVALID, "silu_mul_quantize: gate_up must be rank 2 or 3 with non-negative extents");
+  if (real_kind(vx.dtype) < 0) return fail(ST_NOT_APPLICABLE, "silu_mul_quantize: gate_up must be f32, bf16 or f16");
+  if (vx.cols % 2 != 0) return fail(ST_INVALID, "silu_mul_quantize: rows must be gates and as many factors, got %lld elements", (long long)vx.cols);
+  if (!rows_contiguous(vx)) return fail(ST_NOT_APPLICABLE, "silu_mul_quantize: rows of gate_up must be contiguous");
+  const int64_t k = vx.cols / 2;
+  if (!row_extents_ok(vx.batch, vx.rows, k)) return fail(ST_INVALID, "silu_mul_quantize: extent too large");
+  RowQuantizeParams p = {};
+  const int32_t rc = describe_row_results("silu_mul_quantize", q, scales, gate_up->rank, vx.batch, vx.rows, k, &p);
+  if (rc != ST_OK) return rc;
+  if (vx.batch == 0 || vx.rows == 0 || k == 0) return ST_OK;
+  if (vx.data == nullptr) return fail(ST_INVALID, "silu_mul_quantize: null operand");
+  p.x = vx.data, p.x_bs = vx.bs, p.x_rs = vx.rs;
+  p.batch = static_cast<int32_t>(vx.batch), p.rows = static_cast<int32_t>(vx.rows), p.k = static_cast<int32_t>(k);
+  p.kind = real_kind(vx.dtype);
+  const hipError_t e = launch_silu_mul(p, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(ST_EXEC, "silu_mul_quantize: kernel launch: %s", hipGetErrorString(e));
   return ST_OK;
 }
 

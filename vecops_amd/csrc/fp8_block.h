@@ -40,6 +40,16 @@ struct Fp8MatmulParams {
   float* partial;
 };
 
+// Shares of a product's sums, added in order: c = sum over `splits` of partial[s][batch][m][n], as `out_kind`.
+struct JoinSharesParams {
+  const float* partial;
+  void* c;
+  int64_t c_rs, c_cs, c_bs;
+  int32_t m, n, batch, splits;
+  int32_t out_kind;  // Fp8Real
+};
+hipError_t launch_join_shares(const JoinSharesParams& p, hipStream_t stream);
+
 // block_rows 1 or 128
 hipError_t launch_fp8_quantize(const Fp8QuantizeParams& p, int block_rows, hipStream_t stream);
 

@@ -1,0 +1,41 @@
+// Parameters and launchers of the product of microscaled operands (mx_block.hip).
+#ifndef VECOPS_HIP_MX_BLOCK_H
+#define VECOPS_HIP_MX_BLOCK_H
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "row_quantize.h"
+
+namespace vecops_hip {
+
+struct MxMatmulParams {
+  const uint8_t* a;  // activations [batch][m][k]: e2m1 two a byte, or e4m3; a row's bytes follow one another
+  const uint8_t* b;  // weights [batch][n][k], e2m1
+  const uint8_t* a_scales;  // [batch][m][groups], a row's follow one another
+  const uint8_t* b_scales;  // [batch][n][groups]
+  void* c;                  // [batch][m][n]
+  int64_t lda, ldb, a_bs, b_bs;   // bytes
+  int64_t as_rs, as_bs, bs_rs, bs_bs;
+  int64_t c_rs, c_cs, c_bs;
+  int32_t m, n, batch;
+  int32_t groups;      // blocks of 32 along k, each whole
+  int32_t row_scales;  // scales of a row that can be read: groups, at least four
+  int32_t a_wide;    // a is e4m3
+  int32_t out_kind;  // Fp8Real
+  int32_t splits;    // shares of k; more than one leave through `partial`, [splits][batch][m][n]
+  float* partial;
+};
+
+// The kernels: up to sixteen rows; tiles of 64 x 64, 128 x 128, and 256 weight rows x 256 (with e4m3 activations x 128).
+enum MxKind : int { MX_FEW_ROWS = 0, MX_TILE_64, MX_TILE_128, MX_TILE_256 };
+struct MxPlan {
+  int kind;
+  int splits;  // shares of k; more than one need `partial`
+  int rows_a, rows_b;  // of an operand, that a workgroup reaches by offsets below 2 GiB
+};
+MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int64_t batch, bool a_wide);
+hipError_t launch_mx_matmul(const MxMatmulParams& p, int kind, hipStream_t stream);
+
+}  // namespace vecops_hip
+#endif

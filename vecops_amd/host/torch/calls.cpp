@@ -271,15 +271,18 @@ int matmul_packed_b(PyObject* const* args) {
   });
 }
 
-// describe() for the entry points that take 8-bit floats too.
+// describe() for the entry points that take floats of 8 and 4 bits too.
 bool describe_any(PyObject* object, VecopsHipOperand* o) {
   const at::Tensor* t = plain_tensor(object);
   if (t == nullptr) return false;
-  if (t->scalar_type() != at::kFloat8_e4m3fn) return describe(*t, o);
+  const uint32_t dtype = t->scalar_type() == at::kFloat8_e4m3fn ? VECOPS_HIP_DTYPE_F8E4M3
+                         : t->scalar_type() == at::kFloat8_e8m0fnu ? VECOPS_HIP_DTYPE_F8E8M0
+                         : t->scalar_type() == at::kFloat4_e2m1fn_x2 ? VECOPS_HIP_DTYPE_F4E2M1X2 : 0;
+  if (dtype == 0) return describe(*t, o);
   const int64_t rank = t->dim();
   if (rank > 3) return false;
   memset(o, 0, sizeof(*o));
-  o->dtype = VECOPS_HIP_DTYPE_F8E4M3;
+  o->dtype = dtype;
   o->data = t->data_ptr();
   o->rank = static_cast<uint32_t>(rank);
   for (int64_t i = 0; i < rank; ++i) {
@@ -334,6 +337,44 @@ int matmul_fp8_block(PyObject* const* args) {
     const Workspace workspace(given, vecops_hip_matmul_fp8_block_workspace(&o[0], &o[1], &o[2], &o[3], &o[4]));
     return vecops_hip_matmul_fp8_block(&o[0], &o[1], &o[2], &o[3], &o[4], workspace.data, workspace.size, current_stream());
   });
+}
+
+// quantize_mx(x, q, scales), dequantize_mx(q, scales, out), silu_mul_quantize(gate_up, q, scales)
+template <int32_t (*CALL)(const VecopsHipOperand*, const VecopsHipOperand*, const VecopsHipOperand*, void*)>
+int three_operands(PyObject* const* args) {
+  VecopsHipOperand o[3];
+  for (int i = 0; i < 3; ++i)
+    if (!describe_any(args[i], &o[i])) return kNotPlain;
+  if (!on_current_device({args[0], args[1], args[2]})) return kNotPlain;
+  return without_lock([&] { return CALL(&o[0], &o[1], &o[2], current_stream()); });
+}
+constexpr auto quantize_mx = three_operands<vecops_hip_quantize_mx>;
+constexpr auto dequantize_mx = three_operands<vecops_hip_dequantize_mx>;
+constexpr auto silu_mul_quantize = three_operands<vecops_hip_silu_mul_quantize>;
+
+// matmul_mx(a, a_scales, b, b_scales, c, workspace)
+int matmul_mx(PyObject* const* args) {
+  VecopsHipOperand o[5];
+  for (int i = 0; i < 5; ++i)
+    if (!describe_any(args[i], &o[i])) return kNotPlain;
+  Given given;
+  if (!given.describe(args[5], *plain_tensor(args[4])) || !on_current_device({args[0], args[1], args[2], args[3], args[4], args[5]})) return kNotPlain;
+  return without_lock([&]() -> int {
+    const Workspace workspace(given, vecops_hip_matmul_mx_workspace(&o[0], &o[1], &o[2], &o[3], &o[4]));
+    return vecops_hip_matmul_mx(&o[0], &o[1], &o[2], &o[3], &o[4], workspace.data, workspace.size, current_stream());
+  });
+}
+
+// rms_norm(x, weight, residual, summed, q, scales, out, eps)
+int rms_norm(PyObject* const* args) {
+  VecopsHipOperand x, weight;
+  Optional residual, summed, q, scales, out;
+  if (!describe_any(args[0], &x) || !describe_any(args[1], &weight) || !residual.describe(args[2]) || !summed.describe(args[3]) ||
+      !q.describe(args[4]) || !scales.describe(args[5]) || !out.describe(args[6]) || !PyFloat_Check(args[7]) ||
+      !on_current_device({args[0], args[1], args[2], args[3], args[4], args[5], args[6]}))
+    return kNotPlain;
+  const float eps = static_cast<float>(PyFloat_AS_DOUBLE(args[7]));
+  return without_lock([&] { return vecops_hip_rms_norm(&x, &weight, eps, residual.at, summed.at, q.at, scales.at, out.at, current_stream()); });
 }
 
 // moe_experts(x, ids, weights, gate_up, gate_up_scales, down, down_scales, out, workspace)
@@ -605,6 +646,11 @@ PyMethodDef methods[] = {VECOPS_ENTRY(matmul, 6),
                          VECOPS_ENTRY(matmul_packed_b, 7),
                          VECOPS_ENTRY(quantize_fp8_block, 4),
                          VECOPS_ENTRY(matmul_fp8_block, 6),
+                         VECOPS_ENTRY(quantize_mx, 3),
+                         VECOPS_ENTRY(dequantize_mx, 3),
+                         VECOPS_ENTRY(matmul_mx, 6),
+                         VECOPS_ENTRY(rms_norm, 8),
+                         VECOPS_ENTRY(silu_mul_quantize, 3),
                          VECOPS_ENTRY(moe_experts, 9),
                          VECOPS_ENTRY(moe_layer, 11),
                          {nullptr, nullptr, 0, nullptr}};
