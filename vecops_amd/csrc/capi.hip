@@ -2938,12 +2938,12 @@ uint64_t mx_copy_bytes(const View& v, int64_t k, int64_t rows) {
   return round_up_256(static_cast<uint64_t>(v.bs == 0 ? 1 : v.batch) * static_cast<uint64_t>(v.rows) * static_cast<uint64_t>(mx_row_bytes(v)));
 }
 
-// Scales likewise: a row's follow one another, at least four of them, rows up to 2^20 apart.
-bool mx_scales_ok(const View& v) { return v.cs == 1 && v.cols >= 4 && v.rs >= 0 && v.rs <= (int64_t{1} << 20); }
-int64_t mx_scale_row_bytes(const View& v) { return (v.cols + 3) / 4 * 4; }
-uint64_t mx_scale_copy_bytes(const View& v) {
-  if (v.batch == 0 || v.rows == 0 || v.cols == 0 || mx_scales_ok(v)) return 0;
-  return round_up_256(static_cast<uint64_t>(v.bs == 0 ? 1 : v.batch) * static_cast<uint64_t>(v.rows) * static_cast<uint64_t>(mx_scale_row_bytes(v)));
+// Scales likewise: a row's follow one another, at least as many as the plan's kernel reads at once, rows up to 2^20 apart.
+bool mx_scales_ok(const View& v, int least) { return v.cs == 1 && v.cols >= least && v.rs >= 0 && v.rs <= (int64_t{1} << 20); }
+int64_t mx_scale_row_bytes(const View& v, int least) { return (std::max<int64_t>(v.cols, least) + 3) / 4 * 4; }
+uint64_t mx_scale_copy_bytes(const View& v, int least) {
+  if (v.batch == 0 || v.rows == 0 || v.cols == 0 || mx_scales_ok(v, least)) return 0;
+  return round_up_256(static_cast<uint64_t>(v.bs == 0 ? 1 : v.batch) * static_cast<uint64_t>(v.rows) * static_cast<uint64_t>(mx_scale_row_bytes(v, least)));
 }
 
 struct MxProduct {
@@ -2954,7 +2954,7 @@ struct MxProduct {
 
 uint64_t mx_workspace_bytes(const MxProduct& pr) {
   if (pr.a.batch == 0 || pr.a.rows == 0 || pr.b.rows == 0) return 0;
-  return mx_copy_bytes(pr.a, pr.k, pr.plan.rows_a) + mx_copy_bytes(pr.b, pr.k, pr.plan.rows_b) + mx_scale_copy_bytes(pr.sa) + mx_scale_copy_bytes(pr.sb) +
+  return mx_copy_bytes(pr.a, pr.k, pr.plan.rows_a) + mx_copy_bytes(pr.b, pr.k, pr.plan.rows_b) + mx_scale_copy_bytes(pr.sa, pr.plan.scales) + mx_scale_copy_bytes(pr.sb, pr.plan.scales) +
          (pr.plan.splits == 1 ? 0 : static_cast<uint64_t>(pr.plan.splits) * pr.a.batch * pr.a.rows * pr.b.rows * 4u);
 }
 
@@ -3081,7 +3081,8 @@ int32_t vecops_hip_matmul_mx(const VecopsHipOperand* a, const VecopsHipOperand* 
     return e;
   };
   for (const hipError_t e : {copy(&pr.a, mx_copy_bytes(pr.a, pr.k, pr.plan.rows_a), mx_row_bytes(pr.a)), copy(&pr.b, mx_copy_bytes(pr.b, pr.k, pr.plan.rows_b), mx_row_bytes(pr.b)),
-                             copy(&pr.sa, mx_scale_copy_bytes(pr.sa), mx_scale_row_bytes(pr.sa)), copy(&pr.sb, mx_scale_copy_bytes(pr.sb), mx_scale_row_bytes(pr.sb))})
+                             copy(&pr.sa, mx_scale_copy_bytes(pr.sa, pr.plan.scales), mx_scale_row_bytes(pr.sa, pr.plan.scales)),
+                             copy(&pr.sb, mx_scale_copy_bytes(pr.sb, pr.plan.scales), mx_scale_row_bytes(pr.sb, pr.plan.scales))})
     if (e != hipSuccess) return fail(ST_EXEC, "matmul_mx: kernel launch: %s", hipGetErrorString(e));
   MxMatmulParams p;
   p.a = static_cast<const uint8_t*>(pr.a.data), p.b = static_cast<const uint8_t*>(pr.b.data);
@@ -3092,7 +3093,7 @@ int32_t vecops_hip_matmul_mx(const VecopsHipOperand* a, const VecopsHipOperand* 
   p.c_rs = pr.c.rs, p.c_cs = pr.c.cs, p.c_bs = pr.c.bs;
   p.m = static_cast<int32_t>(pr.a.rows), p.n = static_cast<int32_t>(pr.b.rows), p.batch = static_cast<int32_t>(pr.a.batch);
   p.groups = static_cast<int32_t>(mx_blocks(pr.k));
-  p.row_scales = std::max(p.groups, 4);   // (rows of fewer have been padded with zeros, which stand for numbers; their elements are not there)
+  p.row_scales = std::max(p.groups, pr.plan.scales);   // (rows of fewer have been padded with zeros, which stand for numbers; their elements are not there)
   p.a_wide = pr.a.dtype == DT_E4M3;
   p.out_kind = real_kind(pr.c.dtype);
   p.splits = pr.plan.splits;

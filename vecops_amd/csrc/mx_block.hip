@@ -34,32 +34,23 @@ __device__ __forceinline__ f32x4 mfma_mx(const i32x8& w, const i32x8& x, const f
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 4, A8 ? 0 : 4, OPSEL, static_cast<int>(sw), OPSEL, static_cast<int>(sx));
 }
 
+// The same of 32 x 32 results over 64 k.
+template <bool A8, int OPSEL>
+__device__ __forceinline__ f32x16 mfma_mx_32(const i32x8& w, const i32x8& x, const f32x16& c, uint32_t sw, uint32_t sx) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w, x, c, 4, A8 ? 0 : 4, OPSEL, static_cast<int>(sw), OPSEL, static_cast<int>(sx));
+}
+
 __device__ __forceinline__ i32x8 narrow_fragment(const u32x4& v) {
   return i32x8{static_cast<int>(v[0]), static_cast<int>(v[1]), static_cast<int>(v[2]), static_cast<int>(v[3]), 0, 0, 0, 0};
 }
 
-// One buffer load of 4 bytes a lane that writes LDS itself, as load_16_bytes_into_lds: lane l's land at tile_address + tile_offset + 4 l.
-__device__ __forceinline__ void load_4_bytes_into_lds(const u32x4& descriptor, uint32_t tile_address, uint32_t tile_offset, uint32_t lane_offset) {
-#if defined(__HIP_DEVICE_COMPILE__)
-  asm volatile("s_add_u32 m0, %0, %1\n\ts_nop 0\n\tbuffer_load_dword %2, %3, 0 offen lds"
-               :
-               : "s"(tile_address), "s"(tile_offset), "v"(lane_offset), "s"(descriptor)
-               : "memory", "m0", "scc");
-#else
-  (void)descriptor; (void)tile_address; (void)tile_offset; (void)lane_offset;
-#endif
-}
-
 // Matrix results are read by other instructions only behind this: the compiler has been seen to leave too few wait states where a
 // branch stands between the two.
-template <int N>
-__device__ __forceinline__ void settle(f32x4 (&acc)[N]) {
+__device__ __forceinline__ void settle() {
 #if defined(__HIP_DEVICE_COMPILE__)
-  asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(acc[i]));
-#else
-  (void)acc;
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15\n\ts_nop 7" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
 #endif
 }
 
@@ -69,40 +60,62 @@ __device__ __forceinline__ void settle(f32x4 (&acc)[N]) {
 __device__ __forceinline__ int scale_word_at(int word, int groups) { return min(4 * word, groups - 4); }
 __device__ __forceinline__ uint32_t scale_shift(int word, int groups) { return static_cast<uint32_t>(min(max(4 * word + 4 - groups, 0) * 8, 31)); }
 
-// Many rows: WN x WM wavefronts, each NT x MT blocks of 16 x 16.  A stage is a step of 256 k of both operands and their scales;
-// STAGES of them are under way or in use, by loads that write LDS.
-// The rows of a wavefront's weights are dealt to its 16-row blocks so that a lane's results of two blocks are eight
-// consecutive n (row r of block 2 p + h is n = 32 p + 8 (r / 4) + 4 h + r % 4): sixteen bytes of a 16-bit result a store.
+// Many rows: WN x WM wavefronts, each NT x MT blocks of 32 x 32.  v_mfma_scale_f32_32x32x64_f8f6f4: a lane's e2m1 operand is block
+// l / 32 of two of row l % 32, an e4m3 one k 16 (l / 32) .. and 32 + 16 (l / 32) ..; its scale is that of block l / 32.  (One wavefront
+// on a SIMD keeps the matrix pipe to 8.5 PFLOP/s with it, on operands of zeros, and with the 16 x 16 one to 4.9: an instruction with scales
+// takes two issues.)
+// A stage is 256 k of both operands: whole lines of e2m1 rows (of half lines each is fetched twice).  STAGES of them are under way or
+// in use, by loads that write LDS.  Scales come two stages a run, sixteen bytes of a row a load: each is a request of its own to
+// the cache, which a word a row for each 128 k had by the half of all requests.  A row's last run is its last sixteen scales; what of it
+// has been summed before gets zeros for elements.
+// The rows of a block of weights are dealt so that a lane's sixteen results are neighbouring n (the instruction's row
+// 8 g + 4 h + e, which lane half h holds, is n = 16 h + 4 g + e).
+constexpr int kRunBlocks = 16;
+constexpr int min_of(int a, int b) { return a < b ? a : b; }
 template <int WN, int WM, int NT, int MT, bool A8, int STAGES>
 struct MxTile {
-  static constexpr int kBN = WN * NT * 16, kBM = WM * MT * 16, kWaves = WN * WM, kThreads = 64 * kWaves;
+  static constexpr int kBN = WN * NT * 32, kBM = WM * MT * 32, kWaves = WN * WM, kThreads = 64 * kWaves;
   static constexpr int kRowX = A8 ? 256 : 128, kChunksX = kRowX / 16;
-  static constexpr int kBytesW = kBN * 128, kBytesX = kBM * kRowX, kScalesW = kBytesW + kBytesX, kScalesX = kScalesW + kBN * 8;
-  static constexpr int kLoadsS = (kBN + kBM + 32 * kWaves - 1) / (32 * kWaves);   // (32 rows of scales a load; what the last ones load past the tile's rows is not read)
-  static constexpr int kStage = kScalesW + kLoadsS * kWaves * 256, kLds = STAGES * kStage;
-  static constexpr int kLoadsW = kBytesW / (kThreads * 16), kLoadsX = kBytesX / (kThreads * 16);
-  static constexpr int kLoads = kLoadsW + kLoadsX + kLoadsS;
-  static_assert(NT % 2 == 0, "results of two blocks leave together");
-  static_assert(kBytesW % (kThreads * 16) == 0 && kBytesX % (kThreads * 16) == 0, "whole loads");
-  static_assert(kLds <= 160 * 1024 && STAGES >= 2 && (STAGES - 1) * kLoads < 64, "LDS of a compute unit; the counter of loads");
+  static constexpr int kBytesW = kBN * 128, kBytesX = kBM * kRowX, kStage = kBytesW + kBytesX;
+  static constexpr int kLoadsW = kBytesW / (kThreads * 16), kLoadsX = kBytesX / (kThreads * 16), kLoadsS = (kBN + kBM + 64 * kWaves - 1) / (64 * kWaves);
+  static constexpr int kRuns = STAGES > 3 ? 4 : 2, kRun = kLoadsS * kWaves * 1024;   // (what the last loads of scales bring past the tile's rows is not read)
+  static constexpr int kScales = STAGES * kStage, kLds = kScales + kRuns * kRun;
+  static constexpr int loads(int stage) { return kLoadsW + kLoadsX + (stage % 2 == 0 ? kLoadsS : 0); }   // a run's scales come with its first stage
+  // loads of the stages from..to - 1 (of which only whether they are even matters)
+  static constexpr int loads_between(int from, int to) { return from >= to ? 0 : loads(from) + loads_between(from + 1, to); }
+  // kEarly: of a buffer that is multiplied, only the second pair of block rows is still to be read soon after the stage has begun.  The rest of it -
+  // activations, the first pair's weights (a load is 32 rows, a block row), scales - is refilled from there on: kLate loads less.
+  static constexpr bool kEarly = STAGES == 2 && NT == 4 && kThreads == 256;
+  static constexpr int kLate = kEarly ? kLoadsW / 2 : 0;
+  // nth load of those that come early, and of those that come late
+  static constexpr int early_piece(int nth) { return nth < kLoadsW / 2 ? nth / 2 * 4 + nth % 2 : nth + kLoadsW / 2; }
+  static constexpr int late_piece(int nth) { return nth / 2 * 4 + 2 + nth % 2; }
+  static_assert(NT % 2 == 0 && kBN % 64 == 0 && kBM % 64 == 0 && kBytesW % (kThreads * 16) == 0 && kBytesX % (kThreads * 16) == 0, "pairs of block rows; whole loads");
+  static_assert(kThreads / 8 % 16 == 0 && kThreads / kChunksX % 8 == 0, "a thread's rows have equal keys, or two in turn");
+  static_assert(kLds <= 160 * 1024 && STAGES >= 2 && STAGES <= 4 && STAGES * loads(0) < 64, "LDS of a compute unit; the counter of loads");
 };
 
-// slot of a chunk in its 128 bytes: rows that a fragment reads together lie in different slots
-__device__ __forceinline__ int slot_key_w(int row) { return (row & 3) | ((row >> 1) & 4); }
-__device__ __forceinline__ int slot_key_x(int row) { return row & 7; }
+// Slot of a chunk among a row's.  LDS serves sixteen-byte reads of lanes 0-3, 12-15, 20-27 together, then of 4-11, 16-19, 28-31, and so on: rows
+// of either set (in both orders in which lanes have them) lie in different sixteen bytes of 256.
+template <int BYTES>
+__device__ __forceinline__ int slot_key(int row) { return BYTES == 128 ? (row >> 1) & 7 : row & 15; }
 
-template <int WN, int WM, int NT, int MT, bool A8, int STAGES>
-__global__ __launch_bounds__(64 * WN * WM, 2) void mx_tile_kernel(const MxMatmulParams p, uint32_t tiles_n, uint32_t tiles_m) {
+// One wavefront: two block rows at a time against every block column of the activations, whose fragments stay in registers for the
+// stage.  While a pair's products are formed the next one's weights are fetched, and beside the last pair the next stage's
+// activations, each into the registers that its last product has read.  So in front of the last pair all of the stage has been read: there the next stage
+// has landed, the wavefronts meet, and behind that this stage's buffer is refilled, a load behind each matrix instruction.
+template <int WN, int WM, int NT, int MT, bool A8, int STAGES, int WAVES_A_SIMD>
+__global__ __launch_bounds__(64 * WN * WM, WAVES_A_SIMD) void mx_tile_kernel(const MxMatmulParams p, uint32_t tiles_n, uint32_t tiles_m) {
   using T = MxTile<WN, WM, NT, MT, A8, STAGES>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t lds0 = lds_address_of(lds);
   const int batch = blockIdx.y;
-  // this workgroup's share of the steps
-  const int steps = (p.groups + kStepBlocks - 1) / kStepBlocks;
-  const int g_begin = static_cast<int>(static_cast<int64_t>(steps) * blockIdx.z / p.splits);
-  const int g_end = static_cast<int>(static_cast<int64_t>(steps) * (blockIdx.z + 1) / p.splits);
+  // this workgroup's share of the runs
+  const int runs = (p.groups + kRunBlocks - 1) / kRunBlocks;
+  const int run_begin = static_cast<int>(static_cast<int64_t>(runs) * blockIdx.z / p.splits);
+  const int run_end = static_cast<int>(static_cast<int64_t>(runs) * (blockIdx.z + 1) / p.splits);
 
   // neighbouring tiles on one die: each die's workgroups (every eighth) take a contiguous run of tiles, walked in groups of
   // eight tile rows
@@ -119,142 +132,221 @@ __global__ __launch_bounds__(64 * WN * WM, 2) void mx_tile_kernel(const MxMatmul
   const int last_n = static_cast<int>(min(p.n - n0, static_cast<int64_t>(T::kBN))) - 1;
 
   // Rows past the operand's last one lie past the descriptors' ends: zeros arrive.
-  const uint32_t row_w = static_cast<uint32_t>(p.groups) * 16u, row_x = static_cast<uint32_t>(p.groups) * (A8 ? 32u : 16u);
   u32x4 desc_w = tile_buffer_words((const VECOPS_GLOBAL char*)p.b + batch * p.b_bs + n0 * p.ldb);
   u32x4 desc_x = tile_buffer_words((const VECOPS_GLOBAL char*)p.a + batch * p.a_bs + m0 * p.lda);
-  u32x4 desc_sw = tile_buffer_words((const VECOPS_GLOBAL char*)p.b_scales + batch * p.bs_bs + n0 * p.bs_rs);
-  u32x4 desc_sx = tile_buffer_words((const VECOPS_GLOBAL char*)p.a_scales + batch * p.as_bs + m0 * p.as_rs);
-  const uint32_t end_w = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(last_n * p.ldb) + row_w);
-  const uint32_t end_x = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(last_m * p.lda) + row_x);
-  const uint32_t end_sw = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(last_n * p.bs_rs + p.row_scales));
-  const uint32_t end_sx = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(last_m * p.as_rs + p.row_scales));
+  const uint32_t end_w = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(last_n * p.ldb) + static_cast<uint32_t>(p.groups) * 16u);
+  const uint32_t end_x = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(last_m * p.lda) + static_cast<uint32_t>(p.groups) * (A8 ? 32u : 16u));
 
-  // load i of a thread: sixteen bytes of row i * kRowsW + tid / 8, the chunk whose slot is tid % 8 (rows apart by kRowsW have
-  // equal keys); e4m3 rows have sixteen slots
+  // load i of a thread: sixteen bytes of row i * kRowsW + tid / chunks, the chunk whose slot is tid % chunks
   constexpr int kRowsW = T::kThreads / 8, kRowsX = T::kThreads / T::kChunksX;
-  static_assert(kRowsW % 16 == 0 && kRowsX % 8 == 0, "equal keys");
   const int at_row_w = tid / 8, at_row_x = tid / T::kChunksX;
-  const uint32_t chunk_w = ((tid & 7) ^ slot_key_w(at_row_w)) << 4, chunk_x = ((tid & (T::kChunksX - 1)) ^ slot_key_x(at_row_x)) << 4;
-  const uint32_t from_w = static_cast<uint32_t>(at_row_w * p.ldb) + chunk_w, from_x = static_cast<uint32_t>(at_row_x * p.lda) + chunk_x;
+  const int chunk_w = (tid & 7) ^ slot_key<128>(at_row_w), chunk_x = (tid & (T::kChunksX - 1)) ^ slot_key<T::kRowX>(at_row_x);
+  constexpr int kTurn = kRowsX % 16 == 0 ? 0 : 8;   // (rows sixteen apart have equal keys; eight apart, those of 256 bytes, keys that differ by eight)
+  const uint32_t from_w = static_cast<uint32_t>(at_row_w * p.ldb) + chunk_w * 16, from_x = static_cast<uint32_t>(at_row_x * p.lda) + chunk_x * 16;
+  const uint32_t from_x_odd = static_cast<uint32_t>(at_row_x * p.lda) + (chunk_x ^ kTurn) * 16;
   const uint32_t add_w = static_cast<uint32_t>(kRowsW * p.ldb), add_x = static_cast<uint32_t>(kRowsX * p.lda);
-  // the scales: 32 rows an instruction, a lane one of a row's two words; instruction u of the stage goes to wavefront u % waves
-  uint32_t from_s[T::kLoadsS];
+  const int block_x = A8 ? chunk_x >> 1 : chunk_x, block_x_odd = A8 ? (chunk_x ^ kTurn) >> 1 : chunk_x;   // of the stage's eight
+  // the scales: 64 rows an instruction; instruction u goes to wavefront u % waves
+  u32x4 desc_s[T::kLoadsS];
+  uint32_t end_s[T::kLoadsS], from_s[T::kLoadsS];
 #pragma unroll
   for (int i = 0; i < T::kLoadsS; ++i) {
-    const int u = i * T::kWaves + wave, row = 32 * u + (lane >> 1);
-    from_s[i] = u < T::kBN / 32 ? static_cast<uint32_t>(row * p.bs_rs) : static_cast<uint32_t>((row - T::kBN) * p.as_rs);
+    const int rows = 64 * (i * T::kWaves + wave);
+    const bool weights = rows < T::kBN;
+    const int64_t rs = weights ? p.bs_rs : p.as_rs;
+    desc_s[i] = tile_buffer_words(weights ? (const VECOPS_GLOBAL char*)p.b_scales + batch * p.bs_bs + n0 * p.bs_rs
+                                          : (const VECOPS_GLOBAL char*)p.a_scales + batch * p.as_bs + m0 * p.as_rs);
+    end_s[i] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>((weights ? last_n : last_m) * rs + p.row_scales));
+    from_s[i] = static_cast<uint32_t>((rows - (weights ? 0 : T::kBN) + lane) * rs);
   }
 
-  // load PIECE of those that fill stage `slot` with step g; past the last step nothing is fetched (but as many loads are issued)
-  auto issue_piece = [&](auto piece_tag, int g, int slot) {
-    constexpr int PIECE = decltype(piece_tag)::value;
-    const uint32_t stage = lds0 + slot * T::kStage;
-    const bool there = g < g_end;
+  // load PIECE of those that fill buffer `slot` with half PAR of run `run`; past the last run nothing is fetched (but as many loads are issued)
+  auto issue_piece = [&](auto piece_tag, auto par_tag, int run, int slot) {
+    constexpr int PIECE = decltype(piece_tag)::value, PAR = decltype(par_tag)::value;
+    const bool there = run < run_end;
+    const int first_block = min(run * kRunBlocks, p.row_scales - kRunBlocks);   // the run's sixteen blocks
+    // those before `old` have been summed; those from `most` on are not there
+    const int old = run * kRunBlocks - first_block - 8 * PAR, most = p.groups - first_block - 8 * PAR;
     if constexpr (PIECE < T::kLoadsW) {
-      const uint32_t k0 = static_cast<uint32_t>(g) * 128u;
       desc_w[2] = there ? end_w : 0u;
-      load_16_bytes_into_lds(desc_w, stage, __builtin_amdgcn_readfirstlane(PIECE * (T::kThreads * 16) + wave * 1024),
-                             k0 + chunk_w < row_w ? from_w : kNowhere, __builtin_amdgcn_readfirstlane(PIECE * add_w + k0));
+      load_16_bytes_into_lds(desc_w, lds0 + slot * T::kStage, __builtin_amdgcn_readfirstlane(PIECE * (T::kThreads * 16) + wave * 1024),
+                             chunk_w >= old && chunk_w < most ? from_w : kNowhere,
+                             __builtin_amdgcn_readfirstlane(PIECE * add_w + static_cast<uint32_t>(first_block + 8 * PAR) * 16u));
     } else if constexpr (PIECE < T::kLoadsW + T::kLoadsX) {
       constexpr int AT = PIECE - T::kLoadsW;
-      const uint32_t k0 = static_cast<uint32_t>(g) * T::kRowX;
+      const int block = AT % 2 ? block_x_odd : block_x;
       desc_x[2] = there ? end_x : 0u;
-      load_16_bytes_into_lds(desc_x, stage, __builtin_amdgcn_readfirstlane(T::kBytesW + AT * (T::kThreads * 16) + wave * 1024),
-                             k0 + chunk_x < row_x ? from_x : kNowhere, __builtin_amdgcn_readfirstlane(AT * add_x + k0));
+      load_16_bytes_into_lds(desc_x, lds0 + slot * T::kStage, __builtin_amdgcn_readfirstlane(T::kBytesW + AT * (T::kThreads * 16) + wave * 1024),
+                             block >= old && block < most ? (AT % 2 ? from_x_odd : from_x) : kNowhere,
+                             __builtin_amdgcn_readfirstlane(AT * add_x + static_cast<uint32_t>(first_block + 8 * PAR) * (A8 ? 32u : 16u)));
     } else {
       constexpr int AT = PIECE - T::kLoadsW - T::kLoadsX;
-      const int u = AT * T::kWaves + wave;
-      const bool weights = u < T::kBN / 32;
-      u32x4 desc = weights ? desc_sw : desc_sx;
-      desc[2] = there ? (weights ? end_sw : end_sx) : 0u;
-      load_4_bytes_into_lds(desc, stage, __builtin_amdgcn_readfirstlane(T::kScalesW + u * 256), from_s[AT] + scale_word_at(2 * g + (lane & 1), p.row_scales));
+      desc_s[AT][2] = there ? end_s[AT] : 0u;
+      load_16_bytes_into_lds(desc_s[AT], lds0 + T::kScales + (run & (T::kRuns - 1)) * T::kRun, __builtin_amdgcn_readfirstlane((AT * T::kWaves + wave) * 1024), from_s[AT],
+                             __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(first_block)));
     }
   };
-  auto issue = [&](int g, int slot) { static_for<T::kLoads>([&](auto piece) { issue_piece(piece, g, slot); }); };
 
   const int wn = wave / WM, wm = wave % WM;
-  const int col = lane & 15, quarter = lane >> 4;
+  const int col = lane & 31, half = lane >> 5;
   // a lane's chunks of its row in block 0 (blocks apart by whole rows of equal keys)
-  uint32_t at_w[2], at_x[A8 ? 4 : 2];
-  {
-    const int row = wn * (NT * 16) + 8 * (col >> 2) + (col & 3), row_of_x = wm * (MT * 16) + col;
+  const int row_of_w = wn * (NT * 32) + 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3), row_of_x = wm * (MT * 32) + col;
+  uint32_t at_w[4], at_x[4][A8 ? 2 : 1];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      at_w[h] = lds0 + row * 128 + (((2 * quarter + h) ^ slot_key_w(row)) << 4);
-      if constexpr (A8) {
-        const int chunk = 4 * (quarter >> 1) + (quarter & 1) + 2 * h;   // half quarter % 2 of block 2 (quarter / 2) + h; the other: of that plus four blocks
-        at_x[2 * h] = lds0 + T::kBytesW + row_of_x * 256 + ((chunk ^ slot_key_x(row_of_x)) << 4);
-        at_x[2 * h + 1] = lds0 + T::kBytesW + row_of_x * 256 + (((chunk + 8) ^ slot_key_x(row_of_x)) << 4);
-      } else {
-        at_x[h] = lds0 + T::kBytesW + row_of_x * 128 + (((2 * quarter + h) ^ slot_key_x(row_of_x)) << 4);
-      }
-    }
+  for (int s = 0; s < 4; ++s) {
+    at_w[s] = lds0 + row_of_w * 128 + (((2 * s + half) ^ slot_key<128>(row_of_w)) << 4);
+#pragma unroll
+    for (int h = 0; h < (A8 ? 2 : 1); ++h)
+      at_x[s][h] = lds0 + T::kBytesW + row_of_x * T::kRowX + ((((A8 ? 4 : 2) * s + 2 * h + half) ^ slot_key<T::kRowX>(row_of_x)) << 4);
   }
-  const uint32_t at_sw = lds0 + T::kScalesW + (wn * (NT * 16) + 8 * (col >> 2) + (col & 3)) * 8 + (quarter >> 1) * 4;
-  const uint32_t at_sx = lds0 + T::kScalesX + (wm * (MT * 16) + col) * 8 + (quarter >> 1) * 4;
+  const uint32_t at_sw = lds0 + T::kScales + row_of_w * 16, at_sx = lds0 + T::kScales + (T::kBN + row_of_x) * 16;
 
-  f32x4 acc[NT * MT];
+  f32x16 acc[NT * MT];
 #pragma unroll
-  for (int i = 0; i < NT * MT; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < NT * MT; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
+  i32x8 x[4][MT], w[2][2][4];
+  u32x2 sx[2][MT], sw[2][2];   // a lane's scales of 64 k `s`: byte 2 (s % 2) of word s / 2, shifted down by its half
+  constexpr int kPairs = NT / 2, kMeet = 5;
+  // a stage's scales of one row
+  auto scales_at = [&](uint32_t at, int offset) {
+    const u32x2 v = read_lds_pair(at, offset);
+    return u32x2{v[0] >> (8 * half), v[1] >> (8 * half)};
+  };
+  auto read_w = [&](auto to_tag, auto i_tag, auto s_tag, uint32_t stage) {
+    constexpr int to = decltype(to_tag)::value, i = decltype(i_tag)::value, s = decltype(s_tag)::value;
+    w[to][i & 1][s] = narrow_fragment(read_lds(at_w[s] + stage, i * 4096));
+  };
+  auto read_x = [&](auto s_tag, auto j_tag, uint32_t stage) {
+    constexpr int s = decltype(s_tag)::value, j = decltype(j_tag)::value;
+    if constexpr (A8) x[s][j] = fragment_of(read_lds(at_x[s][0] + stage, j * 8192), read_lds(at_x[s][1] + stage, j * 8192));
+    else x[s][j] = narrow_fragment(read_lds(at_x[s][0] + stage, j * 4096));
+  };
 
-  if (g_begin < g_end) {
-#pragma unroll
-    for (int g = 0; g < STAGES - 1; ++g) issue(g_begin + g, g);
-    int slot = 0;
-    for (int g = g_begin; g < g_end; ++g) {
-      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((STAGES - 2) * T::kLoads) : "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      issue(g + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
-      const uint32_t stage = slot * T::kStage;
-      const uint32_t shift = 16u * (quarter & 1) + scale_shift(2 * g + (quarter >> 1), p.row_scales);
-      i32x8 x[MT][2];
-      uint32_t sx[MT];
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        sx[j] = read_lds_word(at_sx + stage, j * 128) >> min(shift, 31u);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if constexpr (A8) x[j][h] = fragment_of(read_lds(at_x[2 * h] + stage, j * 4096), read_lds(at_x[2 * h + 1] + stage, j * 4096));
-          else x[j][h] = narrow_fragment(read_lds(at_x[h] + stage, j * 2048));
+  // half PAR of a run, in buffer `slot`
+  auto multiply = [&](auto par_tag, int run, int slot) {
+    constexpr int PAR = decltype(par_tag)::value;
+    constexpr int AHEAD = PAR + STAGES;   // the stage, counted from the run's first, that takes this one's buffer
+    const int next_slot = slot + 1 == STAGES ? 0 : slot + 1;
+    const uint32_t stage = slot * T::kStage, next = next_slot * T::kStage;
+    const uint32_t run_at = (run & (T::kRuns - 1)) * T::kRun, next_run_at = PAR == 0 ? run_at : ((run + 1) & (T::kRuns - 1)) * T::kRun;
+    static_for<kPairs>([&](auto pair_tag) {
+      constexpr int pair = decltype(pair_tag)::value, now = (PAR * kPairs + pair) & 1, then = now ^ 1;
+      constexpr bool final_pair = pair + 1 == kPairs;
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (final_pair) {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(T::kEarly ? T::loads(AHEAD) - T::kLate : T::loads_between(PAR + 2, PAR + STAGES)) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+      }
+      // behind matrix instruction AT of the pair: the next pair's weights and scales, the next stage's activations, loads
+      auto beside = [&](auto at_tag) {
+        constexpr int AT = decltype(at_tag)::value, kAll = 8 * MT;
+        constexpr int from = AT * 8 / kAll, to = (AT + 1) * 8 / kAll;   // of eight fragments
+        static_for<to - from>([&](auto nth) {
+          constexpr int f = from + decltype(nth)::value;
+          constexpr int i = final_pair ? f & 1 : 2 * pair + 2 + (f & 1);
+          read_w(std::integral_constant<int, then>{}, std::integral_constant<int, i>{}, std::integral_constant<int, (f >> 1)>{}, final_pair ? next : stage);
+          if constexpr (f < 2)
+            sw[then][f] = scales_at(at_sw + (final_pair ? next_run_at : run_at), i * 512 + 8 * (final_pair ? 1 - PAR : PAR));
+        });
+        if constexpr (final_pair) {
+          if constexpr (AT < MT) sx[1 - PAR][AT] = scales_at(at_sx + next_run_at, AT * 512 + 8 * (1 - PAR));
+          if constexpr (AT % 2 == 1) read_x(std::integral_constant<int, AT / 2 / MT>{}, std::integral_constant<int, AT / 2 % MT>{}, next);
         }
-      }
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        // block 2 p + h starts 32 p + 4 h rows down; 4 rows down the key stays
-        const int down = (i >> 1) * 32 + (i & 1) * 4;
-        const uint32_t sw = read_lds_word(at_sw + stage, down * 8) >> min(shift, 31u);
-        const i32x8 w0 = narrow_fragment(read_lds(at_w[0] + stage, down * 128)), w1 = narrow_fragment(read_lds(at_w[1] + stage, down * 128));
-#pragma unroll
-        for (int j = 0; j < MT; ++j) acc[i * MT + j] = mfma_mx<A8, 0>(w0, x[j][0], acc[i * MT + j], sw, sx[j]);
-#pragma unroll
-        for (int j = 0; j < MT; ++j) acc[i * MT + j] = mfma_mx<A8, 1>(w1, x[j][1], acc[i * MT + j], sw, sx[j]);
-      }
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (this stage may be overwritten behind the next barrier)
-      slot = slot + 1 == STAGES ? 0 : slot + 1;
+        if constexpr (T::kEarly && !final_pair && AT == kMeet) {   // every wavefront has read what is refilled from here on
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+        }
+        constexpr int count = !T::kEarly ? (final_pair ? T::loads(AHEAD) : 0) : final_pair ? T::kLate : T::loads(AHEAD) - T::kLate;
+        constexpr int begin = T::kEarly && !final_pair ? kMeet : 0, per = (count + kAll - begin - 1) / (kAll - begin);
+        constexpr int a = AT < begin ? 0 : min_of((AT - begin) * per, count), b = AT < begin ? 0 : min_of((AT - begin + 1) * per, count);
+        static_for<b - a>([&](auto nth) {
+          constexpr int at = a + decltype(nth)::value, piece = !T::kEarly ? at : final_pair ? T::late_piece(at) : T::early_piece(at);
+          issue_piece(std::integral_constant<int, piece>{}, std::integral_constant<int, AHEAD % 2>{}, run + AHEAD / 2, slot);
+        });
+      };
+      static_for<4>([&](auto s_tag) {
+        static_for<MT>([&](auto j_tag) {
+          static_for<2>([&](auto i_tag) {
+            constexpr int s = decltype(s_tag)::value, j = decltype(j_tag)::value, i = decltype(i_tag)::value, at = (2 * pair + i) * MT + j;
+            acc[at] = mfma_mx_32<A8, 2 * (s & 1)>(w[now][i][s], x[s][j], acc[at], sw[now][i][s >> 1], sx[PAR][j][s >> 1]);
+            __builtin_amdgcn_sched_barrier(0);
+            beside(std::integral_constant<int, (s * MT + j) * 2 + i>{});
+            __builtin_amdgcn_sched_barrier(0);
+          });
+        });
+      });
+    });
+  };
+
+  if (run_begin < run_end) {
+    static_for<STAGES>([&](auto g) {
+      constexpr int G = decltype(g)::value;
+      static_for<T::loads(G)>([&](auto piece) { issue_piece(piece, std::integral_constant<int, G % 2>{}, run_begin + G / 2, G); });
+    });
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(T::loads_between(1, STAGES)) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    const uint32_t run_at = (run_begin & (T::kRuns - 1)) * T::kRun;
+    static_for<8>([&](auto f) {
+      constexpr int F = decltype(f)::value;
+      read_w(std::integral_constant<int, 0>{}, std::integral_constant<int, (F & 1)>{}, std::integral_constant<int, (F >> 1)>{}, 0);
+      if constexpr (F < 2) sw[0][F] = scales_at(at_sw + run_at, F * 512);
+    });
+    static_for<MT>([&](auto j) {
+      sx[0][decltype(j)::value] = scales_at(at_sx + run_at, decltype(j)::value * 512);
+      static_for<4>([&](auto s) { read_x(s, j, 0); });
+    });
+    int slot = 0;
+    const auto following = [](int at) { return at + 1 == STAGES ? 0 : at + 1; };
+    // (past the last stage: reads of a buffer that nothing has been fetched for, and loads that fetch nothing)
+    for (int run = run_begin; run < run_end; ++run) {
+      multiply(std::integral_constant<int, 0>{}, run, slot);
+      slot = following(slot);
+      multiply(std::integral_constant<int, 1>{}, run, slot);
+      slot = following(slot);
     }
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (no load may write LDS once the workgroup is gone)
-  settle(acc);
+  settle();
 
+  // Results leave 32 rows at a time by way of LDS, a wavefront's own part of it, so that a store instruction fills whole lines.
+  // Sixteen bytes of a row lie in slot (place ^ row % 16): neither way has conflicts.
+  const bool shares = p.splits > 1;
+  const int kind = shares ? static_cast<int>(FP8_REAL_F32) : p.out_kind;
+  const int64_t c_rs = shares ? p.n : p.c_rs, c_cs = shares ? 1 : p.c_cs;
+  char* const c = shares ? reinterpret_cast<char*>(p.partial + (static_cast<int64_t>(blockIdx.z) * p.batch + batch) * p.m * p.n)
+                         : static_cast<char*>(p.c) + batch * p.c_bs * (kind == FP8_REAL_F32 ? 4 : 2);
+  constexpr int kRow = NT * 32 * 4, kPieces = NT * 4, kRowsAtOnce = 64 / kPieces;   // bytes of a row; eights of results; rows an instruction
+  static_assert(T::kWaves * 32 * kRow <= T::kLds && kPieces >= 8, "room for 32 rows a wavefront; sixteen slots a row or more");
+  const uint32_t mine = lds0 + wave * (32 * kRow);
+  const int64_t m1 = m0 + wm * (MT * 32) + lane / kPieces, n1 = n0 + wn * (NT * 32) + lane % kPieces * 8;
+  __builtin_amdgcn_s_barrier();   // (other wavefronts may still be reading what this one overwrites)
+  asm volatile("" ::: "memory");
+  static_for<MT>([&](auto j_tag) {
+    constexpr int j = decltype(j_tag)::value;
+    static_for<NT>([&](auto i_tag) {
+      constexpr int i = decltype(i_tag)::value;
+      const f32x16 a = acc[i * MT + j];
 #pragma unroll
-  for (int j = 0; j < MT; ++j) {
-    const int64_t m = m0 + wm * (MT * 16) + j * 16 + col;
-    if (m < p.m) {
-#pragma unroll
-      for (int i = 0; i < NT; i += 2) {
-        const int64_t n = n0 + wn * (NT * 16) + i * 16 + quarter * 8;
-        const f32x4 lo = acc[i * MT + j], hi = acc[(i + 1) * MT + j];
-        const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        if (p.splits == 1) {
-          store_results<8>(p.c, batch * p.c_bs + m * p.c_rs + n * p.c_cs, p.c_cs, p.out_kind, n, p.n, v);
-        } else {
-          const int64_t line = (static_cast<int64_t>(blockIdx.z) * p.batch + batch) * p.m + m;
-          store_results<8>(p.partial, line * p.n + n, 1, FP8_REAL_F32, n, p.n, v);
-        }
-      }
+      for (int e = 0; e < 16; e += 4)
+        write_lds(mine + col * kRow + ((((i * 32 + e) / 4 + half * 4) ^ (col & 15)) << 4),
+                  u32x4{__float_as_uint(a[e]), __float_as_uint(a[e + 1]), __float_as_uint(a[e + 2]), __float_as_uint(a[e + 3])});
+      __builtin_amdgcn_sched_barrier(0);   // (a block at a time leaves the accumulators)
+    });
+#pragma unroll 1
+    for (int r = lane / kPieces; r < 32; r += kRowsAtOnce) {
+      const uint32_t at = mine + r * kRow, place = lane % kPieces * 2;
+      const u32x4 lo = read_lds(at + ((place ^ (r & 15)) << 4), 0), hi = read_lds(at + (((place + 1) ^ (r & 15)) << 4), 0);
+      const int64_t m = m1 + j * 32 + (r - lane / kPieces);
+      const float v[8] = {__uint_as_float(lo[0]), __uint_as_float(lo[1]), __uint_as_float(lo[2]), __uint_as_float(lo[3]),
+                          __uint_as_float(hi[0]), __uint_as_float(hi[1]), __uint_as_float(hi[2]), __uint_as_float(hi[3])};
+      if (m < p.m) store_results<8>(c, m * c_rs + n1 * c_cs, c_cs, kind, n1, p.n, v);
     }
-  }
+  });
 }
 
 // Up to sixteen rows: bound by HBM, so that what counts is how many bytes of the weights are under way.  A workgroup owns sixteen
@@ -329,7 +421,7 @@ __global__ __launch_bounds__(64 * WAVES, A8 ? 3 : 4) void mx_few_rows_kernel(con
       }
     });
   }
-  settle(acc);
+  settle();
 
   sums[wave][lane] = acc[0];
   __syncthreads();
@@ -351,41 +443,39 @@ hipError_t launch_few_rows(const MxMatmulParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <int WN, int WM, int NT, int MT, bool A8, int STAGES>
+template <int WN, int WM, int NT, int MT, bool A8, int STAGES, int WAVES_A_SIMD>
 hipError_t launch_tile(const MxMatmulParams& p, hipStream_t stream) {
   using T = MxTile<WN, WM, NT, MT, A8, STAGES>;
-  const void* kernel = reinterpret_cast<const void*>(&mx_tile_kernel<WN, WM, NT, MT, A8, STAGES>);
+  constexpr auto kernel = &mx_tile_kernel<WN, WM, NT, MT, A8, STAGES, WAVES_A_SIMD>;
   if constexpr (T::kLds > 65536) {
-    const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds);
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds);
     if (e != hipSuccess) return e;
   }
   const uint32_t tiles_n = static_cast<uint32_t>((p.n + T::kBN - 1) / T::kBN), tiles_m = static_cast<uint32_t>((p.m + T::kBM - 1) / T::kBM);
-  hipLaunchKernelGGL((mx_tile_kernel<WN, WM, NT, MT, A8, STAGES>), dim3(tiles_n * tiles_m, static_cast<uint32_t>(p.batch), static_cast<uint32_t>(p.splits)),
-                     dim3(T::kThreads), T::kLds, stream, p, tiles_n, tiles_m);
-  if (p.splits > 1) {
-    const hipError_t e = hipGetLastError();
-    return e != hipSuccess ? e : launch_join_shares({p.partial, p.c, p.c_rs, p.c_cs, p.c_bs, p.m, p.n, p.batch, p.splits, p.out_kind}, stream);
-  }
-  return hipGetLastError();
+  hipLaunchKernelGGL(kernel, dim3(tiles_n * tiles_m, static_cast<uint32_t>(p.batch), static_cast<uint32_t>(p.splits)), dim3(T::kThreads), T::kLds, stream, p, tiles_n,
+                     tiles_m);
+  const hipError_t e = hipGetLastError();
+  if (p.splits == 1 || e != hipSuccess) return e;
+  return launch_join_shares({p.partial, p.c, p.c_rs, p.c_cs, p.c_bs, p.m, p.n, p.batch, p.splits, p.out_kind}, stream);
 }
 
 }  // namespace
 
 MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int64_t batch, bool a_wide) {
   (void)k;
-  if (m <= 16) return {MX_FEW_ROWS, 1, 16, 16};
+  if (m <= 16) return {MX_FEW_ROWS, 1, 16, 16, 4};
   const int64_t big = ((m + (a_wide ? 127 : 255)) / (a_wide ? 128 : 256)) * ((n + 255) / 256) * batch, middle = ((m + 127) / 128) * ((n + 127) / 128) * batch;
-  if (big >= 192) return {MX_TILE_256, 1, a_wide ? 128 : 256, 256};
-  if (middle >= 128) return {MX_TILE_128, 1, 128, 128};
-  return {MX_TILE_64, 1, 64, 64};
+  if (big >= 192) return {MX_TILE_256, 1, a_wide ? 128 : 256, 256, kRunBlocks};
+  if (middle >= 128) return {MX_TILE_128, 1, 128, 128, kRunBlocks};
+  return {MX_TILE_64, 1, 64, 64, kRunBlocks};
 }
 
 hipError_t launch_mx_matmul(const MxMatmulParams& p, int kind, hipStream_t stream) {
   switch (kind) {
     case MX_FEW_ROWS: return p.a_wide ? launch_few_rows<true>(p, stream) : launch_few_rows<false>(p, stream);
-    case MX_TILE_64: return p.a_wide ? launch_tile<2, 2, 2, 2, true, 4>(p, stream) : launch_tile<2, 2, 2, 2, false, 4>(p, stream);
-    case MX_TILE_128: return p.a_wide ? launch_tile<2, 2, 4, 4, true, 3>(p, stream) : launch_tile<2, 2, 4, 4, false, 4>(p, stream);
-    case MX_TILE_256: return p.a_wide ? launch_tile<2, 4, 8, 2, true, 2>(p, stream) : launch_tile<2, 4, 8, 4, false, 2>(p, stream);
+    case MX_TILE_64: return p.a_wide ? launch_tile<1, 2, 2, 1, true, 3, 2>(p, stream) : launch_tile<1, 2, 2, 1, false, 3, 2>(p, stream);
+    case MX_TILE_128: return p.a_wide ? launch_tile<2, 2, 2, 2, true, 2, 2>(p, stream) : launch_tile<2, 2, 2, 2, false, 2, 2>(p, stream);
+    case MX_TILE_256: return p.a_wide ? launch_tile<2, 2, 4, 2, true, 2, 1>(p, stream) : launch_tile<2, 2, 4, 4, false, 2, 1>(p, stream);
   }
   return hipErrorInvalidValue;
 }
