@@ -72,24 +72,29 @@ __device__ __forceinline__ uint32_t scale_shift(int word, int groups) { return s
 // 8 g + 4 h + e, which lane half h holds, is n = 16 h + 4 g + e).
 constexpr int kRunBlocks = 16;
 constexpr int min_of(int a, int b) { return a < b ? a : b; }
-template <int WN, int WM, int NT, int MT, bool A8, int STAGES>
+template <int WN, int WM, int NT, int MT, bool A8, int STAGES, bool GOES_ON>
 struct MxTile {
   static constexpr int kBN = WN * NT * 32, kBM = WM * MT * 32, kWaves = WN * WM, kThreads = 64 * kWaves;
   static constexpr int kRowX = A8 ? 256 : 128, kChunksX = kRowX / 16;
   static constexpr int kBytesW = kBN * 128, kBytesX = kBM * kRowX, kStage = kBytesW + kBytesX;
   static constexpr int kLoadsW = kBytesW / (kThreads * 16), kLoadsX = kBytesX / (kThreads * 16), kLoadsS = (kBN + kBM + 64 * kWaves - 1) / (64 * kWaves);
   static constexpr int kRuns = STAGES > 3 ? 4 : 2, kRun = kLoadsS * kWaves * 1024;   // (what the last loads of scales bring past the tile's rows is not read)
-  static constexpr int kScales = STAGES * kStage, kLds = kScales + kRuns * kRun;
+  // Results leave by way of 4 KiB a wavefront: of their own where the next tile's stages are under way meanwhile
+  static constexpr int kScales = STAGES * kStage, kResults = GOES_ON ? kScales + kRuns * kRun : 0;
+  static constexpr int kLds = kScales + kRuns * kRun + (GOES_ON ? kWaves * 4096 : 0);
   static constexpr int loads(int stage) { return kLoadsW + kLoadsX + (stage % 2 == 0 ? kLoadsS : 0); }   // a run's scales come with its first stage
   // loads of the stages from..to - 1 (of which only whether they are even matters)
   static constexpr int loads_between(int from, int to) { return from >= to ? 0 : loads(from) + loads_between(from + 1, to); }
   // kEarly: of a buffer that is multiplied, only the second pair of block rows is still to be read soon after the stage has begun.  The rest of it -
-  // activations, the first pair's weights (a load is 32 rows, a block row), scales - is refilled from there on: kLate loads less.
+  // activations, the first pair's weights (a load is 32 rows, a block row), scales - is refilled from there on, kFirst loads of it beside the
+  // first pair.
   static constexpr bool kEarly = STAGES == 2 && NT == 4 && kThreads == 256;
-  static constexpr int kLate = kEarly ? kLoadsW / 2 : 0;
-  // nth load of those that come early, and of those that come late
-  static constexpr int early_piece(int nth) { return nth < kLoadsW / 2 ? nth / 2 * 4 + nth % 2 : nth + kLoadsW / 2; }
-  static constexpr int late_piece(int nth) { return nth / 2 * 4 + 2 + nth % 2; }
+  static constexpr int kFirst = kEarly ? 11 : 0;
+  // nth load of a stage
+  static constexpr int piece(int nth, int stage) {
+    return !kEarly ? nth : nth < kLoadsW / 2 ? nth / 2 * 4 + nth % 2 : nth < loads(stage) - kLoadsW / 2 ? nth + kLoadsW / 2 : late(nth - loads(stage) + kLoadsW / 2);
+  }
+  static constexpr int late(int nth) { return nth / 2 * 4 + 2 + nth % 2; }
   static_assert(NT % 2 == 0 && kBN % 64 == 0 && kBM % 64 == 0 && kBytesW % (kThreads * 16) == 0 && kBytesX % (kThreads * 16) == 0, "pairs of block rows; whole loads");
   static_assert(kThreads / 8 % 16 == 0 && kThreads / kChunksX % 8 == 0, "a thread's rows have equal keys, or two in turn");
   static_assert(kLds <= 160 * 1024 && STAGES >= 2 && STAGES <= 4 && STAGES * loads(0) < 64, "LDS of a compute unit; the counter of loads");
@@ -100,13 +105,34 @@ struct MxTile {
 template <int BYTES>
 __device__ __forceinline__ int slot_key(int row) { return BYTES == 128 ? (row >> 1) & 7 : row & 15; }
 
+// Sixteen bytes of a row's results (`row`: the row's place in elements) from column n on; those from n_end on stay unwritten.
+template <int KIND>
+__device__ __forceinline__ void store_sixteen(char* c, int64_t row, int64_t cs, int64_t n, int64_t n_end, const u32x4& v) {
+  constexpr int BYTES = KIND == FP8_REAL_F32 ? 4 : 2, COUNT = 16 / BYTES;
+  VECOPS_GLOBAL char* const to = (VECOPS_GLOBAL char*)c + (row + n * cs) * BYTES;
+  if (cs == 1 && n + COUNT <= n_end) {
+    *(VECOPS_GLOBAL u32x4_anywhere*)to = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < COUNT; ++e) {
+      if (n + e >= n_end) continue;
+      if constexpr (BYTES == 4) *(VECOPS_GLOBAL uint32_t*)(to + e * cs * 4) = v[e];
+      else *(VECOPS_GLOBAL uint16_t*)(to + e * cs * 2) = static_cast<uint16_t>(v[e >> 1] >> (16 * (e & 1)));
+    }
+  }
+}
+
 // One wavefront: two block rows at a time against every block column of the activations, whose fragments stay in registers for the
 // stage.  While a pair's products are formed the next one's weights are fetched, and beside the last pair the next stage's
 // activations, each into the registers that its last product has read.  So in front of the last pair all of the stage has been read: there the next stage
 // has landed, the wavefronts meet, and behind that this stage's buffer is refilled, a load behind each matrix instruction.
-template <int WN, int WM, int NT, int MT, bool A8, int STAGES, int WAVES_A_SIMD>
+// GOES_ON: a workgroup goes from tile to tile, and the next one's first stages are fetched while it writes results: with a workgroup a
+// compute unit nothing else would.
+// OUT: the type in which results leave (a template's argument: with a branch the compiler makes copies of all of the way out and reads every
+// accumulator in front of them).
+template <int WN, int WM, int NT, int MT, bool A8, int STAGES, int WAVES_A_SIMD, bool GOES_ON, int OUT>
 __global__ __launch_bounds__(64 * WN * WM, WAVES_A_SIMD) void mx_tile_kernel(const MxMatmulParams p, uint32_t tiles_n, uint32_t tiles_m) {
-  using T = MxTile<WN, WM, NT, MT, A8, STAGES>;
+  using T = MxTile<WN, WM, NT, MT, A8, STAGES, GOES_ON>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -117,25 +143,23 @@ __global__ __launch_bounds__(64 * WN * WM, WAVES_A_SIMD) void mx_tile_kernel(con
   const int run_begin = static_cast<int>(static_cast<int64_t>(runs) * blockIdx.z / p.splits);
   const int run_end = static_cast<int>(static_cast<int64_t>(runs) * (blockIdx.z + 1) / p.splits);
 
-  // neighbouring tiles on one die: each die's workgroups (every eighth) take a contiguous run of tiles, walked in groups of
-  // eight tile rows
-  uint32_t pid = blockIdx.x;
-  {
-    const uint32_t total = tiles_n * tiles_m, xcd = pid & 7, share = total >> 3, extra = total & 7;
-    pid = xcd * share + min(xcd, extra) + (pid >> 3);
-  }
-  const uint32_t per_group = 8 * tiles_n, group = pid / per_group, first = group * 8;
-  const uint32_t height = min(tiles_m - first, 8u), in_group = pid - group * per_group;
-  const uint32_t tile_m = first + in_group % height, tile_n = in_group / height;
-  const int64_t m0 = static_cast<int64_t>(tile_m) * T::kBM, n0 = static_cast<int64_t>(tile_n) * T::kBN;
-  const int last_m = static_cast<int>(min(p.m - m0, static_cast<int64_t>(T::kBM))) - 1;
-  const int last_n = static_cast<int>(min(p.n - n0, static_cast<int64_t>(T::kBN))) - 1;
-
-  // Rows past the operand's last one lie past the descriptors' ends: zeros arrive.
-  u32x4 desc_w = tile_buffer_words((const VECOPS_GLOBAL char*)p.b + batch * p.b_bs + n0 * p.ldb);
-  u32x4 desc_x = tile_buffer_words((const VECOPS_GLOBAL char*)p.a + batch * p.a_bs + m0 * p.lda);
-  const uint32_t end_w = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(last_n * p.ldb) + static_cast<uint32_t>(p.groups) * 16u);
-  const uint32_t end_x = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(last_m * p.lda) + static_cast<uint32_t>(p.groups) * (A8 ? 32u : 16u));
+  // Neighbouring tiles on one die: each die's units (every eighth) are a contiguous run of tiles, walked in groups of eight tile rows.
+  const uint32_t units = tiles_n * tiles_m;
+  struct Tile {
+    int64_t m0, n0;
+    int last_m, last_n;
+  };
+  auto tile_of = [&](uint32_t unit) {
+    const uint32_t xcd = unit & 7, share = units >> 3, extra = units & 7;
+    const uint32_t pid = xcd * share + min(xcd, extra) + (unit >> 3);
+    const uint32_t per_group = 8 * tiles_n, group = pid / per_group, first = group * 8;
+    const uint32_t height = min(tiles_m - first, 8u), in_group = pid - group * per_group;
+    Tile t;
+    t.m0 = static_cast<int64_t>(first + in_group % height) * T::kBM, t.n0 = static_cast<int64_t>(in_group / height) * T::kBN;
+    t.last_m = static_cast<int>(min(p.m - t.m0, static_cast<int64_t>(T::kBM))) - 1;
+    t.last_n = static_cast<int>(min(p.n - t.n0, static_cast<int64_t>(T::kBN))) - 1;
+    return t;
+  };
 
   // load i of a thread: sixteen bytes of row i * kRowsW + tid / chunks, the chunk whose slot is tid % chunks
   constexpr int kRowsW = T::kThreads / 8, kRowsX = T::kThreads / T::kChunksX;
@@ -147,43 +171,64 @@ __global__ __launch_bounds__(64 * WN * WM, WAVES_A_SIMD) void mx_tile_kernel(con
   const uint32_t add_w = static_cast<uint32_t>(kRowsW * p.ldb), add_x = static_cast<uint32_t>(kRowsX * p.lda);
   const int block_x = A8 ? chunk_x >> 1 : chunk_x, block_x_odd = A8 ? (chunk_x ^ kTurn) >> 1 : chunk_x;   // of the stage's eight
   // the scales: 64 rows an instruction; instruction u goes to wavefront u % waves
-  u32x4 desc_s[T::kLoadsS];
-  uint32_t end_s[T::kLoadsS], from_s[T::kLoadsS];
+  uint32_t from_s[T::kLoadsS];
 #pragma unroll
   for (int i = 0; i < T::kLoadsS; ++i) {
     const int rows = 64 * (i * T::kWaves + wave);
-    const bool weights = rows < T::kBN;
-    const int64_t rs = weights ? p.bs_rs : p.as_rs;
-    desc_s[i] = tile_buffer_words(weights ? (const VECOPS_GLOBAL char*)p.b_scales + batch * p.bs_bs + n0 * p.bs_rs
-                                          : (const VECOPS_GLOBAL char*)p.a_scales + batch * p.as_bs + m0 * p.as_rs);
-    end_s[i] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>((weights ? last_n : last_m) * rs + p.row_scales));
-    from_s[i] = static_cast<uint32_t>((rows - (weights ? 0 : T::kBN) + lane) * rs);
+    from_s[i] = static_cast<uint32_t>(rows < T::kBN ? (rows + lane) * p.bs_rs : (rows - T::kBN + lane) * p.as_rs);
   }
 
-  // load PIECE of those that fill buffer `slot` with half PAR of run `run`; past the last run nothing is fetched (but as many loads are issued)
-  auto issue_piece = [&](auto piece_tag, auto par_tag, int run, int slot) {
+  // What is fetched: a unit's tile, a run of it, and which run that is of the workgroup's.  Rows past the operand's last one lie past the
+  // descriptors' ends: zeros arrive.
+  uint32_t fetch_unit = blockIdx.x, end_w = 0, end_x = 0, end_s[T::kLoadsS], fetch_turn = 0;
+  int fetch_run = run_begin;
+  u32x4 desc_w, desc_x, desc_s[T::kLoadsS];
+  auto aim = [&] {
+    const bool there = fetch_unit < units && run_begin < run_end;   // (past the last tile nothing is fetched, but as many loads are issued)
+    const Tile t = tile_of(there ? fetch_unit : 0);
+    desc_w = tile_buffer_words((const VECOPS_GLOBAL char*)p.b + batch * p.b_bs + t.n0 * p.ldb);
+    desc_x = tile_buffer_words((const VECOPS_GLOBAL char*)p.a + batch * p.a_bs + t.m0 * p.lda);
+    end_w = __builtin_amdgcn_readfirstlane(there ? static_cast<uint32_t>(t.last_n * p.ldb) + static_cast<uint32_t>(p.groups) * 16u : 0u);
+    end_x = __builtin_amdgcn_readfirstlane(there ? static_cast<uint32_t>(t.last_m * p.lda) + static_cast<uint32_t>(p.groups) * (A8 ? 32u : 16u) : 0u);
+    desc_w[2] = end_w;
+    desc_x[2] = end_x;
+#pragma unroll
+    for (int i = 0; i < T::kLoadsS; ++i) {
+      const bool weights = 64 * (i * T::kWaves + wave) < T::kBN;
+      desc_s[i] = tile_buffer_words(weights ? (const VECOPS_GLOBAL char*)p.b_scales + batch * p.bs_bs + t.n0 * p.bs_rs
+                                            : (const VECOPS_GLOBAL char*)p.a_scales + batch * p.as_bs + t.m0 * p.as_rs);
+      end_s[i] = __builtin_amdgcn_readfirstlane(there ? static_cast<uint32_t>((weights ? t.last_n * p.bs_rs : t.last_m * p.as_rs) + p.row_scales) : 0u);
+      desc_s[i][2] = end_s[i];
+    }
+  };
+  auto advance = [&] {   // to the next run
+    ++fetch_turn;
+    if (++fetch_run < run_end) return;
+    fetch_run = run_begin;
+    fetch_unit = GOES_ON ? fetch_unit + gridDim.x : units;
+    aim();
+  };
+
+  // load PIECE of those that fill buffer `slot` with half PAR of the run that is fetched
+  auto issue_piece = [&](auto piece_tag, auto par_tag, int slot) {
     constexpr int PIECE = decltype(piece_tag)::value, PAR = decltype(par_tag)::value;
-    const bool there = run < run_end;
-    const int first_block = min(run * kRunBlocks, p.row_scales - kRunBlocks);   // the run's sixteen blocks
+    const int first_block = min(fetch_run * kRunBlocks, p.row_scales - kRunBlocks);   // the run's sixteen blocks
     // those before `old` have been summed; those from `most` on are not there
-    const int old = run * kRunBlocks - first_block - 8 * PAR, most = p.groups - first_block - 8 * PAR;
+    const int old = fetch_run * kRunBlocks - first_block - 8 * PAR, most = p.groups - first_block - 8 * PAR;
     if constexpr (PIECE < T::kLoadsW) {
-      desc_w[2] = there ? end_w : 0u;
       load_16_bytes_into_lds(desc_w, lds0 + slot * T::kStage, __builtin_amdgcn_readfirstlane(PIECE * (T::kThreads * 16) + wave * 1024),
                              chunk_w >= old && chunk_w < most ? from_w : kNowhere,
                              __builtin_amdgcn_readfirstlane(PIECE * add_w + static_cast<uint32_t>(first_block + 8 * PAR) * 16u));
     } else if constexpr (PIECE < T::kLoadsW + T::kLoadsX) {
       constexpr int AT = PIECE - T::kLoadsW;
       const int block = AT % 2 ? block_x_odd : block_x;
-      desc_x[2] = there ? end_x : 0u;
       load_16_bytes_into_lds(desc_x, lds0 + slot * T::kStage, __builtin_amdgcn_readfirstlane(T::kBytesW + AT * (T::kThreads * 16) + wave * 1024),
                              block >= old && block < most ? (AT % 2 ? from_x_odd : from_x) : kNowhere,
                              __builtin_amdgcn_readfirstlane(AT * add_x + static_cast<uint32_t>(first_block + 8 * PAR) * (A8 ? 32u : 16u)));
     } else {
       constexpr int AT = PIECE - T::kLoadsW - T::kLoadsX;
-      desc_s[AT][2] = there ? end_s[AT] : 0u;
-      load_16_bytes_into_lds(desc_s[AT], lds0 + T::kScales + (run & (T::kRuns - 1)) * T::kRun, __builtin_amdgcn_readfirstlane((AT * T::kWaves + wave) * 1024), from_s[AT],
-                             __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(first_block)));
+      load_16_bytes_into_lds(desc_s[AT], lds0 + T::kScales + (fetch_turn & (T::kRuns - 1)) * T::kRun, __builtin_amdgcn_readfirstlane((AT * T::kWaves + wave) * 1024),
+                             from_s[AT], __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(first_block)));
     }
   };
 
@@ -202,10 +247,6 @@ __global__ __launch_bounds__(64 * WN * WM, WAVES_A_SIMD) void mx_tile_kernel(con
   const uint32_t at_sw = lds0 + T::kScales + row_of_w * 16, at_sx = lds0 + T::kScales + (T::kBN + row_of_x) * 16;
 
   f32x16 acc[NT * MT];
-#pragma unroll
-  for (int i = 0; i < NT * MT; ++i)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
   i32x8 x[4][MT], w[2][2][4];
   u32x2 sx[2][MT], sw[2][2];   // a lane's scales of 64 k `s`: byte 2 (s % 2) of word s / 2, shifted down by its half
   constexpr int kPairs = NT / 2, kMeet = 5;
@@ -224,26 +265,29 @@ __global__ __launch_bounds__(64 * WN * WM, WAVES_A_SIMD) void mx_tile_kernel(con
     else x[s][j] = narrow_fragment(read_lds(at_x[s][0] + stage, j * 4096));
   };
 
-  // half PAR of a run, in buffer `slot`
-  auto multiply = [&](auto par_tag, int run, int slot) {
+  // half PAR of the workgroup's run `turn`, in buffer `slot`
+  auto multiply = [&](auto par_tag, uint32_t turn, int slot) {
     constexpr int PAR = decltype(par_tag)::value;
     constexpr int AHEAD = PAR + STAGES;   // the stage, counted from the run's first, that takes this one's buffer
     const int next_slot = slot + 1 == STAGES ? 0 : slot + 1;
     const uint32_t stage = slot * T::kStage, next = next_slot * T::kStage;
-    const uint32_t run_at = (run & (T::kRuns - 1)) * T::kRun, next_run_at = PAR == 0 ? run_at : ((run + 1) & (T::kRuns - 1)) * T::kRun;
+    const uint32_t run_at = (turn & (T::kRuns - 1)) * T::kRun, next_run_at = PAR == 0 ? run_at : ((turn + 1) & (T::kRuns - 1)) * T::kRun;
+    if constexpr (AHEAD % 2 == 0) advance();
     static_for<kPairs>([&](auto pair_tag) {
       constexpr int pair = decltype(pair_tag)::value, now = (PAR * kPairs + pair) & 1, then = now ^ 1;
       constexpr bool final_pair = pair + 1 == kPairs;
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (final_pair) {
-        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(T::kEarly ? T::loads(AHEAD) - T::kLate : T::loads_between(PAR + 2, PAR + STAGES)) : "memory");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(T::kEarly ? T::kFirst : T::loads_between(PAR + 2, PAR + STAGES)) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
       }
       // behind matrix instruction AT of the pair: the next pair's weights and scales, the next stage's activations, loads
       auto beside = [&](auto at_tag) {
         constexpr int AT = decltype(at_tag)::value, kAll = 8 * MT;
-        constexpr int from = AT * 8 / kAll, to = (AT + 1) * 8 / kAll;   // of eight fragments
+        // of eight fragments (beside the first of several pairs not before the wavefronts have met; all some time before they are waited for)
+        constexpr int start = T::kEarly && !final_pair ? kMeet : 0, step = kAll >= 32 ? 2 : 1, many = (8 * step + kAll - 1) / kAll;
+        constexpr int from = AT < start ? 0 : min_of((AT - start + step - 1) / step * many, 8), to = AT < start ? 0 : min_of((AT - start + step) / step * many, 8);
         static_for<to - from>([&](auto nth) {
           constexpr int f = from + decltype(nth)::value;
           constexpr int i = final_pair ? f & 1 : 2 * pair + 2 + (f & 1);
@@ -260,12 +304,11 @@ __global__ __launch_bounds__(64 * WN * WM, WAVES_A_SIMD) void mx_tile_kernel(con
           __builtin_amdgcn_s_barrier();
           asm volatile("" ::: "memory");
         }
-        constexpr int count = !T::kEarly ? (final_pair ? T::loads(AHEAD) : 0) : final_pair ? T::kLate : T::loads(AHEAD) - T::kLate;
-        constexpr int begin = T::kEarly && !final_pair ? kMeet : 0, per = (count + kAll - begin - 1) / (kAll - begin);
-        constexpr int a = AT < begin ? 0 : min_of((AT - begin) * per, count), b = AT < begin ? 0 : min_of((AT - begin + 1) * per, count);
+        // loads evenly
+        constexpr int all = T::loads(AHEAD), first = final_pair ? T::kFirst : 0, count = final_pair ? all - T::kFirst : T::kFirst, room = kAll - start;
+        constexpr int a = AT < start ? 0 : (AT - start) * count / room, b = AT < start ? 0 : (AT - start + 1) * count / room;
         static_for<b - a>([&](auto nth) {
-          constexpr int at = a + decltype(nth)::value, piece = !T::kEarly ? at : final_pair ? T::late_piece(at) : T::early_piece(at);
-          issue_piece(std::integral_constant<int, piece>{}, std::integral_constant<int, AHEAD % 2>{}, run + AHEAD / 2, slot);
+          issue_piece(std::integral_constant<int, T::piece(first + a + decltype(nth)::value, AHEAD)>{}, std::integral_constant<int, AHEAD % 2>{}, slot);
         });
       };
       static_for<4>([&](auto s_tag) {
@@ -282,71 +325,96 @@ __global__ __launch_bounds__(64 * WN * WM, WAVES_A_SIMD) void mx_tile_kernel(con
     });
   };
 
-  if (run_begin < run_end) {
-    static_for<STAGES>([&](auto g) {
-      constexpr int G = decltype(g)::value;
-      static_for<T::loads(G)>([&](auto piece) { issue_piece(piece, std::integral_constant<int, G % 2>{}, run_begin + G / 2, G); });
-    });
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(T::loads_between(1, STAGES)) : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    const uint32_t run_at = (run_begin & (T::kRuns - 1)) * T::kRun;
-    static_for<8>([&](auto f) {
-      constexpr int F = decltype(f)::value;
-      read_w(std::integral_constant<int, 0>{}, std::integral_constant<int, (F & 1)>{}, std::integral_constant<int, (F >> 1)>{}, 0);
-      if constexpr (F < 2) sw[0][F] = scales_at(at_sw + run_at, F * 512);
-    });
-    static_for<MT>([&](auto j) {
-      sx[0][decltype(j)::value] = scales_at(at_sx + run_at, decltype(j)::value * 512);
-      static_for<4>([&](auto s) { read_x(s, j, 0); });
-    });
-    int slot = 0;
-    const auto following = [](int at) { return at + 1 == STAGES ? 0 : at + 1; };
-    // (past the last stage: reads of a buffer that nothing has been fetched for, and loads that fetch nothing)
-    for (int run = run_begin; run < run_end; ++run) {
-      multiply(std::integral_constant<int, 0>{}, run, slot);
-      slot = following(slot);
-      multiply(std::integral_constant<int, 1>{}, run, slot);
-      slot = following(slot);
-    }
-  }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (no load may write LDS once the workgroup is gone)
-  settle();
-
-  // Results leave 32 rows at a time by way of LDS, a wavefront's own part of it, so that a store instruction fills whole lines.
-  // Sixteen bytes of a row lie in slot (place ^ row % 16): neither way has conflicts.
+  aim();
+  static_for<STAGES>([&](auto g) {
+    constexpr int G = decltype(g)::value;
+    if constexpr (G > 0 && G % 2 == 0) advance();
+    static_for<T::loads(G)>([&](auto piece) { issue_piece(piece, std::integral_constant<int, G % 2>{}, G); });
+  });
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(T::loads_between(1, STAGES)) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  static_for<8>([&](auto f) {
+    constexpr int F = decltype(f)::value;
+    read_w(std::integral_constant<int, 0>{}, std::integral_constant<int, (F & 1)>{}, std::integral_constant<int, (F >> 1)>{}, 0);
+    if constexpr (F < 2) sw[0][F] = scales_at(at_sw, F * 512);
+  });
+  static_for<MT>([&](auto j) {
+    sx[0][decltype(j)::value] = scales_at(at_sx, decltype(j)::value * 512);
+    static_for<4>([&](auto s) { read_x(s, j, 0); });
+  });
   const bool shares = p.splits > 1;
-  const int kind = shares ? static_cast<int>(FP8_REAL_F32) : p.out_kind;
   const int64_t c_rs = shares ? p.n : p.c_rs, c_cs = shares ? 1 : p.c_cs;
   char* const c = shares ? reinterpret_cast<char*>(p.partial + (static_cast<int64_t>(blockIdx.z) * p.batch + batch) * p.m * p.n)
-                         : static_cast<char*>(p.c) + batch * p.c_bs * (kind == FP8_REAL_F32 ? 4 : 2);
-  constexpr int kRow = NT * 32 * 4, kPieces = NT * 4, kRowsAtOnce = 64 / kPieces;   // bytes of a row; eights of results; rows an instruction
-  static_assert(T::kWaves * 32 * kRow <= T::kLds && kPieces >= 8, "room for 32 rows a wavefront; sixteen slots a row or more");
-  const uint32_t mine = lds0 + wave * (32 * kRow);
-  const int64_t m1 = m0 + wm * (MT * 32) + lane / kPieces, n1 = n0 + wn * (NT * 32) + lane % kPieces * 8;
-  __builtin_amdgcn_s_barrier();   // (other wavefronts may still be reading what this one overwrites)
-  asm volatile("" ::: "memory");
-  static_for<MT>([&](auto j_tag) {
-    constexpr int j = decltype(j_tag)::value;
-    static_for<NT>([&](auto i_tag) {
-      constexpr int i = decltype(i_tag)::value;
-      const f32x16 a = acc[i * MT + j];
-#pragma unroll
-      for (int e = 0; e < 16; e += 4)
-        write_lds(mine + col * kRow + ((((i * 32 + e) / 4 + half * 4) ^ (col & 15)) << 4),
-                  u32x4{__float_as_uint(a[e]), __float_as_uint(a[e + 1]), __float_as_uint(a[e + 2]), __float_as_uint(a[e + 3])});
-      __builtin_amdgcn_sched_barrier(0);   // (a block at a time leaves the accumulators)
-    });
+                         : static_cast<char*>(p.c) + batch * p.c_bs * (OUT == FP8_REAL_F32 ? 4 : 2);
+  const uint32_t mine = lds0 + T::kResults + wave * 4096;
+  int slot = 0;
+  uint32_t turn = 0;
+  const auto following = [](int at) { return at + 1 == STAGES ? 0 : at + 1; };
+  // (behind the last tile's last stage: reads of a buffer that nothing has been fetched for, and loads that fetch nothing)
 #pragma unroll 1
-    for (int r = lane / kPieces; r < 32; r += kRowsAtOnce) {
-      const uint32_t at = mine + r * kRow, place = lane % kPieces * 2;
-      const u32x4 lo = read_lds(at + ((place ^ (r & 15)) << 4), 0), hi = read_lds(at + (((place + 1) ^ (r & 15)) << 4), 0);
-      const int64_t m = m1 + j * 32 + (r - lane / kPieces);
-      const float v[8] = {__uint_as_float(lo[0]), __uint_as_float(lo[1]), __uint_as_float(lo[2]), __uint_as_float(lo[3]),
-                          __uint_as_float(hi[0]), __uint_as_float(hi[1]), __uint_as_float(hi[2]), __uint_as_float(hi[3])};
-      if (m < p.m) store_results<8>(c, m * c_rs + n1 * c_cs, c_cs, kind, n1, p.n, v);
+  for (uint32_t unit = blockIdx.x; unit < units; unit = GOES_ON ? unit + gridDim.x : units) {
+#pragma unroll
+    for (int i = 0; i < NT * MT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
+#pragma unroll 1
+    for (int run = run_begin; run < run_end; ++run) {
+      multiply(std::integral_constant<int, 0>{}, turn, slot);
+      slot = following(slot);
+      multiply(std::integral_constant<int, 1>{}, turn, slot);
+      slot = following(slot);
+      ++turn;
     }
-  });
+    settle();
+    if constexpr (!GOES_ON) {   // (no load may write LDS once results pass through it; other wavefronts are done with what they replace)
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    }
+    // 32 rows of 128 bytes at a time pass through LDS, so that a store instruction fills lines: sixteen bytes of a row lie in slot
+    // (place ^ row / 2 % 8) of eight.
+    const Tile t = tile_of(unit);
+    const auto write_row = [&](int place, const u32x4& v) { write_lds(mine + col * 128 + ((place ^ ((col >> 1) & 7)) << 4), v); };
+    const auto read_row = [&](int row, int place) { return read_lds(mine + row * 128 + ((place ^ ((row >> 1) & 7)) << 4), 0); };
+    static_for<MT>([&](auto j_tag) {
+      static_for<NT / 2>([&](auto pair_tag) {
+        constexpr int j = decltype(j_tag)::value, i = 2 * decltype(pair_tag)::value;
+        const int64_t m = t.m0 + wm * (MT * 32) + j * 32 + (lane >> 3), n = t.n0 + wn * (NT * 32) + i * 32;
+        if constexpr (OUT == FP8_REAL_F32) {
+          static_for<2>([&](auto u_tag) {
+            constexpr int u = decltype(u_tag)::value;
+            const f32x16 a = acc[(i + u) * MT + j];
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+              write_row(e / 4 + half * 4, u32x4{__float_as_uint(a[e]), __float_as_uint(a[e + 1]), __float_as_uint(a[e + 2]), __float_as_uint(a[e + 3])});
+#pragma unroll
+            for (int r = 0; r < 32; r += 8)
+              store_sixteen<FP8_REAL_F32>(c, (m + r) * c_rs, c_cs, n + u * 32 + (lane & 7) * 4, m + r < p.m ? p.n : 0, read_row(r + (lane >> 3), lane & 7));
+          });
+        } else {
+          static_for<2>([&](auto u_tag) {
+            constexpr int u = decltype(u_tag)::value;
+            const f32x16 a = acc[(i + u) * MT + j];
+#pragma unroll
+            for (int e = 0; e < 16; e += 8) {
+              u32x4 v;
+#pragma unroll
+              for (int d = 0; d < 4; ++d)
+                v[d] = OUT == FP8_REAL_BF16 ? cvt_pk_bf16(a[e + 2 * d], a[e + 2 * d + 1])
+                                            : f16_bits_rne(a[e + 2 * d]) | static_cast<uint32_t>(f16_bits_rne(a[e + 2 * d + 1])) << 16;
+              write_row(u * 4 + half * 2 + e / 8, v);
+            }
+          });
+#pragma unroll
+          for (int r = 0; r < 32; r += 8)
+            store_sixteen<FP8_REAL_BF16>(c, (m + r) * c_rs, c_cs, n + (lane & 7) * 8, m + r < p.m ? p.n : 0, read_row(r + (lane >> 3), lane & 7));
+        }
+        __builtin_amdgcn_sched_barrier(0);   // (two blocks at a time leave the accumulators)
+      });
+    });
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (no load may write LDS once the workgroup is gone)
 }
 
 // Up to sixteen rows: bound by HBM, so that what counts is how many bytes of the weights are under way.  A workgroup owns sixteen
@@ -443,18 +511,26 @@ hipError_t launch_few_rows(const MxMatmulParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <int WN, int WM, int NT, int MT, bool A8, int STAGES, int WAVES_A_SIMD>
-hipError_t launch_tile(const MxMatmulParams& p, hipStream_t stream) {
-  using T = MxTile<WN, WM, NT, MT, A8, STAGES>;
-  constexpr auto kernel = &mx_tile_kernel<WN, WM, NT, MT, A8, STAGES, WAVES_A_SIMD>;
+template <int WN, int WM, int NT, int MT, bool A8, int STAGES, int WAVES_A_SIMD, bool GOES_ON, int OUT>
+hipError_t launch_tile_as(const MxMatmulParams& p, hipStream_t stream) {
+  using T = MxTile<WN, WM, NT, MT, A8, STAGES, GOES_ON>;
+  constexpr auto kernel = &mx_tile_kernel<WN, WM, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, OUT>;
   if constexpr (T::kLds > 65536) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds);
     if (e != hipSuccess) return e;
   }
   const uint32_t tiles_n = static_cast<uint32_t>((p.n + T::kBN - 1) / T::kBN), tiles_m = static_cast<uint32_t>((p.m + T::kBM - 1) / T::kBM);
-  hipLaunchKernelGGL(kernel, dim3(tiles_n * tiles_m, static_cast<uint32_t>(p.batch), static_cast<uint32_t>(p.splits)), dim3(T::kThreads), T::kLds, stream, p, tiles_n,
+  const uint32_t units = tiles_n * tiles_m;
+  hipLaunchKernelGGL(kernel, dim3(GOES_ON ? std::min(units, 256u) : units, static_cast<uint32_t>(p.batch), static_cast<uint32_t>(p.splits)), dim3(T::kThreads), T::kLds, stream, p, tiles_n,
                      tiles_m);
-  const hipError_t e = hipGetLastError();
+  return hipGetLastError();
+}
+
+template <int WN, int WM, int NT, int MT, bool A8, int STAGES, int WAVES_A_SIMD, bool GOES_ON>
+hipError_t launch_tile(const MxMatmulParams& p, hipStream_t stream) {
+  if (p.splits == 1 && p.out_kind == FP8_REAL_BF16) return launch_tile_as<WN, WM, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, FP8_REAL_BF16>(p, stream);
+  if (p.splits == 1 && p.out_kind == FP8_REAL_F16) return launch_tile_as<WN, WM, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, FP8_REAL_F16>(p, stream);
+  const hipError_t e = launch_tile_as<WN, WM, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, FP8_REAL_F32>(p, stream);
   if (p.splits == 1 || e != hipSuccess) return e;
   return launch_join_shares({p.partial, p.c, p.c_rs, p.c_cs, p.c_bs, p.m, p.n, p.batch, p.splits, p.out_kind}, stream);
 }
@@ -473,9 +549,9 @@ MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int64_t batch, bool a_wide) {
 hipError_t launch_mx_matmul(const MxMatmulParams& p, int kind, hipStream_t stream) {
   switch (kind) {
     case MX_FEW_ROWS: return p.a_wide ? launch_few_rows<true>(p, stream) : launch_few_rows<false>(p, stream);
-    case MX_TILE_64: return p.a_wide ? launch_tile<1, 2, 2, 1, true, 3, 2>(p, stream) : launch_tile<1, 2, 2, 1, false, 3, 2>(p, stream);
-    case MX_TILE_128: return p.a_wide ? launch_tile<2, 2, 2, 2, true, 2, 2>(p, stream) : launch_tile<2, 2, 2, 2, false, 2, 2>(p, stream);
-    case MX_TILE_256: return p.a_wide ? launch_tile<2, 2, 4, 2, true, 2, 1>(p, stream) : launch_tile<2, 2, 4, 4, false, 2, 1>(p, stream);
+    case MX_TILE_64: return p.a_wide ? launch_tile<1, 2, 2, 1, true, 3, 2, false>(p, stream) : launch_tile<1, 2, 2, 1, false, 3, 2, false>(p, stream);
+    case MX_TILE_128: return p.a_wide ? launch_tile<2, 2, 2, 2, true, 2, 2, false>(p, stream) : launch_tile<2, 2, 2, 2, false, 2, 2, false>(p, stream);
+    case MX_TILE_256: return p.a_wide ? launch_tile<2, 2, 4, 2, true, 2, 1, true>(p, stream) : launch_tile<2, 2, 4, 4, false, 2, 1, true>(p, stream);
   }
   return hipErrorInvalidValue;
 }
