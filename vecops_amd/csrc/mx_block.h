@@ -28,7 +28,7 @@ struct MxMatmulParams {
 };
 
 // The kernels: up to sixteen rows; tiles of 64 x 64, 128 x 128, and 256 weight rows x 256 (with e4m3 activations x 128).
-enum MxKind : int { MX_FEW_ROWS = 0, MX_TILE_64, MX_TILE_128, MX_TILE_256 };
+enum MxKind : int { MX_FEW_ROWS = 0, MX_TILE_64, MX_TILE_64_DEEP, MX_TILE_128, MX_TILE_128_DEEP, MX_TILE_256 };
 struct MxPlan {
   int kind;
   int splits;  // shares of k; more than one need `partial`

@@ -60,8 +60,9 @@ __device__ __forceinline__ void settle() {
 __device__ __forceinline__ int scale_word_at(int word, int groups) { return min(4 * word, groups - 4); }
 __device__ __forceinline__ uint32_t scale_shift(int word, int groups) { return static_cast<uint32_t>(min(max(4 * word + 4 - groups, 0) * 8, 31)); }
 
-// Many rows: WN x WM wavefronts, each NT x MT blocks of 32 x 32.  v_mfma_scale_f32_32x32x64_f8f6f4: a lane's e2m1 operand is block
-// l / 32 of two of row l % 32, an e4m3 one k 16 (l / 32) .. and 32 + 16 (l / 32) ..; its scale is that of block l / 32.  (One wavefront
+// Many rows: WN x WM wavefronts, each NT x MT blocks of 32 x 32.  v_mfma_scale_f32_32x32x64_f8f6f4: a lane's e2m1 operand is the
+// place l / 32 of two of row l % 32, an e4m3 one half l / 32 of either place; its scale is that of place l / 32.  Of a stage's eight blocks of
+// 32 k instruction s of four has block 4 q + s in place q: a lane's four scales are one word, the instruction's byte of it a constant.  (One wavefront
 // on a SIMD keeps the matrix pipe to 8.5 PFLOP/s with it, on operands of zeros, and with the 16 x 16 one to 4.9: an instruction with scales
 // takes two issues.)
 // A stage is 256 k of both operands: whole lines of e2m1 rows (of half lines each is fetched twice).  STAGES of them are under way or
@@ -72,9 +73,9 @@ __device__ __forceinline__ uint32_t scale_shift(int word, int groups) { return s
 // 8 g + 4 h + e, which lane half h holds, is n = 16 h + 4 g + e).
 constexpr int kRunBlocks = 16;
 constexpr int min_of(int a, int b) { return a < b ? a : b; }
-template <int WN, int WM, int NT, int MT, bool A8, int STAGES, bool GOES_ON>
+template <int WN, int WM, int WK, int NT, int MT, bool A8, int STAGES, bool GOES_ON>
 struct MxTile {
-  static constexpr int kBN = WN * NT * 32, kBM = WM * MT * 32, kWaves = WN * WM, kThreads = 64 * kWaves;
+  static constexpr int kBN = WN * NT * 32, kBM = WM * MT * 32, kWaves = WN * WM * WK, kThreads = 64 * kWaves;
   static constexpr int kRowX = A8 ? 256 : 128, kChunksX = kRowX / 16;
   static constexpr int kBytesW = kBN * 128, kBytesX = kBM * kRowX, kStage = kBytesW + kBytesX;
   static constexpr int kLoadsW = kBytesW / (kThreads * 16), kLoadsX = kBytesX / (kThreads * 16), kLoadsS = (kBN + kBM + 64 * kWaves - 1) / (64 * kWaves);
@@ -97,7 +98,7 @@ struct MxTile {
   static constexpr int late(int nth) { return nth / 2 * 4 + 2 + nth % 2; }
   static_assert(NT % 2 == 0 && kBN % 64 == 0 && kBM % 64 == 0 && kBytesW % (kThreads * 16) == 0 && kBytesX % (kThreads * 16) == 0, "pairs of block rows; whole loads");
   static_assert(kThreads / 8 % 16 == 0 && kThreads / kChunksX % 8 == 0, "a thread's rows have equal keys, or two in turn");
-  static_assert(kLds <= 160 * 1024 && STAGES >= 2 && STAGES <= 4 && STAGES * loads(0) < 64, "LDS of a compute unit; the counter of loads");
+  static_assert(kLds <= 160 * 1024 && STAGES >= 2 && STAGES <= 6 && loads_between(1, STAGES) < 63, "LDS of a compute unit; places for runs; the counter of loads");
 };
 
 // Slot of a chunk among a row's.  LDS serves sixteen-byte reads of lanes 0-3, 12-15, 20-27 together, then of 4-11, 16-19, 28-31, and so on: rows
@@ -130,9 +131,9 @@ __device__ __forceinline__ void store_sixteen(char* c, int64_t row, int64_t cs, 
 // compute unit nothing else would.
 // OUT: the type in which results leave (a template's argument: with a branch the compiler makes copies of all of the way out and reads every
 // accumulator in front of them).
-template <int WN, int WM, int NT, int MT, bool A8, int STAGES, int WAVES_A_SIMD, bool GOES_ON, int OUT>
-__global__ __launch_bounds__(64 * WN * WM, WAVES_A_SIMD) void mx_tile_kernel(const MxMatmulParams p, uint32_t tiles_n, uint32_t tiles_m) {
-  using T = MxTile<WN, WM, NT, MT, A8, STAGES, GOES_ON>;
+template <int WN, int WM, int WK, int NT, int MT, bool A8, int STAGES, int WAVES_A_SIMD, bool GOES_ON, int OUT>
+__global__ __launch_bounds__(64 * WN * WM * WK, WAVES_A_SIMD) void mx_tile_kernel(const MxMatmulParams p, uint32_t tiles_n, uint32_t tiles_m) {
+  using T = MxTile<WN, WM, WK, NT, MT, A8, STAGES, GOES_ON>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -232,29 +233,27 @@ __global__ __launch_bounds__(64 * WN * WM, WAVES_A_SIMD) void mx_tile_kernel(con
     }
   };
 
-  const int wn = wave / WM, wm = wave % WM;
+  const int wn = wave / (WM * WK), wm = wave / WK % WM, wk = wave % WK;
   const int col = lane & 31, half = lane >> 5;
   // a lane's chunks of its row in block 0 (blocks apart by whole rows of equal keys)
   const int row_of_w = wn * (NT * 32) + 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3), row_of_x = wm * (MT * 32) + col;
-  uint32_t at_w[4], at_x[4][A8 ? 2 : 1];
+  constexpr int kSets = 4 / WK;   // of 64 k, of a stage's four, that a wavefront multiplies
+  uint32_t at_w[kSets], at_x[kSets][A8 ? 2 : 1];
 #pragma unroll
-  for (int s = 0; s < 4; ++s) {
-    at_w[s] = lds0 + row_of_w * 128 + (((2 * s + half) ^ slot_key<128>(row_of_w)) << 4);
+  for (int s = 0; s < kSets; ++s) {
+    at_w[s] = lds0 + row_of_w * 128 + (((4 * half + wk * kSets + s) ^ slot_key<128>(row_of_w)) << 4);
 #pragma unroll
     for (int h = 0; h < (A8 ? 2 : 1); ++h)
-      at_x[s][h] = lds0 + T::kBytesW + row_of_x * T::kRowX + ((((A8 ? 4 : 2) * s + 2 * h + half) ^ slot_key<T::kRowX>(row_of_x)) << 4);
+      at_x[s][h] = lds0 + T::kBytesW + row_of_x * T::kRowX + (((A8 ? 8 * h + 2 * (wk * kSets + s) + half : 4 * half + wk * kSets + s) ^ slot_key<T::kRowX>(row_of_x)) << 4);
   }
-  const uint32_t at_sw = lds0 + T::kScales + row_of_w * 16, at_sx = lds0 + T::kScales + (T::kBN + row_of_x) * 16;
+  const uint32_t at_sw = lds0 + T::kScales + row_of_w * 16 + half * 4 + wk * kSets, at_sx = lds0 + T::kScales + (T::kBN + row_of_x) * 16 + half * 4 + wk * kSets;
 
   f32x16 acc[NT * MT];
-  i32x8 x[4][MT], w[2][2][4];
-  u32x2 sx[2][MT], sw[2][2];   // a lane's scales of 64 k `s`: byte 2 (s % 2) of word s / 2, shifted down by its half
+  i32x8 x[kSets][MT], w[2][2][kSets];
+  uint32_t sx[2][MT], sw[2][2];   // byte s: of set s
   constexpr int kPairs = NT / 2, kMeet = 5;
   // a stage's scales of one row
-  auto scales_at = [&](uint32_t at, int offset) {
-    const u32x2 v = read_lds_pair(at, offset);
-    return u32x2{v[0] >> (8 * half), v[1] >> (8 * half)};
-  };
+  auto scales_at = [&](uint32_t at, int offset) { return WK == 2 ? read_lds_short(at, offset) : read_lds_word(at, offset); };
   auto read_w = [&](auto to_tag, auto i_tag, auto s_tag, uint32_t stage) {
     constexpr int to = decltype(to_tag)::value, i = decltype(i_tag)::value, s = decltype(s_tag)::value;
     w[to][i & 1][s] = narrow_fragment(read_lds(at_w[s] + stage, i * 4096));
@@ -284,10 +283,10 @@ __global__ __launch_bounds__(64 * WN * WM, WAVES_A_SIMD) void mx_tile_kernel(con
       }
       // behind matrix instruction AT of the pair: the next pair's weights and scales, the next stage's activations, loads
       auto beside = [&](auto at_tag) {
-        constexpr int AT = decltype(at_tag)::value, kAll = 8 * MT;
-        // of eight fragments (beside the first of several pairs not before the wavefronts have met; all some time before they are waited for)
-        constexpr int start = T::kEarly && !final_pair ? kMeet : 0, step = kAll >= 32 ? 2 : 1, many = (8 * step + kAll - 1) / kAll;
-        constexpr int from = AT < start ? 0 : min_of((AT - start + step - 1) / step * many, 8), to = AT < start ? 0 : min_of((AT - start + step) / step * many, 8);
+        constexpr int AT = decltype(at_tag)::value, kAll = 2 * kSets * MT, kParts = 2 * kSets;
+        // of the pair's fragments (beside the first of several pairs not before the wavefronts have met; all some time before they are waited for)
+        constexpr int start = T::kEarly && !final_pair ? kMeet : 0, step = kAll >= 32 ? 2 : 1, many = (kParts * step + kAll - 1) / kAll;
+        constexpr int from = AT < start ? 0 : min_of((AT - start + step - 1) / step * many, kParts), to = AT < start ? 0 : min_of((AT - start + step) / step * many, kParts);
         static_for<to - from>([&](auto nth) {
           constexpr int f = from + decltype(nth)::value;
           constexpr int i = final_pair ? f & 1 : 2 * pair + 2 + (f & 1);
@@ -311,11 +310,11 @@ __global__ __launch_bounds__(64 * WN * WM, WAVES_A_SIMD) void mx_tile_kernel(con
           issue_piece(std::integral_constant<int, T::piece(first + a + decltype(nth)::value, AHEAD)>{}, std::integral_constant<int, AHEAD % 2>{}, slot);
         });
       };
-      static_for<4>([&](auto s_tag) {
+      static_for<kSets>([&](auto s_tag) {
         static_for<MT>([&](auto j_tag) {
           static_for<2>([&](auto i_tag) {
             constexpr int s = decltype(s_tag)::value, j = decltype(j_tag)::value, i = decltype(i_tag)::value, at = (2 * pair + i) * MT + j;
-            acc[at] = mfma_mx_32<A8, 2 * (s & 1)>(w[now][i][s], x[s][j], acc[at], sw[now][i][s >> 1], sx[PAR][j][s >> 1]);
+            acc[at] = mfma_mx_32<A8, s>(w[now][i][s], x[s][j], acc[at], sw[now][i], sx[PAR][j]);
             __builtin_amdgcn_sched_barrier(0);
             beside(std::integral_constant<int, (s * MT + j) * 2 + i>{});
             __builtin_amdgcn_sched_barrier(0);
@@ -334,20 +333,20 @@ __global__ __launch_bounds__(64 * WN * WM, WAVES_A_SIMD) void mx_tile_kernel(con
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(T::loads_between(1, STAGES)) : "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
-  static_for<8>([&](auto f) {
+  static_for<2 * kSets>([&](auto f) {
     constexpr int F = decltype(f)::value;
     read_w(std::integral_constant<int, 0>{}, std::integral_constant<int, (F & 1)>{}, std::integral_constant<int, (F >> 1)>{}, 0);
     if constexpr (F < 2) sw[0][F] = scales_at(at_sw, F * 512);
   });
   static_for<MT>([&](auto j) {
     sx[0][decltype(j)::value] = scales_at(at_sx, decltype(j)::value * 512);
-    static_for<4>([&](auto s) { read_x(s, j, 0); });
+    static_for<kSets>([&](auto s) { read_x(s, j, 0); });
   });
   const bool shares = p.splits > 1;
   const int64_t c_rs = shares ? p.n : p.c_rs, c_cs = shares ? 1 : p.c_cs;
   char* const c = shares ? reinterpret_cast<char*>(p.partial + (static_cast<int64_t>(blockIdx.z) * p.batch + batch) * p.m * p.n)
                          : static_cast<char*>(p.c) + batch * p.c_bs * (OUT == FP8_REAL_F32 ? 4 : 2);
-  const uint32_t mine = lds0 + T::kResults + wave * 4096;
+  const uint32_t mine = lds0 + T::kResults + wave / WK * 4096;
   int slot = 0;
   uint32_t turn = 0;
   const auto following = [](int at) { return at + 1 == STAGES ? 0 : at + 1; };
@@ -371,6 +370,36 @@ __global__ __launch_bounds__(64 * WN * WM, WAVES_A_SIMD) void mx_tile_kernel(con
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
+    }
+    if constexpr (WK == 2) {   // the second wavefront's sums onto the first one's, which writes them
+      static_assert(!GOES_ON && T::kWaves / 2 * NT * MT * 4096 <= T::kStage * STAGES, "room for them");
+      const uint32_t meet = lds0 + wave / 2 * (NT * MT * 4096) + lane * 16;
+      if (wk == 1) {
+        static_for<NT * MT>([&](auto i) {
+          constexpr int I = decltype(i)::value;
+#pragma unroll
+          for (int e = 0; e < 16; e += 4)
+            write_lds(meet + I * 4096 + e * 256, u32x4{__float_as_uint(acc[I][e]), __float_as_uint(acc[I][e + 1]), __float_as_uint(acc[I][e + 2]), __float_as_uint(acc[I][e + 3])});
+        });
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (wk == 0) {
+        static_for<NT * MT>([&](auto i) {
+          constexpr int I = decltype(i)::value;
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            const u32x4 v = read_lds(meet + I * 4096, e * 256);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) acc[I][e + d] += __uint_as_float(v[d]);
+          }
+        });
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (wk == 1) return;
     }
     // 32 rows of 128 bytes at a time pass through LDS, so that a store instruction fills lines: sixteen bytes of a row lie in slot
     // (place ^ row / 2 % 8) of eight.
@@ -511,10 +540,10 @@ hipError_t launch_few_rows(const MxMatmulParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <int WN, int WM, int NT, int MT, bool A8, int STAGES, int WAVES_A_SIMD, bool GOES_ON, int OUT>
+template <int WN, int WM, int WK, int NT, int MT, bool A8, int STAGES, int WAVES_A_SIMD, bool GOES_ON, int OUT>
 hipError_t launch_tile_as(const MxMatmulParams& p, hipStream_t stream) {
-  using T = MxTile<WN, WM, NT, MT, A8, STAGES, GOES_ON>;
-  constexpr auto kernel = &mx_tile_kernel<WN, WM, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, OUT>;
+  using T = MxTile<WN, WM, WK, NT, MT, A8, STAGES, GOES_ON>;
+  constexpr auto kernel = &mx_tile_kernel<WN, WM, WK, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, OUT>;
   if constexpr (T::kLds > 65536) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds);
     if (e != hipSuccess) return e;
@@ -526,11 +555,11 @@ hipError_t launch_tile_as(const MxMatmulParams& p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-template <int WN, int WM, int NT, int MT, bool A8, int STAGES, int WAVES_A_SIMD, bool GOES_ON>
+template <int WN, int WM, int WK, int NT, int MT, bool A8, int STAGES, int WAVES_A_SIMD, bool GOES_ON>
 hipError_t launch_tile(const MxMatmulParams& p, hipStream_t stream) {
-  if (p.splits == 1 && p.out_kind == FP8_REAL_BF16) return launch_tile_as<WN, WM, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, FP8_REAL_BF16>(p, stream);
-  if (p.splits == 1 && p.out_kind == FP8_REAL_F16) return launch_tile_as<WN, WM, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, FP8_REAL_F16>(p, stream);
-  const hipError_t e = launch_tile_as<WN, WM, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, FP8_REAL_F32>(p, stream);
+  if (p.splits == 1 && p.out_kind == FP8_REAL_BF16) return launch_tile_as<WN, WM, WK, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, FP8_REAL_BF16>(p, stream);
+  if (p.splits == 1 && p.out_kind == FP8_REAL_F16) return launch_tile_as<WN, WM, WK, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, FP8_REAL_F16>(p, stream);
+  const hipError_t e = launch_tile_as<WN, WM, WK, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, FP8_REAL_F32>(p, stream);
   if (p.splits == 1 || e != hipSuccess) return e;
   return launch_join_shares({p.partial, p.c, p.c_rs, p.c_cs, p.c_bs, p.m, p.n, p.batch, p.splits, p.out_kind}, stream);
 }
@@ -542,16 +571,18 @@ MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int64_t batch, bool a_wide) {
   if (m <= 16) return {MX_FEW_ROWS, 1, 16, 16, 4};
   const int64_t big = ((m + (a_wide ? 127 : 255)) / (a_wide ? 128 : 256)) * ((n + 255) / 256) * batch, middle = ((m + 127) / 128) * ((n + 127) / 128) * batch;
   if (big >= 192) return {MX_TILE_256, 1, a_wide ? 128 : 256, 256, kRunBlocks};
-  if (middle >= 128) return {MX_TILE_128, 1, 128, 128, kRunBlocks};
+  if (middle >= 128) return {a_wide ? MX_TILE_128_DEEP : MX_TILE_128, 1, 128, 128, kRunBlocks};
   return {MX_TILE_64, 1, 64, 64, kRunBlocks};
 }
 
 hipError_t launch_mx_matmul(const MxMatmulParams& p, int kind, hipStream_t stream) {
   switch (kind) {
     case MX_FEW_ROWS: return p.a_wide ? launch_few_rows<true>(p, stream) : launch_few_rows<false>(p, stream);
-    case MX_TILE_64: return p.a_wide ? launch_tile<1, 2, 2, 1, true, 3, 2, false>(p, stream) : launch_tile<1, 2, 2, 1, false, 3, 2, false>(p, stream);
-    case MX_TILE_128: return p.a_wide ? launch_tile<2, 2, 2, 2, true, 2, 2, false>(p, stream) : launch_tile<2, 2, 2, 2, false, 2, 2, false>(p, stream);
-    case MX_TILE_256: return p.a_wide ? launch_tile<2, 2, 4, 2, true, 2, 1, true>(p, stream) : launch_tile<2, 2, 4, 4, false, 2, 1, true>(p, stream);
+    case MX_TILE_64: return p.a_wide ? launch_tile<1, 2, 2, 2, 1, true, 3, 2, false>(p, stream) : launch_tile<1, 2, 2, 2, 1, false, 4, 2, false>(p, stream);
+    case MX_TILE_64_DEEP: return p.a_wide ? launch_tile<1, 2, 2, 2, 1, true, 5, 2, false>(p, stream) : launch_tile<1, 2, 2, 2, 1, false, 6, 2, false>(p, stream);
+    case MX_TILE_128: return p.a_wide ? hipErrorInvalidValue : launch_tile<2, 2, 1, 2, 2, false, 2, 2, false>(p, stream);
+    case MX_TILE_128_DEEP: return p.a_wide ? launch_tile<2, 2, 2, 2, 2, true, 3, 2, false>(p, stream) : launch_tile<2, 2, 2, 2, 2, false, 4, 2, false>(p, stream);
+    case MX_TILE_256: return p.a_wide ? launch_tile<2, 2, 1, 4, 2, true, 2, 1, true>(p, stream) : launch_tile<2, 2, 1, 4, 4, false, 2, 1, true>(p, stream);
   }
   return hipErrorInvalidValue;
 }

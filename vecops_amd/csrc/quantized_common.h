@@ -84,7 +84,8 @@ __device__ __forceinline__ void store_results(void* c, int64_t at, int64_t cs, i
 
 typedef __attribute__((address_space(3))) u32x4 lds_u32x4;
 typedef __attribute__((address_space(3))) float lds_float;
-typedef __attribute__((address_space(3))) u32x2 lds_u32x2;
+typedef __attribute__((address_space(3))) uint32_t lds_word;
+typedef __attribute__((address_space(3))) uint16_t lds_short;
 typedef __attribute__((address_space(3))) char lds_char;
 
 // (`offset`, a constant, goes into the instruction)
@@ -94,8 +95,11 @@ __device__ __forceinline__ u32x4 read_lds(uint32_t at, int offset) {
 __device__ __forceinline__ void write_lds(uint32_t at, const u32x4& v) {
   *reinterpret_cast<lds_u32x4*>(reinterpret_cast<lds_char*>(static_cast<uintptr_t>(at))) = v;
 }
-__device__ __forceinline__ u32x2 read_lds_pair(uint32_t at, int offset) {
-  return *reinterpret_cast<const lds_u32x2*>(reinterpret_cast<const lds_char*>(static_cast<uintptr_t>(at)) + offset);
+__device__ __forceinline__ uint32_t read_lds_word(uint32_t at, int offset) {
+  return *reinterpret_cast<const lds_word*>(reinterpret_cast<const lds_char*>(static_cast<uintptr_t>(at)) + offset);
+}
+__device__ __forceinline__ uint32_t read_lds_short(uint32_t at, int offset) {
+  return *reinterpret_cast<const lds_short*>(reinterpret_cast<const lds_char*>(static_cast<uintptr_t>(at)) + offset);
 }
 __device__ __forceinline__ float read_lds_float(uint32_t at, int offset) {
   return *reinterpret_cast<const lds_float*>(reinterpret_cast<const lds_char*>(static_cast<uintptr_t>(at)) + offset);
