@@ -50,6 +50,33 @@ __device__ __forceinline__ void load_row_eight(const void* base, int64_t at, int
   }
 }
 
+// The same in two steps, so that many loads can be under way: what memory holds, then its numbers.
+template <int KIND>
+struct RawEight {
+  u32x4 w[KIND == FP8_REAL_F32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* base, int64_t at) {
+    const VECOPS_GLOBAL auto* x = (const VECOPS_GLOBAL typename Real<KIND>::type*)base + at;
+    w[0] = load_16(x);
+    if constexpr (KIND == FP8_REAL_F32) w[1] = load_16(x + 4);
+  }
+  __device__ __forceinline__ float operator[](int e) const {
+    if constexpr (KIND == FP8_REAL_F32) return __uint_as_float(w[e >> 2][e & 3]);
+    else return real_bits_to_f32((w[0][e >> 1] >> (16 * (e & 1))) & 0xffffu, KIND);
+  }
+  // where less than eight are there: one by one, zeros behind them
+  __device__ __forceinline__ void load_part(const void* base, int64_t at, int left) {
+    const VECOPS_GLOBAL auto* x = (const VECOPS_GLOBAL typename Real<KIND>::type*)base + at;
+#pragma unroll
+    for (int d = 0; d < (KIND == FP8_REAL_F32 ? 2 : 1); ++d) w[d] = u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (e >= left) continue;
+      if constexpr (KIND == FP8_REAL_F32) w[e >> 2][e & 3] = __float_as_uint(x[e]);
+      else w[0][e >> 1] |= static_cast<uint32_t>(x[e]) << (16 * (e & 1));
+    }
+  }
+};
+
 __device__ __forceinline__ uint32_t most_bits(const float (&v)[8]) {
   uint32_t most = 0;
 #pragma unroll
@@ -220,17 +247,9 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const MxCopyParams p
 enum : int { SOURCE_NORM = 0, SOURCE_GATE = 1 };
 constexpr int kHeld = 4;
 
-// g / (1 + e^-g).  The exponent's product with log2 e is carried as two numbers, the quotient gets one Newton step: within 2 units of
-// the last place where the factors v_exp_f32 and v_rcp_f32 alone are off by up to |g| of them.
-__device__ __forceinline__ float silu(float g) {
-  const float hi = g * -1.44269504f;
-  const float lo = fmaf(g, -1.44269504f, -hi) + g * -1.92596303e-8f;
-  float e = __builtin_amdgcn_exp2f(hi);
-  const bool plain = fabsf(hi) < 126.0f;   // (infinities and what overflows: without the corrections, which would be NaN there)
-  e = plain ? fmaf(e, lo * 0.693147181f, e) : e;
-  const float d = 1.0f + e, r = __builtin_amdgcn_rcpf(d), q = g * r;
-  return plain ? fmaf(fmaf(-q, d, g), r, q) : q;
-}
+// g / (1 + e^-g).  The exponent's product with log2 e is off by 1.25 * 2^-24 of itself, which is as much of e^-g as |g| times that; v_exp_f32,
+// the sum, v_rcp_f32 and the product add a unit of the last place each.  (Where e^-g overflows the result is -0, for -infinity NaN.)
+__device__ __forceinline__ float silu(float g) { return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504f)); }
 
 template <int KIND>
 __device__ __forceinline__ float as_held(float v) {   // rounded to the type
@@ -255,31 +274,46 @@ __global__ __launch_bounds__(1024) void row_quantize_kernel(const RowQuantizePar
     const int64_t residual_at = batch * p.residual_bs + row * p.residual_rs;
     float v[kHeld][8];
 
-    // the pieces of a span from k0 on; `again`: the residual has been added
+    // the pieces of a span from k0 on, all their loads under way at once; `again`: the residual has been added
     auto load = [&](int k0, bool again) {
+      constexpr int kSources = 2;
+      RawEight<KIND> raw[kHeld][kSources];
+      const bool adds = SOURCE == SOURCE_NORM && p.residual != nullptr && !again, two = SOURCE == SOURCE_GATE || adds;
+      const bool sum = SOURCE == SOURCE_NORM && p.residual != nullptr && again;
+      const void* const first = sum ? p.summed : p.x;
+      const void* const second = SOURCE == SOURCE_GATE ? p.x : p.residual;
+      const int64_t first_at = sum ? summed_at : x_at, second_at = SOURCE == SOURCE_GATE ? x_at + p.k : residual_at;
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) {
+        const int k = k0 + (i * threads + own) * 8;
+        if (p.k - k < 8) continue;
+        raw[i][0].load(first, first_at + k);
+        if (two) raw[i][1].load(second, second_at + k);
+      }
 #pragma unroll
       for (int i = 0; i < kHeld; ++i) {
         const int k = k0 + (i * threads + own) * 8, left = p.k - k;
+        if (left < 8) {
+          raw[i][0].load_part(first, first_at + k, left);
+          if (two) raw[i][1].load_part(second, second_at + k, left);
+        }
         if (k0 + i * threads * 8 >= p.k) {   // (uniform)
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
           continue;
         }
         if constexpr (SOURCE == SOURCE_GATE) {
-          float up[8];
-          load_row_eight<KIND>(p.x, x_at + k, 1, left, left >= 8, v[i]);
-          load_row_eight<KIND>(p.x, x_at + p.k + k, 1, left, left >= 8, up);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[i][e] = e < left ? silu(v[i][e]) * up[e] : 0.0f;
-        } else if (p.residual == nullptr || again) {
-          load_row_eight<KIND>(p.residual == nullptr ? p.x : p.summed, (p.residual == nullptr ? x_at : summed_at) + k, 1, left, left >= 8, v[i]);
+          for (int e = 0; e < 8; ++e) v[i][e] = silu(raw[i][0][e]) * raw[i][1][e];   // (what is not there: 0)
         } else {
-          float more[8];
-          load_row_eight<KIND>(p.x, x_at + k, 1, left, left >= 8, v[i]);
-          load_row_eight<KIND>(p.residual, residual_at + k, 1, left, left >= 8, more);
+          if (adds) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[i][e] = as_held<KIND>(v[i][e] + more[e]);
-          store_results<8>(p.summed, summed_at + k, 1, KIND, k, p.k, v[i]);
+            for (int e = 0; e < 8; ++e) v[i][e] = as_held<KIND>(raw[i][0][e] + raw[i][1][e]);
+            store_results<8>(p.summed, summed_at + k, 1, KIND, k, p.k, v[i]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] = raw[i][0][e];
+          }
         }
       }
     };
@@ -295,7 +329,11 @@ __global__ __launch_bounds__(1024) void row_quantize_kernel(const RowQuantizePar
           if (p.weight_kind == KIND) load_row_eight<KIND>(p.weight, k, 1, left, left >= 8, w);
           else load_row_eight<FP8_REAL_F32>(p.weight, k, 1, left, left >= 8, w);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[i][e] = e < left ? v[i][e] * norm * w[e] : 0.0f;
+          for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] * norm * w[e];   // (what is not there: 0, but for a norm that is not finite)
+          if (left < 8) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[i][e] = e < left ? v[i][e] : 0.0f;
+          }
         }
       }
     };
