@@ -113,12 +113,12 @@ def test_dequantize_every_element_and_scale(device, dtype, form):
 
 def check(c, a, sa, b, sb):
     """|error| <= what the additions can lose, times the sum of the terms' sizes, and the rounding of the result.  An instruction adds
-    four blocks' sums to the accumulator: each of the five may lose a unit of the sum's last place in fp32, 2^-23 of the sizes; then
-    up to eight shares are added.  With e4m3 operands, of eight products along k the seven smaller ones may each lose 2^-13 of the
-    largest's power of two."""
+    four blocks' sums to the accumulator, or twice two: each of the five or six may lose a unit of the sum's last place in fp32, 2^-23 of the sizes;
+    then up to eight wavefronts' and four shares of k are added.  With e4m3 operands, of eight products along k the seven smaller ones may each lose
+    2^-13 of the largest's power of two."""
     x, w = values(a, sa), values(b, sb)
     want, size = x @ w.transpose(-1, -2), x.abs() @ w.abs().transpose(-1, -2)
-    bound = (5 * blocks(x.shape[-1], 128) + 8) * 2.0 ** -23 * size
+    bound = (6 * blocks(x.shape[-1], 128) + 12) * 2.0 ** -23 * size
     if a.dtype == FP8:
         bound = bound + 7 * 2.0 ** -13 * size
     unit = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[c.dtype]
@@ -156,6 +156,35 @@ def test_matmul(device, m, n, k, form):
         check(c, a, sa, b, sb)
         c.fill_(7.0)
         assert bool((store == 7.0).all())
+
+
+ROWS = lambda *of: f"mx_slim_kernel<{','.join(map(str, of))}>"  # noqa: E731  (weight rows, activation rows, e4m3, wavefronts, places)
+TILE = lambda *of: f"mx_tile_kernel<{','.join(map(str, of))}"  # noqa: E731  (wavefronts, blocks of 32 a wavefront, e4m3)
+
+
+@pytest.mark.parametrize("m,n,k,form,kernel,shares", [
+    (1, 17, 96, FP4, ROWS(16, 4, 0, 2, 1), 0), (4, 33, 544, FP8, ROWS(16, 4, 1, 2, 1), 0), (3, 5055, 1088, FP4, ROWS(16, 4, 0, 4, 1), 0),
+    (4, 31, 1120, FP8, ROWS(16, 4, 1, 4, 1), 0), (3, 17, 2368, FP4, ROWS(16, 4, 0, 4, 2), 0), (2, 100, 9000, FP8, ROWS(16, 4, 1, 4, 2), 0),
+    (5, 16, 32, FP4, ROWS(16, 16, 0, 4, 1), 0), (16, 50, 1000, FP8, ROWS(16, 16, 1, 4, 1), 0), (17, 100, 5000, FP4, ROWS(16, 16, 0, 4, 2), 0),
+    (16, 17, 2112, FP8, ROWS(16, 16, 1, 8, 1), 0), (65, 17, 32, FP4, ROWS(32, 32, 0, 4, 1), 0), (65, 17, 32, FP8, ROWS(32, 32, 1, 4, 1), 0),
+    (100, 16, 6368, FP4, ROWS(32, 32, 0, 4, 1), 4), (65, 17, 5312, FP8, ROWS(32, 32, 1, 4, 1), 4), (200, 368, 7200, FP8, ROWS(32, 32, 1, 4, 1), 2),
+    (260, 16, 32, FP4, TILE(1, 2, 2, 2, 1, 0), 0), (260, 90, 70, FP8, TILE(1, 2, 2, 2, 1, 1), 0), (300, 22, 4576, FP4, TILE(1, 2, 2, 2, 1, 0), 4),
+    (4100, 17, 6208, FP8, TILE(1, 2, 2, 2, 1, 1), 2), (4100, 453, 32, FP4, TILE(2, 2, 1, 2, 2, 0), 0), (4100, 210, 10176, FP4, TILE(2, 2, 1, 2, 2, 0), 4),
+    (4100, 550, 3488, FP4, TILE(2, 2, 2, 2, 2, 0), 0), (4100, 358, 5760, FP4, TILE(2, 2, 2, 2, 2, 0), 2), (4100, 453, 32, FP8, TILE(2, 2, 2, 2, 2, 1), 0),
+    (4100, 3257, 1312, FP4, TILE(2, 2, 1, 4, 4, 0), 0), (2050, 1083, 15712, FP4, TILE(2, 2, 1, 4, 4, 0), 4), (4100, 989, 32, FP8, TILE(2, 2, 1, 4, 2, 1), 0),
+    (4100, 210, 10176, FP8, TILE(2, 2, 1, 4, 2, 1), 4)])
+def test_every_kernel_of_the_product(device, m, n, k, form, kernel, shares):
+    """Each variant that sizes choose, with shares of k and without, up to odd ends of every extent."""
+    a, sa = operands(m, k, form, seed=11)
+    b, sb = operands(n, k, FP4, seed=12)
+    there = [t.to(device) for t in (a, sa, b, sb)]
+    rows = torch.arange(m) if m <= 300 else torch.cat([torch.arange(70), torch.arange(m - 70, m), torch.randint(0, m, (60,), generator=torch.Generator().manual_seed(m))])
+    for dtype in REAL:
+        c = torch.full((m, n), 7.0, dtype=dtype, device=device)
+        names = launched_kernels(lambda c=c: capi.matmul_mx(*there, c))
+        assert any(name.startswith(kernel) for name in names), names
+        assert ("join_shares_kernel" in "".join(names)) == (shares > 0), names
+        check(c[rows.to(device)], only(a, rows), only(sa, rows), b, sb)
 
 
 @pytest.mark.parametrize("form", [FP4, FP8])
@@ -241,9 +270,9 @@ def test_matmul_nothing_to_sum(device):
     capi.quantize_mx(torch.empty((0, 64), device=device), a, sa)
 
 
-def test_matmul_replayed_in_a_graph(device):
-    """Captured with a workspace that a K split and copies need; replayed among eager work, on new operands."""
-    m, n, k = 64, 512, 8000
+@pytest.mark.parametrize("m,n,k", [(64, 512, 8000), (300, 22, 4576), (100, 64, 300)])
+def test_matmul_replayed_in_a_graph(device, m, n, k):
+    """Captured, also with a workspace for shares of k or for copies; replayed among eager work, on new operands."""
     g = torch.Generator(device=device).manual_seed(1)
     x = torch.randn((m, k), generator=g, device=device)
     w = torch.randn((n, k), generator=g, device=device)

@@ -34,26 +34,26 @@ def test_copies(changes, code, word):
 
 
 def product(**changes):
-    return {"a": operand(F4, 5, 160), "sa": operand(E8, 5, 10), "b": operand(F4, 200, 160), "sb": operand(E8, 200, 10), "c": operand(F32, 5, 200)} | changes
+    return {"a": operand(F4, 5, 320), "sa": operand(E8, 5, 20), "b": operand(F4, 200, 320), "sb": operand(E8, 200, 20), "c": operand(F32, 5, 200)} | changes
 
 
 @pytest.mark.parametrize("changes,code,word", [
-    ({"a": operand(I8, 5, 320)}, NOT_APPLICABLE, "e2m1"),
-    ({"b": operand(F8, 200, 320)}, NOT_APPLICABLE, "b e2m1"),
+    ({"a": operand(I8, 5, 640)}, NOT_APPLICABLE, "e2m1"),
+    ({"b": operand(F8, 200, 640)}, NOT_APPLICABLE, "b e2m1"),
     ({"c": operand(I8, 5, 200)}, NOT_APPLICABLE, "c f32"),
-    ({"b": operand(F4, 200, 161)}, INVALID, "K of a"),
-    ({"a": operand(F8, 5, 160)}, INVALID, "K of a (160) and b (320)"),
+    ({"b": operand(F4, 200, 321)}, INVALID, "K of a"),
+    ({"a": operand(F8, 5, 320)}, INVALID, "K of a (320) and b (640)"),
     ({"c": operand(F32, 5, 201)}, INVALID, "c must be"),
     ({"c": operand(F32, 1, 5, 200)}, INVALID, "ranks"),
-    ({"sa": operand(E8, 5, 9)}, INVALID, "a_scales must be"),
-    ({"sb": operand(E8, 7, 10)}, INVALID, "b_scales must be [N=200"),
-    ({"sb": operand(F32, 200, 10)}, INVALID, "e8m0"),
-    ({"a": operand(F4, 5, 160, data=None)}, INVALID, "null"),
-    ({"sb": operand(E8, 200, 10, data=None)}, INVALID, "null"),
+    ({"sa": operand(E8, 5, 19)}, INVALID, "a_scales must be"),
+    ({"sb": operand(E8, 7, 20)}, INVALID, "b_scales must be [N=200"),
+    ({"sb": operand(F32, 200, 20)}, INVALID, "e8m0"),
+    ({"a": operand(F4, 5, 320, data=None)}, INVALID, "null"),
+    ({"sb": operand(E8, 200, 20, data=None)}, INVALID, "null"),
     ({"c": operand(F32, 5, 200, data=None)}, INVALID, "null"),
-    ({"b": operand(F4, 200, 160, strides=(1, 200))}, INVALID, "workspace"),
-    ({"sa": operand(E8, 5, 10, strides=(2 ** 20 + 1, 1))}, INVALID, "workspace"),
-    ({"a": operand(F4, 5, 160, strides=(-160, 1))}, INVALID, "workspace"),
+    ({"b": operand(F4, 200, 320, strides=(1, 200))}, INVALID, "workspace"),
+    ({"sa": operand(E8, 5, 20, strides=(2 ** 20 + 1, 1))}, INVALID, "workspace"),
+    ({"a": operand(F4, 5, 320, strides=(-320, 1))}, INVALID, "workspace"),
 ])
 def test_matmul(changes, code, word):
     v = product(**changes)
@@ -64,31 +64,31 @@ def test_matmul_batches_extents_and_workspace():
     f, need = capi.lib().vecops_hip_matmul_mx, capi.lib().vecops_hip_matmul_mx_workspace
     names = ("a", "sa", "b", "sb", "c")
     asked = lambda **changes: need(*(ref(product(**changes)[n]) for n in names))  # noqa: E731
-    v = [operand(F4, 2, 5, 160), operand(E8, 2, 5, 10), operand(F4, 3, 200, 160), operand(E8, 2, 200, 10), operand(F32, 2, 5, 200)]
+    v = [operand(F4, 2, 5, 320), operand(E8, 2, 5, 20), operand(F4, 3, 200, 320), operand(E8, 2, 200, 20), operand(F32, 2, 5, 200)]
     refused(f(*map(C.byref, v), None, 0, None), INVALID, "batch")
     assert need(*map(C.byref, v)) == 0
     assert asked() == 0
-    assert asked(b=operand(F4, 200, 160, strides=(333, 1))) == 0
+    assert asked(b=operand(F4, 200, 320, strides=(353, 1))) == 0
     up = lambda n: -(-n // 256) * 256  # noqa: E731
-    assert asked(b=operand(F4, 200, 160, strides=(1, 200))) == up(200 * 160)
-    assert asked(sa=operand(E8, 5, 10, strides=(1, 5))) == up(5 * 12)
-    # a K of no whole blocks: both operands padded; fewer than four scales a row: those too
-    assert asked(a=operand(F4, 5, 159), b=operand(F4, 200, 159)) == up(5 * 160) + up(200 * 160)
-    assert asked(a=operand(F8, 5, 318), b=operand(F4, 200, 159)) == up(5 * 320) + up(200 * 160)
-    assert asked(a=operand(F4, 5, 32), sa=operand(E8, 5, 2), b=operand(F4, 200, 32), sb=operand(E8, 200, 2)) == up(5 * 4) + up(200 * 4)
-    shared = product(a=operand(F4, 7, 5, 160), sa=operand(E8, 7, 5, 10), b=operand(F4, 7, 200, 160, strides=(0, 1, 200)),
-                     sb=operand(E8, 7, 200, 10), c=operand(F32, 7, 5, 200))
-    assert need(*(ref(shared[n]) for n in names)) == up(200 * 160)
-    v = product(b=operand(F4, 200, 160, strides=(1, 200)))
+    assert asked(b=operand(F4, 200, 320, strides=(1, 200))) == up(200 * 320)
+    assert asked(sa=operand(E8, 5, 20, strides=(1, 5))) == up(5 * 20)
+    # a K of no whole blocks: both operands padded; fewer than sixteen scales a row: those too
+    assert asked(a=operand(F4, 5, 319), b=operand(F4, 200, 319)) == up(5 * 320) + up(200 * 320)
+    assert asked(a=operand(F8, 5, 638), b=operand(F4, 200, 319)) == up(5 * 640) + up(200 * 320)
+    assert asked(a=operand(F4, 5, 32), sa=operand(E8, 5, 2), b=operand(F4, 200, 32), sb=operand(E8, 200, 2)) == up(5 * 16) + up(200 * 16)
+    shared = product(a=operand(F4, 7, 5, 320), sa=operand(E8, 7, 5, 20), b=operand(F4, 7, 200, 320, strides=(0, 1, 200)),
+                     sb=operand(E8, 7, 200, 20), c=operand(F32, 7, 5, 200))
+    assert need(*(ref(shared[n]) for n in names)) == up(200 * 320)
+    v = product(b=operand(F4, 200, 320, strides=(1, 200)))
     refused(f(*(ref(v[n]) for n in names), 0x10008, 1 << 20, None), INVALID, "16-byte aligned workspace")
     refused(f(*(ref(v[n]) for n in names), 0x10000, 100, None), INVALID, "workspace of")
     long = 1 << 26
     v = product(a=operand(F8, 300, long), sa=operand(E8, 300, long // 32), b=operand(F4, 300, long // 2), sb=operand(E8, 300, long // 32), c=operand(BF16, 300, 300))
     refused(f(*(ref(v[n]) for n in names), None, 0, None), NOT_APPLICABLE, "too long")
-    v = product(b=operand(F4, 1 << 28, 160), sb=operand(E8, 1 << 28, 10), c=operand(F32, 5, 1 << 28))
+    v = product(b=operand(F4, 1 << 28, 320), sb=operand(E8, 1 << 28, 20), c=operand(F32, 5, 1 << 28))
     refused(f(*(ref(v[n]) for n in names), None, 0, None), INVALID, "too large")
     # nothing to do: nothing is needed
-    v = product(a=operand(F4, 0, 160, data=None), sa=operand(E8, 0, 10, data=None), c=operand(F32, 0, 200, data=None))
+    v = product(a=operand(F4, 0, 320, data=None), sa=operand(E8, 0, 20, data=None), c=operand(F32, 0, 200, data=None))
     assert f(*(ref(v[n]) for n in names), None, 0, None) == 0
 
 

@@ -2978,7 +2978,6 @@ int32_t describe_mx(const VecopsHipOperand* a, const VecopsHipOperand* a_scales,
     return fail(ST_INVALID, "matmul_mx: a_scales must be [M=%lld, ceil(K / 32)=%lld]", (long long)m, (long long)mx_blocks(k));
   if (pr->sb.rows != n || pr->sb.cols != mx_blocks(k))
     return fail(ST_INVALID, "matmul_mx: b_scales must be [N=%lld, ceil(K / 32)=%lld]", (long long)n, (long long)mx_blocks(k));
-  // (a grid holds fewer than 2^32 threads: workgroups of 256 for tiles of 128 x 128 or sixteen columns of a few rows, of 512 for larger tiles)
   if (m > INT32_MAX / 2 || n > (1 << 27) || batch > 65535 || ((m + 63) / 64) * ((n + 63) / 64) >= (1 << 24)) return fail(ST_INVALID, "matmul_mx: extent too large");
   pr->plan = mx_plan(m, n, k, batch, pr->a.dtype == DT_E4M3);
   if (m == 0 || n == 0 || batch == 0) return ST_OK;

@@ -2,9 +2,9 @@
 #include "mx_block.h"
 
 #include <algorithm>
+#include <cmath>
 #include <utility>
 
-#include "lane_exchange.h"
 #include "quantized_common.h"
 
 namespace vecops_hip {
@@ -446,98 +446,180 @@ __global__ __launch_bounds__(64 * WN * WM * WK, WAVES_A_SIMD) void mx_tile_kerne
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // (no load may write LDS once the workgroup is gone)
 }
 
-// Up to sixteen rows: bound by HBM, so that what counts is how many bytes of the weights are under way.  A workgroup owns sixteen
-// weight rows; its wavefronts share the steps of 256 k, a run of neighbouring ones each, with the loads of DEPTH steps of both
-// operands and their scales under way, straight into the registers that the matrix instruction reads.  The wavefronts' sums meet in LDS.
-template <int WAVES, bool A8>
-__global__ __launch_bounds__(64 * WAVES, A8 ? 3 : 4) void mx_few_rows_kernel(const MxMatmulParams p) {
-  constexpr int DEPTH = 4, X = A8 ? 4 : 2;
-  __shared__ f32x4 sums[WAVES][64];
+// Few rows, or few results: R weight rows (16 or 32) and XR activation rows a workgroup, whose wavefronts share k without a barrier: each
+// has its own runs of 512 k, every WAVES-th, and its own DEPTH places for them in LDS, filled by loads that write LDS (whole lines, so that a load is
+// a look-up in the cache for every eight lanes or more).  Bound by HBM, or by what a compute unit can have under way: about 40 GB/s as soon as some of its
+// lines come from beyond its die's cache.
+// R = 16: v_mfma_scale_f32_16x16x128_f8f6f4, place q of instruction t of a run has block 4 q + t of sixteen; R = 32: 32x32x64, place q of
+// instruction t has block 8 q + t.  Either way a lane's scales are whole words whose byte is a constant of the instruction.
+template <int R, int XR, bool A8, int WAVES, int DEPTH>
+struct MxSlim {
+  static constexpr int kRowX = A8 ? 512 : 256, kChunksX = kRowX / 16;
+  static constexpr int kBytesW = R * 256, kBytesX = XR * kRowX, kScales = kBytesW + kBytesX, kPlace = kScales + 2048;
+  static constexpr int kLoadsW = kBytesW / 1024, kLoadsX = kBytesX / 1024, kLoads = kLoadsW + kLoadsX + 2;
+  static constexpr int kColumns = XR < R ? 1 : XR / R;                       // blocks of R activation rows
+  static constexpr int kSum = kColumns * R * R * 4;                         // bytes of a wavefront's sums
+  static constexpr int kLds = WAVES * DEPTH * kPlace > WAVES * kSum ? WAVES * DEPTH * kPlace : WAVES * kSum;
+  static_assert((R == 16 || R == 32) && XR % 4 == 0 && XR <= 64 && kLds <= 160 * 1024 && (DEPTH - 1) * kLoads < 63, "rows of scales a load; LDS; the counter of loads");
+};
+
+template <int R, int XR, bool A8, int WAVES, int DEPTH>
+__global__ __launch_bounds__(64 * WAVES, 2) void mx_slim_kernel(const MxMatmulParams p, uint32_t tiles_m, uint32_t units) {
+  using T = MxSlim<R, XR, A8, WAVES, DEPTH>;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int col = lane & 15, quarter = lane >> 4;
+  const uint32_t lds0 = lds_address_of(lds), own = lds0 + wave * (DEPTH * T::kPlace);
   const int batch = blockIdx.y;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
-  const int last_n = static_cast<int>(min(p.n - n0, static_cast<int64_t>(16))) - 1;
-  const uint32_t row_w = static_cast<uint32_t>(p.groups) * 16u, row_x = static_cast<uint32_t>(p.groups) * (A8 ? 32u : 16u);
+  const int runs = (p.groups + kRunBlocks - 1) / kRunBlocks;
+  const int run_begin = static_cast<int>(static_cast<int64_t>(runs) * blockIdx.z / p.splits);
+  const int run_end = static_cast<int>(static_cast<int64_t>(runs) * (blockIdx.z + 1) / p.splits);
+  // each die a contiguous run of tiles: those of the same weights are neighbours
+  const uint32_t xcd = blockIdx.x & 7, share = units >> 3, extra = units & 7;
+  const uint32_t pid = xcd * share + min(xcd, extra) + (blockIdx.x >> 3);
+  const int64_t n0 = static_cast<int64_t>(pid / tiles_m) * R, m0 = static_cast<int64_t>(pid % tiles_m) * XR;
+  const int last_n = static_cast<int>(min(p.n - n0, static_cast<int64_t>(R))) - 1, last_m = static_cast<int>(min(p.m - m0, static_cast<int64_t>(XR))) - 1;
+
   // Rows past the last one lie past the descriptors' ends: zeros arrive.
-  const auto operand = [](const uint8_t* base, int64_t bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc((void*)uniform_ptr((const VECOPS_GLOBAL char*)base), 0, __builtin_amdgcn_readfirstlane(static_cast<int>(bytes)), 0x00020000);
-  };
-  const __amdgpu_buffer_rsrc_t desc_w = operand(p.b + batch * p.b_bs + n0 * p.ldb, last_n * p.ldb + row_w);
-  const __amdgpu_buffer_rsrc_t desc_x = operand(p.a + batch * p.a_bs, (p.m - 1) * p.lda + row_x);
-  const __amdgpu_buffer_rsrc_t desc_sw = operand(p.b_scales + batch * p.bs_bs + n0 * p.bs_rs, last_n * p.bs_rs + p.row_scales);
-  const __amdgpu_buffer_rsrc_t desc_sx = operand(p.a_scales + batch * p.as_bs, (p.m - 1) * p.as_rs + p.row_scales);
-  // Two neighbouring lanes load thirty-two bytes of one row of weights, once of either's, and exchange them: sixteen bytes of a row
-  // each are a look-up in the cache for every lane.
-  uint32_t from_w[2], chunk_x[X];
-  const uint32_t chunk_w = quarter * 32 + (col & 1) * 16;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) from_w[h] = static_cast<uint32_t>(((col & 14) + h) * p.ldb) + chunk_w;
-#pragma unroll
-  for (int c = 0; c < X; ++c) chunk_x[c] = (A8 ? 4 * (quarter >> 1) + (quarter & 1) + 2 * (c >> 1) + 8 * (c & 1) : 2 * quarter + c) * 16;
-  const uint32_t from_x = static_cast<uint32_t>(col * p.lda);
-  const uint32_t from_sw = static_cast<uint32_t>(col * p.bs_rs), from_sx = static_cast<uint32_t>(col * p.as_rs);
+  const u32x4 desc_w = tile_buffer_words((const VECOPS_GLOBAL char*)p.b + batch * p.b_bs + n0 * p.ldb);
+  const u32x4 desc_x = tile_buffer_words((const VECOPS_GLOBAL char*)p.a + batch * p.a_bs + m0 * p.lda);
+  const u32x4 desc_sw = tile_buffer_words((const VECOPS_GLOBAL char*)p.b_scales + batch * p.bs_bs + n0 * p.bs_rs);
+  const u32x4 desc_sx = tile_buffer_words((const VECOPS_GLOBAL char*)p.a_scales + batch * p.as_bs + m0 * p.as_rs);
+  const uint32_t end_w = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(last_n * p.ldb) + static_cast<uint32_t>(p.groups) * 16u);
+  const uint32_t end_x = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(last_m * p.lda) + static_cast<uint32_t>(p.groups) * (A8 ? 32u : 16u));
+  const uint32_t end_sw = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(last_n * p.bs_rs + p.row_scales));
+  const uint32_t end_sx = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(last_m * p.as_rs + p.row_scales));
 
-  const int steps = (p.groups + kStepBlocks - 1) / kStepBlocks;
-  const int begin = static_cast<int>(static_cast<int64_t>(steps) * wave / WAVES), end = static_cast<int>(static_cast<int64_t>(steps) * (wave + 1) / WAVES);
-  u32x4 wv[DEPTH][2], xv[DEPTH][X];
-  uint32_t sw[DEPTH], sx[DEPTH];
-  auto load = [&](auto slot_tag, int g) {
-    constexpr int slot = decltype(slot_tag)::value;
-    const uint32_t kw = static_cast<uint32_t>(g) * 128u, kx = static_cast<uint32_t>(g) * (A8 ? 256u : 128u);
+  // Slot of a chunk: (chunk ^ (row + 4) % 16), of which LDS serves the rows that it reads together without conflicts (R = 16: of two places,
+  // rows 0-3 and 12-15 of one, 4-11 of the other).  Load i of the weights: rows 4 i + lane / 16, slot lane % 16.
+  const uint32_t from_sw = lane < R ? static_cast<uint32_t>(lane * p.bs_rs) : kNowhere, from_sx = lane < XR ? static_cast<uint32_t>(lane * p.as_rs) : kNowhere;
+  auto issue = [&](int its_run, int place) {
+    const int run = __builtin_amdgcn_readfirstlane(its_run);   // (the same in all lanes, which the compiler does not see)
+    const uint32_t to = __builtin_amdgcn_readfirstlane(own + place * T::kPlace);
+    const bool there = run < run_end;
+    const int first_block = __builtin_amdgcn_readfirstlane(min(run * kRunBlocks, p.row_scales - kRunBlocks)), old = run * kRunBlocks - first_block, most = p.groups - first_block;
+    const uint32_t at_w = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(first_block) * 16u), at_x = __builtin_amdgcn_readfirstlane(at_w * (A8 ? 2u : 1u));
+    const auto ending = [&](const u32x4& desc, uint32_t end) {
+      u32x4 words = {desc[0], desc[1], there ? end : 0u, desc[3]};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) wv[slot][h] = __builtin_amdgcn_raw_buffer_load_b128(desc_w, kw + chunk_w < row_w ? from_w[h] : kNowhere, kw, 0);
-#pragma unroll
-    for (int c = 0; c < X; ++c) xv[slot][c] = __builtin_amdgcn_raw_buffer_load_b128(desc_x, kx + chunk_x[c] < row_x ? from_x + chunk_x[c] : kNowhere, kx, 0);
-    const int word = scale_word_at(2 * g + (quarter >> 1), p.row_scales);
-    sw[slot] = __builtin_amdgcn_raw_buffer_load_b32(desc_sw, from_sw + word, 0, 0);
-    sx[slot] = __builtin_amdgcn_raw_buffer_load_b32(desc_sx, from_sx + word, 0, 0);
-  };
-  f32x4 acc[1] = {f32x4{0.f, 0.f, 0.f, 0.f}};
-  static_for<DEPTH>([&](auto u) {
-    if (begin + decltype(u)::value < end) load(u, begin + decltype(u)::value);
-  });
-  for (int g0 = begin; g0 < end; g0 += DEPTH) {
-    static_for<DEPTH>([&](auto u) {
-      constexpr int slot = decltype(u)::value;
-      const int g = g0 + slot;
-      if (g < end) {
-        const uint32_t shift = min(16u * (quarter & 1) + scale_shift(2 * g + (quarter >> 1), p.row_scales), 31u);
-        const uint32_t by_w = sw[slot] >> shift, by_x = sx[slot] >> shift;
-        exchange_lanes<kNextLane>(wv[slot][0], wv[slot][1], lane & 1);
-        i32x8 x[2];
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if constexpr (A8) x[h] = fragment_of(xv[slot][2 * h], xv[slot][2 * h + 1]);
-          else x[h] = narrow_fragment(xv[slot][h]);
-        }
-        acc[0] = mfma_mx<A8, 0>(narrow_fragment(wv[slot][0]), x[0], acc[0], by_w, by_x);
-        acc[0] = mfma_mx<A8, 1>(narrow_fragment(wv[slot][1]), x[1], acc[0], by_w, by_x);
-        if (g + DEPTH < end) load(u, g + DEPTH);
-      }
+      for (int i = 0; i < 4; ++i) words[i] = __builtin_amdgcn_readfirstlane(words[i]);
+      return words;
+    };
+    const u32x4 of_w = ending(desc_w, end_w), of_x = ending(desc_x, end_x), of_sw = ending(desc_sw, end_sw), of_sx = ending(desc_sx, end_sx);
+    const uint32_t at_s = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(first_block));
+    load_16_bytes_into_lds(of_sw, to, T::kScales, from_sw, at_s);
+    load_16_bytes_into_lds(of_sx, to, T::kScales + 1024, from_sx, at_s);
+    static_for<T::kLoadsW>([&](auto i_tag) {
+      constexpr int i = decltype(i_tag)::value;
+      const int row = 4 * i + (lane >> 4), chunk = (lane & 15) ^ ((row + 4) & 15);
+      load_16_bytes_into_lds(of_w, to, i * 1024, chunk >= old && chunk < most ? static_cast<uint32_t>(row * p.ldb) + chunk * 16 : kNowhere, at_w);
     });
-  }
-  settle();
+    static_for<T::kLoadsX>([&](auto i_tag) {
+      constexpr int i = decltype(i_tag)::value;
+      const int row = A8 ? 2 * i + (lane >> 5) : 4 * i + (lane >> 4), chunk = (lane & (T::kChunksX - 1)) ^ ((row + 4) & 15), block = A8 ? chunk >> 1 : chunk;
+      load_16_bytes_into_lds(of_x, to, T::kBytesW + i * 1024, block >= old && block < most ? static_cast<uint32_t>(row * p.lda) + chunk * 16 : kNowhere, at_x);
+    });
+  };
 
-  sums[wave][lane] = acc[0];
+  constexpr int kSteps = R == 16 ? 4 : 8, kWords = kSteps / 4;
+  const int col = lane & (R - 1), part = lane / R;   // a lane's row, and its place in the instruction
+  const int row_w = R == 16 ? col : 16 * ((col >> 2) & 1) + 4 * (col >> 3) + (col & 3);
+  typedef typename std::conditional<R == 16, f32x4, f32x16>::type Sums;
+  Sums acc[T::kColumns];
+#pragma unroll
+  for (int j = 0; j < T::kColumns; ++j)
+#pragma unroll
+    for (int e = 0; e < (R == 16 ? 4 : 16); ++e) acc[j][e] = 0.f;
+
+  const int mine = run_begin + wave;
+  static_for<DEPTH>([&](auto d) { issue(mine + decltype(d)::value * WAVES, decltype(d)::value); });
+  int place = 0;
+#pragma unroll 1
+  for (int run = mine; run < run_end; run += WAVES) {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 1) * T::kLoads) : "memory");
+    const uint32_t at = own + place * T::kPlace;
+    i32x8 w[kSteps];
+    uint32_t sw[kWords];
+#pragma unroll
+    for (int u = 0; u < kWords; ++u) sw[u] = read_lds_word(at + T::kScales + row_w * 16 + part * (4 * kWords), 4 * u);
+    static_for<kSteps>([&](auto t_tag) {
+      constexpr int t = decltype(t_tag)::value;
+      w[t] = narrow_fragment(read_lds(at + row_w * 256 + (((part * kSteps + t) ^ ((row_w + 4) & 15)) << 4), 0));
+    });
+    static_for<T::kColumns>([&](auto j_tag) {
+      constexpr int j = decltype(j_tag)::value;
+      const int row = min(j * R + col, XR - 1);   // (columns past the last row are not written)
+      uint32_t sx[kWords];
+#pragma unroll
+      for (int u = 0; u < kWords; ++u) sx[u] = read_lds_word(at + T::kScales + 1024 + row * 16 + part * (4 * kWords), 4 * u);
+      static_for<kSteps>([&](auto t_tag) {
+        constexpr int t = decltype(t_tag)::value;
+        const uint32_t x_at = at + T::kBytesW + row * T::kRowX;
+        const int key = (row + 4) & 15;
+        i32x8 x;
+        if constexpr (A8) {   // R = 16: half part % 2 of places part / 2 and 2 + part / 2; R = 32: half `part` of both places
+          const int chunk = R == 16 ? 8 * (part >> 1) + 2 * t + (part & 1) : 2 * t + part;
+          x = fragment_of(read_lds(x_at + ((chunk ^ key) << 4), 0), read_lds(x_at + ((chunk ^ key) << 4), 256));
+        } else {
+          x = narrow_fragment(read_lds(x_at + (((part * kSteps + t) ^ key) << 4), 0));
+        }
+        if constexpr (R == 16) acc[j] = mfma_mx<A8, (t & 3)>(w[t], x, acc[j], sw[0], sx[0]);
+        else acc[j] = mfma_mx_32<A8, (t & 3)>(w[t], x, acc[j], sw[t >> 2], sx[t >> 2]);
+      });
+    });
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (what has been read may be overwritten)
+    issue(run + DEPTH * WAVES, place);
+    place = place + 1 == DEPTH ? 0 : place + 1;
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  settle();
   __syncthreads();
-  if (wave == 0) {
+
+  // The wavefronts' sums meet, [m][n] each: four neighbouring n a thread.
+  static_for<T::kColumns>([&](auto j_tag) {
+    constexpr int j = decltype(j_tag)::value;
+    const uint32_t to = lds0 + wave * T::kSum + (j * R + col) * (R * 4) + part * (R == 16 ? 16 : 64);
+#pragma unroll
+    for (int e = 0; e < (R == 16 ? 4 : 16); e += 4)
+      write_lds(to + e * 4, u32x4{__float_as_uint(acc[j][e]), __float_as_uint(acc[j][e + 1]), __float_as_uint(acc[j][e + 2]), __float_as_uint(acc[j][e + 3])});
+  });
+  __syncthreads();
+  constexpr int kQuads = T::kColumns * R * R / 4;
+#pragma unroll
+  for (int q0 = 0; q0 < kQuads; q0 += 64 * WAVES) {
+    const int q = q0 + tid;
+    if (q >= kQuads) break;
     float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int u = 0; u < WAVES; ++u)
+    for (int u = 0; u < WAVES; ++u) {
+      const u32x4 one = read_lds(lds0 + u * T::kSum + q * 16, 0);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] += sums[u][lane][r];
-    const int64_t n = n0 + quarter * 4;
-    if (col < p.m && n < p.n) store_results<4>(p.c, batch * p.c_bs + col * p.c_rs + n * p.c_cs, p.c_cs, p.out_kind, n, p.n, v);
+      for (int e = 0; e < 4; ++e) v[e] += __uint_as_float(one[e]);
+    }
+    const int64_t m = m0 + q / (R / 4), n = n0 + q % (R / 4) * 4;
+    if (q / (R / 4) > last_m || n >= p.n) continue;
+    if (p.splits == 1) store_results<4>(p.c, batch * p.c_bs + m * p.c_rs + n * p.c_cs, p.c_cs, p.out_kind, n, p.n, v);
+    else store_results<4>(p.partial, ((static_cast<int64_t>(blockIdx.z) * p.batch + batch) * p.m + m) * p.n + n, 1, FP8_REAL_F32, n, p.n, v);
   }
 }
 
-template <bool A8>
-hipError_t launch_few_rows(const MxMatmulParams& p, hipStream_t stream) {
-  const dim3 grid(static_cast<uint32_t>((static_cast<int64_t>(p.n) + 15) / 16), static_cast<uint32_t>(p.batch));
-  hipLaunchKernelGGL((mx_few_rows_kernel<4, A8>), grid, dim3(256), 0, stream, p);
-  return hipGetLastError();
+hipError_t join(const MxMatmulParams& p, hipStream_t stream) {
+  const hipError_t e = hipGetLastError();
+  if (p.splits == 1 || e != hipSuccess) return e;
+  return launch_join_shares({p.partial, p.c, p.c_rs, p.c_cs, p.c_bs, p.m, p.n, p.batch, p.splits, p.out_kind}, stream);
+}
+
+template <int R, int XR, bool A8, int WAVES, int DEPTH>
+hipError_t launch_slim(const MxMatmulParams& p, hipStream_t stream) {
+  using T = MxSlim<R, XR, A8, WAVES, DEPTH>;
+  constexpr auto kernel = &mx_slim_kernel<R, XR, A8, WAVES, DEPTH>;
+  if constexpr (T::kLds > 65536) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds);
+    if (e != hipSuccess) return e;
+  }
+  const uint32_t tiles_m = static_cast<uint32_t>((p.m + XR - 1) / XR), units = static_cast<uint32_t>((static_cast<int64_t>(p.n) + R - 1) / R) * tiles_m;
+  hipLaunchKernelGGL(kernel, dim3(units, static_cast<uint32_t>(p.batch), static_cast<uint32_t>(p.splits)), dim3(64 * WAVES), T::kLds, stream, p, tiles_m, units);
+  return join(p, stream);
 }
 
 template <int WN, int WM, int WK, int NT, int MT, bool A8, int STAGES, int WAVES_A_SIMD, bool GOES_ON, int OUT>
@@ -560,26 +642,77 @@ hipError_t launch_tile(const MxMatmulParams& p, hipStream_t stream) {
   if (p.splits == 1 && p.out_kind == FP8_REAL_BF16) return launch_tile_as<WN, WM, WK, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, FP8_REAL_BF16>(p, stream);
   if (p.splits == 1 && p.out_kind == FP8_REAL_F16) return launch_tile_as<WN, WM, WK, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, FP8_REAL_F16>(p, stream);
   const hipError_t e = launch_tile_as<WN, WM, WK, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, FP8_REAL_F32>(p, stream);
-  if (p.splits == 1 || e != hipSuccess) return e;
-  return launch_join_shares({p.partial, p.c, p.c_rs, p.c_cs, p.c_bs, p.m, p.n, p.batch, p.splits, p.out_kind}, stream);
+  return e != hipSuccess ? e : join(p, stream);
 }
 
 }  // namespace
 
+// Which kernel, and how many shares of k.  A kernel of `units` workgroups (shares included) goes in rounds over 256 compute units with `slots` workgroups
+// each, which their LDS allows; a round of c on a compute unit takes start + runs (alone + more (c - 1)) us, where `runs` are the runs of 512 k that a
+// wavefront has to do, and no product is faster than its bytes.  Shares cost the joining launch and its bytes.  The constants were fitted to 3800 timings
+// of all kernels and 1, 2 and 4 shares at 420 products of random sizes (M 1 .. 4096, N 256 .. 28000, K 512 .. 16384) on weights that no cache
+// held.  What the rule takes is 0.9 % slower than the fastest of them on average and 1.19 times at worst; without shares the best choice would lose 0.9 %
+// (1.42 at worst), without MX_ROWS_32 2.4 %, MX_TILE_256 1.7 %, MX_TILE_128 1.0 %, MX_ROWS_16_DEEP 0.9 %, MX_TILE_128_DEEP 0.7 %, MX_ROWS_4_DEEP 0.5 %,
+// MX_ROWS_4_TWO 0.4 %, MX_ROWS_4 0.2 % (1.14 at worst), while 32 x 64 results a workgroup brought 0.2 % and are left out.
+// Fewer rows than MX_ROWS_32's take no shares: their wavefronts share k already.
 MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int64_t batch, bool a_wide) {
-  (void)k;
-  if (m <= 16) return {MX_FEW_ROWS, 1, 16, 16, 4};
-  const int64_t big = ((m + (a_wide ? 127 : 255)) / (a_wide ? 128 : 256)) * ((n + 255) / 256) * batch, middle = ((m + 127) / 128) * ((n + 127) / 128) * batch;
-  if (big >= 192) return {MX_TILE_256, 1, a_wide ? 128 : 256, 256, kRunBlocks};
-  if (middle >= 128) return {a_wide ? MX_TILE_128_DEEP : MX_TILE_128, 1, 128, 128, kRunBlocks};
-  return {MX_TILE_64, 1, 64, 64, kRunBlocks};
+  struct Cost {
+    int rows_a, rows_b, wavefronts, slots;   // as powers of two; wavefronts that share k by whole runs
+    float once, start, alone, more;          // us
+  };
+  constexpr Cost kCosts[2][MX_KINDS] = {
+      {{2, 4, 1, 3, 2.56f, 0.19f, 0.52f, 0.32f},    // MX_ROWS_4_TWO
+       {2, 4, 2, 2, 2.82f, 0.f, 0.75f, 0.62f},      // MX_ROWS_4
+       {2, 4, 2, 1, 1.21f, 1.96f, 0.42f, 0.83f},    // MX_ROWS_4_DEEP
+       {4, 4, 2, 2, 1.84f, 0.83f, 0.85f, 0.71f},   // MX_ROWS_16
+       {4, 4, 2, 1, 1.50f, 1.80f, 0.48f, 0.97f},   // MX_ROWS_16_DEEP
+       {5, 5, 2, 1, 1.26f, 1.55f, 1.59f, 1.56f},   // MX_ROWS_32
+       {6, 6, 0, 1, 3.12f, 0.83f, 0.80f, 0.86f},   // MX_TILE_64
+       {7, 7, 0, 1, 2.94f, 0.62f, 2.17f, 1.19f}, // MX_TILE_128
+       {7, 7, 0, 0, 1.71f, 4.28f, 1.75f, 0.f},   // MX_TILE_128_DEEP
+       {8, 8, 0, 0, 3.28f, 9.71f, 3.44f, 0.f}},  // MX_TILE_256
+      {{2, 4, 1, 3, 0.f, 2.81f, 0.56f, 0.38f},
+       {2, 4, 2, 2, 1.95f, 0.95f, 0.75f, 0.75f},
+       {2, 4, 2, 1, 1.43f, 1.89f, 0.44f, 0.98f},
+       {4, 4, 2, 1, 1.34f, 1.50f, 0.95f, 0.90f},
+       {4, 4, 3, 0, 0.81f, 1.83f, 1.59f, 0.f},
+       {5, 5, 2, 0, 0.86f, 2.16f, 1.83f, 0.f},
+       {6, 6, 0, 1, 2.11f, 2.16f, 0.83f, 0.99f},
+       {7, 7, 0, -1, 0.f, 0.f, 0.f, 0.f},         // (both operands' tiles in half the LDS: e2m1 only)
+       {7, 7, 0, 0, 1.80f, 5.07f, 1.99f, 0.f},
+       {7, 8, 0, 0, 4.91f, 3.74f, 3.06f, 0.f}}};
+  const int64_t runs = (k + 511) / 512;
+  const auto shared = [](int64_t x, int by) { return (x + (int64_t{1} << by) - 1) >> by; };
+  const float bytes = (static_cast<float>(n) * k * (17 / 32.f) + static_cast<float>(m) * k * (a_wide ? 33 / 32.f : 17 / 32.f) + 2.f * m * n) * batch;
+  MxPlan best{};
+  float least = INFINITY;
+  for (int kind = 0; kind < MX_KINDS; ++kind) {
+    const Cost& cost = kCosts[a_wide][kind];
+    if (cost.slots < 0 || (kind < MX_TILE_64 && m > 1 << (2 * cost.rows_a - 2))) continue;   // (kernels of few rows up to M = 4, 64 and 256, as they were timed)
+    const int64_t tiles = shared(m, cost.rows_a) * shared(n, cost.rows_b);
+    if (tiles > (1 << 22) && kind != MX_TILE_256) continue;   // (a grid holds fewer than 2^32 threads; that kernel's goes from tile to tile)
+    for (int split = 0; split == 0 || (split <= 2 && kind >= MX_ROWS_32 && runs >= (2 << split)); ++split) {
+      const int64_t each = shared(shared(runs, split), cost.wavefronts), depth = shared((tiles * batch) << split, 8), rounds = depth >> cost.slots;
+      const int slots = 1 << cost.slots, rest = static_cast<int>(depth - (rounds << cost.slots));
+      float us = cost.once + rounds * (cost.start + (cost.alone + cost.more * (slots - 1)) * each);
+      if (rest > 0) us += cost.start + (cost.alone + cost.more * (rest - 1)) * each;
+      us = std::max(us, 2.5f + bytes / 5.5e6f);
+      if (split > 0) us += 3.2f + 1.4e-6f * (static_cast<float>(m) * n * batch) * (1 << split);
+      if (us < least) least = us, best = {kind, 1 << split, 1 << cost.rows_a, 1 << cost.rows_b, kRunBlocks};
+    }
+  }
+  return best;
 }
 
 hipError_t launch_mx_matmul(const MxMatmulParams& p, int kind, hipStream_t stream) {
   switch (kind) {
-    case MX_FEW_ROWS: return p.a_wide ? launch_few_rows<true>(p, stream) : launch_few_rows<false>(p, stream);
+    case MX_ROWS_4_TWO: return p.a_wide ? launch_slim<16, 4, true, 2, 1>(p, stream) : launch_slim<16, 4, false, 2, 1>(p, stream);
+    case MX_ROWS_4: return p.a_wide ? launch_slim<16, 4, true, 4, 1>(p, stream) : launch_slim<16, 4, false, 4, 1>(p, stream);
+    case MX_ROWS_4_DEEP: return p.a_wide ? launch_slim<16, 4, true, 4, 2>(p, stream) : launch_slim<16, 4, false, 4, 2>(p, stream);
+    case MX_ROWS_16: return p.a_wide ? launch_slim<16, 16, true, 4, 1>(p, stream) : launch_slim<16, 16, false, 4, 1>(p, stream);
+    case MX_ROWS_16_DEEP: return p.a_wide ? launch_slim<16, 16, true, 8, 1>(p, stream) : launch_slim<16, 16, false, 4, 2>(p, stream);
+    case MX_ROWS_32: return p.a_wide ? launch_slim<32, 32, true, 4, 1>(p, stream) : launch_slim<32, 32, false, 4, 1>(p, stream);
     case MX_TILE_64: return p.a_wide ? launch_tile<1, 2, 2, 2, 1, true, 3, 2, false>(p, stream) : launch_tile<1, 2, 2, 2, 1, false, 4, 2, false>(p, stream);
-    case MX_TILE_64_DEEP: return p.a_wide ? launch_tile<1, 2, 2, 2, 1, true, 5, 2, false>(p, stream) : launch_tile<1, 2, 2, 2, 1, false, 6, 2, false>(p, stream);
     case MX_TILE_128: return p.a_wide ? hipErrorInvalidValue : launch_tile<2, 2, 1, 2, 2, false, 2, 2, false>(p, stream);
     case MX_TILE_128_DEEP: return p.a_wide ? launch_tile<2, 2, 2, 2, 2, true, 3, 2, false>(p, stream) : launch_tile<2, 2, 2, 2, 2, false, 4, 2, false>(p, stream);
     case MX_TILE_256: return p.a_wide ? launch_tile<2, 2, 1, 4, 2, true, 2, 1, true>(p, stream) : launch_tile<2, 2, 1, 4, 4, false, 2, 1, true>(p, stream);
