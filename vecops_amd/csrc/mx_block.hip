@@ -647,57 +647,58 @@ hipError_t launch_tile(const MxMatmulParams& p, hipStream_t stream) {
 
 }  // namespace
 
-// Which kernel, and how many shares of k.  A kernel of `units` workgroups (shares included) goes in rounds over 256 compute units with `slots` workgroups
-// each, which their LDS allows; a round of c on a compute unit takes start + runs (alone + more (c - 1)) us, where `runs` are the runs of 512 k that a
-// wavefront has to do, and no product is faster than its bytes.  Shares cost the joining launch and its bytes.  The constants were fitted to 3800 timings
-// of all kernels and 1, 2 and 4 shares at 420 products of random sizes (M 1 .. 4096, N 256 .. 28000, K 512 .. 16384) on weights that no cache
-// held.  What the rule takes is 0.9 % slower than the fastest of them on average and 1.19 times at worst; without shares the best choice would lose 0.9 %
-// (1.42 at worst), without MX_ROWS_32 2.4 %, MX_TILE_256 1.7 %, MX_TILE_128 1.0 %, MX_ROWS_16_DEEP 0.9 %, MX_TILE_128_DEEP 0.7 %, MX_ROWS_4_DEEP 0.5 %,
-// MX_ROWS_4_TWO 0.4 %, MX_ROWS_4 0.2 % (1.14 at worst), while 32 x 64 results a workgroup brought 0.2 % and are left out.
-// Fewer rows than MX_ROWS_32's take no shares: their wavefronts share k already.
+// Which kernel, and how many shares of k: the least of fitted times.  A kernel's workgroups (those of all shares) go in rounds over 256 compute units
+// with `slots` of them each, as their LDS allows; a round of c on a compute unit takes start + runs (alone + more (c - 1)) us, where `runs` are the runs of
+// 512 k that a wavefront has to do, and the bytes at 5.5 TB/s and 2 us are joined to that as a fourth power (the longer of the two counts, the other
+// decides between equals).  Shares cost the joining launch and its bytes.  The constants were fitted to 3700 timings of every kernel and of 1, 2 and 4
+// shares at 520 products of random sizes (M 1 .. 4096, N 256 .. 28000, K 512 .. 16384) on weights that no cache held.  What the rule takes is 0.8 %
+// slower than the fastest of them on average and 1.18 times at worst.  The best choice without one of them would be slower by 2.4 % (MX_ROWS_4),
+// 1.7 % (MX_TILE_256), 1.3 % (MX_TILE_128), 1.1 % (MX_ROWS_32), 0.9 % (MX_ROWS_4_DEEP), 0.6 % (MX_ROWS_16_DEEP, MX_TILE_128_DEEP) and 0.4 % (shares, 1.38 times at
+// worst; four shares rather than two, or of few rows, 0.04 %); 32 x 64 results a workgroup and 4 x 16 by four wavefronts brought 0.2 % each and are left
+// out.  Up to four rows only kernels of four are weighed: on a tie of latencies the fit's errors would decide.
 MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int64_t batch, bool a_wide) {
   struct Cost {
     int rows_a, rows_b, wavefronts, slots;   // as powers of two; wavefronts that share k by whole runs
     float once, start, alone, more;          // us
   };
   constexpr Cost kCosts[2][MX_KINDS] = {
-      {{2, 4, 1, 3, 2.56f, 0.19f, 0.52f, 0.32f},    // MX_ROWS_4_TWO
-       {2, 4, 2, 2, 2.82f, 0.f, 0.75f, 0.62f},      // MX_ROWS_4
-       {2, 4, 2, 1, 1.21f, 1.96f, 0.42f, 0.83f},    // MX_ROWS_4_DEEP
-       {4, 4, 2, 2, 1.84f, 0.83f, 0.85f, 0.71f},   // MX_ROWS_16
-       {4, 4, 2, 1, 1.50f, 1.80f, 0.48f, 0.97f},   // MX_ROWS_16_DEEP
-       {5, 5, 2, 1, 1.26f, 1.55f, 1.59f, 1.56f},   // MX_ROWS_32
-       {6, 6, 0, 1, 3.12f, 0.83f, 0.80f, 0.86f},   // MX_TILE_64
-       {7, 7, 0, 1, 2.94f, 0.62f, 2.17f, 1.19f}, // MX_TILE_128
-       {7, 7, 0, 0, 1.71f, 4.28f, 1.75f, 0.f},   // MX_TILE_128_DEEP
-       {8, 8, 0, 0, 3.28f, 9.71f, 3.44f, 0.f}},  // MX_TILE_256
-      {{2, 4, 1, 3, 0.f, 2.81f, 0.56f, 0.38f},
-       {2, 4, 2, 2, 1.95f, 0.95f, 0.75f, 0.75f},
-       {2, 4, 2, 1, 1.43f, 1.89f, 0.44f, 0.98f},
-       {4, 4, 2, 1, 1.34f, 1.50f, 0.95f, 0.90f},
-       {4, 4, 3, 0, 0.81f, 1.83f, 1.59f, 0.f},
-       {5, 5, 2, 0, 0.86f, 2.16f, 1.83f, 0.f},
-       {6, 6, 0, 1, 2.11f, 2.16f, 0.83f, 0.99f},
-       {7, 7, 0, -1, 0.f, 0.f, 0.f, 0.f},         // (both operands' tiles in half the LDS: e2m1 only)
-       {7, 7, 0, 0, 1.80f, 5.07f, 1.99f, 0.f},
-       {7, 8, 0, 0, 4.91f, 3.74f, 3.06f, 0.f}}};
+      {{2, 4, 1, 3, 2.24f, 0.33f, 0.52f, 0.24f},    // MX_ROWS_4
+       {2, 4, 2, 1, 1.22f, 1.76f, 0.38f, 0.58f},    // MX_ROWS_4_DEEP
+       {4, 4, 2, 2, 1.84f, 0.69f, 0.79f, 0.57f},    // MX_ROWS_16
+       {4, 4, 2, 1, 1.36f, 1.70f, 0.49f, 0.76f},    // MX_ROWS_16_DEEP
+       {5, 5, 2, 1, 1.56f, 1.17f, 1.50f, 1.38f},    // MX_ROWS_32
+       {6, 6, 0, 1, 2.35f, 1.96f, 0.66f, 0.86f},    // MX_TILE_64
+       {7, 7, 0, 1, 1.78f, 2.91f, 1.90f, 1.12f},    // MX_TILE_128
+       {7, 7, 0, 0, 1.70f, 4.94f, 1.57f, 0.f},      // MX_TILE_128_DEEP
+       {8, 8, 0, 0, 2.91f, 10.85f, 3.17f, 0.f}},    // MX_TILE_256
+      {{2, 4, 1, 3, 2.13f, 0.42f, 0.56f, 0.25f},
+       {2, 4, 2, 1, 0.97f, 2.12f, 0.42f, 0.55f},
+       {4, 4, 2, 1, 1.24f, 1.35f, 0.97f, 0.66f},
+       {4, 4, 3, 0, 1.01f, 1.29f, 1.63f, 0.f},
+       {5, 5, 2, 0, 0.86f, 1.92f, 1.86f, 0.f},
+       {6, 6, 0, 1, 1.79f, 2.68f, 0.82f, 0.88f},
+       {7, 7, 0, -1, 0.f, 0.f, 0.f, 0.f},           // (two workgroups of such tiles a compute unit: of e2m1 only)
+       {7, 7, 0, 0, 1.79f, 5.14f, 1.96f, 0.f},
+       {7, 8, 0, 0, 4.90f, 3.96f, 3.05f, 0.f}}};
   const int64_t runs = (k + 511) / 512;
   const auto shared = [](int64_t x, int by) { return (x + (int64_t{1} << by) - 1) >> by; };
   const float bytes = (static_cast<float>(n) * k * (17 / 32.f) + static_cast<float>(m) * k * (a_wide ? 33 / 32.f : 17 / 32.f) + 2.f * m * n) * batch;
+  const float moved = 2.f + bytes / 5.5e6f;
   MxPlan best{};
   float least = INFINITY;
   for (int kind = 0; kind < MX_KINDS; ++kind) {
     const Cost& cost = kCosts[a_wide][kind];
-    if (cost.slots < 0 || (kind < MX_TILE_64 && m > 1 << (2 * cost.rows_a - 2))) continue;   // (kernels of few rows up to M = 4, 64 and 256, as they were timed)
+    if (cost.slots < 0 || (m <= 4 && kind >= MX_ROWS_16) || (kind < MX_TILE_64 && m > 1 << (2 * cost.rows_a))) continue;   // (few rows up to M = 16, 256 and 1024, as they were timed)
     const int64_t tiles = shared(m, cost.rows_a) * shared(n, cost.rows_b);
-    if (tiles > (1 << 22) && kind != MX_TILE_256) continue;   // (a grid holds fewer than 2^32 threads; that kernel's goes from tile to tile)
-    for (int split = 0; split == 0 || (split <= 2 && kind >= MX_ROWS_32 && runs >= (2 << split)); ++split) {
+    // (a grid holds fewer than 2^32 threads, of which a workgroup has up to 512; those of MX_TILE_256 go from tile to tile)
+    if (tiles > (kind == MX_ROWS_16_DEEP || kind == MX_TILE_128_DEEP ? 1 << 22 : 1 << 23) && kind != MX_TILE_256) continue;
+    for (int split = 0; split == 0 || (split == 1 && kind >= MX_TILE_64 && runs >= 4); ++split) {
       const int64_t each = shared(shared(runs, split), cost.wavefronts), depth = shared((tiles * batch) << split, 8), rounds = depth >> cost.slots;
       const int slots = 1 << cost.slots, rest = static_cast<int>(depth - (rounds << cost.slots));
       float us = cost.once + rounds * (cost.start + (cost.alone + cost.more * (slots - 1)) * each);
       if (rest > 0) us += cost.start + (cost.alone + cost.more * (rest - 1)) * each;
-      us = std::max(us, 2.5f + bytes / 5.5e6f);
-      if (split > 0) us += 3.2f + 1.4e-6f * (static_cast<float>(m) * n * batch) * (1 << split);
+      us = std::sqrt(std::sqrt(us * us * us * us + moved * moved * moved * moved));
+      if (split > 0) us += 3.2f + 2.8e-6f * (static_cast<float>(m) * n * batch);
       if (us < least) least = us, best = {kind, 1 << split, 1 << cost.rows_a, 1 << cost.rows_b, kRunBlocks};
     }
   }
@@ -706,8 +707,7 @@ MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int64_t batch, bool a_wide) {
 
 hipError_t launch_mx_matmul(const MxMatmulParams& p, int kind, hipStream_t stream) {
   switch (kind) {
-    case MX_ROWS_4_TWO: return p.a_wide ? launch_slim<16, 4, true, 2, 1>(p, stream) : launch_slim<16, 4, false, 2, 1>(p, stream);
-    case MX_ROWS_4: return p.a_wide ? launch_slim<16, 4, true, 4, 1>(p, stream) : launch_slim<16, 4, false, 4, 1>(p, stream);
+    case MX_ROWS_4: return p.a_wide ? launch_slim<16, 4, true, 2, 1>(p, stream) : launch_slim<16, 4, false, 2, 1>(p, stream);
     case MX_ROWS_4_DEEP: return p.a_wide ? launch_slim<16, 4, true, 4, 2>(p, stream) : launch_slim<16, 4, false, 4, 2>(p, stream);
     case MX_ROWS_16: return p.a_wide ? launch_slim<16, 16, true, 4, 1>(p, stream) : launch_slim<16, 16, false, 4, 1>(p, stream);
     case MX_ROWS_16_DEEP: return p.a_wide ? launch_slim<16, 16, true, 8, 1>(p, stream) : launch_slim<16, 16, false, 4, 2>(p, stream);
