@@ -238,14 +238,15 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const MxCopyParams p
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Rows.  T threads a row (64: four rows a workgroup, no barrier; else a workgroup a row), eight elements a thread a piece, kHeld
-// pieces of a thread in registers: a row of up to 32 T elements is read once.  A longer one is read again behind each sum or
+// Rows.  T threads a row (64: four rows a workgroup, no barrier; else a workgroup a row), eight elements a thread a piece, HELD
+// pieces of a thread in registers: a row of up to 8 HELD T elements is read once.  A longer one is read again behind each sum or
 // maximum over it, by the threads that read (and wrote) the same places before.  Bound by HBM, for a few rows by the launch and one
-// row's way through memory and barriers.
+// row's way through memory and barriers: rows that a piece a thread holds have kernels of their own, a quarter as much code to fetch, and weights
+// under way beside the row (FIGURES).
 // ---------------------------------------------------------------------------------------------------------------------
 
 enum : int { SOURCE_NORM = 0, SOURCE_GATE = 1 };
-constexpr int kHeld = 4;
+constexpr int kHeld = 4;   // of rows that one piece a thread does not hold
 
 // g / (1 + e^-g).  The exponent's product with log2 e is off by 1.25 * 2^-24 of itself, which is as much of e^-g as |g| times that; v_exp_f32,
 // the sum, v_rcp_f32 and the product add a unit of the last place each.  (Where e^-g overflows the result is -0, for -infinity NaN.)
@@ -258,46 +259,59 @@ __device__ __forceinline__ float as_held(float v) {   // rounded to the type
   else return v;
 }
 
-template <int SOURCE, int KIND, int FORMAT>
+template <int SOURCE, int KIND, int FORMAT, int HELD>
 __global__ __launch_bounds__(1024) void row_quantize_kernel(const RowQuantizeParams p, int threads, uint32_t lines) {
   __shared__ float sums[2][16];
   __shared__ uint32_t mosts[2][16];
   const int waves = threads >> 6, own = threads == 64 ? threadIdx.x & 63 : threadIdx.x, wave = threadIdx.x >> 6;
   const uint32_t rows_here = threads == 64 ? blockDim.x >> 6 : 1u;
-  const int span = threads * (8 * kHeld);
-  const bool held = p.k <= span;   // (uniform)
+  const int span = threads * (8 * HELD);
+  const bool held = HELD == 1 || p.k <= span;   // (uniform)
+  const int spans_end = HELD == 1 ? 1 : p.k;
   int turn = 0;
 
   for (uint32_t line = blockIdx.x * rows_here + (threads == 64 ? static_cast<uint32_t>(wave) : 0u); line < lines; line += gridDim.x * rows_here) {
     const uint32_t batch = line / static_cast<uint32_t>(p.rows), row = line - batch * p.rows;
     const int64_t x_at = batch * p.x_bs + row * p.x_rs, summed_at = batch * p.summed_bs + row * p.summed_rs;
     const int64_t residual_at = batch * p.residual_bs + row * p.residual_rs;
-    float v[kHeld][8];
+    float v[HELD][8];
+    constexpr bool kWeightsToo = SOURCE == SOURCE_NORM && HELD == 1;   // (of more pieces they would take the registers of other rows)
+    RawEight<KIND> weight;
+    RawEight<FP8_REAL_F32> wide_weight;
+    const bool same_kind = p.weight_kind == KIND;
 
     // the pieces of a span from k0 on, all their loads under way at once; `again`: the residual has been added
     auto load = [&](int k0, bool again) {
       constexpr int kSources = 2;
-      RawEight<KIND> raw[kHeld][kSources];
+      RawEight<KIND> raw[HELD][kSources];
       const bool adds = SOURCE == SOURCE_NORM && p.residual != nullptr && !again, two = SOURCE == SOURCE_GATE || adds;
       const bool sum = SOURCE == SOURCE_NORM && p.residual != nullptr && again;
       const void* const first = sum ? p.summed : p.x;
       const void* const second = SOURCE == SOURCE_GATE ? p.x : p.residual;
       const int64_t first_at = sum ? summed_at : x_at, second_at = SOURCE == SOURCE_GATE ? x_at + p.k : residual_at;
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i) {
+      for (int i = 0; i < HELD; ++i) {
         const int k = k0 + (i * threads + own) * 8;
         if (p.k - k < 8) continue;
         raw[i][0].load(first, first_at + k);
         if (two) raw[i][1].load(second, second_at + k);
+        if constexpr (kWeightsToo) {
+          if (same_kind) weight.load(p.weight, k);
+          else wide_weight.load(p.weight, k);
+        }
       }
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i) {
+      for (int i = 0; i < HELD; ++i) {
         const int k = k0 + (i * threads + own) * 8, left = p.k - k;
         if (left < 8) {
           raw[i][0].load_part(first, first_at + k, left);
           if (two) raw[i][1].load_part(second, second_at + k, left);
+          if constexpr (kWeightsToo) {
+            if (same_kind) weight.load_part(p.weight, k, left);
+            else wide_weight.load_part(p.weight, k, left);
+          }
         }
-        if (k0 + i * threads * 8 >= p.k) {   // (uniform)
+        if (HELD > 1 && k0 + i * threads * 8 >= p.k) {   // (uniform)
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[i][e] = 0.0f;
           continue;
@@ -322,11 +336,14 @@ __global__ __launch_bounds__(1024) void row_quantize_kernel(const RowQuantizePar
     auto finish = [&](int k0) {
       if constexpr (SOURCE == SOURCE_NORM) {
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) {
+        for (int i = 0; i < HELD; ++i) {
           const int k = k0 + (i * threads + own) * 8, left = p.k - k;
-          if (k0 + i * threads * 8 >= p.k) continue;
+          if (HELD > 1 && k0 + i * threads * 8 >= p.k) continue;
           float w[8];
-          if (p.weight_kind == KIND) load_row_eight<KIND>(p.weight, k, 1, left, left >= 8, w);
+          if constexpr (kWeightsToo) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = same_kind ? weight[e] : wide_weight[e];
+          } else if (same_kind) load_row_eight<KIND>(p.weight, k, 1, left, left >= 8, w);
           else load_row_eight<FP8_REAL_F32>(p.weight, k, 1, left, left >= 8, w);
 #pragma unroll
           for (int e = 0; e < 8; ++e) v[i][e] = v[i][e] * norm * w[e];   // (what is not there: 0, but for a norm that is not finite)
@@ -340,10 +357,10 @@ __global__ __launch_bounds__(1024) void row_quantize_kernel(const RowQuantizePar
 
     if constexpr (SOURCE == SOURCE_NORM) {
       float sum = 0.0f;
-      for (int k0 = 0; k0 < p.k; k0 += span) {
+      for (int k0 = 0; k0 < spans_end; k0 += span) {
         load(k0, false);
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i)
+        for (int i = 0; i < HELD; ++i)
 #pragma unroll
           for (int e = 0; e < 8; ++e) sum = fmaf(v[i][e], v[i][e], sum);
       }
@@ -359,11 +376,11 @@ __global__ __launch_bounds__(1024) void row_quantize_kernel(const RowQuantizePar
     float row_scale = 0.0f;
     if constexpr (FORMAT == ROW_INT8) {
       uint32_t most = 0;
-      for (int k0 = 0; k0 < p.k; k0 += span) {
+      for (int k0 = 0; k0 < spans_end; k0 += span) {
         if (SOURCE == SOURCE_GATE || !held) load(k0, true);
         finish(k0);
 #pragma unroll
-        for (int i = 0; i < kHeld; ++i) most = max(most, most_bits(v[i]));
+        for (int i = 0; i < HELD; ++i) most = max(most, most_bits(v[i]));
       }
       most = most_of_64(most);
       if (waves > 1) {
@@ -377,13 +394,13 @@ __global__ __launch_bounds__(1024) void row_quantize_kernel(const RowQuantizePar
     }
     turn ^= 1;   // (a wavefront that is a row ahead writes beside what others still read; two ahead it cannot be)
 
-    for (int k0 = 0; k0 < p.k; k0 += span) {
+    for (int k0 = 0; k0 < spans_end; k0 += span) {
       if ((SOURCE == SOURCE_GATE && FORMAT != ROW_INT8) || !held) load(k0, true);
       if (FORMAT != ROW_INT8 || !held) finish(k0);
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i) {
+      for (int i = 0; i < HELD; ++i) {
         const int k = k0 + (i * threads + own) * 8, left = p.k - k;
-        if (k0 + i * threads * 8 >= p.k) continue;   // (uniform: the moves between lanes below have all of them)
+        if (HELD > 1 && k0 + i * threads * 8 >= p.k) continue;   // (uniform: the moves between lanes below have all of them)
         if constexpr (SOURCE == SOURCE_NORM)
           if (p.out != nullptr && left > 0) store_results<8>(p.out, batch * p.out_bs + row * p.out_rs + k, 1, KIND, k, p.k, v[i]);
         const int64_t q_at = batch * p.q_bs + row * p.q_rs, s_at = batch * p.s_bs + row * p.s_rs;
@@ -419,29 +436,35 @@ __global__ __launch_bounds__(1024) void row_quantize_kernel(const RowQuantizePar
   }
 }
 
-template <int SOURCE, int KIND>
-hipError_t launch_rows_as(const RowQuantizeParams& p, hipStream_t stream) {
+template <int SOURCE, int KIND, int HELD>
+hipError_t launch_rows_held(const RowQuantizeParams& p, int threads, hipStream_t stream) {
   const int64_t lines = static_cast<int64_t>(p.batch) * p.rows;
-  // as few threads as hold a row, but enough wavefronts for the chip and a piece for each thread
-  int threads = 64;
-  while (threads < 1024 && (threads * 8 * kHeld < p.k || (threads * 8 < p.k && lines * threads < 256 * 1024))) threads *= 2;
   const int64_t rows_here = threads == 64 ? 4 : 1, groups = (lines + rows_here - 1) / rows_here;
   const dim3 grid(static_cast<uint32_t>(std::min<int64_t>(groups, 1 << 20))), block(threads == 64 ? 256 : threads);
   const uint32_t n = static_cast<uint32_t>(lines);
   switch (p.format) {
-    case ROW_INT8: hipLaunchKernelGGL((row_quantize_kernel<SOURCE, KIND, ROW_INT8>), grid, block, 0, stream, p, threads, n); break;
-    case ROW_E4M3_128: hipLaunchKernelGGL((row_quantize_kernel<SOURCE, KIND, ROW_E4M3_128>), grid, block, 0, stream, p, threads, n); break;
-    case ROW_MX_E4M3: hipLaunchKernelGGL((row_quantize_kernel<SOURCE, KIND, ROW_MX_E4M3>), grid, block, 0, stream, p, threads, n); break;
-    case ROW_MX_E2M1: hipLaunchKernelGGL((row_quantize_kernel<SOURCE, KIND, ROW_MX_E2M1>), grid, block, 0, stream, p, threads, n); break;
+    case ROW_INT8: hipLaunchKernelGGL((row_quantize_kernel<SOURCE, KIND, ROW_INT8, HELD>), grid, block, 0, stream, p, threads, n); break;
+    case ROW_E4M3_128: hipLaunchKernelGGL((row_quantize_kernel<SOURCE, KIND, ROW_E4M3_128, HELD>), grid, block, 0, stream, p, threads, n); break;
+    case ROW_MX_E4M3: hipLaunchKernelGGL((row_quantize_kernel<SOURCE, KIND, ROW_MX_E4M3, HELD>), grid, block, 0, stream, p, threads, n); break;
+    case ROW_MX_E2M1: hipLaunchKernelGGL((row_quantize_kernel<SOURCE, KIND, ROW_MX_E2M1, HELD>), grid, block, 0, stream, p, threads, n); break;
     default:
       if constexpr (SOURCE == SOURCE_NORM) {
-        hipLaunchKernelGGL((row_quantize_kernel<SOURCE, KIND, ROW_NONE>), grid, block, 0, stream, p, threads, n);
+        hipLaunchKernelGGL((row_quantize_kernel<SOURCE, KIND, ROW_NONE, HELD>), grid, block, 0, stream, p, threads, n);
         break;
       } else {
         return hipErrorInvalidValue;
       }
   }
   return hipGetLastError();
+}
+
+template <int SOURCE, int KIND>
+hipError_t launch_rows_as(const RowQuantizeParams& p, hipStream_t stream) {
+  const int64_t lines = static_cast<int64_t>(p.batch) * p.rows;
+  // as few threads as hold a row, but enough wavefronts for the chip and a piece for each thread
+  int threads = 64;
+  while (threads < 1024 && (threads * 8 * kHeld < p.k || (threads * 8 < p.k && lines * threads < 256 * 1024))) threads *= 2;
+  return threads * 8 >= p.k ? launch_rows_held<SOURCE, KIND, 1>(p, threads, stream) : launch_rows_held<SOURCE, KIND, kHeld>(p, threads, stream);
 }
 
 template <int SOURCE>
