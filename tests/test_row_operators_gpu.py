@@ -176,6 +176,21 @@ def test_gate(device, dtype, form, shape):
 
 
 @pytest.mark.parametrize("form", FORMATS)
+@pytest.mark.parametrize("shape", [(5000, 1030), (2100, 4100), (130, 70002)])
+def test_many_rows(device, form, shape):
+    """So many that a thread takes several pieces of a row, and rows that are read again."""
+    torch.manual_seed(shape[0])
+    k = shape[-1]
+    x = torch.randn(shape[0], 2 * k).bfloat16()
+    q, scales = results(shape[:-1], k, form)
+    capi.silu_mul_quantize(x.to(device), q, scales)
+    check(q, scales, gate64(x), form, gate_slack(x))
+    x, weight = x[:, :k], torch.randn(k)
+    capi.rms_norm(x.to(device), weight.to(device), q=q, scales=scales, eps=1e-5)
+    check(q, scales, norm64(x, None, weight, 1e-5)[1], form, norm_slack(k))
+
+
+@pytest.mark.parametrize("form", FORMATS)
 def test_gate_of_numbers_at_the_edges(device, form):
     """Gates far from zero on both sides, infinities, NaN: what silu gives, and the rows beside."""
     x = torch.randn(6, 512)
