@@ -212,6 +212,40 @@ def test_matmul_strides_and_batches(device, m, form):
         assert bool((store == 3.0).all()), at
 
 
+@pytest.mark.parametrize("m", [1, 3, 40, 300])
+def test_matmul_rows_that_overlap(device, m):
+    """Rows that lie in one another, that are all the same one, and a single row with a stride that says nothing."""
+    n, k = 90, 640
+    a, sa = operands(m, k, FP8)
+    line, scales = operands(1, 8 * k, FP4, seed=9)
+    line, scales = line.view(torch.uint8).flatten(), scales.view(torch.uint8).flatten()
+    for apart, scales_apart in ((16, 1), (0, 0)):
+        b = line.to(device).as_strided((n, k // 2), (apart, 1)).view(FP4)
+        sb = scales.to(device).as_strided((n, k // 32), (scales_apart, 1)).view(E8M0)
+        there_a, there_sa = a.to(device), sa.to(device)
+        if m == 1:
+            there_a, there_sa = (t.view(torch.uint8).as_strided((1, t.shape[1]), (1 << 40, 1)).view(t.dtype) for t in (there_a, there_sa))
+        c = torch.empty(m, n, device=device)
+        capi.matmul_mx(there_a, there_sa, b, sb, c)
+        check(c, a, sa, b.view(torch.uint8).cpu().contiguous().view(FP4), sb.view(torch.uint8).cpu().contiguous().view(E8M0))
+
+
+def test_matmul_in_a_workspace_of_its_caller(device):
+    """Copies and shares of k in memory that held other things; one that is too small is left alone."""
+    for m, n, k in ((7, 33, 300), (1030, 19, 4928), (65, 40, 90)):
+        a, sa = operands(m, k, FP4)
+        b, sb = operands(n, k, FP4, seed=4)
+        c = torch.empty(m, n, device=device)
+        there = [t.to(device) for t in (a, sa, b, sb)]
+        room_for_it = torch.full((1 << 21,), 0xFF, dtype=torch.uint8, device=device)
+        capi.matmul_mx(*there, c, workspace=room_for_it)
+        check(c, a, sa, b, sb)
+        room_for_it.fill_(0xFF)
+        capi.matmul_mx(*there, c.fill_(7.0), workspace=room_for_it[:256])
+        check(c, a, sa, b, sb)
+        assert bool((room_for_it == 0xFF).all())
+
+
 @pytest.mark.parametrize("form", [FP4, FP8])
 @pytest.mark.parametrize("m", [3, 50, 200, 1000])
 def test_matmul_scales_that_are_not_numbers(device, m, form):

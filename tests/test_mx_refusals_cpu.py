@@ -54,6 +54,8 @@ def product(**changes):
     ({"b": operand(F4, 200, 320, strides=(1, 200))}, INVALID, "workspace"),
     ({"sa": operand(E8, 5, 20, strides=(2 ** 20 + 1, 1))}, INVALID, "workspace"),
     ({"a": operand(F4, 5, 320, strides=(-320, 1))}, INVALID, "workspace"),
+    ({"b": operand(F4, 200, 320, strides=(319, 1))}, INVALID, "workspace"),
+    ({"sb": operand(E8, 200, 20, strides=(1, 1))}, INVALID, "workspace"),
 ])
 def test_matmul(changes, code, word):
     v = product(**changes)
@@ -69,6 +71,9 @@ def test_matmul_batches_extents_and_workspace():
     assert need(*map(C.byref, v)) == 0
     assert asked() == 0
     assert asked(b=operand(F4, 200, 320, strides=(353, 1))) == 0
+    assert asked(b=operand(F4, 200, 320, strides=(0, 1)), sb=operand(E8, 200, 20, strides=(0, 1))) == 0
+    # a single row's stride says nothing
+    assert asked(a=operand(F4, 1, 320, strides=(1, 1)), sa=operand(E8, 1, 20, strides=(1 << 40, 1)), c=operand(F32, 1, 200)) == 0
     up = lambda n: -(-n // 256) * 256  # noqa: E731
     assert asked(b=operand(F4, 200, 320, strides=(1, 200))) == up(200 * 320)
     assert asked(sa=operand(E8, 5, 20, strides=(1, 5))) == up(5 * 20)

@@ -2931,7 +2931,9 @@ int32_t describe_mx_copy(const char* name, const VecopsHipOperand* x, const Veco
 // What the product reads an operand through: its own rows where their bytes follow one another, their blocks are whole and they lie near enough
 // to one another for the offsets of the plan's kernel, `rows` of them, else a copy in the workspace, padded to whole blocks with zeros.
 bool mx_rows_reached(int64_t rows, int64_t ld, int64_t bytes) { return ld <= INT32_MAX && (rows - 1) * ld + bytes + 512 < (int64_t{1} << 31); }
-bool mx_rows_ok(const View& v, int64_t k, int64_t rows) { return (v.cs == 1 || v.cols == 1) && k % kMxBlock == 0 && v.rs >= 0 && mx_rows_reached(rows, v.rs, v.cols); }
+// (rows that overlap would let rows past the last one, which the kernels keep out by their offsets, reach past the operand's end)
+bool mx_rows_apart(const View& v) { return v.rs == 0 || v.rs >= v.cols; }
+bool mx_rows_ok(const View& v, int64_t k, int64_t rows) { return (v.cs == 1 || v.cols == 1) && k % kMxBlock == 0 && mx_rows_apart(v) && mx_rows_reached(rows, v.rs, v.cols); }
 int64_t mx_row_bytes(const View& v) { return mx_blocks(v.dtype == DT_E2M1X2 ? 2 * v.cols : v.cols) * (v.dtype == DT_E2M1X2 ? kMxBlock / 2 : kMxBlock); }
 uint64_t mx_copy_bytes(const View& v, int64_t k, int64_t rows) {
   if (v.batch == 0 || v.rows == 0 || k == 0 || mx_rows_ok(v, k, rows)) return 0;
@@ -2939,7 +2941,7 @@ uint64_t mx_copy_bytes(const View& v, int64_t k, int64_t rows) {
 }
 
 // Scales likewise: a row's follow one another, at least as many as the plan's kernel reads at once, rows up to 2^20 apart.
-bool mx_scales_ok(const View& v, int least) { return v.cs == 1 && v.cols >= least && v.rs >= 0 && v.rs <= (int64_t{1} << 20); }
+bool mx_scales_ok(const View& v, int least) { return v.cs == 1 && v.cols >= least && mx_rows_apart(v) && v.rs <= (int64_t{1} << 20); }
 int64_t mx_scale_row_bytes(const View& v, int least) { return (std::max<int64_t>(v.cols, least) + 3) / 4 * 4; }
 uint64_t mx_scale_copy_bytes(const View& v, int least) {
   if (v.batch == 0 || v.rows == 0 || v.cols == 0 || mx_scales_ok(v, least)) return 0;
@@ -2980,6 +2982,8 @@ int32_t describe_mx(const VecopsHipOperand* a, const VecopsHipOperand* a_scales,
     return fail(ST_INVALID, "matmul_mx: b_scales must be [N=%lld, ceil(K / 32)=%lld]", (long long)n, (long long)mx_blocks(k));
   if (m > INT32_MAX / 2 || n > (1 << 27) || batch > 65535 || ((m + 63) / 64) * ((n + 63) / 64) >= (1 << 24)) return fail(ST_INVALID, "matmul_mx: extent too large");
   pr->plan = mx_plan(m, n, k, batch, pr->a.dtype == DT_E4M3);
+  for (View* v : {&pr->a, &pr->sa, &pr->b, &pr->sb})
+    if (v->rows == 1) v->rs = v->cols;   // (a single row's stride says nothing)
   if (m == 0 || n == 0 || batch == 0) return ST_OK;
   for (const auto& [v, rows] : {std::make_pair(&pr->a, pr->plan.rows_a), std::make_pair(&pr->b, pr->plan.rows_b)}) {
     if (mx_copy_bytes(*v, k, rows) == 0) continue;
