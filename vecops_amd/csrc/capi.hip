@@ -2942,7 +2942,7 @@ uint64_t mx_copy_bytes(const View& v, int64_t k, int64_t rows) {
 
 // Scales likewise: a row's follow one another, at least as many as the plan's kernel reads at once, rows up to 2^20 apart.
 bool mx_scales_ok(const View& v, int least) { return v.cs == 1 && v.cols >= least && mx_rows_apart(v) && v.rs <= (int64_t{1} << 20); }
-int64_t mx_scale_row_bytes(const View& v, int least) { return (std::max<int64_t>(v.cols, least) + 3) / 4 * 4; }
+int64_t mx_scale_row_bytes(const View& v, int least) { return (std::max<int64_t>(v.cols, least) + 15) / 16 * 16; }
 uint64_t mx_scale_copy_bytes(const View& v, int least) {
   if (v.batch == 0 || v.rows == 0 || v.cols == 0 || mx_scales_ok(v, least)) return 0;
   return round_up_256(static_cast<uint64_t>(v.bs == 0 ? 1 : v.batch) * static_cast<uint64_t>(v.rows) * static_cast<uint64_t>(mx_scale_row_bytes(v, least)));
@@ -2989,7 +2989,6 @@ int32_t describe_mx(const VecopsHipOperand* a, const VecopsHipOperand* a_scales,
     if (mx_copy_bytes(*v, k, rows) == 0) continue;
     // a copy brings rows together, but no nearer than their length
     if (!mx_rows_reached(rows, mx_row_bytes(*v), v->cols)) return fail(ST_NOT_APPLICABLE, "matmul_mx: K=%lld is too long: %d rows must lie within 2 GiB", (long long)k, rows);
-    if (((v->rows + 63) / 64) * ((v->cols + 63) / 64) >= (1 << 24)) return fail(ST_INVALID, "matmul_mx: extent too large");
   }
   return ST_OK;
 }
@@ -3072,21 +3071,26 @@ int32_t vecops_hip_matmul_mx(const VecopsHipOperand* a, const VecopsHipOperand* 
     return fail(ST_INVALID, "matmul_mx: needs a 16-byte aligned workspace of %llu bytes", (unsigned long long)need);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   uint8_t* room = static_cast<uint8_t*>(workspace);
+  MxCopies copies;
+  copies.count = 0;
   const auto copy = [&](View* v, uint64_t bytes, int64_t ld) {
-    if (bytes == 0) return hipSuccess;
-    const hipError_t e = launch_fp8_rows(static_cast<const uint8_t*>(v->data), v->bs, v->rs, v->cs, room, ld, static_cast<int32_t>(v->bs == 0 ? 1 : v->batch),
-                                         static_cast<int32_t>(v->rows), static_cast<int32_t>(v->cols), s);
+    if (bytes == 0) return;
+    copies.of[copies.count++] = {static_cast<const uint8_t*>(v->data), room, v->bs, v->rs, v->cols == 1 ? 1 : v->cs, ld, static_cast<int32_t>(v->bs == 0 ? 1 : v->batch),
+                                 static_cast<int32_t>(v->rows), static_cast<int32_t>(v->cols), 0};
     v->data = room;
     v->bs = v->bs == 0 ? 0 : v->rows * ld;
     v->rs = ld;
     v->cs = 1;
     room += bytes;
-    return e;
   };
-  for (const hipError_t e : {copy(&pr.a, mx_copy_bytes(pr.a, pr.k, pr.plan.rows_a), mx_row_bytes(pr.a)), copy(&pr.b, mx_copy_bytes(pr.b, pr.k, pr.plan.rows_b), mx_row_bytes(pr.b)),
-                             copy(&pr.sa, mx_scale_copy_bytes(pr.sa, pr.plan.scales), mx_scale_row_bytes(pr.sa, pr.plan.scales)),
-                             copy(&pr.sb, mx_scale_copy_bytes(pr.sb, pr.plan.scales), mx_scale_row_bytes(pr.sb, pr.plan.scales))})
+  copy(&pr.a, mx_copy_bytes(pr.a, pr.k, pr.plan.rows_a), mx_row_bytes(pr.a));
+  copy(&pr.b, mx_copy_bytes(pr.b, pr.k, pr.plan.rows_b), mx_row_bytes(pr.b));
+  copy(&pr.sa, mx_scale_copy_bytes(pr.sa, pr.plan.scales), mx_scale_row_bytes(pr.sa, pr.plan.scales));
+  copy(&pr.sb, mx_scale_copy_bytes(pr.sb, pr.plan.scales), mx_scale_row_bytes(pr.sb, pr.plan.scales));
+  if (copies.count > 0) {
+    const hipError_t e = launch_mx_copies(copies, s);
     if (e != hipSuccess) return fail(ST_EXEC, "matmul_mx: kernel launch: %s", hipGetErrorString(e));
+  }
   MxMatmulParams p;
   p.a = static_cast<const uint8_t*>(pr.a.data), p.b = static_cast<const uint8_t*>(pr.b.data);
   p.a_scales = static_cast<const uint8_t*>(pr.sa.data), p.b_scales = static_cast<const uint8_t*>(pr.sb.data);

@@ -603,6 +603,44 @@ __global__ __launch_bounds__(64 * WAVES, 2) void mx_slim_kernel(const MxMatmulPa
   }
 }
 
+// Operands whose rows are laid out in another way, all of them by one launch (with one each, 1 x 640 x 256, whose scales are too few a row, took 10.5 us a
+// call, now 6.4; 171 x 426 x 12582, whose K is no whole blocks, byte by byte 28.7, now 15.2).  A unit of work is 256 times sixteen bytes of rows that are contiguous, else 64 x 64 bytes through LDS, each side in its
+// own order.
+__global__ __launch_bounds__(256) void mx_copies_kernel(const MxCopies copies) {
+  __shared__ uint8_t tile[64][68];
+  for (int64_t unit = blockIdx.x; unit < copies.of[copies.count - 1].end; unit += gridDim.x) {
+    int which = 0;
+    while (unit >= copies.of[which].end) ++which;   // (uniform)
+    const MxCopy c = copies.of[which];
+    const int64_t begin = which == 0 ? 0 : copies.of[which - 1].end, per_batch = (c.end - begin) / c.batch, batch = (unit - begin) / per_batch;
+    const int64_t at = unit - begin - batch * per_batch;
+    const VECOPS_GLOBAL uint8_t* in = (const VECOPS_GLOBAL uint8_t*)c.in + batch * c.bs;
+    VECOPS_GLOBAL uint8_t* out = (VECOPS_GLOBAL uint8_t*)c.out + batch * c.rows * c.ld;
+    if (c.cs == 1) {
+      const int64_t pieces = c.ld / 16, piece = at * 256 + threadIdx.x, row = piece / pieces, from = (piece - row * pieces) * 16;
+      if (row >= c.rows) continue;
+      u32x4 v = {0u, 0u, 0u, 0u};
+      if (from + 16 <= c.cols) {
+        v = load_16(in + row * c.rs + from);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (from + e < c.cols) v[e >> 2] |= static_cast<uint32_t>(in[row * c.rs + from + e]) << (8 * (e & 3));
+      }
+      *(VECOPS_GLOBAL u32x4*)(out + piece * 16) = v;
+    } else {
+      const int64_t tiles = (c.ld + 63) / 64, r0 = at / tiles * 64, k0 = (at - at / tiles * tiles) * 64;
+      const int x = threadIdx.x & 63, y = threadIdx.x >> 6;
+      for (int i = y; i < 64; i += 4)   // consecutive lanes: consecutive rows (the contiguous side of a [K, rows] matrix)
+        tile[x][i] = r0 + x < c.rows && k0 + i < c.cols ? in[(r0 + x) * c.rs + (k0 + i) * c.cs] : 0;
+      __syncthreads();
+      for (int i = y; i < 64; i += 4)
+        if (r0 + i < c.rows && k0 + x < c.ld) out[(r0 + i) * c.ld + k0 + x] = tile[i][x];
+      __syncthreads();
+    }
+  }
+}
+
 hipError_t join(const MxMatmulParams& p, hipStream_t stream) {
   const hipError_t e = hipGetLastError();
   if (p.splits == 1 || e != hipSuccess) return e;
@@ -703,6 +741,17 @@ MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int64_t batch, bool a_wide) {
     }
   }
   return best;
+}
+
+hipError_t launch_mx_copies(MxCopies& copies, hipStream_t stream) {
+  int64_t end = 0;
+  for (int i = 0; i < copies.count; ++i) {
+    MxCopy& c = copies.of[i];
+    end += c.batch * (c.cs == 1 ? (c.rows * (c.ld / 16) + 255) / 256 : (static_cast<int64_t>(c.rows) + 63) / 64 * ((c.ld + 63) / 64));
+    c.end = end;
+  }
+  hipLaunchKernelGGL(mx_copies_kernel, dim3(static_cast<uint32_t>(std::min<int64_t>(end, 1 << 20))), dim3(256), 0, stream, copies);
+  return hipGetLastError();
 }
 
 hipError_t launch_mx_matmul(const MxMatmulParams& p, int kind, hipStream_t stream) {
