@@ -69,6 +69,8 @@ __device__ __forceinline__ uint32_t scale_shift(int word, int groups) { return s
 // in use, by loads that write LDS.  Scales come two stages a run, sixteen bytes of a row a load: each is a request of its own to
 // the cache, which a word a row for each 128 k had by the half of all requests.  A row's last run is its last sixteen scales; what of it
 // has been summed before gets zeros for elements.
+// 4096 x 11008 x 4096: e2m1 98-101 us (3.7 PFLOP/s; the matrix pipes busy 54 % of the cycles of a clock that they pull down to 1.65 GHz, 38 GB/s of loads a
+// compute unit, and 8 us a tile in which all of them write), e4m3 167 us (2.2 PFLOP/s).
 // The rows of a block of weights are dealt so that a lane's sixteen results are neighbouring n (the instruction's row
 // 8 g + 4 h + e, which lane half h holds, is n = 16 h + 4 g + e).
 constexpr int kRunBlocks = 16;
@@ -449,7 +451,10 @@ __global__ __launch_bounds__(64 * WN * WM * WK, WAVES_A_SIMD) void mx_tile_kerne
 // Few rows, or few results: R weight rows (16 or 32) and XR activation rows a workgroup, whose wavefronts share k without a barrier: each
 // has its own runs of 512 k, every WAVES-th, and its own DEPTH places for them in LDS, filled by loads that write LDS (whole lines, so that a load is
 // a look-up in the cache for every eight lanes or more).  Bound by HBM, or by what a compute unit can have under way: about 40 GB/s as soon as some of its
-// lines come from beyond its die's cache.
+// lines come from beyond its die's cache.  On weights that no cache holds: 1 x 14336 x 4096 8.3 us and 1 x 28672 x 4096 13.8 (3.8 and 4.5 TB/s), 16 x 14336 x
+// 4096 10.5, 64 x 4096 x 4096 7.1 (as 64 x 64 tiles 10.4), with e4m3 16 x 4096 x 14336 11.3 (fragments fetched into registers, four wavefronts: 16.3) and
+// 32 x 4096 x 14336 17.9 (64 x 64 tiles 29.5).  Two wavefronts of four rows where workgroups are many (1 x 28672 x 4096 13.8 us, with four 14.2, with two
+// places each 16), four with two places where they are few (1 x 4096 x 14336 8.2, 10.0 with one place, 14.1 with two wavefronts).
 // R = 16: v_mfma_scale_f32_16x16x128_f8f6f4, place q of instruction t of a run has block 4 q + t of sixteen; R = 32: 32x32x64, place q of
 // instruction t has block 8 q + t.  Either way a lane's scales are whole words whose byte is a constant of the instruction.
 template <int R, int XR, bool A8, int WAVES, int DEPTH>
