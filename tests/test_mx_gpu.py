@@ -349,3 +349,39 @@ def test_python_and_native_calls_agree(device, monkeypatch):
         results.append((q.view(torch.uint8), s.view(torch.uint8), c, out))
     for one, other in zip(*results):
         assert torch.equal(one, other)
+
+
+def test_two_streams_and_two_graphs(device):
+    """Calls with copies and shares of k at once on two streams, named and current ones, and two graphs replayed in turn: none has another's scratch."""
+    cases = []
+    for m, n, k in ((1030, 19, 4928), (300, 200, 300)):
+        a, sa = operands(m, k, FP4)
+        b, sb = operands(n, k, FP4, seed=6)
+        there = [t.to(device) for t in (a, sa, b, sb)]
+        cases.append((there, capi.matmul_mx(*there, torch.empty(m, n, device=device)), torch.zeros(m, n, device=device)))
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for turn in range(20):
+        for stream, (there, _, c) in zip(streams, cases):
+            if turn % 2:
+                capi.matmul_mx(*there, c, stream=stream)
+            else:
+                with torch.cuda.stream(stream):
+                    capi.matmul_mx(*there, c)
+    torch.cuda.synchronize()
+    graphs = []
+    for there, want, c in cases:
+        assert torch.equal(c, want)
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            capi.matmul_mx(*there, c)
+    for _ in range(3):
+        for (_, _, c), stream in zip(cases, streams):
+            c.zero_()
+            stream.wait_stream(torch.cuda.current_stream())
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, want, c in cases:
+            assert torch.equal(c, want)
