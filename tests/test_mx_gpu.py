@@ -168,9 +168,10 @@ TILE = lambda *of: f"mx_tile_kernel<{','.join(map(str, of))}"  # noqa: E731  (wa
     (17, 16, 32, FP4, ROWS(16, 16, 0, 4, 1), 0), (50, 30, 70, FP8, ROWS(16, 16, 1, 4, 1), 0), (40, 100, 5000, FP4, ROWS(16, 16, 0, 4, 2), 0),
     (40, 17, 2208, FP8, ROWS(16, 16, 1, 8, 1), 0), (260, 17, 32, FP4, ROWS(32, 32, 0, 4, 1), 0), (260, 17, 32, FP8, ROWS(32, 32, 1, 4, 1), 0),
     (1030, 18, 32, FP4, TILE(1, 2, 2, 2, 1, 0), 0), (1030, 90, 70, FP8, TILE(1, 2, 2, 2, 1, 1), 0), (1030, 19, 4928, FP4, TILE(1, 2, 2, 2, 1, 0), 2),
-    (1030, 19, 5200, FP8, TILE(1, 2, 2, 2, 1, 1), 2), (4100, 453, 32, FP4, TILE(2, 2, 1, 2, 2, 0), 0), (65, 9472, 4736, FP4, TILE(2, 2, 1, 2, 2, 0), 2),
+    (1030, 19, 5200, FP8, TILE(1, 2, 2, 2, 1, 1), 2), (4100, 453, 32, FP4, TILE(2, 2, 1, 2, 2, 0), 0), (4100, 248, 2400, FP4, TILE(2, 1, 2, 2, 2, 0), 0), (4100, 207, 1536, FP8, TILE(2, 1, 2, 2, 2, 1), 0),
+    (4100, 113, 14560, FP8, TILE(2, 1, 2, 2, 2, 1), 2),
     (4100, 550, 3488, FP4, TILE(2, 2, 2, 2, 2, 0), 0), (4100, 210, 10176, FP4, TILE(2, 2, 2, 2, 2, 0), 2), (4100, 453, 32, FP8, TILE(2, 2, 2, 2, 2, 1), 0),
-    (4100, 210, 10176, FP8, TILE(2, 2, 2, 2, 2, 1), 2), (4100, 3257, 1312, FP4, TILE(2, 2, 1, 4, 4, 0), 0), (4100, 980, 10656, FP4, TILE(2, 2, 1, 4, 4, 0), 2),
+    (4100, 210, 10176, FP8, TILE(2, 2, 2, 2, 2, 1), 2), (4100, 3257, 1312, FP4, TILE(2, 2, 1, 4, 4, 0), 0), (2050, 2041, 12288, FP4, TILE(2, 2, 1, 4, 4, 0), 2),
     (4100, 989, 32, FP8, TILE(2, 2, 1, 4, 2, 1), 0), (2050, 1083, 15712, FP8, TILE(2, 2, 1, 4, 2, 1), 2)])
 def test_every_kernel_of_the_product(device, m, n, k, form, kernel, shares):
     """Each variant that sizes choose, with shares of k and without, up to odd ends of every extent."""

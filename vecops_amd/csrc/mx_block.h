@@ -42,8 +42,8 @@ struct MxCopies {
 hipError_t launch_mx_copies(MxCopies& copies, hipStream_t stream);
 
 // The kernels.  MX_ROWS_r: r activation rows by 16 (r = 4, 16) or 32 weight rows a workgroup, whose wavefronts share k; MX_TILE_t: tiles of t x t,
-// MX_TILE_256 of 256 weight rows by 256, with e4m3 activations by 128.  _DEEP: more of k under way a workgroup, for products of few workgroups.
-enum MxKind : int { MX_ROWS_4 = 0, MX_ROWS_4_DEEP, MX_ROWS_16, MX_ROWS_16_DEEP, MX_ROWS_32, MX_TILE_64, MX_TILE_128, MX_TILE_128_DEEP, MX_TILE_256, MX_KINDS };
+// MX_TILE_128X64 of 128 weight rows by 64, MX_TILE_256 of 256 by 256, with e4m3 activations by 128.  _DEEP: more of k under way a workgroup, for products of few workgroups.
+enum MxKind : int { MX_ROWS_4 = 0, MX_ROWS_4_DEEP, MX_ROWS_16, MX_ROWS_16_DEEP, MX_ROWS_32, MX_TILE_64, MX_TILE_128X64, MX_TILE_128, MX_TILE_128_DEEP, MX_TILE_256, MX_KINDS };
 struct MxPlan {
   int kind;
   int splits;  // shares of k; more than one need `partial`

@@ -71,6 +71,8 @@ __device__ __forceinline__ uint32_t scale_shift(int word, int groups) { return s
 // has been summed before gets zeros for elements.
 // 4096 x 11008 x 4096: e2m1 98-101 us (3.7 PFLOP/s; the matrix pipes busy 54 % of the cycles of a clock that they pull down to 1.65 GHz, 38 GB/s of loads a
 // compute unit, and 8 us a tile in which all of them write), e4m3 167 us (2.2 PFLOP/s).
+// 128 weight rows by 64, two wavefronts sharing k: a third less to load a result than 64 x 64; 128 x 11008 x 4096 with e4m3 16.4 us rather than 20.4,
+// 512 x 4096 x 11008 35.4 rather than 44, 1024 x 2048 x 8192 25.7 rather than 31.6 (e2m1 22.4 and 23.5).
 // The rows of a block of weights are dealt so that a lane's sixteen results are neighbouring n (the instruction's row
 // 8 g + 4 h + e, which lane half h holds, is n = 16 h + 4 g + e).
 constexpr int kRunBlocks = 16;
@@ -693,36 +695,38 @@ hipError_t launch_tile(const MxMatmulParams& p, hipStream_t stream) {
 // Which kernel, and how many shares of k: the least of fitted times.  A kernel's workgroups (those of all shares) go in rounds over 256 compute units
 // with `slots` of them each, as their LDS allows; a round of c on a compute unit takes start + runs (alone + more (c - 1)) us, where `runs` are the runs of
 // 512 k that a wavefront has to do, and the bytes at 5.5 TB/s and 2 us are joined to that as a fourth power (the longer of the two counts, the other
-// decides between equals).  Shares cost the joining launch and its bytes.  The constants were fitted to 3700 timings of every kernel and of 1, 2 and 4
-// shares at 520 products of random sizes (M 1 .. 4096, N 256 .. 28000, K 512 .. 16384) on weights that no cache held.  What the rule takes is 0.8 %
-// slower than the fastest of them on average and 1.18 times at worst.  The best choice without one of them would be slower by 2.4 % (MX_ROWS_4),
-// 1.7 % (MX_TILE_256), 1.3 % (MX_TILE_128), 1.1 % (MX_ROWS_32), 0.9 % (MX_ROWS_4_DEEP), 0.6 % (MX_ROWS_16_DEEP, MX_TILE_128_DEEP) and 0.4 % (shares, 1.38 times at
-// worst; four shares rather than two, or of few rows, 0.04 %); 32 x 64 results a workgroup and 4 x 16 by four wavefronts brought 0.2 % each and are left
-// out.  Up to four rows only kernels of four are weighed: on a tie of latencies the fit's errors would decide.
+// decides between equals).  Shares cost the joining launch and its bytes.  The constants were fitted to 4200 timings of every kernel and of 1 and 2
+// shares at 620 products of random sizes (M 1 .. 4096, N 256 .. 28000, K 512 .. 16384) on weights that no cache held.  What the rule takes is 0.6 %
+// slower than the fastest of them on average and 1.19 times at worst.  The best choice without one of them would be slower by 2.2 % (MX_ROWS_4),
+// 2.1 % (MX_TILE_256), 1.5 % (MX_TILE_128), 1.1 % (MX_ROWS_32), 0.9 % (MX_ROWS_4_DEEP), 0.6 % (MX_TILE_128X64, MX_TILE_128_DEEP), 0.5 % (MX_ROWS_16_DEEP) and
+// 0.3 % (shares, 1.38 times at worst; four shares rather than two, or of few rows, 0.04 %); 32 x 64 results a workgroup and 4 x 16 by four wavefronts
+// brought 0.2 % each and are left out.  Up to four rows only kernels of four are weighed: on a tie of latencies the fit's errors would decide.
 MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int64_t batch, bool a_wide) {
   struct Cost {
     int rows_a, rows_b, wavefronts, slots;   // as powers of two; wavefronts that share k by whole runs
     float once, start, alone, more;          // us
   };
   constexpr Cost kCosts[2][MX_KINDS] = {
-      {{2, 4, 1, 3, 2.24f, 0.33f, 0.52f, 0.24f},    // MX_ROWS_4
-       {2, 4, 2, 1, 1.22f, 1.76f, 0.38f, 0.58f},    // MX_ROWS_4_DEEP
-       {4, 4, 2, 2, 1.84f, 0.69f, 0.79f, 0.57f},    // MX_ROWS_16
-       {4, 4, 2, 1, 1.36f, 1.70f, 0.49f, 0.76f},    // MX_ROWS_16_DEEP
-       {5, 5, 2, 1, 1.56f, 1.17f, 1.50f, 1.38f},    // MX_ROWS_32
-       {6, 6, 0, 1, 2.35f, 1.96f, 0.66f, 0.86f},    // MX_TILE_64
-       {7, 7, 0, 1, 1.78f, 2.91f, 1.90f, 1.12f},    // MX_TILE_128
-       {7, 7, 0, 0, 1.70f, 4.94f, 1.57f, 0.f},      // MX_TILE_128_DEEP
-       {8, 8, 0, 0, 2.91f, 10.85f, 3.17f, 0.f}},    // MX_TILE_256
-      {{2, 4, 1, 3, 2.13f, 0.42f, 0.56f, 0.25f},
-       {2, 4, 2, 1, 0.97f, 2.12f, 0.42f, 0.55f},
-       {4, 4, 2, 1, 1.24f, 1.35f, 0.97f, 0.66f},
-       {4, 4, 3, 0, 1.01f, 1.29f, 1.63f, 0.f},
-       {5, 5, 2, 0, 0.86f, 1.92f, 1.86f, 0.f},
-       {6, 6, 0, 1, 1.79f, 2.68f, 0.82f, 0.88f},
+      {{2, 4, 1, 3, 1.99f, 0.64f, 0.51f, 0.22f},    // MX_ROWS_4
+       {2, 4, 2, 1, 1.06f, 1.85f, 0.52f, 0.42f},    // MX_ROWS_4_DEEP
+       {4, 4, 2, 2, 1.58f, 0.94f, 0.85f, 0.50f},    // MX_ROWS_16
+       {4, 4, 2, 1, 1.24f, 1.72f, 0.56f, 0.72f},    // MX_ROWS_16_DEEP
+       {5, 5, 2, 1, 1.83f, 0.85f, 1.50f, 1.23f},    // MX_ROWS_32
+       {6, 6, 0, 1, 1.87f, 2.37f, 0.70f, 0.75f},    // MX_TILE_64
+       {6, 7, 0, 1, 1.96f, 3.53f, 1.15f, 0.90f},    // MX_TILE_128X64
+       {7, 7, 0, 1, 1.16f, 3.47f, 1.89f, 0.86f},    // MX_TILE_128
+       {7, 7, 0, 0, 1.60f, 5.14f, 1.48f, 0.f},      // MX_TILE_128_DEEP
+       {8, 8, 0, 0, 4.85f, 9.57f, 3.14f, 0.f}},     // MX_TILE_256
+      {{2, 4, 1, 3, 2.46f, 0.f, 0.60f, 0.26f},
+       {2, 4, 2, 1, 1.04f, 1.94f, 0.46f, 0.64f},
+       {4, 4, 2, 1, 1.33f, 1.21f, 1.02f, 0.62f},
+       {4, 4, 3, 0, 0.91f, 1.30f, 1.69f, 0.f},
+       {5, 5, 2, 0, 1.04f, 1.66f, 1.98f, 0.f},
+       {6, 6, 0, 1, 1.73f, 2.56f, 0.93f, 0.87f},
+       {6, 7, 0, 0, 2.07f, 3.44f, 1.37f, 0.f},
        {7, 7, 0, -1, 0.f, 0.f, 0.f, 0.f},           // (two workgroups of such tiles a compute unit: of e2m1 only)
-       {7, 7, 0, 0, 1.79f, 5.14f, 1.96f, 0.f},
-       {7, 8, 0, 0, 4.90f, 3.96f, 3.05f, 0.f}}};
+       {7, 7, 0, 0, 2.06f, 4.88f, 1.96f, 0.f},
+       {7, 8, 0, 0, 5.70f, 3.25f, 2.98f, 0.f}}};
   const int64_t runs = (k + 511) / 512;
   const auto shared = [](int64_t x, int by) { return (x + (int64_t{1} << by) - 1) >> by; };
   const float bytes = (static_cast<float>(n) * k * (17 / 32.f) + static_cast<float>(m) * k * (a_wide ? 33 / 32.f : 17 / 32.f) + 2.f * m * n) * batch;
@@ -767,6 +771,7 @@ hipError_t launch_mx_matmul(const MxMatmulParams& p, int kind, hipStream_t strea
     case MX_ROWS_16_DEEP: return p.a_wide ? launch_slim<16, 16, true, 8, 1>(p, stream) : launch_slim<16, 16, false, 4, 2>(p, stream);
     case MX_ROWS_32: return p.a_wide ? launch_slim<32, 32, true, 4, 1>(p, stream) : launch_slim<32, 32, false, 4, 1>(p, stream);
     case MX_TILE_64: return p.a_wide ? launch_tile<1, 2, 2, 2, 1, true, 3, 2, false>(p, stream) : launch_tile<1, 2, 2, 2, 1, false, 4, 2, false>(p, stream);
+    case MX_TILE_128X64: return p.a_wide ? launch_tile<2, 1, 2, 2, 2, true, 3, 2, false>(p, stream) : launch_tile<2, 1, 2, 2, 2, false, 3, 2, false>(p, stream);
     case MX_TILE_128: return p.a_wide ? hipErrorInvalidValue : launch_tile<2, 2, 1, 2, 2, false, 2, 2, false>(p, stream);
     case MX_TILE_128_DEEP: return p.a_wide ? launch_tile<2, 2, 2, 2, 2, true, 3, 2, false>(p, stream) : launch_tile<2, 2, 2, 2, 2, false, 4, 2, false>(p, stream);
     case MX_TILE_256: return p.a_wide ? launch_tile<2, 2, 1, 4, 2, true, 2, 1, true>(p, stream) : launch_tile<2, 2, 1, 4, 4, false, 2, 1, true>(p, stream);
