@@ -584,8 +584,8 @@ VECOPS_HIP_EXPORT int32_t vecops_hip_dequantize_mx(const VecopsHipOperand* q, co
  * results of its row or column NaN.
  * workspace: vecops_hip_matmul_mx_workspace bytes (0 for operands that the call refuses), 16-byte aligned.  It holds the sums of
  * parts of K, where few tiles would leave the chip short of work (added in a fixed order), and copies of operands whose rows are not contiguous, lie too far
- * apart, overlap, or have a K that is no multiple of 32, and of scales of which a row's are not contiguous, fewer than sixteen, overlap, or whose rows are more
- * than 2^20 apart.  The rows of a tile, up to 256 of either operand, are reached by offsets below 2 GiB: a K so long that even a copy does not fit there is
+ * apart, overlap, or have a K that is no multiple of 32, and of scales of which a row's are not contiguous, whose rows overlap, are more than 2^20 apart, or
+ * (with large M and N) have fewer than sixteen.  The rows of a tile, up to 256 of either operand, are reached by offsets below 2 GiB: a K so long that even a copy does not fit there is
  * refused.
  */
 VECOPS_HIP_EXPORT uint64_t vecops_hip_matmul_mx_workspace(const VecopsHipOperand* a, const VecopsHipOperand* a_scales,

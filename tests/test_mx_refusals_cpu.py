@@ -77,10 +77,12 @@ def test_matmul_batches_extents_and_workspace():
     up = lambda n: -(-n // 256) * 256  # noqa: E731
     assert asked(b=operand(F4, 200, 320, strides=(1, 200))) == up(200 * 320)
     assert asked(sa=operand(E8, 5, 20, strides=(1, 5))) == up(5 * 20)
-    # a K of no whole blocks: both operands padded; fewer than sixteen scales a row: those too
+    # a K of no whole blocks: both operands padded; scales of rows apart: in place, however few
     assert asked(a=operand(F4, 5, 319), b=operand(F4, 200, 319)) == up(5 * 320) + up(200 * 320)
     assert asked(a=operand(F8, 5, 638), b=operand(F4, 200, 319)) == up(5 * 640) + up(200 * 320)
-    assert asked(a=operand(F4, 5, 32), sa=operand(E8, 5, 2), b=operand(F4, 200, 32), sb=operand(E8, 200, 2)) == up(5 * 16) + up(200 * 16)
+    assert asked(a=operand(F4, 5, 32), sa=operand(E8, 5, 2), b=operand(F4, 200, 32), sb=operand(E8, 200, 2)) == 0
+    # the largest tiles read sixteen scales of a row at once
+    assert asked(a=operand(F8, 2050, 224), sa=operand(E8, 2050, 7), b=operand(F4, 4100, 112), sb=operand(E8, 4100, 7), c=operand(BF16, 2050, 4100)) == up(2050 * 16) + up(4100 * 16)
     shared = product(a=operand(F4, 7, 5, 320), sa=operand(E8, 7, 5, 20), b=operand(F4, 7, 200, 320, strides=(0, 1, 200)),
                      sb=operand(E8, 7, 200, 20), c=operand(F32, 7, 5, 200))
     assert need(*(ref(shared[n]) for n in names)) == up(200 * 320)

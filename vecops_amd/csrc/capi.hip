@@ -2941,7 +2941,7 @@ uint64_t mx_copy_bytes(const View& v, int64_t k, int64_t rows) {
 }
 
 // Scales likewise: a row's follow one another, at least as many as the plan's kernel reads at once, rows up to 2^20 apart.
-bool mx_scales_ok(const View& v, int least) { return v.cs == 1 && v.cols >= least && mx_rows_apart(v) && v.rs <= (int64_t{1} << 20); }
+bool mx_scales_ok(const View& v, int least) { return (v.cs == 1 || v.cols == 1) && v.cols >= least && mx_rows_apart(v) && v.rs <= (int64_t{1} << 20); }
 int64_t mx_scale_row_bytes(const View& v, int least) { return (std::max<int64_t>(v.cols, least) + 15) / 16 * 16; }
 uint64_t mx_scale_copy_bytes(const View& v, int least) {
   if (v.batch == 0 || v.rows == 0 || v.cols == 0 || mx_scales_ok(v, least)) return 0;

@@ -20,7 +20,7 @@ struct MxMatmulParams {
   int64_t c_rs, c_cs, c_bs;
   int32_t m, n, batch;
   int32_t groups;      // blocks of 32 along k, each whole
-  int32_t row_scales;  // scales of a row that can be read: groups, at least as many as the kernel reads at once
+  int32_t row_scales;  // scales of a row that can be read: groups, or sixteen where rows of fewer have been padded (what MX_TILE_256 needs)
   int32_t a_wide;    // a is e4m3
   int32_t out_kind;  // Fp8Real
   int32_t splits;    // shares of k; more than one leave through `partial`, [splits][batch][m][n]
@@ -48,7 +48,7 @@ struct MxPlan {
   int kind;
   int splits;  // shares of k; more than one need `partial`
   int rows_a, rows_b;  // of an operand, that a workgroup reaches by offsets below 2 GiB
-  int scales;          // of a row, that are read at once
+  int scales;          // the fewest of a row
 };
 MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int64_t batch, bool a_wide);
 hipError_t launch_mx_matmul(const MxMatmulParams& p, int kind, hipStream_t stream);

@@ -60,6 +60,18 @@ __device__ __forceinline__ void settle() {
 __device__ __forceinline__ int scale_word_at(int word, int groups) { return min(4 * word, groups - 4); }
 __device__ __forceinline__ uint32_t scale_shift(int word, int groups) { return static_cast<uint32_t>(min(max(4 * word + 4 - groups, 0) * 8, 31)); }
 
+// Rows of fewer scales than a load fetches (K < 512): a lane reads those that there are, byte by byte, and writes them to LDS itself, with zeros
+// behind, where a load has left zeros (1 x 640 x 256 4.9 us a call, 109 x 3200 x 256 6.5; with rows laid out in the workspace first 6.4 and 8.7.  It costs 64 x 64
+// tiles of longer rows 0.15 us of 7.6).  MX_TILE_256, whose workgroups go on to other tiles, has them laid out.
+__device__ __forceinline__ u32x4 few_scales(const uint8_t* base, int64_t at, int groups, bool there) {
+  u32x4 v = {0u, 0u, 0u, 0u};
+  const VECOPS_GLOBAL uint8_t* from = (const VECOPS_GLOBAL uint8_t*)base + at;
+#pragma unroll
+  for (int e = 0; e < 15; ++e)
+    if (there && e < groups) v[e >> 2] |= static_cast<uint32_t>(from[e]) << (8 * (e & 3));
+  return v;
+}
+
 // Many rows: WN x WM wavefronts, each NT x MT blocks of 32 x 32.  v_mfma_scale_f32_32x32x64_f8f6f4: a lane's e2m1 operand is the
 // place l / 32 of two of row l % 32, an e4m3 one half l / 32 of either place; its scale is that of place l / 32.  Of a stage's eight blocks of
 // 32 k instruction s of four has block 4 q + s in place q: a lane's four scales are one word, the instruction's byte of it a constant.  (One wavefront
@@ -188,6 +200,8 @@ __global__ __launch_bounds__(64 * WN * WM * WK, WAVES_A_SIMD) void mx_tile_kerne
   uint32_t fetch_unit = blockIdx.x, end_w = 0, end_x = 0, end_s[T::kLoadsS], fetch_turn = 0;
   int fetch_run = run_begin;
   u32x4 desc_w, desc_x, desc_s[T::kLoadsS];
+  const bool few = !GOES_ON && p.row_scales < kRunBlocks;
+  const int last_first = few ? 0 : p.row_scales - kRunBlocks;
   auto aim = [&] {
     const bool there = fetch_unit < units && run_begin < run_end;   // (past the last tile nothing is fetched, but as many loads are issued)
     const Tile t = tile_of(there ? fetch_unit : 0);
@@ -202,7 +216,7 @@ __global__ __launch_bounds__(64 * WN * WM * WK, WAVES_A_SIMD) void mx_tile_kerne
       const bool weights = 64 * (i * T::kWaves + wave) < T::kBN;
       desc_s[i] = tile_buffer_words(weights ? (const VECOPS_GLOBAL char*)p.b_scales + batch * p.bs_bs + t.n0 * p.bs_rs
                                             : (const VECOPS_GLOBAL char*)p.a_scales + batch * p.as_bs + t.m0 * p.as_rs);
-      end_s[i] = __builtin_amdgcn_readfirstlane(there ? static_cast<uint32_t>((weights ? t.last_n * p.bs_rs : t.last_m * p.as_rs) + p.row_scales) : 0u);
+      end_s[i] = __builtin_amdgcn_readfirstlane(there && !few ? static_cast<uint32_t>((weights ? t.last_n * p.bs_rs : t.last_m * p.as_rs) + p.row_scales) : 0u);
       desc_s[i][2] = end_s[i];
     }
   };
@@ -217,7 +231,7 @@ __global__ __launch_bounds__(64 * WN * WM * WK, WAVES_A_SIMD) void mx_tile_kerne
   // load PIECE of those that fill buffer `slot` with half PAR of the run that is fetched
   auto issue_piece = [&](auto piece_tag, auto par_tag, int slot) {
     constexpr int PIECE = decltype(piece_tag)::value, PAR = decltype(par_tag)::value;
-    const int first_block = min(fetch_run * kRunBlocks, p.row_scales - kRunBlocks);   // the run's sixteen blocks
+    const int first_block = min(fetch_run * kRunBlocks, last_first);   // the run's sixteen blocks
     // those before `old` have been summed; those from `most` on are not there
     const int old = fetch_run * kRunBlocks - first_block - 8 * PAR, most = p.groups - first_block - 8 * PAR;
     if constexpr (PIECE < T::kLoadsW) {
@@ -337,6 +351,18 @@ __global__ __launch_bounds__(64 * WN * WM * WK, WAVES_A_SIMD) void mx_tile_kerne
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(T::loads_between(1, STAGES)) : "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
+  if (__builtin_expect(few, 0)) {
+    const Tile t = tile_of(blockIdx.x);
+    for (int row = tid; row < T::kBN + T::kBM; row += T::kThreads) {
+      const bool weights = row < T::kBN;
+      const int64_t n = t.n0 + row, m = t.m0 + row - T::kBN;
+      write_lds(lds0 + T::kScales + row * 16, weights ? few_scales(p.b_scales, batch * p.bs_bs + n * p.bs_rs, p.groups, n < p.n)
+                                                      : few_scales(p.a_scales, batch * p.as_bs + m * p.as_rs, p.groups, m < p.m));
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  }
   static_for<2 * kSets>([&](auto f) {
     constexpr int F = decltype(f)::value;
     read_w(std::integral_constant<int, 0>{}, std::integral_constant<int, (F & 1)>{}, std::integral_constant<int, (F >> 1)>{}, 0);
@@ -494,8 +520,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void mx_slim_kernel(const MxMatmulPa
   const u32x4 desc_sx = tile_buffer_words((const VECOPS_GLOBAL char*)p.a_scales + batch * p.as_bs + m0 * p.as_rs);
   const uint32_t end_w = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(last_n * p.ldb) + static_cast<uint32_t>(p.groups) * 16u);
   const uint32_t end_x = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(last_m * p.lda) + static_cast<uint32_t>(p.groups) * (A8 ? 32u : 16u));
-  const uint32_t end_sw = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(last_n * p.bs_rs + p.row_scales));
-  const uint32_t end_sx = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(last_m * p.as_rs + p.row_scales));
+  const bool few = p.row_scales < kRunBlocks;
+  const int last_first = few ? 0 : p.row_scales - kRunBlocks;
+  const uint32_t end_sw = __builtin_amdgcn_readfirstlane(few ? 0u : static_cast<uint32_t>(last_n * p.bs_rs + p.row_scales));
+  const uint32_t end_sx = __builtin_amdgcn_readfirstlane(few ? 0u : static_cast<uint32_t>(last_m * p.as_rs + p.row_scales));
 
   // Slot of a chunk: (chunk ^ (row + 4) % 16), of which LDS serves the rows that it reads together without conflicts (R = 16: of two places,
   // rows 0-3 and 12-15 of one, 4-11 of the other).  Load i of the weights: rows 4 i + lane / 16, slot lane % 16.
@@ -504,7 +532,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void mx_slim_kernel(const MxMatmulPa
     const int run = __builtin_amdgcn_readfirstlane(its_run);   // (the same in all lanes, which the compiler does not see)
     const uint32_t to = __builtin_amdgcn_readfirstlane(own + place * T::kPlace);
     const bool there = run < run_end;
-    const int first_block = __builtin_amdgcn_readfirstlane(min(run * kRunBlocks, p.row_scales - kRunBlocks)), old = run * kRunBlocks - first_block, most = p.groups - first_block;
+    const int first_block = __builtin_amdgcn_readfirstlane(min(run * kRunBlocks, last_first)), old = run * kRunBlocks - first_block, most = p.groups - first_block;
     const uint32_t at_w = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(first_block) * 16u), at_x = __builtin_amdgcn_readfirstlane(at_w * (A8 ? 2u : 1u));
     const auto ending = [&](const u32x4& desc, uint32_t end) {
       u32x4 words = {desc[0], desc[1], there ? end : 0u, desc[3]};
@@ -545,6 +573,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void mx_slim_kernel(const MxMatmulPa
   for (int run = mine; run < run_end; run += WAVES) {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 1) * T::kLoads) : "memory");
     const uint32_t at = own + place * T::kPlace;
+    if (__builtin_expect(few, 0)) {   // (the only run)
+      if (lane < R) write_lds(at + T::kScales + lane * 16, few_scales(p.b_scales, batch * p.bs_bs + (n0 + lane) * p.bs_rs, p.groups, lane <= last_n));
+      if (lane < XR) write_lds(at + T::kScales + 1024 + lane * 16, few_scales(p.a_scales, batch * p.as_bs + (m0 + lane) * p.as_rs, p.groups, lane <= last_m));
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    }
     i32x8 w[kSteps];
     uint32_t sw[kWords];
 #pragma unroll
@@ -610,9 +643,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void mx_slim_kernel(const MxMatmulPa
   }
 }
 
-// Operands whose rows are laid out in another way, all of them by one launch (with one each, 1 x 640 x 256, whose scales are too few a row, took 10.5 us a
-// call, now 6.4; 171 x 426 x 12582, whose K is no whole blocks, byte by byte 28.7, now 15.2).  A unit of work is 256 times sixteen bytes of rows that are contiguous, else 64 x 64 bytes through LDS, each side in its
-// own order.
+// Operands whose rows are laid out in another way, all of them by one launch (171 x 426 x 12582, whose K is no whole blocks, 15.3 us a call; with a launch
+// each that moves single bytes 28.7).  A unit of work is 256 times sixteen bytes of rows that are contiguous, else 64 x 64 bytes through LDS, each side in
+// its own order.
 __global__ __launch_bounds__(256) void mx_copies_kernel(const MxCopies copies) {
   __shared__ uint8_t tile[64][68];
   for (int64_t unit = blockIdx.x; unit < copies.of[copies.count - 1].end; unit += gridDim.x) {
@@ -745,8 +778,9 @@ MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int64_t batch, bool a_wide) {
       float us = cost.once + rounds * (cost.start + (cost.alone + cost.more * (slots - 1)) * each);
       if (rest > 0) us += cost.start + (cost.alone + cost.more * (rest - 1)) * each;
       us = std::sqrt(std::sqrt(us * us * us * us + moved * moved * moved * moved));
+      if (kind == MX_TILE_256 && runs <= 1) us += 2.5f;   // (for the launch that lays out scales too few a row)
       if (split > 0) us += 3.2f + 2.8e-6f * (static_cast<float>(m) * n * batch);
-      if (us < least) least = us, best = {kind, 1 << split, 1 << cost.rows_a, 1 << cost.rows_b, kRunBlocks};
+      if (us < least) least = us, best = {kind, 1 << split, 1 << cost.rows_a, 1 << cost.rows_b, kind == MX_TILE_256 ? kRunBlocks : 0};
     }
   }
   return best;
