@@ -22,7 +22,9 @@ namespace {
 // two instructions, and instruction h has block 2 q + h in place q.  A lane then holds the scales of neighbouring blocks.
 // e2m1 times e2m1 is exact up to one rounding to fp32 an instruction (measured: 3e-8 of the terms' sizes).  With e4m3 the instruction aligns
 // each eight products along k to the largest and drops what is below 2^-13 of it: 1.4e-5 of a result on normally distributed
-// operands.  A scale that is NaN makes the result NaN, also over elements of zero.
+// operands, which goes unnoticed in results of 16 bits.  For results in f32 the activations are taken in two parts by size, an instruction each, whose products
+// are exact as e2m1's are: 30 to 70 % more time where many rows share weights (4096 x 11008 x 4096 290 us rather than 177, 128 x 11008 x 4096 21.6 rather than 17.1),
+// none to speak of for a few rows.  A scale that is NaN makes the result NaN, also over elements of zero.
 // ---------------------------------------------------------------------------------------------------------------------
 
 constexpr int kStepBlocks = 8;                  // blocks of 32 k in a step
@@ -42,6 +44,17 @@ __device__ __forceinline__ f32x16 mfma_mx_32(const i32x8& w, const i32x8& x, con
 
 __device__ __forceinline__ i32x8 narrow_fragment(const u32x4& v) {
   return i32x8{static_cast<int>(v[0]), static_cast<int>(v[1]), static_cast<int>(v[2]), static_cast<int>(v[3]), 0, 0, 0, 0};
+}
+
+// e4m3 elements of 2 and more (bit 6 of a byte; NaN has it too) with zeros for the others, and the others.  A product with e2m1 is a multiple of 2^-4 of its
+// element's power of two, and a part has at most eight of these powers: none of eight products has a bit that is dropped beside the largest.
+__device__ __forceinline__ void part_by_size(const i32x8& x, i32x8& high, i32x8& low) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t v = static_cast<uint32_t>(x[i]), there = (v >> 6) & 0x01010101u, mask = (there << 8) - there;
+    high[i] = static_cast<int>(v & mask);
+    low[i] = static_cast<int>(v & ~mask);
+  }
 }
 
 // Matrix results are read by other instructions only behind this: the compiler has been seen to leave too few wait states where a
@@ -147,7 +160,7 @@ __device__ __forceinline__ void store_sixteen(char* c, int64_t row, int64_t cs, 
 // compute unit nothing else would.
 // OUT: the type in which results leave (a template's argument: with a branch the compiler makes copies of all of the way out and reads every
 // accumulator in front of them).
-template <int WN, int WM, int WK, int NT, int MT, bool A8, int STAGES, int WAVES_A_SIMD, bool GOES_ON, int OUT>
+template <int WN, int WM, int WK, int NT, int MT, bool A8, int STAGES, int WAVES_A_SIMD, bool GOES_ON, int OUT, bool PARTS>
 __global__ __launch_bounds__(64 * WN * WM * WK, WAVES_A_SIMD) void mx_tile_kernel(const MxMatmulParams p, uint32_t tiles_n, uint32_t tiles_m) {
   using T = MxTile<WN, WM, WK, NT, MT, A8, STAGES, GOES_ON>;
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -330,9 +343,16 @@ __global__ __launch_bounds__(64 * WN * WM * WK, WAVES_A_SIMD) void mx_tile_kerne
       };
       static_for<kSets>([&](auto s_tag) {
         static_for<MT>([&](auto j_tag) {
+          i32x8 high, low;
+          if constexpr (PARTS) {
+            constexpr int s = decltype(s_tag)::value, j = decltype(j_tag)::value, at = 2 * pair * MT + j;
+            part_by_size(x[s][j], high, low);
+            acc[at] = mfma_mx_32<A8, s>(w[now][0][s], low, acc[at], sw[now][0], sx[PAR][j]);
+            acc[at + MT] = mfma_mx_32<A8, s>(w[now][1][s], low, acc[at + MT], sw[now][1], sx[PAR][j]);
+          }
           static_for<2>([&](auto i_tag) {
             constexpr int s = decltype(s_tag)::value, j = decltype(j_tag)::value, i = decltype(i_tag)::value, at = (2 * pair + i) * MT + j;
-            acc[at] = mfma_mx_32<A8, s>(w[now][i][s], x[s][j], acc[at], sw[now][i], sx[PAR][j]);
+            acc[at] = mfma_mx_32<A8, s>(w[now][i][s], PARTS ? high : x[s][j], acc[at], sw[now][i], sx[PAR][j]);
             __builtin_amdgcn_sched_barrier(0);
             beside(std::integral_constant<int, (s * MT + j) * 2 + i>{});
             __builtin_amdgcn_sched_barrier(0);
@@ -569,47 +589,66 @@ __global__ __launch_bounds__(64 * WAVES, 2) void mx_slim_kernel(const MxMatmulPa
   const int mine = run_begin + wave;
   static_for<DEPTH>([&](auto d) { issue(mine + decltype(d)::value * WAVES, decltype(d)::value); });
   int place = 0;
+  // all of this wavefront's runs; PARTS: e4m3 activations in two parts
+  auto all_runs = [&](auto parts_tag) {
+    constexpr bool PARTS = decltype(parts_tag)::value;
 #pragma unroll 1
-  for (int run = mine; run < run_end; run += WAVES) {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 1) * T::kLoads) : "memory");
-    const uint32_t at = own + place * T::kPlace;
-    if (__builtin_expect(few, 0)) {   // (the only run)
-      if (lane < R) write_lds(at + T::kScales + lane * 16, few_scales(p.b_scales, batch * p.bs_bs + (n0 + lane) * p.bs_rs, p.groups, lane <= last_n));
-      if (lane < XR) write_lds(at + T::kScales + 1024 + lane * 16, few_scales(p.a_scales, batch * p.as_bs + (m0 + lane) * p.as_rs, p.groups, lane <= last_m));
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
-    i32x8 w[kSteps];
-    uint32_t sw[kWords];
+    for (int run = mine; run < run_end; run += WAVES) {
+      asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 1) * T::kLoads) : "memory");
+      const uint32_t at = own + place * T::kPlace;
+      if (__builtin_expect(few, 0)) {   // (the only run)
+        if (lane < R) write_lds(at + T::kScales + lane * 16, few_scales(p.b_scales, batch * p.bs_bs + (n0 + lane) * p.bs_rs, p.groups, lane <= last_n));
+        if (lane < XR) write_lds(at + T::kScales + 1024 + lane * 16, few_scales(p.a_scales, batch * p.as_bs + (m0 + lane) * p.as_rs, p.groups, lane <= last_m));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
+      i32x8 w[kSteps];
+      uint32_t sw[kWords];
 #pragma unroll
-    for (int u = 0; u < kWords; ++u) sw[u] = read_lds_word(at + T::kScales + row_w * 16 + part * (4 * kWords), 4 * u);
-    static_for<kSteps>([&](auto t_tag) {
-      constexpr int t = decltype(t_tag)::value;
-      w[t] = narrow_fragment(read_lds(at + row_w * 256 + (((part * kSteps + t) ^ ((row_w + 4) & 15)) << 4), 0));
-    });
-    static_for<T::kColumns>([&](auto j_tag) {
-      constexpr int j = decltype(j_tag)::value;
-      const int row = min(j * R + col, XR - 1);   // (columns past the last row are not written)
-      uint32_t sx[kWords];
-#pragma unroll
-      for (int u = 0; u < kWords; ++u) sx[u] = read_lds_word(at + T::kScales + 1024 + row * 16 + part * (4 * kWords), 4 * u);
+      for (int u = 0; u < kWords; ++u) sw[u] = read_lds_word(at + T::kScales + row_w * 16 + part * (4 * kWords), 4 * u);
       static_for<kSteps>([&](auto t_tag) {
         constexpr int t = decltype(t_tag)::value;
-        const uint32_t x_at = at + T::kBytesW + row * T::kRowX;
-        const int key = (row + 4) & 15;
-        i32x8 x;
-        if constexpr (A8) {   // R = 16: half part % 2 of places part / 2 and 2 + part / 2; R = 32: half `part` of both places
-          const int chunk = R == 16 ? 8 * (part >> 1) + 2 * t + (part & 1) : 2 * t + part;
-          x = fragment_of(read_lds(x_at + ((chunk ^ key) << 4), 0), read_lds(x_at + ((chunk ^ key) << 4), 256));
-        } else {
-          x = narrow_fragment(read_lds(x_at + (((part * kSteps + t) ^ key) << 4), 0));
-        }
-        if constexpr (R == 16) acc[j] = mfma_mx<A8, (t & 3)>(w[t], x, acc[j], sw[0], sx[0]);
-        else acc[j] = mfma_mx_32<A8, (t & 3)>(w[t], x, acc[j], sw[t >> 2], sx[t >> 2]);
+        w[t] = narrow_fragment(read_lds(at + row_w * 256 + (((part * kSteps + t) ^ ((row_w + 4) & 15)) << 4), 0));
       });
-    });
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (what has been read may be overwritten)
-    issue(run + DEPTH * WAVES, place);
-    place = place + 1 == DEPTH ? 0 : place + 1;
+      static_for<T::kColumns>([&](auto j_tag) {
+        constexpr int j = decltype(j_tag)::value;
+        const int row = min(j * R + col, XR - 1);   // (columns past the last row are not written)
+        uint32_t sx[kWords];
+#pragma unroll
+        for (int u = 0; u < kWords; ++u) sx[u] = read_lds_word(at + T::kScales + 1024 + row * 16 + part * (4 * kWords), 4 * u);
+        static_for<kSteps>([&](auto t_tag) {
+          constexpr int t = decltype(t_tag)::value;
+          const uint32_t x_at = at + T::kBytesW + row * T::kRowX;
+          const int key = (row + 4) & 15;
+          const auto multiply = [&](const i32x8& x) {
+            if constexpr (R == 16) acc[j] = mfma_mx<A8, (t & 3)>(w[t], x, acc[j], sw[0], sx[0]);
+            else acc[j] = mfma_mx_32<A8, (t & 3)>(w[t], x, acc[j], sw[t >> 2], sx[t >> 2]);
+          };
+          if constexpr (A8) {   // R = 16: half part % 2 of places part / 2 and 2 + part / 2; R = 32: half `part` of both places
+            const int chunk = R == 16 ? 8 * (part >> 1) + 2 * t + (part & 1) : 2 * t + part;
+            const i32x8 x = fragment_of(read_lds(x_at + ((chunk ^ key) << 4), 0), read_lds(x_at + ((chunk ^ key) << 4), 256));
+            if constexpr (PARTS) {
+              i32x8 high, low;
+              part_by_size(x, high, low);
+              multiply(low);
+              multiply(high);
+            } else {
+              multiply(x);
+            }
+          } else {
+            multiply(narrow_fragment(read_lds(x_at + (((part * kSteps + t) ^ key) << 4), 0)));
+          }
+        });
+      });
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // (what has been read may be overwritten)
+      issue(run + DEPTH * WAVES, place);
+      place = place + 1 == DEPTH ? 0 : place + 1;
+    }
+  };
+  if constexpr (A8) {   // (uniform; one loop with a branch in it cost 16-bit results of 32 rows 4 %)
+    if (p.out_kind == FP8_REAL_F32) all_runs(std::true_type{});
+    else all_runs(std::false_type{});
+  } else {
+    all_runs(std::false_type{});
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   settle();
@@ -700,10 +739,10 @@ hipError_t launch_slim(const MxMatmulParams& p, hipStream_t stream) {
   return join(p, stream);
 }
 
-template <int WN, int WM, int WK, int NT, int MT, bool A8, int STAGES, int WAVES_A_SIMD, bool GOES_ON, int OUT>
+template <int WN, int WM, int WK, int NT, int MT, bool A8, int STAGES, int WAVES_A_SIMD, bool GOES_ON, int OUT, bool PARTS = false>
 hipError_t launch_tile_as(const MxMatmulParams& p, hipStream_t stream) {
   using T = MxTile<WN, WM, WK, NT, MT, A8, STAGES, GOES_ON>;
-  constexpr auto kernel = &mx_tile_kernel<WN, WM, WK, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, OUT>;
+  constexpr auto kernel = &mx_tile_kernel<WN, WM, WK, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, OUT, PARTS>;
   if constexpr (T::kLds > 65536) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, T::kLds);
     if (e != hipSuccess) return e;
@@ -719,7 +758,9 @@ template <int WN, int WM, int WK, int NT, int MT, bool A8, int STAGES, int WAVES
 hipError_t launch_tile(const MxMatmulParams& p, hipStream_t stream) {
   if (p.splits == 1 && p.out_kind == FP8_REAL_BF16) return launch_tile_as<WN, WM, WK, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, FP8_REAL_BF16>(p, stream);
   if (p.splits == 1 && p.out_kind == FP8_REAL_F16) return launch_tile_as<WN, WM, WK, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, FP8_REAL_F16>(p, stream);
-  const hipError_t e = launch_tile_as<WN, WM, WK, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, FP8_REAL_F32>(p, stream);
+  // (shares of 16-bit results too are added in fp32, but of products as those have them)
+  const hipError_t e = A8 && p.out_kind == FP8_REAL_F32 ? launch_tile_as<WN, WM, WK, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, FP8_REAL_F32, A8>(p, stream)
+                                                        : launch_tile_as<WN, WM, WK, NT, MT, A8, STAGES, WAVES_A_SIMD, GOES_ON, FP8_REAL_F32>(p, stream);
   return e != hipSuccess ? e : join(p, stream);
 }
 
