@@ -555,7 +555,7 @@ VECOPS_HIP_EXPORT int32_t vecops_hip_matmul_fp8_block(const VecopsHipOperand* a,
  * Microscaled floats (OCP MX): elements with a power of two for each block of 32 along a row.  Elements are e4m3 as above, or
  * e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), two a byte, the one with the lower index in the lower four bits: extents and
  * strides of such operands count bytes, so that a row of K elements has K / 2 of them (K is even).  Scales are e8m0: byte E stands for
- * 2^(E - 127), 255 for NaN.
+ * 2^(E - 127), 255 for NaN.  Results of the calls from here to vecops_hip_silu_mul_quantize whose own elements share memory (a stride of 0, rows that overlap) are refused.
  */
 #define VECOPS_HIP_DTYPE_F4E2M1X2 65u
 #define VECOPS_HIP_DTYPE_F8E8M0 66u
@@ -606,6 +606,7 @@ VECOPS_HIP_EXPORT int32_t vecops_hip_matmul_mx(const VecopsHipOperand* a, const 
  *   e4m3 and f32 [..,M,ceil(K/128)]: as vecops_hip_quantize_fp8_block with block_rows 1
  *   e4m3 or e2m1 and e8m0 [..,M,ceil(K/32)]: as vecops_hip_quantize_mx
  * Ranks 2 or 3.  Rows of x, residual, summed, out and q are contiguous (at any alignment); other strides, and those of scales, are free.  Sums are held in fp32.
+ * Results share memory with nothing but as said here: not out with the sum, nor two rows with one another (a residual that all rows share needs a summed of its own).
  */
 VECOPS_HIP_EXPORT int32_t vecops_hip_rms_norm(const VecopsHipOperand* x, const VecopsHipOperand* weight, float eps,
                                               const VecopsHipOperand* residual, const VecopsHipOperand* summed,

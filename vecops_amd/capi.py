@@ -851,7 +851,7 @@ def matmul_mx(a, a_scales, b, b_scales, c, workspace=None, stream=None):
 
 def rms_norm(x, weight, q=None, scales=None, out=None, residual=None, summed=None, eps: float = 1e-6, stream=None):
     """y = h / sqrt(mean(h^2) + eps) * weight for the rows h = x + residual, which are written to ``summed`` (None: in the
-    residual's place).  ``out`` gets y in x's type; ``q`` and ``scales`` get it quantised, by their types: int8 with float32
+    residual's place, which no two rows may share then).  ``out`` gets y in x's type; ``q`` and ``scales`` get it quantised, by their types: int8 with float32
     [.., M, 1] (activations and row scales of ``matmul_i8_dequant``), ``float8_e4m3fn`` with float32 [.., M, ceil(K / 128)] (of
     ``matmul_fp8_block``), ``float8_e4m3fn`` or ``float4_e2m1fn_x2`` with ``float8_e8m0fnu`` (of ``matmul_mx``).  Returns what
     was asked for, (q, scales), out, or (q, scales, out)."""

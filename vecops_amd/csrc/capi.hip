@@ -1,6 +1,7 @@
 // C ABI of libvecops_hip.so (declared in include/vecops_hip.h): operand
 // validation, the GPU kernel-selection rule table and the kernel launches.
 #include <algorithm>
+#include <numeric>
 #include <hip/hip_runtime.h>
 
 #include <atomic>
@@ -2895,8 +2896,22 @@ int64_t mx_blocks(int64_t extent) { return (extent + kMxBlock - 1) / kMxBlock; }
 bool rows_contiguous(const View& v) { return v.cs == 1 || v.cols <= 1; }
 bool same_shape(const View& a, const View& b) { return a.batch == b.batch && a.rows == b.rows && a.cols == b.cols; }
 
-// A matrix and its microscaled copy; *nothing: there is no element.
-int32_t describe_mx_copy(const char* name, const VecopsHipOperand* x, const VecopsHipOperand* q, const VecopsHipOperand* scales, MxCopyParams* p,
+// Whether i s = j t for some |i| < n and |j| < m that are not both 0: the least of them are i = t / g and j = s / g.
+bool steps_meet(int64_t n, int64_t s, int64_t m, int64_t t) {
+  const uint64_t us = s < 0 ? uint64_t{0} - static_cast<uint64_t>(s) : static_cast<uint64_t>(s), ut = t < 0 ? uint64_t{0} - static_cast<uint64_t>(t) : static_cast<uint64_t>(t);
+  const uint64_t g = std::gcd(us, ut);
+  if (g == 0) return n > 1 || m > 1;
+  return ut / g < static_cast<uint64_t>(n) && us / g < static_cast<uint64_t>(m);
+}
+// Two elements of a result at one address: of those in one batch, one row or one column.
+bool shares_memory(const View& v) {
+  if (v.batch == 0 || v.rows == 0 || v.cols == 0) return false;
+  return steps_meet(v.rows, v.rs, v.cols, v.cs) || (v.batch > 1 && (steps_meet(v.batch, v.bs, v.rows, v.rs) || steps_meet(v.batch, v.bs, v.cols, v.cs)));
+}
+int32_t fail_shared(const char* name, const char* result) { return fail(ST_INVALID, "%s: %s: elements share memory", name, result); }
+
+// A matrix and its microscaled copy; *nothing: there is no element.  `back`: the matrix is the result.
+int32_t describe_mx_copy(const char* name, const VecopsHipOperand* x, const VecopsHipOperand* q, const VecopsHipOperand* scales, bool back, MxCopyParams* p,
                          bool* nothing) {
   View vx, vq, vs;
   if (!normalise(x, &vx) || !normalise(q, &vq) || !normalise(scales, &vs))
@@ -2912,6 +2927,9 @@ int32_t describe_mx_copy(const char* name, const VecopsHipOperand* x, const Veco
     return fail(ST_INVALID, "%s: scales must be [%lld, %lld]", name, (long long)vx.rows, (long long)groups);
   *nothing = vx.batch == 0 || vx.rows == 0 || vx.cols == 0;
   if (*nothing) return ST_OK;
+  if (back && shares_memory(vx)) return fail_shared(name, "out");
+  if (!back && shares_memory(vq)) return fail_shared(name, "q");
+  if (!back && shares_memory(vs)) return fail_shared(name, "scales");
   if (vx.data == nullptr || vq.data == nullptr || vs.data == nullptr) return fail(ST_INVALID, "%s: null operand", name);
   if (vx.batch > INT32_MAX || vx.rows > INT32_MAX || vx.cols > INT32_MAX / 2 || vx.batch * vx.rows > INT32_MAX / (4 * groups))
     return fail(ST_INVALID, "%s: extent too large", name);
@@ -2975,6 +2993,7 @@ int32_t describe_mx(const VecopsHipOperand* a, const VecopsHipOperand* a_scales,
   if (pr->a.cols * (pr->a.dtype == DT_E2M1X2 ? 2 : 1) != k)
     return fail(ST_INVALID, "matmul_mx: K of a (%lld) and b (%lld) differ", (long long)(pr->a.cols * (pr->a.dtype == DT_E2M1X2 ? 2 : 1)), (long long)k);
   if (pr->c.rows != m || pr->c.cols != n) return fail(ST_INVALID, "matmul_mx: c must be [M=%lld, N=%lld]", (long long)m, (long long)n);
+  if (shares_memory(pr->c)) return fail_shared("matmul_mx", "c");
   if (pr->b.batch != batch || pr->c.batch != batch || pr->sa.batch != batch || pr->sb.batch != batch) return fail(ST_INVALID, "matmul_mx: batch extents differ");
   if (pr->sa.rows != m || pr->sa.cols != mx_blocks(k))
     return fail(ST_INVALID, "matmul_mx: a_scales must be [M=%lld, ceil(K / 32)=%lld]", (long long)m, (long long)mx_blocks(k));
@@ -3018,6 +3037,8 @@ int32_t describe_row_results(const char* name, const VecopsHipOperand* q, const 
   const int64_t groups = p->format == ROW_INT8 ? 1 : p->format == ROW_E4M3_128 ? fp8_blocks(k) : mx_blocks(k);
   if (vs.batch != batch || vs.rows != rows || vs.cols != groups) return fail(ST_INVALID, "%s: scales must be [%lld, %lld]", name, (long long)rows, (long long)groups);
   if (!rows_contiguous(vq)) return fail(ST_NOT_APPLICABLE, "%s: rows of q must be contiguous", name);
+  if (k > 0 && shares_memory(vq)) return fail_shared(name, "q");
+  if (k > 0 && shares_memory(vs)) return fail_shared(name, "scales");
   if (batch * rows * k > 0 && (vq.data == nullptr || vs.data == nullptr)) return fail(ST_INVALID, "%s: null operand", name);
   p->q = static_cast<uint8_t*>(vq.data);
   p->scales = vs.data;
@@ -3034,7 +3055,7 @@ bool row_extents_ok(int64_t batch, int64_t rows, int64_t k) { return batch <= IN
 int32_t vecops_hip_quantize_mx(const VecopsHipOperand* x, const VecopsHipOperand* q, const VecopsHipOperand* scales, void* stream) {
   MxCopyParams p;
   bool nothing;
-  const int32_t rc = describe_mx_copy("quantize_mx", x, q, scales, &p, &nothing);
+  const int32_t rc = describe_mx_copy("quantize_mx", x, q, scales, false, &p, &nothing);
   if (rc != ST_OK || nothing) return rc;
   const hipError_t e = launch_mx_quantize(p, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return fail(ST_EXEC, "quantize_mx: kernel launch: %s", hipGetErrorString(e));
@@ -3044,7 +3065,7 @@ int32_t vecops_hip_quantize_mx(const VecopsHipOperand* x, const VecopsHipOperand
 int32_t vecops_hip_dequantize_mx(const VecopsHipOperand* q, const VecopsHipOperand* scales, const VecopsHipOperand* out, void* stream) {
   MxCopyParams p;
   bool nothing;
-  const int32_t rc = describe_mx_copy("dequantize_mx", out, q, scales, &p, &nothing);
+  const int32_t rc = describe_mx_copy("dequantize_mx", out, q, scales, true, &p, &nothing);
   if (rc != ST_OK || nothing) return rc;
   const hipError_t e = launch_mx_dequantize(p, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return fail(ST_EXEC, "dequantize_mx: kernel launch: %s", hipGetErrorString(e));
@@ -3134,8 +3155,10 @@ int32_t vecops_hip_rms_norm(const VecopsHipOperand* x, const VecopsHipOperand* w
     if (!normalise(b.operand, b.view) || b.operand->rank != x->rank || !same_shape(*b.view, vx)) return fail(ST_INVALID, "rms_norm: %s must have x's shape", b.name);
     if (b.view->dtype != vx.dtype) return fail(ST_NOT_APPLICABLE, "rms_norm: %s must be of x's type", b.name);
     if (!rows_contiguous(*b.view)) return fail(ST_NOT_APPLICABLE, "rms_norm: rows of %s must be contiguous", b.name);
+    if (b.view != &vr && shares_memory(*b.view)) return fail_shared("rms_norm", b.name);
     if (vx.batch * vx.rows * k > 0 && b.view->data == nullptr) return fail(ST_INVALID, "rms_norm: null operand");
   }
+  if (vx.batch * vx.rows * k > 0 && out != nullptr && summed != nullptr && vo.data == vh.data) return fail(ST_INVALID, "rms_norm: out and summed are two results");
   if (!rows_contiguous(vx)) return fail(ST_NOT_APPLICABLE, "rms_norm: rows of x must be contiguous");
   if (!row_extents_ok(vx.batch, vx.rows, k)) return fail(ST_INVALID, "rms_norm: extent too large");
   RowQuantizeParams p = {};
