@@ -239,11 +239,14 @@ def _check(rc: int) -> None:
         raise VecopsHipError(rc, lib().vecops_hip_last_error().decode())
 
 
+# (by name: a torch without the microscaled types has calls on the others all the same)
+_TORCH_DTYPES = {"torch.int8": I8, "torch.uint8": U8, "torch.int32": I32, "torch.float16": F16, "torch.bfloat16": BF16,
+                 "torch.float32": F32, "torch.float64": F64, "torch.float8_e4m3fn": F8E4M3, "torch.float4_e2m1fn_x2": F4E2M1X2,
+                 "torch.float8_e8m0fnu": F8E8M0}
+
+
 def _torch_dtype_code(t) -> int:
-    import torch
-    return {torch.int8: I8, torch.uint8: U8, torch.int32: I32, torch.float16: F16, torch.bfloat16: BF16,
-            torch.float32: F32, torch.float64: F64, torch.float8_e4m3fn: F8E4M3, torch.float4_e2m1fn_x2: F4E2M1X2,
-            torch.float8_e8m0fnu: F8E8M0}[t.dtype]
+    return _TORCH_DTYPES[str(t.dtype)]
 
 
 def operand(t) -> Operand:

@@ -12,6 +12,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/jit/python/pybind_utils.h>
 #include <torch/library.h>
+#include <torch/version.h>
 
 #include <ATen/ATen.h>
 #include <c10/hip/HIPFunctions.h>
@@ -275,9 +276,11 @@ int matmul_packed_b(PyObject* const* args) {
 bool describe_any(PyObject* object, VecopsHipOperand* o) {
   const at::Tensor* t = plain_tensor(object);
   if (t == nullptr) return false;
-  const uint32_t dtype = t->scalar_type() == at::kFloat8_e4m3fn ? VECOPS_HIP_DTYPE_F8E4M3
-                         : t->scalar_type() == at::kFloat8_e8m0fnu ? VECOPS_HIP_DTYPE_F8E8M0
-                         : t->scalar_type() == at::kFloat4_e2m1fn_x2 ? VECOPS_HIP_DTYPE_F4E2M1X2 : 0;
+  uint32_t dtype = t->scalar_type() == at::kFloat8_e4m3fn ? VECOPS_HIP_DTYPE_F8E4M3 : 0;
+#if TORCH_VERSION_MAJOR > 2 || TORCH_VERSION_MINOR >= 8   // (those before have no tensors of the microscaled types)
+  if (t->scalar_type() == at::kFloat8_e8m0fnu) dtype = VECOPS_HIP_DTYPE_F8E8M0;
+  if (t->scalar_type() == at::kFloat4_e2m1fn_x2) dtype = VECOPS_HIP_DTYPE_F4E2M1X2;
+#endif
   if (dtype == 0) return describe(*t, o);
   const int64_t rank = t->dim();
   if (rank > 3) return false;
