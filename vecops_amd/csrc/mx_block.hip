@@ -774,7 +774,9 @@ hipError_t launch_tile(const MxMatmulParams& p, hipStream_t stream) {
 // slower than the fastest of them on average and 1.19 times at worst.  The best choice without one of them would be slower by 2.2 % (MX_ROWS_4),
 // 2.1 % (MX_TILE_256), 1.5 % (MX_TILE_128), 1.1 % (MX_ROWS_32), 0.9 % (MX_ROWS_4_DEEP), 0.6 % (MX_TILE_128X64, MX_TILE_128_DEEP), 0.5 % (MX_ROWS_16_DEEP) and
 // 0.3 % (shares, 1.38 times at worst; four shares rather than two, or of few rows, 0.04 %); 32 x 64 results a workgroup and 4 x 16 by four wavefronts
-// brought 0.2 % each and are left out.  Up to four rows only kernels of four are weighed: on a tie of latencies the fit's errors would decide.
+// brought 0.2 % each and are left out.  K of up to 512 lie at the fit's edge or past it: of 92 such products (M 256 .. 8192, N 2048 .. 16384, K 128, 256, 480, 512)
+// with e4m3 what it takes is 0.1 % slower than the fastest, 1.04 times at worst, with e2m1 5 % and 1.51 times (MX_TILE_128 where MX_TILE_256 has three rounds and
+// more: 4096 x 16384 x 480 71 us rather than 47).  Up to four rows only kernels of four are weighed: on a tie of latencies the fit's errors would decide.
 MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int64_t batch, bool a_wide) {
   struct Cost {
     int rows_a, rows_b, wavefronts, slots;   // as powers of two; wavefronts that share k by whole runs
@@ -819,7 +821,7 @@ MxPlan mx_plan(int64_t m, int64_t n, int64_t k, int64_t batch, bool a_wide) {
       float us = cost.once + rounds * (cost.start + (cost.alone + cost.more * (slots - 1)) * each);
       if (rest > 0) us += cost.start + (cost.alone + cost.more * (rest - 1)) * each;
       us = std::sqrt(std::sqrt(us * us * us * us + moved * moved * moved * moved));
-      if (kind == MX_TILE_256 && runs <= 1) us += 2.5f;   // (for the launch that lays out scales too few a row)
+      if (kind == MX_TILE_256 && k % kMxBlock == 0 && k / kMxBlock < kRunBlocks) us += 2.5f;   // (for the launch that lays out scales too few a row; a K of no whole blocks has one anyway)
       if (split > 0) us += 3.2f + 2.8e-6f * (static_cast<float>(m) * n * batch);
       if (us < least) least = us, best = {kind, 1 << split, 1 << cost.rows_a, 1 << cost.rows_b, kind == MX_TILE_256 ? kRunBlocks : 0};
     }
