@@ -18,16 +18,15 @@ namespace {
 // A lane's e2m1 operand is 32 k of one row (16 bytes), lanes 16 q .. 16 q + 15 block q of four, and its scale is that block's.
 // An e4m3 operand is 32 bytes: k 16 q .. 16 q + 15 and 64 + 16 q .., so that block b lies in the lanes of 2 b and 2 b + 1 (of
 // eight halves), while its scale is still taken from the lanes of quarter b.
-// Which block of a row goes into which of the four places is free, as long as both operands and scales agree: a step of 256 k is
-// two instructions, and instruction h has block 2 q + h in place q.  A lane then holds the scales of neighbouring blocks.
+// Which block of a row goes into which of the four places is free, as long as both operands and scales agree: blocks are dealt so that a lane's scales of
+// several instructions are neighbours, bytes of one word.
 // e2m1 times e2m1 is exact up to one rounding to fp32 an instruction (measured: 3e-8 of the terms' sizes).  With e4m3 the instruction aligns
 // each eight products along k to the largest and drops what is below 2^-13 of it: 1.4e-5 of a result on normally distributed
-// operands, which goes unnoticed in results of 16 bits.  For results in f32 the activations are taken in two parts by size, an instruction each, whose products
+// operands, at worst 7 * 2^-13 of the terms' sizes.  Results of 16 bits, whose own rounding is 2^-8 or 2^-11, are left with it.  For results in f32 the activations are taken in two parts by size, an instruction each, whose products
 // are exact as e2m1's are: 30 to 70 % more time where many rows share weights (4096 x 11008 x 4096 290 us rather than 177, 128 x 11008 x 4096 21.6 rather than 17.1),
 // none to speak of for a few rows.  A scale that is NaN makes the result NaN, also over elements of zero.
 // ---------------------------------------------------------------------------------------------------------------------
 
-constexpr int kStepBlocks = 8;                  // blocks of 32 k in a step
 constexpr uint32_t kNowhere = 0x80000000u;      // an offset past every descriptor's end: zeros arrive
 
 // OPSEL: which byte of the scales' registers counts.
@@ -67,14 +66,8 @@ __device__ __forceinline__ void settle() {
 #endif
 }
 
-// Scales arrive as words of four blocks; a row's last word is its last four bytes, so that no load passes a row's end (rows have at least
-// four).  Word `word` of a row of `groups` is fetched from byte scale_word_at() on, and holds its own blocks from bit scale_shift() on (with blocks
-// past the row's end as zeros, which stand for 2^-127).
-__device__ __forceinline__ int scale_word_at(int word, int groups) { return min(4 * word, groups - 4); }
-__device__ __forceinline__ uint32_t scale_shift(int word, int groups) { return static_cast<uint32_t>(min(max(4 * word + 4 - groups, 0) * 8, 31)); }
-
-// Rows of fewer scales than a load fetches (K < 512): a lane reads those that there are, byte by byte, and writes them to LDS itself, with zeros
-// behind, where a load has left zeros (1 x 640 x 256 4.9 us a call, 109 x 3200 x 256 6.5; with rows laid out in the workspace first 6.4 and 8.7.  It costs 64 x 64
+// Scales arrive sixteen of a row a load, a row's last sixteen by one that ends with the row.  Rows of fewer (K of up to 480): a lane reads those that there are,
+// byte by byte, and writes them to LDS itself, with zeros behind, where a load has left zeros (1 x 640 x 256 4.9 us a call, 109 x 3200 x 256 6.5; with rows laid out in the workspace first 6.4 and 8.7.  It costs 64 x 64
 // tiles of longer rows 0.15 us of 7.6).  MX_TILE_256, whose workgroups go on to other tiles, has them laid out.
 __device__ __forceinline__ u32x4 few_scales(const uint8_t* base, int64_t at, int groups, bool there) {
   u32x4 v = {0u, 0u, 0u, 0u};
