@@ -24,7 +24,7 @@ namespace {
 // each eight products along k to the largest and drops what is below 2^-13 of it: 1.4e-5 of a result on normally distributed
 // operands, at worst 7 * 2^-13 of the terms' sizes.  Results of 16 bits, whose own rounding is 2^-8 or 2^-11, are left with it.  For results in f32 the activations are taken in two parts by size, an instruction each, whose products
 // are exact as e2m1's are: 30 to 70 % more time where many rows share weights (4096 x 11008 x 4096 290 us rather than 177, 128 x 11008 x 4096 21.6 rather than 17.1),
-// none to speak of for a few rows.  A scale that is NaN makes the result NaN, also over elements of zero.
+// for a few rows 1 us of 7 (M up to 4) or less.  A scale that is NaN makes the result NaN, also over elements of zero.
 // ---------------------------------------------------------------------------------------------------------------------
 
 constexpr uint32_t kNowhere = 0x80000000u;      // an offset past every descriptor's end: zeros arrive
@@ -87,9 +87,9 @@ __device__ __forceinline__ u32x4 few_scales(const uint8_t* base, int64_t at, int
 // in use, by loads that write LDS.  Scales come two stages a run, sixteen bytes of a row a load: each is a request of its own to
 // the cache, which a word a row for each 128 k had by the half of all requests.  A row's last run is its last sixteen scales; what of it
 // has been summed before gets zeros for elements.
-// 4096 x 11008 x 4096: e2m1 98-101 us (3.7 PFLOP/s; the matrix pipes busy 54 % of the cycles of a clock that they pull down to 1.65 GHz, 38 GB/s of loads a
-// compute unit, and 8 us a tile in which all of them write), e4m3 167 us (2.2 PFLOP/s).
-// 128 weight rows by 64, two wavefronts sharing k: a third less to load a result than 64 x 64; 128 x 11008 x 4096 with e4m3 16.4 us rather than 20.4,
+// 4096 x 11008 x 4096 on weights that no cache holds: e2m1 102 us (3.6 PFLOP/s; the matrix pipes busy 54 % of the cycles of a clock that they pull down to
+// 1.65 GHz, 38 GB/s of loads a compute unit, and 8 us a tile in which all of them write), e4m3 167 us (2.2 PFLOP/s).
+// 128 weight rows by 64, two wavefronts sharing k: a third less to load a result than 64 x 64; on such weights 128 x 11008 x 4096 with e4m3 16.4 us rather than 20.4,
 // 512 x 4096 x 11008 35.4 rather than 44, 1024 x 2048 x 8192 25.7 rather than 31.6 (e2m1 22.4 and 23.5).
 // The rows of a block of weights are dealt so that a lane's sixteen results are neighbouring n (the instruction's row
 // 8 g + 4 h + e, which lane half h holds, is n = 16 h + 4 g + e).

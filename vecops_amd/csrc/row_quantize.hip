@@ -170,7 +170,8 @@ __device__ __forceinline__ void store_bytes(uint8_t* base, int64_t at, int64_t c
   }
 }
 
-// Eight elements a lane, four lanes a block.  Bound by HBM: 11008 x 4096 bf16 to e2m1 23.2 us, and back 22.0 (4.9 and 5.2 TB/s read and written).
+// Eight elements a lane, four lanes a block.  Bound by HBM: 11008 x 4096 bf16 to e2m1 29.3 us, and back 21.2 (3.9 and 5.4 TB/s read and written; of a matrix
+// that the last cache holds 21.8 and 20.8).
 template <int KIND, int FORMAT>
 __global__ __launch_bounds__(256) void mx_quantize_kernel(const MxCopyParams p, uint32_t total) {
   const uint32_t per_line = static_cast<uint32_t>(p.groups) * 4u;
@@ -240,8 +241,8 @@ __global__ __launch_bounds__(256) void mx_dequantize_kernel(const MxCopyParams p
 // ---------------------------------------------------------------------------------------------------------------------
 // Rows.  T threads a row (64: four rows a workgroup, no barrier; else a workgroup a row), eight elements a thread a piece, HELD
 // pieces of a thread in registers: a row of up to 8 HELD T elements is read once.  A longer one is read again behind each sum or
-// maximum over it, by the threads that read (and wrote) the same places before.  Bound by HBM (4096 x 8192 bf16 with the residual to e4m3 by 32 50.8 us, 4.7 TB/s;
-// the gate of 1999 x 11000 f16 to e4m3 by 128 25 us, 4.4 TB/s), for a few rows by the launch and one
+// maximum over it, by the threads that read (and wrote) the same places before.  Bound by HBM (4096 x 8192 bf16 with the residual to e4m3 by 32 50.8 us, 4.6 TB/s, and 42 where
+// the last cache holds most of the operands; the gate of 1999 x 11000 f16 to e4m3 by 128 26-27 us, 4.1 TB/s, and 24), for a few rows by the launch and one
 // row's way through memory and barriers: rows that a piece a thread holds have kernels of their own, a quarter as much code to fetch, and weights
 // under way beside the row (4 x 4096 with the residual, bf16 to e4m3 by 128: 4.0 us a call rather than 5.0; a launch alone is 2.5).
 // ---------------------------------------------------------------------------------------------------------------------
