@@ -605,7 +605,8 @@ VECOPS_HIP_EXPORT int32_t vecops_hip_matmul_mx(const VecopsHipOperand* a, const 
  *                          row_scales of vecops_hip_matmul_i8_dequant (a NaN in the row makes its scale NaN, an infinity infinite)
  *   e4m3 and f32 [..,M,ceil(K/128)]: as vecops_hip_quantize_fp8_block with block_rows 1
  *   e4m3 or e2m1 and e8m0 [..,M,ceil(K/32)]: as vecops_hip_quantize_mx
- * Ranks 2 or 3.  Rows of x, residual, summed, out and q are contiguous (at any alignment); other strides, and those of scales, are free.  Sums are held in fp32.
+ * Ranks 2 or 3.  Rows of x, residual, summed, out and q are contiguous (at any alignment); other strides, and those of scales, are free.  Sums are held in fp32
+ * (so that a row whose squares leave its range, of |h| past 1.8e19, becomes zeros).
  * Rows of no elements (K = 0) have no results: nothing is written, the scale that an int8 row otherwise has included.
  * Results share memory with nothing but as said here: not out with the sum, nor two rows with one another (a residual that all rows share needs a summed of its own).
  */

@@ -1,4 +1,4 @@
-"""Rows without elements: the row operators and quantisers write nothing, as their header says, scales of int8 rows included."""
+"""Rows without elements, of which the row operators and quantisers write nothing, scales of int8 rows included, and rows whose squares fp32 does not hold."""
 import pytest
 import torch
 
@@ -25,3 +25,20 @@ def test_nothing_is_written(device, form, lead):
         capi.dequantize_mx(q, scales, out)
     torch.cuda.synchronize()
     assert torch.equal(scales.view(torch.uint8), before)
+
+
+@pytest.mark.parametrize("form", FORMATS)
+def test_squares_past_fp32(device, form):
+    """A sum of squares that fp32 does not hold: its row becomes zeros, as the header says, and the rows beside it stay."""
+    x = torch.randn((3, 640), generator=torch.Generator().manual_seed(1)).to(device)
+    x[1, 77] = 1e20
+    weight = torch.ones(640, device=device)
+    found = []
+    for rows in (x, x[0::2].contiguous()):
+        q, scales = results(rows.shape[:1], 640, form)
+        out = torch.empty_like(rows)
+        capi.rms_norm(rows, weight, q=q, scales=scales, out=out)
+        found.append((out, q.view(torch.uint8), scales.view(torch.uint8)))
+    assert bool((found[0][0][1] == 0).all()) and bool(torch.isfinite(found[0][0]).all())
+    for some, others in zip(*found):
+        assert torch.equal(some[0::2], others)
